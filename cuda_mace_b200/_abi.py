@@ -82,6 +82,14 @@ SIGNATURES = {
     "cmace_linear_tc_f32": [_P, _P, _P, _P, _I, _L, _I, _I, _D, _P, _P, _P],
     "cmace_bounded_wait_probe": [_P, _I, _D, _P],
     "cmace_gemm3x_gradr_f32": [_P, _P, _P, _P, _P, _P, _L, _I, _I, _P, _P, _P],
+    "cmace_gated_ff_workspace_bytes": [_I, _L, _I, _I, _I],
+    "cmace_gated_ff_fwd_f32": [_P, _P, _P, _P, _L, _I, _I, _I, _P, _P, _L, _P, _P],
+    "cmace_gated_ff_fwd_bf16": [_P, _P, _P, _P, _L, _I, _I, _I, _P, _P, _L, _P, _P],
+    "cmace_gated_ff_bwd_f32": [_P, _P, _P, _P, _P, _L, _I, _I, _I, _P, _P, _P, _P, _P, _L, _P, _P],
+    "cmace_gated_ff_bwd_bf16": [_P, _P, _P, _P, _P, _L, _I, _I, _I, _P, _P, _P, _P, _P, _L, _P, _P],
+    "cmace_orthogonalize_workspace_bytes": [_I, _L, _L, _I],
+    "cmace_orthogonalize_f32": [_P, _L, _L, _I, _I, _D, _D, _D, _D, _P, _P, _L, _P, _P],
+    "cmace_orthogonalize_bf16": [_P, _L, _L, _I, _I, _D, _D, _D, _D, _P, _P, _L, _P, _P],
     "cmace_radial_hidden_saved_floats": [_L],
     "cmace_radial_hidden_fwd_f32": [_P, _I, _P, _P, _P, _L, _P, _P, _P, _P],
     "cmace_radial_hidden_bwd_f32": [_P, _P, _P, _P, _P, _I, _L, _P, _P, _P],
@@ -118,6 +126,8 @@ _RESTYPES = {
     "cmace_sender_order_workspace_bytes": _L,
     "cmace_imp_bwd_scratch_elems": _L,
     "cmace_gemm_packed_floats": _L,
+    "cmace_gated_ff_workspace_bytes": _L,
+    "cmace_orthogonalize_workspace_bytes": _L,
     "cmace_radial_hidden_saved_floats": _L,
     "cmace_nl_num_cells": _L,
     "cmace_nl_workspace_bytes": _L,
@@ -128,7 +138,7 @@ _RESTYPES = {
     "cmace_symcon_plan_destroy": None,
 }
 # functions whose integer result is a value, not a status
-_VALUE_FUNCS = {"cmace_abi_version", "cmace_sender_order_workspace_bytes", "cmace_imp_bwd_scratch_elems",
+_VALUE_FUNCS = {"cmace_abi_version", "cmace_gated_ff_workspace_bytes", "cmace_orthogonalize_workspace_bytes", "cmace_sender_order_workspace_bytes", "cmace_imp_bwd_scratch_elems",
                 "cmace_gemm_packed_floats", "cmace_imp_bwd_edge_f64_noalloc_max_elems",
                 "cmace_radial_hidden_saved_floats", "cmace_nl_num_cells", "cmace_nl_workspace_bytes", "cmace_scan_workspace_bytes",
                 "cmace_imp_staged_stalled", "cmace_step_workspace_bytes", "cmace_step_count", "cmace_step_struct_bytes", "cmace_step_name",
@@ -146,6 +156,7 @@ KERNEL_LAUNCHES = {
     "cmace_spline_fwd": 1, "cmace_spline_bwd": 1, "cmace_imp_fwd": 1, "cmace_imp_bwd_edge": 1, "cmace_imp_bwd_edge_f64_noalloc": 2,
     "cmace_imp_bwd_node": 1, "cmace_imp_bwd_node_edges": 1, "cmace_linear": 1, "cmace_symcon_fwd": 1, "cmace_symcon_bwd": 1,
     "cmace_gemm_pack_weights": 1, "cmace_gemm3x": 1, "cmace_gemm": 1, "cmace_gemm3x_gradr": 1, "cmace_bounded_wait_probe": 1, "cmace_linear_tc": 1,
+    "cmace_gated_ff_fwd": 3, "cmace_gated_ff_fwd_bf16": 2, "cmace_gated_ff_bwd": 5, "cmace_gated_ff_bwd_bf16": 4,
     "cmace_radial_hidden_fwd": 1, "cmace_radial_hidden_bwd": 1, "cmace_imp_radial_fused_fwd": 1,
     "cmace_symcon_effective_weights": 1, "cmace_symcon_apply": 1, "cmace_nl_build": 4, "cmace_nl_emit": 1, "cmace_nl_cell_ids": 1, "cmace_nl_count": 1, "cmace_exclusive_scan_i32": 1, "cmace_nl_fill": 1,
 }

@@ -1,0 +1,430 @@
+// The gated feed-forward block y = (act(x Wg) * (x Wu)) Wd on rows of node features, and its backward.  x [M, C], Wg and Wu [C, H],
+// Wd [H, C], act = SiLU or GELU (with erf).
+//
+//   forward   h = act(x Wg) * (x Wu)          one kernel: both projections are one product with 256 columns a tile, the gate is
+//             y = h Wd                        applied to the accumulators; h [M, H] goes out once, in the operands' form
+//   backward  g, u as above, dh = dy Wd^T     one kernel: three products a tile, h, dg = dh u act'(g) and du = dh act(g) out
+//             dx = dg Wg^T + du Wu^T          one product over 2 H
+//             dWg = x^T dg, dWu = x^T du, dWd = h^T dy    one launch of three products over M, split where M is long
+// Only x and the weights are kept for the backward: forming g and u again costs 4 M C H operations, keeping them in float32 16 bytes
+// a hidden value written and read (what would be as exact as the products are), which pays from C of about 1 000 only.
+//
+// float32 goes as pairs of fp16 values (tile_product.cuh); a first kernel splits x and the weights.  bf16 is read where it lies;
+// rows that TMA cannot address (a width that is not a multiple of eight, an address that is not one of 16 bytes) are copied first.
+// In bf16, h, dg and du are rounded once to bf16 between the products, as the operands of a 16-bit product have to be; with the
+// rounding of the results that makes 1.4 times the error of a result that is rounded alone.  Sums over M are float32.
+#include <algorithm>
+
+#include "tile_product.cuh"
+
+namespace cmace {
+
+// ---- operands: float32 to pairs, bf16 rows to rows of a multiple of 16 bytes ------------------------------------------------
+struct PrepJob {
+  const void *src;
+  void *hi, *lo;       // lo null: copy
+  float *scale;        // inverse scales of the blocks
+  int64_t rows, first; // first block of this job
+  int cols, ld, blocks_n;
+};
+struct PrepArgs {
+  PrepJob job[5];
+  int jobs;
+};
+constexpr int PREP_THREADS = 256;
+
+// One block of 64 x 64 values a CTA: a thread takes four columns of every 16th row, or one column of every 4th.
+__global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const __grid_constant__ PrepArgs p) {
+  __shared__ float most_of[PREP_THREADS / 32];
+  grid_begin();
+  int j = 0;
+  while (j + 1 < p.jobs && (int64_t)blockIdx.x >= p.job[j + 1].first) j++;
+  const PrepJob &J = p.job[j];
+  const int64_t b = blockIdx.x - J.first;
+  const int64_t rb = b / J.blocks_n;
+  const int cb = (int)(b - rb * J.blocks_n);
+  const int64_t row0 = rb * 64;
+  const int col0 = cb * 64, t = threadIdx.x;
+  if (J.lo == nullptr) {
+    const uint16_t *s = static_cast<const uint16_t *>(J.src);
+    uint16_t *d = static_cast<uint16_t *>(J.hi);
+    const int col = col0 + (t & 63);
+    if (col < J.cols)
+      for (int r = t >> 6; r < 64 && row0 + r < J.rows; r += 4) d[(row0 + r) * J.ld + col] = s[(row0 + r) * J.cols + col];
+    return;
+  }
+  const float *s = static_cast<const float *>(J.src);
+  const bool wide = (J.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(J.src) & 15) == 0;
+  float v[16];
+  float most = 0.f;
+  if (wide) {
+    const int col = col0 + 4 * (t & 15);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int64_t r = row0 + (t >> 4) + 16 * i;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < J.rows && col < J.cols) x = __ldg(reinterpret_cast<const float4 *>(s + r * J.cols + col));
+      v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+    }
+  } else {
+    const int col = col0 + (t & 63);
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const int64_t r = row0 + (t >> 6) + 4 * i;
+      v[i] = r < J.rows && col < J.cols ? __ldg(s + r * J.cols + col) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; i++) most = fmaxf(most, tp_finite_abs(v[i]));
+  most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+  if ((t & 31) == 0) most_of[t >> 5] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < PREP_THREADS / 32; w++) most = fmaxf(most, most_of[w]);
+  const float scale = tp_scale(most);
+  if (t == 0) J.scale[b] = 1.0f / scale;
+  __half *hi = static_cast<__half *>(J.hi), *lo = static_cast<__half *>(J.lo);
+  if (wide) {
+    const int col = col0 + 4 * (t & 15);
+    if (col >= J.cols) return;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int64_t r = row0 + (t >> 4) + 16 * i;
+      if (r >= J.rows) break;
+      uint2 h, l;
+      tp_split2(v[4 * i] * scale, v[4 * i + 1] * scale, h.x, l.x);
+      tp_split2(v[4 * i + 2] * scale, v[4 * i + 3] * scale, h.y, l.y);
+      *reinterpret_cast<uint2 *>(hi + r * J.ld + col) = h;
+      *reinterpret_cast<uint2 *>(lo + r * J.ld + col) = l;
+    }
+  } else {
+    const int col = col0 + (t & 63);
+    if (col >= J.cols) return;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const int64_t r = row0 + (t >> 6) + 4 * i;
+      if (r >= J.rows) break;
+      uint32_t h, l;
+      tp_split2(v[i] * scale, 0.f, h, l);
+      hi[r * J.ld + col] = __ushort_as_half((unsigned short)h);
+      lo[r * J.ld + col] = __ushort_as_half((unsigned short)l);
+    }
+  }
+}
+
+// ---- weight gradients: the splits' sums, the third transposed ------------------------------------------------------------------
+struct WeightReduce {
+  const float *partial;   // [splits][3][C][ld]
+  void *out[3];
+  int64_t ld;
+  int splits, C, H;
+};
+// A block sums 32 x 32 values of one matrix, in the order of the splits.
+template <typename T>
+__global__ void __launch_bounds__(256) weight_reduce_kernel(const WeightReduce p) {
+  __shared__ float tile[32][33];
+  grid_begin();
+  const int which = blockIdx.z, c0 = blockIdx.y * 32, h0 = blockIdx.x * 32;
+  T *out = static_cast<T *>(p.out[which]);
+  if (out == nullptr) return;
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t matrix = (int64_t)p.C * p.ld;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int c = c0 + y + 8 * i, h = h0 + x;
+    float sum = 0.f;
+    if (c < p.C && h < p.H) {
+      const float *v = p.partial + which * matrix + (int64_t)c * p.ld + h;
+      for (int s = 0; s < p.splits; s++) sum += __ldcg(v + (int64_t)s * 3 * matrix);
+      if (which < 2) out[(int64_t)c * p.H + h] = (T)sum;
+    }
+    tile[y + 8 * i][x] = sum;
+  }
+  if (which < 2) return;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int h = h0 + y + 8 * i, c = c0 + x;
+    if (c < p.C && h < p.H) out[(int64_t)h * p.C + c] = (T)tile[x][y + 8 * i];
+  }
+}
+
+// ---- a call -----------------------------------------------------------------------------------------------------------------
+struct FeedForward {
+  bool f32;
+  const void *x, *wg, *wu, *wd, *gy;
+  int64_t M;
+  int C, H, act;
+  int32_t *status;
+  cudaStream_t st;
+  const char *what;
+};
+
+// A caller's matrix: read where it lies, or laid out in the workspace by the job that is added.
+static Matrix take_matrix(Carve &w, PrepArgs &prep, int64_t &blocks, bool f32, const void *src, int64_t rows, int cols) {
+  if (!f32 && cols % 8 == 0 && aligned16(src)) {
+    Matrix m;
+    m.hi = const_cast<void *>(src);
+    m.rows = rows, m.cols = cols, m.ld = cols;
+    return m;
+  }
+  const Matrix m = new_matrix(w, f32, rows, cols, 1);
+  PrepJob &j = prep.job[prep.jobs++];
+  j = PrepJob{src, m.hi, m.lo, m.scale, rows, blocks, cols, (int)m.ld, (int)m.blocks_n()};
+  blocks += m.blocks_m() * m.blocks_n();
+  return m;
+}
+
+static int set_hidden_out(TpArgs &g, const Matrix &m, int box_cols, bool bf16, const char *what) {
+  const void *base[2] = {m.hi, m.lo};
+  for (int t = 0; t < (m.lo ? 2 : 1); t++) {
+    const int rc = encode_tile_map(&g.out[t].map, base[t], 2, bf16, m.cols, m.rows, m.batches, m.ld, m.rows * m.ld, box_cols, 32, what);
+    if (rc) return rc;
+    g.out[t].use_map = 1;
+  }
+  for (int p = 0; p < 3 && m.scale; p++) g.out_scale[p] = m.scale + (m.batches > 1 ? p : 0) * m.blocks_m() * m.blocks_n();
+  g.out_scale_ld = m.blocks_n();
+  return CMACE_OK;
+}
+// rows of a caller's array: by TMA where it can address them
+static int set_user_out(TpArgs &g, void *ptr, bool f32, int64_t rows, int cols, const char *what) {
+  TpOut &o = g.out[0];
+  o.ptr = ptr;
+  o.ld = cols;
+  o.batch = rows * (int64_t)cols;
+  g.out_bf16 = !f32;
+  const int bytes = f32 ? 4 : 2;
+  o.use_map = aligned16(ptr) && (int64_t)cols * bytes % 16 == 0;
+  if (o.use_map) return encode_tile_map(&o.map, ptr, bytes, !f32, cols, rows, 1, cols, rows * (int64_t)cols, f32 ? 32 : 64, 32, what);
+  return CMACE_OK;
+}
+
+template <int KIND, int ACT>
+static int launch_kind(bool pair, TpArgs &g, cudaStream_t st, const char *what) {
+  return pair ? tp_launch<KIND, true, 128, ACT>(g, st, what) : tp_launch<KIND, false, 128, ACT>(g, st, what);
+}
+template <int KIND>
+static int launch_hidden(const FeedForward &f, TpArgs &g) {
+  return f.act == TP_SILU ? launch_kind<KIND, TP_SILU>(f.f32, g, f.st, f.what) : launch_kind<KIND, TP_GELU>(f.f32, g, f.st, f.what);
+}
+static int launch_plain(bool pair, int tn, TpArgs &g, cudaStream_t st, const char *what) {
+  if (tn == 256) return pair ? tp_launch<TP_PLAIN, true, 256>(g, st, what) : tp_launch<TP_PLAIN, false, 256>(g, st, what);
+  return pair ? tp_launch<TP_PLAIN, true, 128>(g, st, what) : tp_launch<TP_PLAIN, false, 128>(g, st, what);
+}
+
+static int run_prep(const PrepArgs &p, int64_t blocks, cudaStream_t st, const char *what) {
+  if (blocks == 0) return CMACE_OK;
+  if (blocks >= (int64_t)1 << 31) return fail(CMACE_ERR_UNSUPPORTED, "%s: too many rows", what);
+  launch_chained(prep_kernel, dim3((unsigned)blocks), dim3(PREP_THREADS), (size_t)0, st, p);
+  return check_launch(what);
+}
+
+// Splits of the weight gradients' sum over M: rounds of tiles times the length of one, a few blocks of 64 rows for filling the ring
+// and handing over the sums, and the traffic of the partial sums.
+static int weight_splits(int64_t M, int C, int H, int tn) {
+  const int64_t tiles = 3 * ((C + 127) / 128) * (int64_t)((H + tn - 1) / tn), kb = blocks64(M);
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 64 && s <= kb; s++) {
+    const double cost = (double)((tiles * s + 147) / 148) * ((double)((kb + s - 1) / s) + 6.0) + s * 3.0 * C * H * 1.5e-6;
+    if (s == 1 || cost < least) best = s, least = cost;
+  }
+  return best;
+}
+
+static int forward(const FeedForward &f, void *y, Carve &w) {
+  PrepArgs prep;
+  memset(&prep, 0, sizeof(prep));
+  int64_t blocks = 0;
+  const Matrix x = take_matrix(w, prep, blocks, f.f32, f.x, f.M, f.C);
+  const Matrix wg = take_matrix(w, prep, blocks, f.f32, f.wg, f.C, f.H);
+  const Matrix wu = take_matrix(w, prep, blocks, f.f32, f.wu, f.C, f.H);
+  const Matrix wd = take_matrix(w, prep, blocks, f.f32, f.wd, f.H, f.C);
+  const Matrix h = new_matrix(w, f.f32, f.M, f.H, 1);
+  if (!w.base) return CMACE_OK;
+  int rc = run_prep(prep, blocks, f.st, f.what);
+  const bool bf16 = !f.f32;
+  {
+    TpArgs g = new_args(f.M, f.H, f.status);
+    if (!rc) rc = set_operand(g.a[0], x, true, 128, bf16, f.what);
+    if (!rc) rc = set_operand(g.b[0], wg, false, 64, bf16, f.what);
+    if (!rc) rc = set_operand(g.b[1], wu, false, 64, bf16, f.what);
+    if (!rc) rc = set_hidden_out(g, h, 64, bf16, f.what);
+    g.kblocks[0] = blocks64(f.C);
+    if (!rc) rc = launch_hidden<TP_GATED>(f, g);
+  }
+  TpArgs g = new_args(f.M, f.C, f.status);
+  const int tn = tile_columns(f.M, f.C, 1);
+  if (!rc) rc = set_operand(g.a[0], h, true, 128, bf16, f.what);
+  if (!rc) rc = set_operand(g.b[0], wd, false, 64, bf16, f.what);
+  if (!rc) rc = set_user_out(g, y, f.f32, f.M, f.C, f.what);
+  g.kblocks[0] = blocks64(f.H);
+  if (!rc) rc = launch_plain(f.f32, tn, g, f.st, f.what);
+  return rc;
+}
+
+static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want_x, bool want_w, Carve &w) {
+  PrepArgs prep;
+  memset(&prep, 0, sizeof(prep));
+  int64_t blocks = 0;
+  const Matrix x = take_matrix(w, prep, blocks, f.f32, f.x, f.M, f.C);
+  const Matrix wg = take_matrix(w, prep, blocks, f.f32, f.wg, f.C, f.H);
+  const Matrix wu = take_matrix(w, prep, blocks, f.f32, f.wu, f.C, f.H);
+  const Matrix wd = take_matrix(w, prep, blocks, f.f32, f.wd, f.H, f.C);
+  const Matrix gy = take_matrix(w, prep, blocks, f.f32, f.gy, f.M, f.C);
+  const Matrix hidden = new_matrix(w, f.f32, f.M, f.H, 3);   // dg, du, h
+  const int64_t ld = up(f.H, 4);
+  const int tn = f.H > 128 ? 256 : 128;
+  const int splits = weight_splits(f.M, f.C, f.H, tn);
+  float *partial = want_w ? w.take<float>((int64_t)splits * 3 * f.C * ld) : nullptr;
+  if (!w.base) return CMACE_OK;
+  int rc = run_prep(prep, blocks, f.st, f.what);
+  const bool bf16 = !f.f32;
+  {
+    TpArgs g = new_args(f.M, f.H, f.status);
+    if (!rc) rc = set_operand(g.a[0], x, true, 128, bf16, f.what);
+    if (!rc) rc = set_operand(g.a[1], gy, true, 128, bf16, f.what);
+    if (!rc) rc = set_operand(g.b[0], wg, false, 64, bf16, f.what);
+    if (!rc) rc = set_operand(g.b[1], wu, false, 64, bf16, f.what);
+    if (!rc) rc = set_operand(g.b[2], wd, true, 64, bf16, f.what);
+    if (!rc) rc = set_hidden_out(g, hidden, 32, bf16, f.what);
+    g.segments = 2;
+    g.kblocks[0] = g.kblocks[1] = blocks64(f.C);
+    if (!rc) rc = launch_hidden<TP_BACK>(f, g);
+  }
+  const auto part = [&](int p) {   // one of the three hidden arrays as a matrix of its own
+    Matrix m = hidden;
+    m.batches = 1;
+    m.hi = static_cast<uint16_t *>(hidden.hi) + p * hidden.rows * hidden.ld;
+    if (hidden.lo) {
+      m.lo = static_cast<uint16_t *>(hidden.lo) + p * hidden.rows * hidden.ld;
+      m.scale = hidden.scale + p * hidden.blocks_m() * hidden.blocks_n();
+    }
+    return m;
+  };
+  if (want_x) {
+    TpArgs g = new_args(f.M, f.C, f.status);
+    const int tx = tile_columns(f.M, f.C, 1);
+    if (!rc) rc = set_operand(g.a[0], part(0), true, 128, bf16, f.what);
+    if (!rc) rc = set_operand(g.a[1], part(1), true, 128, bf16, f.what);
+    if (!rc) rc = set_operand(g.b[0], wg, true, tx, bf16, f.what);
+    if (!rc) rc = set_operand(g.b[1], wu, true, tx, bf16, f.what);
+    if (!rc) rc = set_user_out(g, gx, f.f32, f.M, f.C, f.what);
+    g.segments = 2;
+    g.kblocks[0] = g.kblocks[1] = blocks64(f.H);
+    if (!rc) rc = launch_plain(f.f32, tx, g, f.st, f.what);
+  }
+  if (want_w) {
+    // batches dg, du and h: x^T dg, x^T du and, as its transpose, dy^T h
+    TpArgs g = new_args(f.C, f.H, f.status);
+    if (!rc) rc = set_operand(g.a[0], x, false, 64, bf16, f.what);
+    if (!rc) rc = set_operand(g.a[1], gy, false, 64, bf16, f.what);
+    if (!rc) rc = set_operand(g.b[0], hidden, false, 64, bf16, f.what);
+    g.batches = 3;
+    g.splits = splits;
+    g.a_of_last = 1;
+    g.kblocks[0] = blocks64(f.M);
+    g.out[0].use_map = 1;
+    if (!rc) rc = encode_tile_map(&g.out[0].map, partial, 4, false, f.H, f.C, (int64_t)splits * 3, ld, (int64_t)f.C * ld, 32, 32, f.what);
+    if (!rc) rc = launch_plain(f.f32, tn, g, f.st, f.what);
+    WeightReduce r{partial, {gw[0], gw[1], gw[2]}, ld, splits, f.C, f.H};
+    const dim3 grid((unsigned)((f.H + 31) / 32), (unsigned)((f.C + 31) / 32), 3);
+    if (!rc) {
+      if (f.f32) launch_chained(weight_reduce_kernel<float>, grid, dim3(256), (size_t)0, f.st, r);
+      else launch_chained(weight_reduce_kernel<__nv_bfloat16>, grid, dim3(256), (size_t)0, f.st, r);
+      rc = check_launch(f.what);
+    }
+  }
+  return rc;
+}
+
+static int check_sizes(const char *what, int64_t M, int C, int H, int act) {
+  if (M < 0 || M >= (int64_t)1 << 31 || C < 1 || H < 1) return fail(CMACE_ERR_ARG, "%s: bad sizes: %lld rows, width %d, hidden width %d", what, (long long)M, C, H);
+  if (C > 1 << 20 || H > 1 << 20) return fail(CMACE_ERR_UNSUPPORTED, "%s: widths up to 2^20", what);
+  if (act != TP_SILU && act != TP_GELU) return fail(CMACE_ERR_ARG, "%s: unknown activation %d", what, act);
+  return CMACE_OK;
+}
+
+static int run_forward(bool f32, const void *x, const void *wg, const void *wu, const void *wd, int64_t M, int C, int H, int act, void *y,
+                       void *workspace, int64_t bytes, int32_t *status, cmace_stream_t stream, const char *what) {
+  if (int rc = check_sizes(what, M, C, H, act)) return rc;
+  if (M == 0) return CMACE_OK;
+  if (!x || !wg || !wu || !wd || !y || !workspace) return fail(CMACE_ERR_ARG, "%s: null pointer", what);
+  if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(CMACE_ERR_ARG, "%s: the workspace has to be aligned to 256 bytes", what);
+  FeedForward f{f32, x, wg, wu, wd, nullptr, M, C, H, act, status, (cudaStream_t)stream, what};
+  Carve count{nullptr};
+  forward(f, y, count);
+  if (bytes < count.used) return fail(CMACE_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes, (long long)count.used);
+  ChainScope chain;
+  chain_launches() = Chain::from_second;
+  Carve w{static_cast<char *>(workspace)};
+  return forward(f, y, w);
+}
+
+static int run_backward(bool f32, const void *x, const void *wg, const void *wu, const void *wd, const void *gy, int64_t M, int C, int H, int act,
+                        void *gx, void *gwg, void *gwu, void *gwd, void *workspace, int64_t bytes, int32_t *status, cmace_stream_t stream,
+                        const char *what) {
+  if (int rc = check_sizes(what, M, C, H, act)) return rc;
+  void *const gw[3] = {gwg, gwu, gwd};
+  const bool want_w = gwg || gwu || gwd;
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (M == 0) {   // a sum over no rows
+    for (void *p : gw)
+      if (p && cudaMemsetAsync(p, 0, (size_t)C * H * (f32 ? 4 : 2), st) != cudaSuccess) return check_launch(what);
+    return CMACE_OK;
+  }
+  if (!gx && !want_w) return CMACE_OK;
+  if (!x || !wg || !wu || !wd || !gy || !workspace) return fail(CMACE_ERR_ARG, "%s: null pointer", what);
+  if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(CMACE_ERR_ARG, "%s: the workspace has to be aligned to 256 bytes", what);
+  FeedForward f{f32, x, wg, wu, wd, gy, M, C, H, act, status, st, what};
+  Carve count{nullptr};
+  backward(f, gx, gw, gx != nullptr, want_w, count);
+  if (bytes < count.used) return fail(CMACE_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes, (long long)count.used);
+  ChainScope chain;
+  chain_launches() = Chain::from_second;
+  Carve w{static_cast<char *>(workspace)};
+  return backward(f, gx, gw, gx != nullptr, want_w, w);
+}
+
+}  // namespace cmace
+
+using namespace cmace;
+
+extern "C" {
+
+int64_t cmace_gated_ff_workspace_bytes(int is_f32, int64_t rows, int width, int hidden, int backward_pass) {
+  if (check_sizes("cmace_gated_ff_workspace_bytes", rows, width, hidden, TP_SILU)) return -1;
+  if (rows == 0) return 256;
+  // addresses are not known here: room for copies of all arrays of a width that is not a multiple of eight, and of those that are
+  FeedForward f{is_f32 != 0, (const void *)1, (const void *)1, (const void *)1, (const void *)1, (const void *)1, rows, width, hidden, TP_SILU, nullptr, nullptr, ""};
+  Carve count{nullptr};
+  void *const none[3] = {nullptr, nullptr, nullptr};
+  if (backward_pass) backward(f, nullptr, none, true, true, count);
+  else forward(f, nullptr, count);
+  return count.used;
+}
+
+int cmace_gated_ff_fwd_f32(const float *x, const float *w_gate, const float *w_up, const float *w_down, int64_t rows, int width, int hidden,
+                           int activation, float *y, void *workspace, int64_t workspace_bytes, int32_t *status, cmace_stream_t stream) {
+  return run_forward(true, x, w_gate, w_up, w_down, rows, width, hidden, activation, y, workspace, workspace_bytes, status, stream,
+                     "cmace_gated_ff_fwd_f32");
+}
+int cmace_gated_ff_fwd_bf16(const void *x, const void *w_gate, const void *w_up, const void *w_down, int64_t rows, int width, int hidden,
+                            int activation, void *y, void *workspace, int64_t workspace_bytes, int32_t *status, cmace_stream_t stream) {
+  return run_forward(false, x, w_gate, w_up, w_down, rows, width, hidden, activation, y, workspace, workspace_bytes, status, stream,
+                     "cmace_gated_ff_fwd_bf16");
+}
+int cmace_gated_ff_bwd_f32(const float *x, const float *w_gate, const float *w_up, const float *w_down, const float *grad_y, int64_t rows, int width,
+                           int hidden, int activation, float *grad_x, float *grad_gate, float *grad_up, float *grad_down, void *workspace,
+                           int64_t workspace_bytes, int32_t *status, cmace_stream_t stream) {
+  return run_backward(true, x, w_gate, w_up, w_down, grad_y, rows, width, hidden, activation, grad_x, grad_gate, grad_up, grad_down, workspace,
+                      workspace_bytes, status, stream, "cmace_gated_ff_bwd_f32");
+}
+int cmace_gated_ff_bwd_bf16(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *grad_y, int64_t rows, int width,
+                            int hidden, int activation, void *grad_x, void *grad_gate, void *grad_up, void *grad_down, void *workspace,
+                            int64_t workspace_bytes, int32_t *status, cmace_stream_t stream) {
+  return run_backward(false, x, w_gate, w_up, w_down, grad_y, rows, width, hidden, activation, grad_x, grad_gate, grad_up, grad_down, workspace,
+                      workspace_bytes, status, stream, "cmace_gated_ff_bwd_bf16");
+}
+
+}  // extern "C"

@@ -1252,6 +1252,13 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 static EncodeTiledFn encode_tiled_fn() {
   static EncodeTiledFn fn = nullptr;
+  // The encoder is a driver call and needs the context to be current, which it is not yet in a thread whose first CUDA call this is
+  // (autograd's, when a backward begins here).
+  static thread_local bool current = false;
+  if (!current) {
+    int device;
+    current = cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess;
+  }
   if (fn == nullptr) {
     void *p = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -1292,6 +1299,25 @@ int encode_half_rows_tensor_map(CUtensorMap *tmap, const void *base, int64_t row
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(CMACE_ERR_CUDA, "%s: cuTensorMapEncodeTiled (fp16 rows) failed (%d)", what, (int)r);
+  return CMACE_OK;
+}
+
+// [batches, rows, cols] of 16-bit or float32 values, rows ld elements apart, as boxes of box_cols x box_rows of one batch; the swizzle
+// spans a box's row of 64 or 128 bytes
+int encode_tile_map(CUtensorMap *map, const void *base, int bytes, bool bf16, int64_t cols, int64_t rows, int64_t batches, int64_t ld,
+                    int64_t batch_stride, int box_cols, int box_rows, const char *what) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (enc == nullptr) return fail(CMACE_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available", what);
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batches};
+  const cuuint64_t strides[2] = {(cuuint64_t)(ld * bytes), (cuuint64_t)(batch_stride * bytes)};
+  const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType type =
+      bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : (bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+  const CUresult r = enc(map, type, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         box_cols * bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(CMACE_ERR_CUDA, "%s: cuTensorMapEncodeTiled (tile) failed (%d)", what, (int)r);
   return CMACE_OK;
 }
 

@@ -1,0 +1,841 @@
+// Products of 16-bit operands on tcgen05 (kind::f16, float32 accumulator in tensor memory) with the epilogues that the dense
+// operators need: the gated feed-forward block (gated_feed_forward.cu) and the Newton-Schulz products (orthogonalize.cu).
+//
+//   D[i, j] = sum over segments, k of A_s[i, k] B_s[k, j]
+//
+// Operands are read where they lie, row-major with rows of a multiple of 16 bytes: the contracted index may be the inner one
+// (K-major) or the outer one (MN-major), so neither a weight nor an activation is ever transposed.  TMA brings tiles of 64 k
+// into a ring of stages (128-byte swizzle, zeros outside the array, which is all that ragged sizes need).
+//
+// Two precisions:
+//  * 16-bit operands (bf16, or fp16 where the caller knows the range): one MMA a k step, the sum stays in tensor memory for
+//    the whole of K.
+//  * PAIR: float32 values as two fp16 values, x = (hi + lo) / scale, hi and lo rounded to nearest: at most 2^-22 |x| off, about 2^-24
+//    on the average.  Three MMAs a k step (lo hi, hi lo, hi hi; lo lo is below 2^-22 of hi hi).  fp16 lacks float32's range, so
+//    every block of 64 x 64 values has a power of two of its own, from the block's largest value: within a block the precision
+//    holds over 2^18 below that value and degrades to an absolute 2^-39 of it beyond.  A block of 64 k is one chunk: its sum goes
+//    to its own accumulator columns and the epilogue warps add it, times the two blocks' scales, to float32 registers, rounding to
+//    nearest.  That also keeps the tensor core's own accumulation, which truncates, to 12 instructions: summed in tensor
+//    memory over K = 512, three terms of it are off by 4e-6 of the largest value; in chunks by 3e-7.
+//    Compared with TF32 in three terms the operands are half as large and the instructions twice as fast.
+//
+// One persistent CTA an SM, ten warps: eight for the epilogue (two a quarter of the 128 tensor-memory lanes, each half of
+// the columns), one thread that issues the copies, one that issues the MMAs.  Two sets of accumulator columns: the
+// products of the next chunk or tile run while the epilogue reads this one's.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstring>
+
+#include "common.cuh"
+#include "tc_ptx.cuh"
+
+namespace cmace {
+
+constexpr int TP_EPILOGUE_WARPS = 8;
+constexpr int TP_THREADS = (TP_EPILOGUE_WARPS + 2) * 32;   // 204 registers a thread: 128 sums of a PAIR tile and their handling
+constexpr int TP_STAGING = 4096;                           // bytes an epilogue warp stages its output in
+constexpr int TP_SMEM_BUDGET = 227 * 1024 - 1024;          // without the static barriers
+constexpr int TP_BUFFER_COLS = 256;                        // one set of accumulator columns
+constexpr int TP_MAX_STAGES = 8;
+
+// GATED: D = act(x Wg) * (x Wu).  BACK: what the block's backward needs of a hidden value: h, and the gradients of both
+// projections.  GRAM, POLY, APPLY: the three products of a Newton-Schulz step.
+enum TpKind { TP_PLAIN, TP_GATED, TP_BACK, TP_GRAM, TP_POLY, TP_APPLY };
+enum TpAct { TP_SILU = 0, TP_GELU = 1 };
+
+struct TpOperand {
+  CUtensorMap map[2];      // 16-bit values, or hi and lo
+  const float *scale;      // PAIR: inverse scales of the blocks (1 / scale), null where there are none
+  int64_t sc_i, sc_k, sc_b;  // their strides over blocks of the free index, of k, and over batches
+  int mn_major;            // the contracted index is the outer one
+  int batched;             // coordinates take the batch index
+};
+
+struct TpOut {
+  CUtensorMap map;         // boxes of 32 rows
+  void *ptr;               // rows that TMA cannot address (not a multiple of 16 bytes): stored by the warps
+  int64_t ld, batch;       // elements a row and a batch, for ptr
+  int use_map;
+};
+
+struct TpArgs {
+  TpOperand a[2], b[3];
+  TpOut out[4];
+  float *out_scale[3];           // PAIR outputs with block scales: inverse scale of every 64 x 64 block
+  int64_t out_scale_ld, out_scale_batch;
+  const void *cin[2];            // POLY: the Gram matrix (16-bit, or hi and lo); APPLY: X in float32
+  int64_t cin_ld, cin_batch;
+  float alpha, beta, cin_scale, pair_scale;   // D = alpha * product + beta * cin / ..., see the epilogues
+  int32_t *status;
+  int64_t rows, cols;            // of the output
+  int kblocks[2], segments;      // blocks of 64 k a segment
+  int batches, splits, mt, nt;
+  int64_t total;                 // tiles
+  int stages;
+  int a_of_last;                 // the last batch takes a[1] (its own, unbatched operand) in place of a[0]
+  int out_bf16;                  // PLAIN, APPLY's result: 16-bit output
+  int in_f16;                    // 16-bit operands are fp16, not bf16
+};
+
+__device__ __forceinline__ void umma_16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Operand image of rows of 128 bytes with the 128-byte swizzle.  K-major: a row is 64 k of one i, groups of eight rows 1 024 bytes
+// apart.  MN-major: a row is 64 i of one k, groups of eight k 1 024 bytes apart (stride offset), runs of 64 i 8 192 (leading offset).
+__device__ __forceinline__ uint64_t tp_desc(uint32_t smem, int mn_major) {
+  return (uint64_t)((smem & 0x3FFFF) >> 4) | ((uint64_t)(mn_major ? 512 : 1) << 16) | ((uint64_t)64 << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)2 << 61);
+}
+// kind::f16: D float32, A and B fp16 (0) or bf16 (1) at bits 7 and 10, MN-major operands at bits 15 and 16
+__device__ __forceinline__ uint32_t tp_idesc(int n, int bf16, int a_mn, int b_mn) {
+  return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+template <int KIND, bool PAIR, int TN>
+struct TpShape {
+  static constexpr int B_ROWS = KIND == TP_BACK ? 128 : (KIND == TP_GATED ? 256 : TN);   // rows of B in a stage
+  static constexpr int OUT_N = KIND == TP_BACK ? 64 : (KIND == TP_GATED ? 128 : TN);     // output columns of a tile
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128;
+  static constexpr int STAGE = (A_BYTES + B_BYTES) * (PAIR ? 2 : 1);
+  static constexpr int STAGES =
+      (TP_SMEM_BUDGET - 1024 - TP_EPILOGUE_WARPS * TP_STAGING) / STAGE < TP_MAX_STAGES
+          ? (TP_SMEM_BUDGET - 1024 - TP_EPILOGUE_WARPS * TP_STAGING) / STAGE : TP_MAX_STAGES;
+  static constexpr int SMEM = STAGE * STAGES + TP_EPILOGUE_WARPS * TP_STAGING + 1024;
+};
+
+struct TpTile {
+  int64_t row0;
+  int n0, batch, split;
+};
+__device__ __forceinline__ TpTile tp_tile(const TpArgs &g, int64_t t, int out_n) {
+  TpTile T;
+  const uint32_t u = (uint32_t)t, nt = (uint32_t)g.nt, mt = (uint32_t)g.mt;
+  const uint32_t v = u / nt;
+  T.n0 = (int)(u - v * nt) * out_n;
+  const uint32_t w = v / mt;
+  T.row0 = (int64_t)(v - w * mt) * 128;
+  T.split = (int)(w / (uint32_t)g.batches);
+  T.batch = (int)(w - (uint32_t)T.split * (uint32_t)g.batches);
+  return T;
+}
+// k blocks of a split
+__device__ __forceinline__ void tp_range(const TpArgs &g, int split, int seg, int &k0, int &k1) {
+  const int n = g.kblocks[seg];
+  k0 = (int)((int64_t)n * split / g.splits);
+  k1 = (int)((int64_t)n * (split + 1) / g.splits);
+}
+
+__device__ __forceinline__ void tp_report(const TpArgs &g, int code) {
+  if (g.status) atomicCAS(g.status, 0, code);
+}
+// named barrier of a part of the epilogue warps
+__device__ __forceinline__ void tp_bar(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+// power of two that brings `most` (finite, >= 0) into [2^14, 2^15)
+__device__ __forceinline__ float tp_scale(float most) {
+  int k = 14 - (int)((__float_as_uint(most) >> 23) - 127);   // a subnormal counts as 2^-127
+  if (most == 0.f) k = 0;
+  k = k > 126 ? 126 : k;
+  return __uint_as_float((uint32_t)(k + 127) << 23);
+}
+__device__ __forceinline__ float tp_finite_abs(float x) {
+  const float a = fabsf(x);
+  return a < CUDART_INF_F ? a : 0.f;   // infinities and NaN do not set a block's scale
+}
+// two values as (hi, lo) pairs of fp16; what is not finite goes to hi alone
+__device__ __forceinline__ void tp_split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  float dx = x - f.x, dy = y - f.y;
+  dx = fabsf(f.x) < CUDART_INF_F ? dx : 0.f;
+  dy = fabsf(f.y) < CUDART_INF_F ? dy : 0.f;
+  const __half2 l = __floats2half2_rn(dx, dy);
+  hi = *reinterpret_cast<const uint32_t *>(&h);
+  lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+__device__ __forceinline__ uint32_t tp_bf16x2(float x, float y) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t tp_f16x2(float x, float y) {
+  const __half2 v = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// act(g); with the derivative
+template <int ACT>
+__device__ __forceinline__ float tp_act(float g) {
+  if (ACT == TP_SILU) return g * sigmoid_fast(g);
+  return g * (0.5f * (1.0f + erff(g * 0.70710678118654752f)));
+}
+template <int ACT>
+__device__ __forceinline__ float tp_act(float g, float &d) {
+  if (ACT == TP_SILU) {
+    const float s = sigmoid_fast(g);
+    const float a = g * s;
+    d = s * (1.0f + (g - a));
+    return a;
+  }
+  const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+  d = cdf + g * (0.39894228040143268f * exp2f(-0.72134752044448170f * g * g));
+  return g * cdf;
+}
+
+// ---- an epilogue warp's stores ------------------------------------------------------------------------------------------
+struct TpStager {
+  uint32_t smem;
+  int lane;
+  int64_t rows, cols;   // of the output: a box that starts outside is not stored
+  __device__ __forceinline__ void begin() const {   // the copy engine has read what was staged before
+    if (elect_one()) tma_store_wait_read();
+    __syncwarp();
+  }
+  // COLS 32-bit words of this lane's row at `at` (bytes into the staging buffer): rows of 128 bytes (32 words) or 64 (16)
+  template <int WORDS>
+  __device__ __forceinline__ void put(uint32_t at, const uint32_t (&w)[WORDS]) const {
+#pragma unroll
+    for (int c = 0; c < WORDS / 4; c++)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                       smem + at + (uint32_t)(WORDS == 32 ? sw128_offset(lane, c) : sw64_offset(lane, c))),
+                   "r"(w[4 * c]), "r"(w[4 * c + 1]), "r"(w[4 * c + 2]), "r"(w[4 * c + 3])
+                   : "memory");
+  }
+  __device__ __forceinline__ void send(const CUtensorMap *map, uint32_t at, int col, int64_t row, int batch) const {
+    fence_proxy_async();
+    __syncwarp();
+    if (row < rows && col < cols && elect_one()) tma_store_3d(map, col, (int)row, batch, smem + at);
+  }
+  __device__ __forceinline__ uint32_t word(int row, int w) const {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(smem + (uint32_t)sw128_offset(row, w >> 2) + 4u * (uint32_t)(w & 3)) : "memory");
+    return v;
+  }
+  // rows that TMA cannot address: 32 float32 columns (one a lane) or 64 16-bit ones (two a lane)
+  __device__ __forceinline__ void send_rows(const TpOut &o, bool sixteen, int col, int64_t row, int batch) const {
+    __syncwarp();
+    const int64_t base = (int64_t)batch * o.batch;
+    const int n = rows - row < 32 ? (int)(rows - row) : 32;
+    for (int r = 0; r < n; r++) {
+      const uint32_t v = word(r, lane);
+      const int64_t at = base + (row + r) * o.ld + col;
+      if (!sixteen) {
+        if (col + lane < cols) static_cast<uint32_t *>(o.ptr)[at + lane] = v;
+      } else {
+        uint16_t *p = static_cast<uint16_t *>(o.ptr) + at + 2 * lane;
+        if (col + 2 * lane < cols) p[0] = (uint16_t)v;
+        if (col + 2 * lane + 1 < cols) p[1] = (uint16_t)(v >> 16);
+      }
+    }
+    __syncwarp();
+  }
+};
+
+template <int KIND, bool PAIR, int TN, int ACT>
+__global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __grid_constant__ TpArgs g) {
+  using S = TpShape<KIND, PAIR, TN>;
+  constexpr int TERMS = PAIR ? 2 : 1;
+  constexpr int STAGES = S::STAGES;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 5];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ float block_most[3][TP_EPILOGUE_WARPS];   // GATED: of alternating tiles; BACK: of the three outputs
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t staging = smem + (uint32_t)(STAGES * S::STAGE);
+  const uint32_t full = smem_u32(&bars[0]), empty = smem_u32(&bars[TP_MAX_STAGES]);
+  const uint32_t acc_full = smem_u32(&bars[2 * TP_MAX_STAGES]), acc_empty = smem_u32(&bars[2 * TP_MAX_STAGES + 2]);
+  const uint32_t drain = smem_u32(&bars[2 * TP_MAX_STAGES + 4]);
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; s++) {
+      mbar_init(full + 8 * s, 1);    // the copies' expect_tx
+      mbar_init(empty + 8 * s, 1);   // one commit
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(acc_full + 8 * b, 1);                    // one commit
+      mbar_init(acc_empty + 8 * b, TP_EPILOGUE_WARPS);   // one arrival a warp
+    }
+    mbar_init(drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == TP_EPILOGUE_WARPS) tmem_alloc(smem_u32(&tmem_base_slot), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = (uint32_t)uniform((int)tmem_base_slot);
+  grid_wait();
+  grid_release();   // after the allocation
+
+  if (warp == TP_EPILOGUE_WARPS) {
+    // ================================ copies ================================
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0, used = 0;   // used: bit per stage that has been filled at least once
+      bool ok = true;
+      for (int64_t t = blockIdx.x; ok && t < g.total; t += gridDim.x) {
+        const TpTile T = tp_tile(g, t, S::OUT_N);
+        for (int seg = 0; ok && seg < g.segments; seg++) {
+          const bool last = g.a_of_last && T.batch == g.batches - 1;
+          const TpOperand &A = g.a[last ? 1 : seg];
+          const int a_batch = A.batched ? T.batch : 0;
+          int k0, k1;
+          tp_range(g, T.split, seg, k0, k1);
+          constexpr int PARTS0 = KIND == TP_GATED || KIND == TP_BACK ? 2 : 1;
+          const int parts = KIND == TP_BACK && seg == 1 ? 1 : PARTS0;
+          const int first = KIND == TP_BACK ? 2 * seg : (KIND == TP_GATED ? 0 : seg);
+          constexpr int PART_ROWS = KIND == TP_BACK ? 64 : (KIND == TP_GATED ? 128 : TN);
+          const uint32_t bytes = (uint32_t)(TERMS * (S::A_BYTES + parts * PART_ROWS * 128));
+          for (int kb = k0; kb < k1; kb++) {
+            if (!mbar_wait(empty + 8 * stage, phase ^ 1)) {
+              tp_report(g, 40);
+              ok = false;
+              break;
+            }
+            const uint32_t bar = full + 8 * stage, sA = smem + (uint32_t)(stage * S::STAGE);
+            const uint32_t sB = sA + TERMS * S::A_BYTES;
+            mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+            for (int term = 0; term < TERMS; term++) {
+              const uint32_t dA = sA + term * S::A_BYTES;
+              if (A.mn_major) {
+                tma_load_3d(dA, &A.map[term], (int)T.row0, kb * 64, a_batch, bar);
+                tma_load_3d(dA + 8192, &A.map[term], (int)T.row0 + 64, kb * 64, a_batch, bar);
+              } else {
+                tma_load_3d(dA, &A.map[term], kb * 64, (int)T.row0, a_batch, bar);
+              }
+              for (int p = 0; p < parts; p++) {
+                const TpOperand &B = g.b[first + p];
+                const int b_batch = B.batched ? T.batch : 0;
+                const uint32_t dB = sB + term * S::B_BYTES + (uint32_t)(p * PART_ROWS * 128);
+                if (B.mn_major) {
+#pragma unroll
+                  for (int i = 0; i < PART_ROWS / 64; i++)
+                    tma_load_3d(dB + 8192u * i, &B.map[term], T.n0 + 64 * i, kb * 64, b_batch, bar);
+                } else {
+                  tma_load_3d(dB, &B.map[term], kb * 64, T.n0, b_batch, bar);
+                }
+              }
+            }
+            used |= 1u << stage;
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+        }
+      }
+      if (!ok) {   // no copy outlives the block: the fills that nobody took
+        for (int s = 0; s < STAGES; s++)
+          if (used >> s & 1) mbar_wait(full + 8 * s, s < stage ? phase : phase ^ 1);
+      }
+    }
+  } else if (warp == TP_EPILOGUE_WARPS + 1) {
+    // ================================ products ================================
+    if (elect_one()) {
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, buf_phase[2] = {0, 0};
+      bool ok = true;
+      const int bf16 = g.in_f16 || PAIR ? 0 : 1;
+      for (int64_t t = blockIdx.x; ok && t < g.total; t += gridDim.x) {
+        const TpTile T = tp_tile(g, t, S::OUT_N);
+        if (!PAIR) {
+          if (!mbar_wait(acc_empty + 8 * buf, buf_phase[buf] ^ 1)) {
+            tp_report(g, 41);
+            break;
+          }
+          tc_fence_after();
+        }
+        uint32_t begun = 0;
+        for (int seg = 0; ok && seg < g.segments; seg++) {
+          int k0, k1;
+          tp_range(g, T.split, seg, k0, k1);
+          const bool last = g.a_of_last && T.batch == g.batches - 1;
+          const int a_mn = g.a[last ? 1 : seg].mn_major;
+          const int b_mn = g.b[KIND == TP_BACK ? 2 * seg : (KIND == TP_GATED ? 0 : seg)].mn_major;
+          const int n = KIND == TP_BACK ? (seg == 0 ? 128 : 64) : S::B_ROWS;
+          const uint32_t idesc = tp_idesc(n, bf16, a_mn, b_mn);
+          const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;   // 16 k, in units of 16 bytes
+          if (KIND == TP_BACK && seg == 1) begun = 0;
+          for (int kb = k0; kb < k1; kb++) {
+            if (PAIR) {
+              if (!mbar_wait(acc_empty + 8 * buf, buf_phase[buf] ^ 1)) {
+                tp_report(g, 42);
+                ok = false;
+                break;
+              }
+              begun = 0;
+            }
+            if (!mbar_wait(full + 8 * stage, phase)) {
+              tp_report(g, 43);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t d = tmem + (uint32_t)(buf * TP_BUFFER_COLS) + (KIND == TP_BACK && !PAIR && seg == 1 ? 128u : 0u);
+            const uint32_t sA = smem + (uint32_t)(stage * S::STAGE), sB = sA + TERMS * S::A_BYTES;
+            const uint64_t a_hi = tp_desc(sA, a_mn), b_hi = tp_desc(sB, b_mn);
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++) {
+              if (PAIR) {
+                const uint64_t a_lo = tp_desc(sA + S::A_BYTES, a_mn), b_lo = tp_desc(sB + S::B_BYTES, b_mn);
+                umma_16(d, a_lo + ks * a_step, b_hi + ks * b_step, idesc, begun);
+                umma_16(d, a_hi + ks * a_step, b_lo + ks * b_step, idesc, 1);
+                umma_16(d, a_hi + ks * a_step, b_hi + ks * b_step, idesc, 1);
+              } else {
+                umma_16(d, a_hi + ks * a_step, b_hi + ks * b_step, idesc, begun);
+              }
+              begun = 1;
+            }
+            umma_commit(empty + 8 * stage);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+            if (PAIR) {
+              umma_commit(acc_full + 8 * buf);
+              buf_phase[buf] ^= 1;
+              buf ^= 1;
+            }
+          }
+        }
+        if (!PAIR && ok) {
+          umma_commit(acc_full + 8 * buf);
+          buf_phase[buf] ^= 1;
+          buf ^= 1;
+        }
+      }
+      umma_commit(drain);   // nothing of this block's products is in flight when the columns are given back
+      if (!mbar_wait(drain, 0)) tp_report(g, 44);
+    }
+  } else {
+    // ================================ epilogue ================================
+    const int q = warp & 3, half = warp >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+    const TpStager st{staging + (uint32_t)(warp * TP_STAGING), lane, g.rows, g.cols};
+    int buf = 0;
+    uint32_t buf_phase[2] = {0, 0};
+    bool ok = true;
+    // groups of 32 columns of the sum that this warp owns
+    constexpr int GROUPS = KIND == TP_BACK ? 3 : (KIND == TP_GATED ? 4 : TN / 64);
+    constexpr int SEG0_GROUPS = KIND == TP_BACK ? 2 : GROUPS;
+    // first column of group i inside the accumulator (BACK: the third group has an accumulator, or columns, of its own)
+    const auto column = [&](int i) -> uint32_t {
+      if (KIND == TP_GATED) return (uint32_t)((i >> 1) * 128 + 64 * half + 32 * (i & 1));
+      if (KIND == TP_BACK) return (uint32_t)(i < 2 ? 64 * i + 32 * half : (PAIR ? 32 * half : 128 + 32 * half));
+      return (uint32_t)(half * (TN / 2) + 32 * i);
+    };
+    // A warp whose wait gave up goes through the rest of its tiles without waiting: others meet it at the named barriers.
+    int odd = 0;
+    for (int64_t t = blockIdx.x; t < g.total; t += gridDim.x, odd ^= 1) {
+      const TpTile T = tp_tile(g, t, S::OUT_N);
+      const int64_t row = T.row0 + 32 * q;   // first row of this warp
+      float acc[PAIR ? GROUPS : 1][32];
+      if (PAIR) {
+#pragma unroll
+        for (int i = 0; i < (PAIR ? GROUPS : 1); i++)
+#pragma unroll
+          for (int j = 0; j < 32; j++) acc[i][j] = 0.f;
+#pragma unroll
+        for (int seg = 0; seg < 2; seg++) {
+          if (seg >= g.segments) break;
+          const int i0 = KIND == TP_BACK && seg == 1 ? SEG0_GROUPS : 0;
+          const int i1 = KIND == TP_BACK && seg == 0 ? SEG0_GROUPS : GROUPS;
+          int k0, k1;
+          tp_range(g, T.split, seg, k0, k1);
+          const bool last = g.a_of_last && T.batch == g.batches - 1;
+          const TpOperand &A = g.a[last ? 1 : seg];
+          const TpOperand &B0 = g.b[KIND == TP_BACK ? 2 * seg : (KIND == TP_GATED ? 0 : seg)];
+          const TpOperand &B1 = g.b[KIND == TP_GATED || (KIND == TP_BACK && seg == 0) ? 1 : (KIND == TP_BACK ? 2 : seg)];
+          // scales: one block of rows a warp; two blocks of columns at most: of both projections (GATED, BACK), or side by side
+          const int cb = T.n0 / 64 + (KIND == TP_GATED ? half : (KIND == TP_BACK ? 0 : half * (TN / 128)));
+          const float *pa = A.scale ? A.scale + (A.batched ? T.batch * A.sc_b : 0) + (row >> 6) * A.sc_i : nullptr;
+          const float *pb0 = B0.scale ? B0.scale + (B0.batched ? T.batch * B0.sc_b : 0) + cb * B0.sc_i : nullptr;
+          const bool two = KIND == TP_GATED || (KIND == TP_BACK && seg == 0) || TN == 256;
+          const float *pb1 = !two ? pb0 : (KIND == TP_GATED || KIND == TP_BACK
+                                 ? (B1.scale ? B1.scale + (B1.batched ? T.batch * B1.sc_b : 0) + cb * B1.sc_i : nullptr)
+                                 : (pb0 && (cb + 1) * 64 < g.cols ? pb0 + B0.sc_i : pb0));   // past the last block: zeros in any scale
+          const bool a_rows = row < g.rows;   // a warp of rows past the end has zeros and no scale
+          const bool b_cols = (int64_t)cb * 64 < g.cols;
+          float na = 1.f, nb0 = 1.f, nb1 = 1.f;
+          const auto fetch = [&](int kb) {
+            if (pa && a_rows) na = __ldcg(pa + kb * A.sc_k);
+            if (pb0 && b_cols) nb0 = __ldcg(pb0 + kb * B0.sc_k);
+            if (pb1 && b_cols) nb1 = __ldcg(pb1 + kb * B1.sc_k);
+          };
+          fetch(k0);
+          for (int kb = k0; kb < k1; kb++) {
+            const float s0 = na * nb0, s1 = na * nb1;
+            if (kb + 1 < k1) fetch(kb + 1);
+            if (ok && !warp_wait(acc_full + 8 * buf, buf_phase[buf], lane)) {
+              if (lane == 0) tp_report(g, 45);
+              ok = false;
+            }
+            tc_fence_after();
+            const uint32_t at = lanes + (uint32_t)(buf * TP_BUFFER_COLS);
+#pragma unroll
+            for (int i = 0; i < (PAIR ? GROUPS : 1); i++) {
+              if (i < i0 || i >= i1) continue;
+              uint32_t v[32];
+              tmem_ld32(at + column(i), v);
+              const float s = (KIND == TP_GATED ? i >= 2 : (KIND == TP_BACK ? i == 1 : i >= 2)) ? s1 : s0;
+#pragma unroll
+              for (int j = 0; j < 32; j++) acc[i][j] = fmaf(__uint_as_float(v[j]), s, acc[i][j]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(acc_empty + 8 * buf);
+            buf_phase[buf] ^= 1;
+            buf ^= 1;
+          }
+        }
+      } else {
+        if (ok && !warp_wait(acc_full + 8 * buf, buf_phase[buf], lane)) {
+          if (lane == 0) tp_report(g, 46);
+          ok = false;
+        }
+        tc_fence_after();
+      }
+      const uint32_t at = lanes + (uint32_t)(buf * TP_BUFFER_COLS);
+      // group i of the finished sums
+      const auto take = [&](int i, float (&v)[32]) {
+        if (PAIR) {
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[j] = acc[PAIR ? i : 0][j];
+        } else {
+          uint32_t u[32];
+          tmem_ld32(at + column(i), u);
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[j] = __uint_as_float(u[j]);
+        }
+      };
+
+      if constexpr (KIND == TP_GATED) {
+        const int col = T.n0 + 64 * half;
+        if constexpr (PAIR) {
+          float most = 0.f;
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              acc[i][j] = tp_act<ACT>(acc[i][j]) * acc[PAIR ? 2 + i : 0][j];
+              most = fmaxf(most, tp_finite_abs(acc[i][j]));
+            }
+          // the block of 64 rows is this warp's and the next (or previous) quarter's of the same columns
+          most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+          if (lane == 0) block_most[odd][warp] = most;
+          tp_bar(1 + 2 * half + (q >> 1), 64);
+          const float scale = tp_scale(fmaxf(most, block_most[odd][warp ^ 1]));
+          if (lane == 0 && (q & 1) == 0 && row < g.rows && col < g.cols)
+            g.out_scale[0][(row >> 6) * g.out_scale_ld + (col >> 6)] = 1.0f / scale;
+          uint32_t w[32], lo[32];
+#pragma unroll
+          for (int j = 0; j < 32; j++)
+            tp_split2(acc[j >> 4][2 * (j & 15)] * scale, acc[j >> 4][2 * (j & 15) + 1] * scale, w[j], lo[j]);
+          st.begin();
+          st.put(0, w);
+          st.send(&g.out[0].map, 0, col, row, 0);
+          st.begin();
+          st.put(0, lo);
+          st.send(&g.out[1].map, 0, col, row, 0);
+        } else {
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            float a[32], u[32];
+            take(i, a);
+            take(2 + i, u);
+#pragma unroll
+            for (int j = 0; j < 16; j++) w[16 * i + j] = tp_bf16x2(tp_act<ACT>(a[2 * j]) * u[2 * j], tp_act<ACT>(a[2 * j + 1]) * u[2 * j + 1]);
+          }
+          st.begin();
+          st.put(0, w);
+          st.send(&g.out[0].map, 0, col, row, 0);
+        }
+      } else if constexpr (KIND == TP_BACK) {
+        // h = act(g) u, dL/dg = dL/dh u act'(g), dL/du = dL/dh act(g)
+        const int col = T.n0 + 32 * half;
+        float a[32], u[32], dh[32];
+        take(0, a);
+        take(1, u);
+        take(2, dh);
+        float most[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+          float d;
+          const float act = tp_act<ACT>(a[j], d);
+          const float h = act * u[j], dg = dh[j] * (u[j] * d), du = dh[j] * act;
+          a[j] = h;
+          u[j] = dg;
+          dh[j] = du;
+          if (PAIR) {
+            most[0] = fmaxf(most[0], tp_finite_abs(dg));
+            most[1] = fmaxf(most[1], tp_finite_abs(du));
+            most[2] = fmaxf(most[2], tp_finite_abs(h));
+          }
+        }
+        float scale[3] = {1.f, 1.f, 1.f};
+        if (PAIR) {
+#pragma unroll
+          for (int p = 0; p < 3; p++) {
+            most[p] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most[p])));
+            if (lane == 0) block_most[p][warp] = most[p];
+          }
+          tp_bar(1 + (q >> 1), 128);   // 64 rows x 64 columns: two quarters, both halves
+#pragma unroll
+          for (int p = 0; p < 3; p++) {
+            const float m = fmaxf(fmaxf(block_most[p][warp], block_most[p][warp ^ 1]), fmaxf(block_most[p][warp ^ 4], block_most[p][warp ^ 5]));
+            scale[p] = tp_scale(m);
+            if (lane == 0 && (q & 1) == 0 && half == 0 && row < g.rows && T.n0 < g.cols)
+              g.out_scale[p][(row >> 6) * g.out_scale_ld + (T.n0 >> 6)] = 1.0f / scale[p];
+          }
+          tp_bar(1 + (q >> 1), 128);   // read by all before the next tile's are written
+        }
+#pragma unroll
+        for (int p = 0; p < 3; p++) {
+          uint32_t w[16], lo[16];
+#pragma unroll
+          for (int j = 0; j < 16; j++) {
+            const float x = p == 0 ? u[2 * j] : (p == 1 ? dh[2 * j] : a[2 * j]);
+            const float y = p == 0 ? u[2 * j + 1] : (p == 1 ? dh[2 * j + 1] : a[2 * j + 1]);
+            if (PAIR) tp_split2(x * scale[p], y * scale[p], w[j], lo[j]);
+            else w[j] = tp_bf16x2(x, y);
+          }
+          if (PAIR || p != 1) st.begin();
+          const uint32_t where = PAIR ? 0u : (p == 1 ? 2048u : 0u);
+          st.put(where, w);
+          if (PAIR) st.put(2048, lo);
+          st.send(&g.out[0].map, where, col, row, p);
+          if (PAIR) st.send(&g.out[1].map, 2048, col, row, p);
+        }
+      } else if constexpr (KIND == TP_PLAIN) {
+        const int col0 = T.n0 + half * (TN / 2);
+        const int batch = T.split * g.batches + T.batch;
+        if (g.out_bf16) {
+#pragma unroll
+          for (int i = 0; i < GROUPS; i += 2) {
+            if (col0 + 32 * i >= g.cols) break;
+            uint32_t w[32];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              float v[32];
+              take(i + k, v);
+#pragma unroll
+              for (int j = 0; j < 16; j++) w[16 * k + j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
+            }
+            st.begin();
+            st.put(0, w);
+            if (g.out[0].use_map) st.send(&g.out[0].map, 0, col0 + 32 * i, row, batch);
+            else st.send_rows(g.out[0], true, col0 + 32 * i, row, batch);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < GROUPS; i++) {
+            if (col0 + 32 * i >= g.cols) break;
+            float v[32];
+            take(i, v);
+            uint32_t w[32];
+#pragma unroll
+            for (int j = 0; j < 32; j++) w[j] = __float_as_uint(v[j]);
+            st.begin();
+            st.put(0, w);
+            if (g.out[0].use_map) st.send(&g.out[0].map, 0, col0 + 32 * i, row, batch);
+            else st.send_rows(g.out[0], false, col0 + 32 * i, row, batch);
+          }
+        }
+      } else {
+        // Newton-Schulz: values in float32, then hi and lo (or one fp16) at a power of two that the caller has from its bounds
+        const int col0 = T.n0 + half * (TN / 2);
+        const bool in_rows = row + lane < g.rows;
+#pragma unroll
+        for (int i = 0; i < GROUPS; i++) {
+          const int col = col0 + 32 * i;
+          if (col >= g.cols) break;
+          float v[32];
+          take(i, v);
+          if constexpr (KIND == TP_GRAM) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] *= g.alpha;
+          } else if constexpr (KIND == TP_POLY) {
+            // alpha * (S S) + beta * S; rows of S have a multiple of 64 elements, so a group never runs over one's end
+            const int64_t at16 = (int64_t)T.batch * g.cin_batch + (row + lane) * g.cin_ld + col;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+              uint4 h = make_uint4(0, 0, 0, 0), l = h;
+              if (in_rows) {
+                h = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(g.cin[0]) + at16) + c);
+                if (PAIR) l = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(g.cin[1]) + at16) + c);
+              }
+              const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+              for (int k = 0; k < 4; k++) {
+                float2 s = __half22float2(*reinterpret_cast<const __half2 *>(&hw[k]));
+                if (PAIR) {
+                  const float2 e = __half22float2(*reinterpret_cast<const __half2 *>(&lw[k]));
+                  s.x += e.x;
+                  s.y += e.y;
+                }
+                v[8 * c + 2 * k] = g.alpha * v[8 * c + 2 * k] + g.beta * s.x;
+                v[8 * c + 2 * k + 1] = g.alpha * v[8 * c + 2 * k + 1] + g.beta * s.y;
+              }
+            }
+          } else {
+            const float *x = static_cast<const float *>(g.cin[0]) + (int64_t)T.batch * g.cin_batch + (row + lane) * g.cin_ld + col;
+#pragma unroll
+            for (int c = 0; c < 8; c++) {
+              float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (in_rows) s = __ldcg(reinterpret_cast<const float4 *>(x) + c);
+              v[4 * c] = g.alpha * v[4 * c] + g.beta * s.x;
+              v[4 * c + 1] = g.alpha * v[4 * c + 1] + g.beta * s.y;
+              v[4 * c + 2] = g.alpha * v[4 * c + 2] + g.beta * s.z;
+              v[4 * c + 3] = g.alpha * v[4 * c + 3] + g.beta * s.w;
+            }
+          }
+          if (KIND == TP_APPLY) {
+            // out[2]: float32, the X of the next step or the result
+            uint32_t w[32];
+#pragma unroll
+            for (int j = 0; j < 32; j++) w[j] = __float_as_uint(v[j]);
+            if (!g.out_bf16) {
+              st.begin();
+              st.put(0, w);
+              if (g.out[2].use_map) st.send(&g.out[2].map, 0, col, row, T.batch);
+              else st.send_rows(g.out[2], false, col, row, T.batch);
+            } else {
+              if (g.out[2].use_map) {
+                uint32_t w16[16];
+#pragma unroll
+                for (int j = 0; j < 16; j++) w16[j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
+                st.begin();
+                st.put(0, w16);
+                st.send(&g.out[2].map, 0, col, row, T.batch);
+              } else {
+                __nv_bfloat16 *o =
+                    static_cast<__nv_bfloat16 *>(g.out[2].ptr) + (int64_t)T.batch * g.out[2].batch + (row + lane) * g.out[2].ld + col;
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                  if (in_rows && col + j < g.cols) o[j] = __float2bfloat16_rn(v[j]);
+              }
+            }
+          }
+          if (KIND != TP_APPLY || g.pair_scale != 0.f) {
+            uint32_t w[16], lo[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+              if (PAIR) tp_split2(v[2 * j] * g.pair_scale, v[2 * j + 1] * g.pair_scale, w[j], lo[j]);
+              else w[j] = tp_f16x2(v[2 * j] * g.pair_scale, v[2 * j + 1] * g.pair_scale);
+            }
+            st.begin();
+            st.put(0, w);
+            if (PAIR) st.put(2048, lo);
+            st.send(&g.out[0].map, 0, col, row, T.batch);
+            if (PAIR) st.send(&g.out[1].map, 2048, col, row, T.batch);
+          }
+        }
+      }
+      if (!PAIR) {
+        tc_fence_before();
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(acc_empty + 8 * buf);
+        buf_phase[buf] ^= 1;
+        buf ^= 1;
+      }
+    }
+    if (elect_one()) tma_store_wait_all();   // the copy engine reads this warp's staging buffer
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == TP_EPILOGUE_WARPS) tmem_dealloc(tmem, 512);
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+// [batch][rows][cols] of 16-bit or float32 values, rows ld elements apart, as boxes of box_cols x box_rows (gemm_tc.cu)
+int encode_tile_map(CUtensorMap *map, const void *base, int bytes, bool bf16, int64_t cols, int64_t rows, int64_t batches, int64_t ld,
+                    int64_t batch_stride, int box_cols, int box_rows, const char *what);
+
+// ---- layout of a call's workspace -------------------------------------------------------------------------------------------
+inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+struct Carve {   // consecutive pieces of the workspace; without a base it only counts
+  char *base;
+  int64_t used = 0;
+  template <typename T>
+  T *take(int64_t n) {
+    char *p = base ? base + used : nullptr;
+    used += up(n * (int64_t)sizeof(T), 256);
+    return reinterpret_cast<T *>(p);
+  }
+};
+
+// a matrix [batches][rows][cols] as an operand of the products
+struct Matrix {
+  void *hi = nullptr, *lo = nullptr;
+  float *scale = nullptr;
+  int64_t rows = 0, ld = 0, batches = 1;
+  int cols = 0;
+  int64_t blocks_m() const { return (rows + 63) / 64; }
+  int64_t blocks_n() const { return (cols + 63) / 64; }
+};
+
+// values apart by rows of a multiple of `align` elements; PAIR values with or without scales of their blocks
+inline Matrix new_matrix(Carve &w, bool pair, int64_t rows, int cols, int64_t batches, int align = 8, bool scales = true) {
+  Matrix m;
+  m.rows = rows, m.cols = cols, m.batches = batches, m.ld = up(cols, align);
+  m.hi = w.take<uint16_t>(batches * rows * m.ld);
+  if (pair) {
+    m.lo = w.take<uint16_t>(batches * rows * m.ld);
+    if (scales) m.scale = w.take<float>(batches * m.blocks_m() * m.blocks_n());
+  }
+  return m;
+}
+
+// m as an operand: k_inner: the contracted index runs along a row; box_rows: rows (of the free index) a copy takes then
+inline int set_operand(TpOperand &o, const Matrix &m, bool k_inner, int box_rows, bool bf16, const char *what) {
+  o.mn_major = !k_inner;
+  o.batched = m.batches > 1;
+  o.scale = m.scale;
+  o.sc_i = k_inner ? m.blocks_n() : 1;
+  o.sc_k = k_inner ? 1 : m.blocks_n();
+  o.sc_b = m.blocks_m() * m.blocks_n();
+  const void *base[2] = {m.hi, m.lo};
+  for (int t = 0; t < (m.lo ? 2 : 1); t++) {
+    const int rc = encode_tile_map(&o.map[t], base[t], 2, bf16, m.cols, m.rows, m.batches, m.ld, m.rows * m.ld, 64, k_inner ? box_rows : 64, what);
+    if (rc) return rc;
+  }
+  return CMACE_OK;
+}
+inline TpArgs new_args(int64_t rows, int64_t cols, int32_t *status) {
+  TpArgs g;
+  memset(&g, 0, sizeof(g));
+  g.rows = rows, g.cols = cols, g.status = status;
+  g.segments = g.batches = g.splits = 1;
+  return g;
+}
+inline int blocks64(int64_t n) { return (int)((n + 63) / 64); }
+
+// 256 columns a tile where that fills the SMs, 128 otherwise
+inline int tile_columns(int64_t rows, int cols, int64_t times) { return cols > 128 && (rows + 127) / 128 * ((cols + 255) / 256) * times >= 148 ? 256 : 128; }
+template <int KIND, bool PAIR, int TN, int ACT = TP_SILU>
+int tp_launch(TpArgs &g, cudaStream_t st, const char *what) {
+  using S = TpShape<KIND, PAIR, TN>;
+  static_assert(S::STAGES >= 2, "a ring of two stages at least");
+  g.mt = (int)((g.rows + 127) / 128);
+  g.nt = (int)((g.cols + S::OUT_N - 1) / S::OUT_N);
+  g.total = (int64_t)g.mt * g.nt * g.batches * g.splits;
+  if (g.total >= (int64_t)1 << 31) return fail(CMACE_ERR_UNSUPPORTED, "%s: too many tiles", what);
+  const auto kernel = tile_product_kernel<KIND, PAIR, TN, ACT>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  if (e != cudaSuccess) return fail(CMACE_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  const int grid = (int)(g.total < 148 ? g.total : 148);
+  launch_chained(kernel, dim3(grid), dim3(TP_THREADS), (size_t)S::SMEM, st, g);
+  return check_launch(what);
+}
+
+}  // namespace cmace

@@ -271,6 +271,113 @@ def tensor_core_ok(dtype, K, N):
 
 
 # --------------------------------------------------------------------------------------
+# gated feed-forward block
+# --------------------------------------------------------------------------------------
+_ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _workspace(device, nbytes):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+class _GatedFeedForwardFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, activation):
+        rows = x.reshape(-1, x.shape[-1]).contiguous()
+        weights = tuple(w.contiguous() for w in (w_gate, w_up, w_down))
+        M, C = rows.shape
+        H = weights[0].shape[1]
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        f32 = x.dtype == torch.float32
+        nbytes = _abi.call("cmace_gated_ff_workspace_bytes", int(f32), M, C, H, 0)
+        ws = _workspace(x.device, nbytes)
+        _abi.call("cmace_gated_ff_fwd_" + ("f32" if f32 else "bf16"), _ptr(rows), *map(_ptr, weights), M, C, H, activation,
+                  _ptr(y), _ptr(ws), nbytes, _ptr(_status_tensor(x.device)), _stream())
+        ctx.save_for_backward(rows, *weights)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_y):
+        rows, w_gate, w_up, w_down = ctx.saved_tensors
+        M, C = rows.shape
+        H = w_gate.shape[1]
+        gy = grad_y.contiguous()
+        f32 = rows.dtype == torch.float32
+        need = ctx.needs_input_grad
+        grads = [torch.empty(grad_y.shape, dtype=rows.dtype, device=rows.device) if need[0] else None]
+        grads += [torch.empty_like(w) if n else None for w, n in zip((w_gate, w_up, w_down), need[1:4])]
+        nbytes = _abi.call("cmace_gated_ff_workspace_bytes", int(f32), M, C, H, 1)
+        ws = _workspace(rows.device, nbytes)
+        _abi.call("cmace_gated_ff_bwd_" + ("f32" if f32 else "bf16"), _ptr(rows), _ptr(w_gate), _ptr(w_up), _ptr(w_down),
+                  _ptr(gy), M, C, H, ctx.activation, *map(_ptr, grads), _ptr(ws), nbytes,
+                  _ptr(_status_tensor(rows.device)), _stream())
+        return (*grads, None)
+
+
+def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
+    """(act(x @ w_gate) * (x @ w_up)) @ w_down for rows of node features x [..., C], w_gate and w_up [C, H], w_down [H, C], all
+    float32 or all bfloat16; `activation` is "silu" or "gelu" (with erf).  Differentiable (once) in x and the three weights.
+    Sums are float32 in both types; float32 runs on the tensor cores in three terms (cmace_gated_ff_fwd_f32), bfloat16 rounds the hidden
+    values to bfloat16 between the products.  The backward keeps x and the weights only and forms the hidden values again."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"gated_feed_forward: activation {activation!r} is none of {sorted(_ACTIVATIONS)}")
+    _check_cuda(x, w_gate, w_up, w_down)
+    if x.dtype not in (torch.float32, torch.bfloat16) or any(w.dtype != x.dtype for w in (w_gate, w_up, w_down)):
+        raise TypeError("gated_feed_forward needs float32 or bfloat16 operands of one type")
+    if x.dim() < 1 or w_gate.dim() != 2:
+        raise RuntimeError("gated_feed_forward needs rows and weight matrices")
+    C, H = w_gate.shape
+    if x.shape[-1] != C or w_up.shape != (C, H) or w_down.shape != (H, C) or C < 1 or H < 1:
+        raise RuntimeError(f"shape mismatch: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, "
+                           f"w_down {tuple(w_down.shape)}")
+    return _GatedFeedForwardFunction.apply(x, w_gate, w_up, w_down, _ACTIVATIONS[activation])
+
+
+class GatedFeedForward(torch.nn.Module):
+    """gated_feed_forward() with its weights as parameters: w_gate, w_up [C, H], w_down [H, C]."""
+
+    def __init__(self, w_gate, w_up, w_down, activation="silu"):
+        super().__init__()
+        self.w_gate, self.w_up, self.w_down = (torch.nn.Parameter(w.detach().clone()) for w in (w_gate, w_up, w_down))
+        self.activation = activation
+
+    def forward(self, x):
+        return gated_feed_forward(x, self.w_gate, self.w_up, self.w_down, self.activation)
+
+
+# --------------------------------------------------------------------------------------
+# orthogonalised updates
+# --------------------------------------------------------------------------------------
+def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """Matrices of `update` [..., m, n] brought near their orthogonal factors by Newton-Schulz products: X = U / (|U| + eps)
+    with the Frobenius norm of each matrix, then `steps` times X <- a X + (b S + c S S) X with S = X X^T and
+    (a, b, c) = `coefficients`.  float32 or bfloat16; a new tensor of the same shape and type.  For the updates of weight
+    matrices, stacks like Linear's [4, K, N] and ElementalLinear's [Z, 4, K, N] included; has no gradient."""
+    _check_cuda(update)
+    if update.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"orthogonalize needs float32 or bfloat16, got {update.dtype}")
+    if update.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("orthogonalize has no gradient: detach the update or call it under torch.no_grad()")
+    if update.dim() < 2 or update.shape[-1] < 1 or update.shape[-2] < 1:
+        raise RuntimeError(f"orthogonalize needs matrices [..., m, n], got {tuple(update.shape)}")
+    a, b, c = (float(v) for v in coefficients)
+    u = update.detach().contiguous()
+    m, n = u.shape[-2:]
+    out = torch.empty_like(u)
+    count = u.numel() // (m * n)
+    f32 = u.dtype == torch.float32
+    nbytes = _abi.call("cmace_orthogonalize_workspace_bytes", int(f32), count, m, n)
+    ws = _workspace(u.device, max(nbytes, 0))
+    name = "cmace_orthogonalize_" + ("f32" if f32 else "bf16")
+    _abi.call(name, _ptr(u), count, m, n, int(steps), a, b, c, float(eps), _ptr(out), _ptr(ws), nbytes,
+              _ptr(_status_tensor(u.device)), _stream())
+    _abi.launch_count += 2 + 3 * int(steps)
+    return out
+
+
+# --------------------------------------------------------------------------------------
 # edge topology
 # --------------------------------------------------------------------------------------
 class EdgeTopology:

@@ -272,6 +272,43 @@ int cmace_gemm3x_gradr_f32(const float *X, const float *G, const float *Y, const
                            const int32_t *receiver, const float *packed, int64_t nedges, int channels, int N,
                            float *out, int32_t *status, cmace_stream_t stream);
 
+/* ---- gated feed-forward block on rows of node features (no counterpart in the reference) -------------
+ * y = (act(x Wg) * (x Wu)) Wd with x [rows, width], Wg and Wu [width, hidden], Wd [hidden, width], all contiguous; activation 0: SiLU,
+ * 1: GELU (erf).  _f32 takes float, _bf16 bfloat16 (sums in float32).  The backward recomputes what it needs from x and the weights;
+ * every gradient may be NULL and is not formed then.  No rows: y and grad_x have none, the weights' gradients are zeros.
+ * workspace: cmace_gated_ff_workspace_bytes(...) bytes, aligned to 256, not shared by calls that may overlap; what it holds afterwards is not
+ * for the caller.  A row of x with an infinity or a NaN makes that row of y and grad_x, and the weights' gradients, not finite, no other row.
+ * status: as for cmace_gemm3x_f32. */
+int64_t cmace_gated_ff_workspace_bytes(int is_f32, int64_t rows, int width, int hidden, int backward_pass);
+int cmace_gated_ff_fwd_f32(const float *x, const float *w_gate, const float *w_up, const float *w_down, int64_t rows,
+                           int width, int hidden, int activation, float *y, void *workspace, int64_t workspace_bytes,
+                           int32_t *status, cmace_stream_t stream);
+int cmace_gated_ff_fwd_bf16(const void *x, const void *w_gate, const void *w_up, const void *w_down, int64_t rows,
+                            int width, int hidden, int activation, void *y, void *workspace, int64_t workspace_bytes,
+                            int32_t *status, cmace_stream_t stream);
+int cmace_gated_ff_bwd_f32(const float *x, const float *w_gate, const float *w_up, const float *w_down,
+                           const float *grad_y, int64_t rows, int width, int hidden, int activation, float *grad_x,
+                           float *grad_gate, float *grad_up, float *grad_down, void *workspace, int64_t workspace_bytes,
+                           int32_t *status, cmace_stream_t stream);
+int cmace_gated_ff_bwd_bf16(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *grad_y,
+                            int64_t rows, int width, int hidden, int activation, void *grad_x, void *grad_gate,
+                            void *grad_up, void *grad_down, void *workspace, int64_t workspace_bytes, int32_t *status,
+                            cmace_stream_t stream);
+
+/* ---- orthogonalised updates (no counterpart in the reference) -----------------------------------------
+ * out = Newton-Schulz products of update [count, rows, cols], contiguous: X = U / (|U| + eps) with the Frobenius norm of each matrix,
+ * then steps (1 to 100) times X <- a X + (b S + c S S) X, S = X X^T (rows > cols: X <- a X + X (b S + c S S), S = X^T X, the same values).
+ * float or bfloat16 in and out; X is held in float32.  Coefficients under which a singular value in [0, 1] could pass 1e12 are refused.
+ * out may be update itself.  workspace: cmace_orthogonalize_workspace_bytes(...) bytes, aligned to 256, not shared by calls that may
+ * overlap.  A matrix with an infinity or a NaN comes out not finite, no other one.  status: as for cmace_gemm3x_f32. */
+int64_t cmace_orthogonalize_workspace_bytes(int is_f32, int64_t count, int64_t rows, int cols);
+int cmace_orthogonalize_f32(const float *update, int64_t count, int64_t rows, int cols, int steps, double a, double b,
+                            double c, double eps, float *out, void *workspace, int64_t workspace_bytes, int32_t *status,
+                            cmace_stream_t stream);
+int cmace_orthogonalize_bf16(const void *update, int64_t count, int64_t rows, int cols, int steps, double a, double b,
+                             double c, double eps, void *out, void *workspace, int64_t workspace_bytes, int32_t *status,
+                             cmace_stream_t stream);
+
 /* ---- hidden layers of the radial multilayer perceptron in one kernel (float32) ---------------------
  * basis [E, nb] -> h3 = silu(silu(silu(basis W1) W2) W3) [E, 64], nb in {8, 16, 24, 32}, hidden width 64: the
  * network upstream MACE evaluates with torch (e3nn FullyConnectedNet) and the reference tabulates into its

@@ -226,7 +226,7 @@ static int weight_splits(int64_t M, int C, int H, int tn) {
   int best = 1;
   double least = 0;
   for (int s = 1; s <= 64 && s <= kb; s++) {
-    const double cost = (double)((tiles * s + 147) / 148) * ((double)((kb + s - 1) / s) + 6.0) + s * 3.0 * C * H * 1.5e-6;
+    const double cost = (double)((tiles * s + 147) / 148) * ((double)((kb + s - 1) / s) + 6.0) + s * 3.0 * C * H * 6e-6;
     if (s == 1 || cost < least) best = s, least = cost;
   }
   return best;

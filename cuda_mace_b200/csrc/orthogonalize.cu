@@ -62,8 +62,10 @@ __global__ void __launch_bounds__(NS_THREADS) ns_prep_kernel(const NsPrep p) {
   const int nb = (p.cols + 31) / 32;
   const int64_t row0 = b / nb * 32;
   const int col = (int)(b - b / nb * nb) * 32 + (threadIdx.x & 31);
-  double s = 0;
-  for (int c = 0; c < p.chunks; c++) s += __ldcg(p.partial + m * p.chunks + c);
+  double s = 0;   // every warp sums the partial sums, in the same order
+  for (int c = threadIdx.x & 31; c < p.chunks; c += 32) s += __ldcg(p.partial + m * p.chunks + c);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
   const float inv = (float)(1.0 / (sqrt(s) + p.eps));
   if (col >= p.cols) return;
 #pragma unroll
@@ -82,6 +84,314 @@ __global__ void __launch_bounds__(NS_THREADS) ns_prep_kernel(const NsPrep p) {
       p.hi[at] = __float2half_rn(v * p.scale);
     }
   }
+}
+
+// ---- all steps in one kernel, for matrices whose shorter side fits a tile ------------------------------------------------------
+// X [side <= 128, columns] (a tall matrix is read and written transposed) stays on the SM: as fp16 pairs in shared memory, which
+// serve S = X X^T (contracted index inside a row) and P X (contracted index over the rows) from the same image, and in float32 in
+// tensor memory, 128 lanes x 256 columns.  S, then P = b S + c S S in its place, are a second image.  A matrix of more than 256 columns
+// (128 in a cluster) is spread over the CTAs of a cluster: each has its columns of X and a part of S, which they sum
+// through distributed shared memory (each its share of the rows, in the order of the ranks) and hand to all.
+//
+// The three products of a step and what stands between them form a chain, so the block works on one thing at a time: 16 warps for the
+// elementwise phases (a warp of each quarter of the lanes has a quarter of the columns), one thread issues MMAs.  Terms with a low part come
+// first: the sum is small while they are added, and the truncating additions that count are the 4 a 64 k of hi hi.
+constexpr int NSF_THREADS = 512;
+constexpr int NSF_STAGE_LD = 65;          // floats a row of the transposing buffer
+constexpr int NSF_IMAGE = 128 * 128;      // 128 rows of 64 fp16
+constexpr int NSF_S_BYTES = 4 * NSF_IMAGE;   // two chunks, hi and lo
+constexpr int NSF_MAX_STEPS = 100;
+
+struct NsFused {
+  const void *src;
+  void *out;
+  int64_t count;
+  int side, length, tall, bf16, steps, columns, chunks;   // columns of a CTA, its chunks of 64
+  int cluster;
+  float a, b, c;
+  double eps;
+  int32_t *status;
+  float sx[NSF_MAX_STEPS + 1], ss[NSF_MAX_STEPS], sp[NSF_MAX_STEPS];   // powers of two of X, S and P of every step
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 peer_load4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void peer_store2(uint32_t addr, uint32_t x, uint32_t y) {
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void smem_store4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ uint4 smem_load4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+// hi and lo of COLS values of one row (16-byte pieces `piece`, ... of its 128 bytes) into the images at hi and lo
+template <int COLS>
+__device__ __forceinline__ void put_pairs(uint32_t hi, uint32_t lo, int row, int piece, const float (&v)[COLS], float scale) {
+#pragma unroll
+  for (int c = 0; c < COLS / 8; c++) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) tp_split2(v[8 * c + 2 * k] * scale, v[8 * c + 2 * k + 1] * scale, h[k], l[k]);
+    const uint32_t at = (uint32_t)sw128_offset(row, piece + c);
+    smem_store4(hi + at, h[0], h[1], h[2], h[3]);
+    smem_store4(lo + at, l[0], l[1], l[2], l[3]);
+  }
+}
+
+template <bool CLUSTER>
+__global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_constant__ NsFused g) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t done_bar;
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ double sums[NSF_THREADS / 32 + 1];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  unsigned char *const generic = smem_raw + (base - raw);
+  const uint32_t x_hi = base, x_lo = base + (uint32_t)(g.chunks * NSF_IMAGE), s_hi = base + (uint32_t)(2 * g.chunks * NSF_IMAGE);
+  const uint32_t s_lo = s_hi + 2 * NSF_IMAGE, part = s_hi + NSF_S_BYTES;   // part: CLUSTER, this CTA's S in float32
+  float *const stage = reinterpret_cast<float *>(generic + (s_hi - base));   // before and after the steps
+  const uint32_t bar = smem_u32(&done_bar);
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31, q = warp & 3, group = warp >> 2;
+  const int row = 32 * q + lane;
+  const uint32_t rank = CLUSTER ? cluster_rank() : 0;
+
+  if (tid == 0) {
+    mbar_init(bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) tmem_alloc(smem_u32(&tmem_base_slot), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = (uint32_t)uniform((int)tmem_base_slot);
+  const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16), master = acc + 256;
+  grid_begin();
+  const int64_t matrix = blockIdx.x / (unsigned)g.cluster;
+  const int64_t size = (int64_t)g.side * g.length;
+  const int col0 = (int)rank * g.columns;
+  uint32_t phase = 0;
+  bool ok = true;
+
+  // ---- the update into tensor memory, and its norm -----------------------------------------------------------------------
+  double square = 0;
+  for (int ch = 0; ch < g.chunks; ch++) {
+    float v[16];
+    if (!g.tall) {
+#pragma unroll
+      for (int k = 0; k < 16; k++) {
+        const int e = tid + NSF_THREADS * k, r = e >> 6, cc = 64 * ch + (e & 63), c = col0 + cc;
+        v[k] = r < g.side && cc < g.columns && c < g.length ? ns_load(g.src, matrix * size + (int64_t)r * g.length + c, g.bf16) : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; k++) {
+        const int e = tid + NSF_THREADS * k, r = e & 127, cc = 64 * ch + (e >> 7), c = col0 + cc;
+        v[k] = r < g.side && cc < g.columns && c < g.length ? ns_load(g.src, matrix * size + (int64_t)c * g.side + r, g.bf16) : 0.f;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+      const int e = tid + NSF_THREADS * k;
+      if (!g.tall) stage[(e >> 6) * NSF_STAGE_LD + (e & 63)] = v[k];
+      else stage[(e & 127) * NSF_STAGE_LD + (e >> 7)] = v[k];
+      square = fma((double)v[k], (double)v[k], square);
+    }
+    __syncthreads();
+    uint32_t w[16];
+#pragma unroll
+    for (int k = 0; k < 16; k++) w[k] = __float_as_uint(stage[row * NSF_STAGE_LD + 16 * group + k]);
+    tmem_st16(master + (uint32_t)(64 * ch + 16 * group), w);
+  }
+  tmem_st_wait();
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
+  if (lane == 0) sums[warp] = square;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < NSF_THREADS / 32; w++) square += sums[w];
+    sums[NSF_THREADS / 32] = square;
+  }
+  if (CLUSTER) {
+    cluster_sync();
+    square = 0;
+    for (int r = 0; r < g.cluster; r++) {
+      double v;
+      asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(peer_smem(smem_u32(&sums[NSF_THREADS / 32]), (uint32_t)r)) : "memory");
+      square += v;
+    }
+  } else {
+    __syncthreads();
+    square = sums[NSF_THREADS / 32];
+  }
+  const float inv = (float)(1.0 / (sqrt(square) + g.eps));
+  for (int ch = 0; ch < g.chunks; ch++) {
+    const uint32_t at = master + (uint32_t)(64 * ch + 16 * group);
+    uint32_t w[16];
+    float v[16];
+    tmem_ld16_nowait(at, w);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 16; k++) v[k] = __uint_as_float(w[k]) * inv;
+#pragma unroll
+    for (int k = 0; k < 16; k++) w[k] = __float_as_uint(v[k]);
+    tmem_st16(at, w);
+    put_pairs(x_hi + (uint32_t)(ch * NSF_IMAGE), x_lo + (uint32_t)(ch * NSF_IMAGE), row, 2 * group, v, g.sx[0]);
+  }
+  tmem_st_wait();
+
+  const int side16 = (g.side + 15) & ~15, n_x = 64 * g.chunks;
+  const uint32_t idesc_s = tp_idesc(side16, 0, 0, 0), idesc_x = tp_idesc(n_x, 0, 0, 1);
+  // operands are written, sums are read: products a*b of `steps16` times 16 k, three terms, the ones with a low part first
+  const auto products = [&](uint32_t a_hi, uint32_t a_lo, uint32_t b_hi, uint32_t b_lo, int steps16, bool b_mn, uint32_t idesc) {
+    fence_proxy_async();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0 && elect_one()) {
+      tc_fence_after();
+      const auto A = [&](uint32_t image, int k) { return tp_desc(image + (uint32_t)((k >> 2) * NSF_IMAGE + (k & 3) * 32), 0); };
+      const auto B = [&](uint32_t image, int k) {
+        // MN-major: 16 rows of the image a step, runs of 64 columns an image apart
+        if (b_mn) return (tp_desc(image + (uint32_t)(k * 2048), 1) & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(NSF_IMAGE >> 4) << 16);
+        return tp_desc(image + (uint32_t)((k >> 2) * NSF_IMAGE + (k & 3) * 32), 0);
+      };
+      for (int k = 0; k < steps16; k++) {
+        umma_16(tmem, A(a_lo, k), B(b_hi, k), idesc, k > 0);
+        umma_16(tmem, A(a_hi, k), B(b_lo, k), idesc, 1);
+      }
+      for (int k = 0; k < steps16; k++) umma_16(tmem, A(a_hi, k), B(b_hi, k), idesc, 1);
+      umma_commit(bar);
+    }
+    if (ok && !warp_wait(bar, phase, lane)) {   // a block that gave up goes on: the others of its cluster meet it at the barriers
+      if (lane == 0 && g.status) atomicCAS(g.status, 0, 47);
+      ok = false;
+    }
+    phase ^= 1;
+    tc_fence_after();
+  };
+  const int s_chunk = group >> 1, s_piece = 4 * (group & 1);   // this thread's 32 columns of S
+  const uint32_t s_at = (uint32_t)(s_chunk * NSF_IMAGE);
+  const int x_steps = (min(g.columns, g.length - col0 > 0 ? g.length - col0 : 1) + 15) / 16;
+
+  for (int step = 0; step < g.steps; step++) {
+    const float sx = g.sx[step], ss = g.ss[step], sp = g.sp[step];
+    uint32_t u[32];
+    float v[32];
+    // S = X X^T
+    products(x_hi, x_lo, x_hi, x_lo, x_steps, false, idesc_s);
+    tmem_ld32(acc + (uint32_t)(32 * group), u);
+    const float to_s = 1.0f / (sx * sx);
+    const bool mine = 32 * group < side16;   // columns that the product has written
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] = mine && 32 * group + j < side16 ? __uint_as_float(u[j]) * to_s : 0.f;
+    if (!CLUSTER) {
+      put_pairs(s_hi + s_at, s_lo + s_at, row, s_piece, v, ss);
+    } else {
+      // part: [128 rows][32 pieces of four columns], the piece changed by the row so that a warp's stores and loads meet all banks
+#pragma unroll
+      for (int c = 0; c < 8; c++)
+        smem_store4(part + (uint32_t)(row * 512 + (((8 * group + c) ^ (row & 31)) << 4)), __float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]),
+                    __float_as_uint(v[4 * c + 2]), __float_as_uint(v[4 * c + 3]));
+      cluster_sync();
+      const int rows_each = 128 / g.cluster;
+      for (int e = tid; e < rows_each * 32; e += NSF_THREADS) {
+        const int r = (int)rank * rows_each + (e >> 5), piece = e & 31;
+        const uint32_t at = part + (uint32_t)(r * 512 + ((piece ^ (r & 31)) << 4));
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = 0; p < g.cluster; p++) {
+          const float4 x = peer_load4(peer_smem(at, (uint32_t)p));
+          sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+        }
+        uint32_t h0, h1, l0, l1;
+        tp_split2(sum.x * ss, sum.y * ss, h0, l0);
+        tp_split2(sum.z * ss, sum.w * ss, h1, l1);
+        const uint32_t to = (uint32_t)((piece >> 4) * NSF_IMAGE + sw128_offset(r, (piece & 15) >> 1) + (piece & 1) * 8);
+        for (int p = 0; p < g.cluster; p++) {
+          peer_store2(peer_smem(s_hi + to, (uint32_t)p), h0, h1);
+          peer_store2(peer_smem(s_lo + to, (uint32_t)p), l0, l1);
+        }
+      }
+      asm volatile("fence.proxy.async;" ::: "memory");   // the images are read by tensor cores of all CTAs
+      cluster_sync();
+    }
+    // P = b S + c S S, in the place of S
+    products(s_hi, s_lo, s_hi, s_lo, side16 / 16, false, idesc_s);
+    tmem_ld32(acc + (uint32_t)(32 * group), u);
+    const float from_ss = g.c / (ss * ss), from_s = g.b / ss;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const uint32_t at = s_at + (uint32_t)sw128_offset(row, s_piece + c);
+      const uint4 h = smem_load4(s_hi + at), l = smem_load4(s_lo + at);
+      const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&hw[k])), y = __half22float2(*reinterpret_cast<const __half2 *>(&lw[k]));
+        const int j = 8 * c + 2 * k;
+        v[j] = mine && 32 * group + j < side16 ? __uint_as_float(u[j]) * from_ss + from_s * (x.x + y.x) : 0.f;
+        v[j + 1] = mine && 32 * group + j < side16 ? __uint_as_float(u[j + 1]) * from_ss + from_s * (x.y + y.y) : 0.f;
+      }
+    }
+    put_pairs(s_hi + s_at, s_lo + s_at, row, s_piece, v, sp);
+    // X = a X + P X
+    products(s_hi, s_lo, x_hi, x_lo, side16 / 16, true, idesc_x);
+    const float from_p = 1.0f / (sp * sx);
+    const bool last = step + 1 == g.steps;
+    for (int ch = 0; ch < g.chunks; ch++) {
+      const uint32_t col = (uint32_t)(64 * ch + 16 * group);
+      uint32_t w[16], m[16];
+      float x[16];
+      tmem_ld16_nowait(acc + col, w);
+      tmem_ld16_nowait(master + col, m);
+      tmem_ld_wait();
+#pragma unroll
+      for (int k = 0; k < 16; k++) x[k] = g.a * __uint_as_float(m[k]) + from_p * __uint_as_float(w[k]);
+      if (!last) {
+#pragma unroll
+        for (int k = 0; k < 16; k++) m[k] = __float_as_uint(x[k]);
+        tmem_st16(master + col, m);
+        put_pairs(x_hi + (uint32_t)(ch * NSF_IMAGE), x_lo + (uint32_t)(ch * NSF_IMAGE), row, 2 * group, x, g.sx[step + 1]);
+      } else {
+        __syncthreads();   // every warp has its sums: the image of P is free; and the stores of the chunk before are done
+#pragma unroll
+        for (int k = 0; k < 16; k++) stage[row * NSF_STAGE_LD + 16 * group + k] = x[k];
+        __syncthreads();
+#pragma unroll 4
+        for (int k = 0; k < 16; k++) {
+          const int e = tid + NSF_THREADS * k;
+          const int r = g.tall ? e & 127 : e >> 6, in = g.tall ? e >> 7 : e & 63, c = col0 + 64 * ch + in;
+          if (r < g.side && 64 * ch + in < g.columns && c < g.length) {
+            const int64_t at = matrix * size + (g.tall ? (int64_t)c * g.side + r : (int64_t)r * g.length + c);
+            const float y = stage[r * NSF_STAGE_LD + in];
+            if (g.bf16) static_cast<__nv_bfloat16 *>(g.out)[at] = __float2bfloat16_rn(y);
+            else static_cast<float *>(g.out)[at] = y;
+          }
+        }
+      }
+    }
+    tmem_st_wait();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
 // largest |p| over [0, most] of a polynomial c1 t + c3 t^3 + c5 t^5 (odd) or c1 t + c2 t^2, from its ends and the zeros of its derivative
@@ -138,11 +448,68 @@ static int set_split_out(TpArgs &g, const Matrix &m, const char *what) {
 }
 template <int KIND>
 static int launch_ns(bool pair, int tn, TpArgs &g, cudaStream_t st, const char *what) {
-  if (tn == 256) return pair ? tp_launch<KIND, true, 256>(g, st, what) : tp_launch<KIND, false, 256>(g, st, what);
+  if (tn == 256) return tp_launch<KIND, false, 256>(g, st, what);   // pairs: the sums and their handling do not fit 168 registers
   return pair ? tp_launch<KIND, true, 128>(g, st, what) : tp_launch<KIND, false, 128>(g, st, what);
 }
 
+// CTAs a matrix for the kernel above, 0: it does not fit
+static int fused_cluster(int64_t count, int64_t rows, int cols) {
+  const int64_t side = std::min<int64_t>(rows, cols), length = std::max<int64_t>(rows, cols);
+  if (side > 128 || length > 1024) return 0;
+  if (length <= 128 || (length <= 256 && count > 74)) return 1;
+  int p = 2;
+  while (p * 128 < length) p *= 2;
+  return p;
+}
+
+static int run_fused(const NsCall &f, int cluster) {
+  NsFused g;
+  memset(&g, 0, sizeof(g));
+  g.src = f.src, g.out = f.out, g.count = f.count;
+  g.tall = f.rows > f.cols;
+  g.side = (int)std::min<int64_t>(f.rows, f.cols), g.length = (int)std::max<int64_t>(f.rows, f.cols);
+  g.bf16 = !f.f32, g.steps = f.steps, g.cluster = cluster;
+  g.columns = (int)up((g.length + cluster - 1) / cluster, 16);
+  g.chunks = (g.columns + 63) / 64;
+  g.a = (float)f.a, g.b = (float)f.b, g.c = (float)f.c, g.eps = f.eps, g.status = f.status;
+  double most = 1.0;
+  for (int k = 0; k < f.steps; k++) {
+    g.sx[k] = fp16_scale(most);
+    g.ss[k] = fp16_scale(most * most);
+    g.sp[k] = fp16_scale(most_square(f.b, f.c, most * most));
+    most = most_odd(f.a, f.b, f.c, most);
+  }
+  const int smem = 2 * g.chunks * NSF_IMAGE + NSF_S_BYTES + (cluster > 1 ? 128 * 512 : 0) + 1024;
+  const auto kernel = cluster > 1 ? ns_fused_kernel<true> : ns_fused_kernel<false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)cluster, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(f.count * cluster));
+  cfg.blockDim = dim3(NSF_THREADS);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = f.st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, g);
+  if (e != cudaSuccess) return fail(CMACE_ERR_CUDA, "%s: %s", f.what, cudaGetErrorString(e));
+  return check_launch(f.what);
+}
+// how far singular values can grow is what fp16 operands and float32 sums have to hold
+static int check_growth(const NsCall &f) {
+  double most = 1.0;
+  for (int k = 0; k < f.steps; k++) {
+    const double p = most_square(f.b, f.c, most * most), next = most_odd(f.a, f.b, f.c, most);
+    if (!(next < 1e12) || !(p < 1e12))
+      return fail(CMACE_ERR_ARG, "%s: coefficients %g, %g, %g: singular values may grow to %g in step %d", f.what, f.a, f.b, f.c, next, k + 1);
+    most = next;
+  }
+  return CMACE_OK;
+}
+
 static int orthogonalize(const NsCall &f, Carve &w) {
+  if (const int cluster = fused_cluster(f.count, f.rows, f.cols)) return w.base ? run_fused(f, cluster) : CMACE_OK;
   const bool wide = f.rows <= f.cols;   // S = X X^T, else X^T X
   const int side = wide ? (int)f.rows : f.cols;
   const int64_t n = f.rows * f.cols;
@@ -150,7 +517,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   double *partial = w.take<double>(f.count * chunks);
   Matrix x[2];
   for (Matrix &m : x) m = new_matrix(w, f.f32, f.rows, f.cols, f.count, 64, false);
-  const Matrix s = new_matrix(w, f.f32, side, side, f.count, 64, false), poly = new_matrix(w, f.f32, side, side, f.count, 64, false);
+  const Matrix s = new_matrix(w, true, side, side, f.count, 64, false), poly = new_matrix(w, f.f32, side, side, f.count, 64, false);
   float *master = w.take<float>(f.count * f.rows * x[0].ld);
   if (!w.base) return CMACE_OK;
 
@@ -161,12 +528,10 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   launch_chained(ns_norm_kernel, dim3((unsigned)(f.count * chunks)), dim3(NS_THREADS), (size_t)0, f.st, p);
   launch_chained(ns_prep_kernel, dim3((unsigned)(f.count * ((f.rows + 31) / 32) * ((f.cols + 31) / 32))), dim3(NS_THREADS), (size_t)0, f.st, p);
   int rc = check_launch(f.what);
-  const int t_s = tile_columns(side, side, f.count), t_x = tile_columns(f.rows, f.cols, f.count);
+  const int t_s = f.f32 ? 128 : tile_columns(side, side, f.count), t_x = f.f32 ? 128 : tile_columns(f.rows, f.cols, f.count);
   for (int step = 0; step < f.steps && !rc; step++) {
     const Matrix &now = x[step & 1], &next = x[(step + 1) & 1];
     const double most_s = most * most, most_p = most_square(f.b, f.c, most_s), most_next = most_odd(f.a, f.b, f.c, most);
-    if (!(most_next < 1e12) || !(most_p < 1e12))
-      return fail(CMACE_ERR_ARG, "%s: coefficients %g, %g, %g: singular values may grow to %g in step %d", f.what, f.a, f.b, f.c, most_next, step + 1);
     const float ss = fp16_scale(most_s), sp = fp16_scale(most_p), sn = fp16_scale(most_next);
     const bool last = step + 1 == f.steps;
     TpArgs g = new_args(side, side, f.status);
@@ -233,6 +598,7 @@ static int run_orthogonalize(bool f32, const void *update, int64_t count, int64_
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(CMACE_ERR_ARG, "%s: the workspace has to be aligned to 256 bytes", what);
   if (!(std::isfinite(a) && std::isfinite(b) && std::isfinite(c)) || !(eps >= 0)) return fail(CMACE_ERR_ARG, "%s: bad coefficients or eps", what);
   NsCall f{f32, update, out, count, rows, cols, steps, a, b, c, eps, status, (cudaStream_t)stream, what};
+  if (int rc = check_growth(f)) return rc;
   Carve need{nullptr};
   orthogonalize(f, need);
   if (bytes < need.used) return fail(CMACE_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes, (long long)need.used);

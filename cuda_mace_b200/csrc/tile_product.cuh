@@ -35,7 +35,6 @@ namespace cmace {
 
 constexpr int TP_EPILOGUE_WARPS = 8;
 constexpr int TP_THREADS = (TP_EPILOGUE_WARPS + 2) * 32;   // 204 registers a thread: 128 sums of a PAIR tile and their handling
-constexpr int TP_STAGING = 4096;                           // bytes an epilogue warp stages its output in
 constexpr int TP_SMEM_BUDGET = 227 * 1024 - 1024;          // without the static barriers
 constexpr int TP_BUFFER_COLS = 256;                        // one set of accumulator columns
 constexpr int TP_MAX_STAGES = 8;
@@ -105,10 +104,11 @@ struct TpShape {
   static constexpr int OUT_N = KIND == TP_BACK ? 64 : (KIND == TP_GATED ? 128 : TN);     // output columns of a tile
   static constexpr int A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128;
   static constexpr int STAGE = (A_BYTES + B_BYTES) * (PAIR ? 2 : 1);
-  static constexpr int STAGES =
-      (TP_SMEM_BUDGET - 1024 - TP_EPILOGUE_WARPS * TP_STAGING) / STAGE < TP_MAX_STAGES
-          ? (TP_SMEM_BUDGET - 1024 - TP_EPILOGUE_WARPS * TP_STAGING) / STAGE : TP_MAX_STAGES;
-  static constexpr int SMEM = STAGE * STAGES + TP_EPILOGUE_WARPS * TP_STAGING + 1024;
+  // bytes an epilogue warp stages its output in: one piece of 32 rows of 128 bytes, or two where the stages leave room
+  static constexpr int STAGING = KIND >= TP_GRAM && !PAIR ? 8192 : 4096;
+  static constexpr int FIT = (TP_SMEM_BUDGET - 1024 - TP_EPILOGUE_WARPS * STAGING) / STAGE;
+  static constexpr int STAGES = FIT < TP_MAX_STAGES ? FIT : TP_MAX_STAGES;
+  static constexpr int SMEM = STAGE * STAGES + TP_EPILOGUE_WARPS * STAGING + 1024;
 };
 
 struct TpTile {
@@ -196,6 +196,10 @@ struct TpStager {
   int64_t rows, cols;   // of the output: a box that starts outside is not stored
   __device__ __forceinline__ void begin() const {   // the copy engine has read what was staged before
     if (elect_one()) tma_store_wait_read();
+    __syncwarp();
+  }
+  __device__ __forceinline__ void begin_but_last() const {   // ... all but the last store's piece
+    if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
     __syncwarp();
   }
   // COLS 32-bit words of this lane's row at `at` (bytes into the staging buffer): rows of 128 bytes (32 words) or 64 (16)
@@ -419,7 +423,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
     // ================================ epilogue ================================
     const int q = warp & 3, half = warp >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
-    const TpStager st{staging + (uint32_t)(warp * TP_STAGING), lane, g.rows, g.cols};
+    const TpStager st{staging + (uint32_t)(warp * S::STAGING), lane, g.rows, g.cols};
     int buf = 0;
     uint32_t buf_phase[2] = {0, 0};
     bool ok = true;
@@ -437,6 +441,23 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
     for (int64_t t = blockIdx.x; t < g.total; t += gridDim.x, odd ^= 1) {
       const TpTile T = tp_tile(g, t, S::OUT_N);
       const int64_t row = T.row0 + 32 * q;   // first row of this warp
+      // What a Newton-Schulz epilogue adds to the product, a group of 32 columns ahead: S (hi and lo; rows of a multiple of 64 elements,
+      // so that a group never runs over one's end) or X in float32.
+      const int col0 = T.n0 + half * (TN / 2);
+      uint4 cin[KIND == TP_POLY || KIND == TP_APPLY ? 8 : 1];
+      const auto fetch_cin = [&](int col) {
+        if constexpr (KIND == TP_POLY || KIND == TP_APPLY) {
+          const int64_t from = (int64_t)T.batch * g.cin_batch + (row + lane) * g.cin_ld + col;
+          const bool in_rows = row + lane < g.rows;
+#pragma unroll
+          for (int c = 0; c < 8; c++) {
+            const uint4 *p = KIND == TP_APPLY ? reinterpret_cast<const uint4 *>(static_cast<const float *>(g.cin[0]) + from) + c
+                                              : reinterpret_cast<const uint4 *>(static_cast<const __half *>(g.cin[c >> 2]) + from) + (c & 3);
+            cin[c] = in_rows ? __ldcg(p) : make_uint4(0, 0, 0, 0);
+          }
+        }
+      };
+      if (col0 < g.cols) fetch_cin(col0);
       float acc[PAIR ? GROUPS : 1][32];
       if (PAIR) {
 #pragma unroll
@@ -616,7 +637,6 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           if (PAIR) st.send(&g.out[1].map, 2048, col, row, p);
         }
       } else if constexpr (KIND == TP_PLAIN) {
-        const int col0 = T.n0 + half * (TN / 2);
         const int batch = T.split * g.batches + T.batch;
         if (g.out_bf16) {
 #pragma unroll
@@ -652,8 +672,6 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         }
       } else {
         // Newton-Schulz: values in float32, then hi and lo (or one fp16) at a power of two that the caller has from its bounds
-        const int col0 = T.n0 + half * (TN / 2);
-        const bool in_rows = row + lane < g.rows;
 #pragma unroll
         for (int i = 0; i < GROUPS; i++) {
           const int col = col0 + 32 * i;
@@ -664,79 +682,67 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] *= g.alpha;
           } else if constexpr (KIND == TP_POLY) {
-            // alpha * (S S) + beta * S; rows of S have a multiple of 64 elements, so a group never runs over one's end
-            const int64_t at16 = (int64_t)T.batch * g.cin_batch + (row + lane) * g.cin_ld + col;
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-              uint4 h = make_uint4(0, 0, 0, 0), l = h;
-              if (in_rows) {
-                h = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(g.cin[0]) + at16) + c);
-                if (PAIR) l = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(g.cin[1]) + at16) + c);
-              }
-              const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
+              const uint32_t hw[4] = {cin[c].x, cin[c].y, cin[c].z, cin[c].w}, lw[4] = {cin[4 + c].x, cin[4 + c].y, cin[4 + c].z, cin[4 + c].w};
 #pragma unroll
               for (int k = 0; k < 4; k++) {
-                float2 s = __half22float2(*reinterpret_cast<const __half2 *>(&hw[k]));
-                if (PAIR) {
-                  const float2 e = __half22float2(*reinterpret_cast<const __half2 *>(&lw[k]));
-                  s.x += e.x;
-                  s.y += e.y;
-                }
-                v[8 * c + 2 * k] = g.alpha * v[8 * c + 2 * k] + g.beta * s.x;
-                v[8 * c + 2 * k + 1] = g.alpha * v[8 * c + 2 * k + 1] + g.beta * s.y;
+                const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&hw[k])), e = __half22float2(*reinterpret_cast<const __half2 *>(&lw[k]));
+                v[8 * c + 2 * k] = g.alpha * v[8 * c + 2 * k] + g.beta * (a.x + e.x);
+                v[8 * c + 2 * k + 1] = g.alpha * v[8 * c + 2 * k + 1] + g.beta * (a.y + e.y);
               }
             }
           } else {
-            const float *x = static_cast<const float *>(g.cin[0]) + (int64_t)T.batch * g.cin_batch + (row + lane) * g.cin_ld + col;
 #pragma unroll
             for (int c = 0; c < 8; c++) {
-              float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (in_rows) s = __ldcg(reinterpret_cast<const float4 *>(x) + c);
-              v[4 * c] = g.alpha * v[4 * c] + g.beta * s.x;
-              v[4 * c + 1] = g.alpha * v[4 * c + 1] + g.beta * s.y;
-              v[4 * c + 2] = g.alpha * v[4 * c + 2] + g.beta * s.z;
-              v[4 * c + 3] = g.alpha * v[4 * c + 3] + g.beta * s.w;
+              v[4 * c] = g.alpha * v[4 * c] + g.beta * __uint_as_float(cin[c].x);
+              v[4 * c + 1] = g.alpha * v[4 * c + 1] + g.beta * __uint_as_float(cin[c].y);
+              v[4 * c + 2] = g.alpha * v[4 * c + 2] + g.beta * __uint_as_float(cin[c].z);
+              v[4 * c + 3] = g.alpha * v[4 * c + 3] + g.beta * __uint_as_float(cin[c].w);
             }
           }
+          if (i + 1 < GROUPS && col + 32 < g.cols) fetch_cin(col + 32);   // on its way while this group is put down
           if (KIND == TP_APPLY) {
             // out[2]: float32, the X of the next step or the result
-            uint32_t w[32];
-#pragma unroll
-            for (int j = 0; j < 32; j++) w[j] = __float_as_uint(v[j]);
             if (!g.out_bf16) {
-              st.begin();
+              uint32_t w[32];
+#pragma unroll
+              for (int j = 0; j < 32; j++) w[j] = __float_as_uint(v[j]);
+              if (PAIR) st.begin();
+              else st.begin_but_last();   // the pairs' piece may still be read
               st.put(0, w);
               if (g.out[2].use_map) st.send(&g.out[2].map, 0, col, row, T.batch);
               else st.send_rows(g.out[2], false, col, row, T.batch);
+            } else if (g.out[2].use_map) {
+              uint32_t w[16];
+#pragma unroll
+              for (int j = 0; j < 16; j++) w[j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
+              st.begin();
+              st.put(0, w);
+              st.send(&g.out[2].map, 0, col, row, T.batch);
             } else {
-              if (g.out[2].use_map) {
-                uint32_t w16[16];
+              __nv_bfloat16 *o =
+                  static_cast<__nv_bfloat16 *>(g.out[2].ptr) + (int64_t)T.batch * g.out[2].batch + (row + lane) * g.out[2].ld + col;
 #pragma unroll
-                for (int j = 0; j < 16; j++) w16[j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
-                st.begin();
-                st.put(0, w16);
-                st.send(&g.out[2].map, 0, col, row, T.batch);
-              } else {
-                __nv_bfloat16 *o =
-                    static_cast<__nv_bfloat16 *>(g.out[2].ptr) + (int64_t)T.batch * g.out[2].batch + (row + lane) * g.out[2].ld + col;
-#pragma unroll
-                for (int j = 0; j < 32; j++)
-                  if (in_rows && col + j < g.cols) o[j] = __float2bfloat16_rn(v[j]);
-              }
+              for (int j = 0; j < 32; j++)
+                if (row + lane < g.rows && col + j < g.cols) o[j] = __float2bfloat16_rn(v[j]);
             }
           }
           if (KIND != TP_APPLY || g.pair_scale != 0.f) {
+            constexpr uint32_t where = PAIR ? 0u : 4096u;
+            constexpr bool LOW = PAIR || KIND == TP_GRAM;   // S is also added as it is: with its low part
             uint32_t w[16], lo[16];
 #pragma unroll
             for (int j = 0; j < 16; j++) {
-              if (PAIR) tp_split2(v[2 * j] * g.pair_scale, v[2 * j + 1] * g.pair_scale, w[j], lo[j]);
+              if (LOW) tp_split2(v[2 * j] * g.pair_scale, v[2 * j + 1] * g.pair_scale, w[j], lo[j]);
               else w[j] = tp_f16x2(v[2 * j] * g.pair_scale, v[2 * j + 1] * g.pair_scale);
             }
-            st.begin();
-            st.put(0, w);
-            if (PAIR) st.put(2048, lo);
-            st.send(&g.out[0].map, 0, col, row, T.batch);
-            if (PAIR) st.send(&g.out[1].map, 2048, col, row, T.batch);
+            if (PAIR || KIND != TP_APPLY) st.begin();
+            else st.begin_but_last();   // this group's float32 piece may still be read
+            st.put(where, w);
+            if (LOW) st.put(where + 2048, lo);
+            st.send(&g.out[0].map, where, col, row, T.batch);
+            if (LOW) st.send(&g.out[1].map, where + 2048, col, row, T.batch);
           }
         }
       }

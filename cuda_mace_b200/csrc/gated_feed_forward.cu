@@ -164,31 +164,30 @@ struct FeedForward {
 static Matrix take_matrix(Carve &w, PrepArgs &prep, int64_t &blocks, bool f32, const void *src, int64_t rows, int cols) {
   if (!f32 && cols % 8 == 0 && aligned16(src)) {
     Matrix m;
-    m.hi = const_cast<void *>(src);
+    m.at = static_cast<uint16_t *>(const_cast<void *>(src));
     m.rows = rows, m.cols = cols, m.ld = cols;
     return m;
   }
   const Matrix m = new_matrix(w, f32, rows, cols, 1);
   PrepJob &j = prep.job[prep.jobs++];
-  j = PrepJob{src, m.hi, m.lo, m.scale, rows, blocks, cols, (int)m.ld, (int)m.blocks_n()};
+  j = PrepJob{src, m.at, f32 ? m.at + m.plane() : nullptr, m.scale, rows, blocks, cols, (int)m.ld, (int)m.blocks_n()};
   blocks += m.blocks_m() * m.blocks_n();
   return m;
 }
-
+static int encode_all(std::initializer_list<Matrix *> all, bool bf16, const char *what) {
+  for (Matrix *m : all)
+    if (const int rc = encode_matrix(&m->map, *m, 64, 64, bf16, what)) return rc;
+  return CMACE_OK;
+}
 static int set_hidden_out(TpArgs &g, const Matrix &m, int box_cols, bool bf16, const char *what) {
-  const void *base[2] = {m.hi, m.lo};
-  for (int t = 0; t < (m.lo ? 2 : 1); t++) {
-    const int rc = encode_tile_map(&g.out[t].map, base[t], 2, bf16, m.cols, m.rows, m.batches, m.ld, m.rows * m.ld, box_cols, 32, what);
-    if (rc) return rc;
-    g.out[t].use_map = 1;
-  }
+  g.out[0].use_map = 1;
   for (int p = 0; p < 3 && m.scale; p++) g.out_scale[p] = m.scale + (m.batches > 1 ? p : 0) * m.blocks_m() * m.blocks_n();
   g.out_scale_ld = m.blocks_n();
-  return CMACE_OK;
+  return encode_matrix(&g.out[0].map, m, box_cols, 32, bf16, what);
 }
 // rows of a caller's array: by TMA where it can address them
 static int set_user_out(TpArgs &g, void *ptr, bool f32, int64_t rows, int cols, const char *what) {
-  TpOut &o = g.out[0];
+  TpOut &o = g.out[1];
   o.ptr = ptr;
   o.ld = cols;
   o.batch = rows * (int64_t)cols;
@@ -236,30 +235,28 @@ static int forward(const FeedForward &f, void *y, Carve &w) {
   PrepArgs prep;
   memset(&prep, 0, sizeof(prep));
   int64_t blocks = 0;
-  const Matrix x = take_matrix(w, prep, blocks, f.f32, f.x, f.M, f.C);
-  const Matrix wg = take_matrix(w, prep, blocks, f.f32, f.wg, f.C, f.H);
-  const Matrix wu = take_matrix(w, prep, blocks, f.f32, f.wu, f.C, f.H);
-  const Matrix wd = take_matrix(w, prep, blocks, f.f32, f.wd, f.H, f.C);
-  const Matrix h = new_matrix(w, f.f32, f.M, f.H, 1);
+  Matrix x = take_matrix(w, prep, blocks, f.f32, f.x, f.M, f.C);
+  Matrix wg = take_matrix(w, prep, blocks, f.f32, f.wg, f.C, f.H);
+  Matrix wu = take_matrix(w, prep, blocks, f.f32, f.wu, f.C, f.H);
+  Matrix wd = take_matrix(w, prep, blocks, f.f32, f.wd, f.H, f.C);
+  Matrix h = new_matrix(w, f.f32, f.M, f.H, 1);
   if (!w.base) return CMACE_OK;
-  int rc = run_prep(prep, blocks, f.st, f.what);
   const bool bf16 = !f.f32;
-  {
-    TpArgs g = new_args(f.M, f.H, f.status);
-    if (!rc) rc = set_operand(g.a[0], x, true, 128, bf16, f.what);
-    if (!rc) rc = set_operand(g.b[0], wg, false, 64, bf16, f.what);
-    if (!rc) rc = set_operand(g.b[1], wu, false, 64, bf16, f.what);
-    if (!rc) rc = set_hidden_out(g, h, 64, bf16, f.what);
-    g.kblocks[0] = blocks64(f.C);
-    if (!rc) rc = launch_hidden<TP_GATED>(f, g);
-  }
-  TpArgs g = new_args(f.M, f.C, f.status);
-  const int tn = tile_columns(f.M, f.C, 1);
-  if (!rc) rc = set_operand(g.a[0], h, true, 128, bf16, f.what);
-  if (!rc) rc = set_operand(g.b[0], wd, false, 64, bf16, f.what);
-  if (!rc) rc = set_user_out(g, y, f.f32, f.M, f.C, f.what);
+  int rc = run_prep(prep, blocks, f.st, f.what);
+  if (!rc) rc = encode_all({&x, &wg, &wu, &wd, &h}, bf16, f.what);
+  TpArgs g = new_args(f.M, f.H, f.status);
+  set_operand(g.a[0], x, true);
+  set_operand(g.b[0], wg, false);
+  set_operand(g.b[1], wu, false);
+  g.kblocks[0] = blocks64(f.C);
+  if (!rc) rc = set_hidden_out(g, h, 64, bf16, f.what);
+  if (!rc) rc = launch_hidden<TP_GATED>(f, g);
+  g = new_args(f.M, f.C, f.status);
+  set_operand(g.a[0], h, true);
+  set_operand(g.b[0], wd, false);
   g.kblocks[0] = blocks64(f.H);
-  if (!rc) rc = launch_plain(f.f32, tn, g, f.st, f.what);
+  if (!rc) rc = set_user_out(g, y, f.f32, f.M, f.C, f.what);
+  if (!rc) rc = launch_plain(f.f32, tile_columns(f.M, f.C, 1), g, f.st, f.what);
   return rc;
 }
 
@@ -267,65 +264,53 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   PrepArgs prep;
   memset(&prep, 0, sizeof(prep));
   int64_t blocks = 0;
-  const Matrix x = take_matrix(w, prep, blocks, f.f32, f.x, f.M, f.C);
-  const Matrix wg = take_matrix(w, prep, blocks, f.f32, f.wg, f.C, f.H);
-  const Matrix wu = take_matrix(w, prep, blocks, f.f32, f.wu, f.C, f.H);
-  const Matrix wd = take_matrix(w, prep, blocks, f.f32, f.wd, f.H, f.C);
-  const Matrix gy = take_matrix(w, prep, blocks, f.f32, f.gy, f.M, f.C);
-  const Matrix hidden = new_matrix(w, f.f32, f.M, f.H, 3);   // dg, du, h
+  Matrix x = take_matrix(w, prep, blocks, f.f32, f.x, f.M, f.C);
+  Matrix wg = take_matrix(w, prep, blocks, f.f32, f.wg, f.C, f.H);
+  Matrix wu = take_matrix(w, prep, blocks, f.f32, f.wu, f.C, f.H);
+  Matrix wd = take_matrix(w, prep, blocks, f.f32, f.wd, f.H, f.C);
+  Matrix gy = take_matrix(w, prep, blocks, f.f32, f.gy, f.M, f.C);
+  Matrix hidden = new_matrix(w, f.f32, f.M, f.H, 3);   // dg, du, h
   const int64_t ld = up(f.H, 4);
   const int tn = f.H > 128 ? 256 : 128;
   const int splits = weight_splits(f.M, f.C, f.H, tn);
   float *partial = want_w ? w.take<float>((int64_t)splits * 3 * f.C * ld) : nullptr;
   if (!w.base) return CMACE_OK;
-  int rc = run_prep(prep, blocks, f.st, f.what);
   const bool bf16 = !f.f32;
-  {
-    TpArgs g = new_args(f.M, f.H, f.status);
-    if (!rc) rc = set_operand(g.a[0], x, true, 128, bf16, f.what);
-    if (!rc) rc = set_operand(g.a[1], gy, true, 128, bf16, f.what);
-    if (!rc) rc = set_operand(g.b[0], wg, false, 64, bf16, f.what);
-    if (!rc) rc = set_operand(g.b[1], wu, false, 64, bf16, f.what);
-    if (!rc) rc = set_operand(g.b[2], wd, true, 64, bf16, f.what);
-    if (!rc) rc = set_hidden_out(g, hidden, 32, bf16, f.what);
-    g.segments = 2;
-    g.kblocks[0] = g.kblocks[1] = blocks64(f.C);
-    if (!rc) rc = launch_hidden<TP_BACK>(f, g);
-  }
-  const auto part = [&](int p) {   // one of the three hidden arrays as a matrix of its own
-    Matrix m = hidden;
-    m.batches = 1;
-    m.hi = static_cast<uint16_t *>(hidden.hi) + p * hidden.rows * hidden.ld;
-    if (hidden.lo) {
-      m.lo = static_cast<uint16_t *>(hidden.lo) + p * hidden.rows * hidden.ld;
-      m.scale = hidden.scale + p * hidden.blocks_m() * hidden.blocks_n();
-    }
-    return m;
-  };
+  int rc = run_prep(prep, blocks, f.st, f.what);
+  if (!rc) rc = encode_all({&x, &wg, &wu, &wd, &gy, &hidden}, bf16, f.what);
+  TpArgs g = new_args(f.M, f.H, f.status);
+  set_operand(g.a[0], x, true);
+  set_operand(g.a[1], gy, true);
+  set_operand(g.b[0], wg, false);
+  set_operand(g.b[1], wu, false);
+  set_operand(g.b[2], wd, true);
+  g.segments = 2;
+  g.kblocks[0] = g.kblocks[1] = blocks64(f.C);
+  if (!rc) rc = set_hidden_out(g, hidden, 32, bf16, f.what);
+  if (!rc) rc = launch_hidden<TP_BACK>(f, g);
   if (want_x) {
-    TpArgs g = new_args(f.M, f.C, f.status);
-    const int tx = tile_columns(f.M, f.C, 1);
-    if (!rc) rc = set_operand(g.a[0], part(0), true, 128, bf16, f.what);
-    if (!rc) rc = set_operand(g.a[1], part(1), true, 128, bf16, f.what);
-    if (!rc) rc = set_operand(g.b[0], wg, true, tx, bf16, f.what);
-    if (!rc) rc = set_operand(g.b[1], wu, true, tx, bf16, f.what);
-    if (!rc) rc = set_user_out(g, gx, f.f32, f.M, f.C, f.what);
+    g = new_args(f.M, f.C, f.status);
+    set_operand(g.a[0], hidden.part(0), true);
+    set_operand(g.a[1], hidden.part(1), true);
+    set_operand(g.b[0], wg, true);
+    set_operand(g.b[1], wu, true);
     g.segments = 2;
     g.kblocks[0] = g.kblocks[1] = blocks64(f.H);
-    if (!rc) rc = launch_plain(f.f32, tx, g, f.st, f.what);
+    if (!rc) rc = set_user_out(g, gx, f.f32, f.M, f.C, f.what);
+    if (!rc) rc = launch_plain(f.f32, tile_columns(f.M, f.C, 1), g, f.st, f.what);
   }
   if (want_w) {
     // batches dg, du and h: x^T dg, x^T du and, as its transpose, dy^T h
-    TpArgs g = new_args(f.C, f.H, f.status);
-    if (!rc) rc = set_operand(g.a[0], x, false, 64, bf16, f.what);
-    if (!rc) rc = set_operand(g.a[1], gy, false, 64, bf16, f.what);
-    if (!rc) rc = set_operand(g.b[0], hidden, false, 64, bf16, f.what);
+    g = new_args(f.C, f.H, f.status);
+    set_operand(g.a[0], x, false);
+    set_operand(g.a[1], gy, false);
+    set_operand(g.b[0], hidden, false);
     g.batches = 3;
     g.splits = splits;
     g.a_of_last = 1;
     g.kblocks[0] = blocks64(f.M);
-    g.out[0].use_map = 1;
-    if (!rc) rc = encode_tile_map(&g.out[0].map, partial, 4, false, f.H, f.C, (int64_t)splits * 3, ld, (int64_t)f.C * ld, 32, 32, f.what);
+    g.out[1].use_map = 1;
+    if (!rc) rc = encode_tile_map(&g.out[1].map, partial, 4, false, f.H, f.C, (int64_t)splits * 3, ld, (int64_t)f.C * ld, 32, 32, f.what);
     if (!rc) rc = launch_plain(f.f32, tn, g, f.st, f.what);
     WeightReduce r{partial, {gw[0], gw[1], gw[2]}, ld, splits, f.C, f.H};
     const dim3 grid((unsigned)((f.H + 31) / 32), (unsigned)((f.C + 31) / 32), 3);

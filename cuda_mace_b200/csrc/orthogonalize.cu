@@ -22,7 +22,8 @@ struct NsPrep {
   const void *src;
   double *partial;   // [count][chunks]
   float *x;          // [count][rows][ld]
-  __half *hi, *lo;   // [count][rows][ld]
+  __half *h;         // [count][terms][rows][ld]
+  int terms;
   int64_t count, rows;
   int cols, ld, chunks, bf16;
   double eps;
@@ -75,14 +76,11 @@ __global__ void __launch_bounds__(NS_THREADS) ns_prep_kernel(const NsPrep p) {
     const float v = ns_load(p.src, (m * p.rows + row) * p.cols + col, p.bf16) * inv;
     const int64_t at = (m * p.rows + row) * p.ld + col;
     p.x[at] = v;
-    if (p.lo) {
-      uint32_t h, l;
-      tp_split2(v * p.scale, 0.f, h, l);
-      p.hi[at] = __ushort_as_half((unsigned short)h);
-      p.lo[at] = __ushort_as_half((unsigned short)l);
-    } else {
-      p.hi[at] = __float2half_rn(v * p.scale);
-    }
+    const int64_t plane = p.rows * p.ld, to = m * p.terms * plane + row * p.ld + col;
+    uint32_t h, l;
+    tp_split2(v * p.scale, 0.f, h, l);
+    p.h[to] = __ushort_as_half((unsigned short)h);
+    if (p.terms == 2) p.h[to + plane] = __ushort_as_half((unsigned short)l);
   }
 }
 
@@ -437,15 +435,6 @@ struct NsCall {
   const char *what;
 };
 
-static int set_split_out(TpArgs &g, const Matrix &m, const char *what) {
-  const void *base[2] = {m.hi, m.lo};
-  for (int t = 0; t < (m.lo ? 2 : 1); t++) {
-    const int rc = encode_tile_map(&g.out[t].map, base[t], 2, false, m.cols, m.rows, m.batches, m.ld, m.rows * m.ld, 32, 32, what);
-    if (rc) return rc;
-    g.out[t].use_map = 1;
-  }
-  return CMACE_OK;
-}
 template <int KIND>
 static int launch_ns(bool pair, int tn, TpArgs &g, cudaStream_t st, const char *what) {
   if (tn == 256) return tp_launch<KIND, false, 256>(g, st, what);   // pairs: the sums and their handling do not fit 168 registers
@@ -481,7 +470,7 @@ static int run_fused(const NsCall &f, int cluster) {
   }
   const int smem = 2 * g.chunks * NSF_IMAGE + NSF_S_BYTES + (cluster > 1 ? 128 * 512 : 0) + 1024;
   const auto kernel = cluster > 1 ? ns_fused_kernel<true> : ns_fused_kernel<false>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (const int rc = cluster > 1 ? allow_smem<ns_fused_kernel<true>>(smem, f.what) : allow_smem<ns_fused_kernel<false>>(smem, f.what)) return rc;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = (unsigned)cluster, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
@@ -492,7 +481,7 @@ static int run_fused(const NsCall &f, int cluster) {
   cfg.stream = f.st;
   cfg.attrs = &attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, g);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, g);
   if (e != cudaSuccess) return fail(CMACE_ERR_CUDA, "%s: %s", f.what, cudaGetErrorString(e));
   return check_launch(f.what);
 }
@@ -517,64 +506,67 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   double *partial = w.take<double>(f.count * chunks);
   Matrix x[2];
   for (Matrix &m : x) m = new_matrix(w, f.f32, f.rows, f.cols, f.count, 64, false);
-  const Matrix s = new_matrix(w, true, side, side, f.count, 64, false), poly = new_matrix(w, f.f32, side, side, f.count, 64, false);
-  float *master = w.take<float>(f.count * f.rows * x[0].ld);
+  Matrix s = new_matrix(w, true, side, side, f.count, 64, false), poly = new_matrix(w, f.f32, side, side, f.count, 64, false);
+  const int64_t ld = x[0].ld;
+  float *master = w.take<float>(f.count * f.rows * ld);
   if (!w.base) return CMACE_OK;
 
   double most = 1.0;   // bound of the singular values
   float sx = fp16_scale(most);
-  NsPrep p{f.src, partial, master, static_cast<__half *>(x[0].hi), static_cast<__half *>(x[0].lo), f.count, f.rows, f.cols, (int)x[0].ld, chunks,
-           f.f32 ? 0 : 1, f.eps, sx};
+  NsPrep p{f.src, partial, master, reinterpret_cast<__half *>(x[0].at), x[0].terms, f.count, f.rows, f.cols, (int)ld, chunks, f.f32 ? 0 : 1, f.eps, sx};
   launch_chained(ns_norm_kernel, dim3((unsigned)(f.count * chunks)), dim3(NS_THREADS), (size_t)0, f.st, p);
   launch_chained(ns_prep_kernel, dim3((unsigned)(f.count * ((f.rows + 31) / 32) * ((f.cols + 31) / 32))), dim3(NS_THREADS), (size_t)0, f.st, p);
   int rc = check_launch(f.what);
+  // maps, read and written: of X twice, S, P, the float32 X and the result
+  CUtensorMap to_x[2], to_s, to_poly;
+  TpOut to_master, to_out;
+  memset(&to_master, 0, sizeof(to_master));
+  memset(&to_out, 0, sizeof(to_out));
+  for (Matrix *m : {&x[0], &x[1], &s, &poly})
+    if (!rc) rc = encode_matrix(&m->map, *m, 64, 64, false, f.what);
+  for (int k = 0; k < 2 && !rc; k++) rc = encode_matrix(&to_x[k], x[k], 32, 32, false, f.what);
+  if (!rc) rc = encode_matrix(&to_s, s, 32, 32, false, f.what);
+  if (!rc) rc = encode_matrix(&to_poly, poly, 32, 32, false, f.what);
+  to_master.use_map = 1;
+  if (!rc) rc = encode_tile_map(&to_master.map, master, 4, false, f.cols, f.rows, f.count, ld, f.rows * ld, 32, 32, f.what);
+  const int bytes = f.f32 ? 4 : 2;
+  to_out.ptr = f.out, to_out.ld = f.cols, to_out.batch = n;
+  to_out.use_map = aligned16(f.out) && (int64_t)f.cols * bytes % 16 == 0;
+  if (!rc && to_out.use_map) rc = encode_tile_map(&to_out.map, f.out, bytes, !f.f32, f.cols, f.rows, f.count, f.cols, n, 32, 32, f.what);
+
   const int t_s = f.f32 ? 128 : tile_columns(side, side, f.count), t_x = f.f32 ? 128 : tile_columns(f.rows, f.cols, f.count);
   for (int step = 0; step < f.steps && !rc; step++) {
-    const Matrix &now = x[step & 1], &next = x[(step + 1) & 1];
-    const double most_s = most * most, most_p = most_square(f.b, f.c, most_s), most_next = most_odd(f.a, f.b, f.c, most);
-    const float ss = fp16_scale(most_s), sp = fp16_scale(most_p), sn = fp16_scale(most_next);
+    const Matrix &now = x[step & 1];
+    const double most_s = most * most, most_next = most_odd(f.a, f.b, f.c, most);
+    const float ss = fp16_scale(most_s), sp = fp16_scale(most_square(f.b, f.c, most_s)), sn = fp16_scale(most_next);
     const bool last = step + 1 == f.steps;
     TpArgs g = new_args(side, side, f.status);
     g.batches = (int)f.count;
     g.in_f16 = 1;
     g.kblocks[0] = blocks64(wide ? f.cols : f.rows);
-    if (!rc) rc = set_operand(g.a[0], now, wide, 128, false, f.what);
-    if (!rc) rc = set_operand(g.b[0], now, wide, t_s, false, f.what);
-    if (!rc) rc = set_split_out(g, s, f.what);
+    set_operand(g.a[0], now, wide);
+    set_operand(g.b[0], now, wide);
+    g.out[0].map = to_s;
     g.alpha = 1.0f / (sx * sx);
     g.pair_scale = ss;
-    if (!rc) rc = launch_ns<TP_GRAM>(f.f32, t_s, g, f.st, f.what);
+    rc = launch_ns<TP_GRAM>(f.f32, t_s, g, f.st, f.what);
 
     g.kblocks[0] = blocks64(side);
-    if (!rc) rc = set_operand(g.a[0], s, true, 128, false, f.what);
-    if (!rc) rc = set_operand(g.b[0], s, true, t_s, false, f.what);
-    if (!rc) rc = set_split_out(g, poly, f.what);
-    g.cin[0] = s.hi, g.cin[1] = s.lo, g.cin_ld = s.ld, g.cin_batch = side * s.ld;
+    set_operand(g.a[0], s, true);
+    set_operand(g.b[0], s, true);
+    g.out[0].map = to_poly;
+    g.cin = s.at, g.cin_ld = s.ld, g.cin_batch = 2 * s.plane(), g.cin_lo = s.plane();
     g.alpha = (float)f.c / (ss * ss), g.beta = (float)f.b / ss, g.pair_scale = sp;
     if (!rc) rc = launch_ns<TP_POLY>(f.f32, t_s, g, f.st, f.what);
 
     g.rows = f.rows, g.cols = f.cols;
-    if (wide) {
-      if (!rc) rc = set_operand(g.a[0], poly, true, 128, false, f.what);
-      if (!rc) rc = set_operand(g.b[0], now, false, 64, false, f.what);
-    } else {
-      if (!rc) rc = set_operand(g.a[0], now, true, 128, false, f.what);
-      if (!rc) rc = set_operand(g.b[0], poly, true, t_x, false, f.what);
-    }
-    if (!rc) rc = set_split_out(g, next, f.what);
-    g.cin[0] = master, g.cin_ld = now.ld, g.cin_batch = f.rows * now.ld;
+    set_operand(g.a[0], wide ? poly : now, true);
+    set_operand(g.b[0], wide ? now : poly, !wide);
+    g.out[0].map = to_x[(step + 1) & 1];
+    g.out[1] = last ? to_out : to_master;
+    g.out_bf16 = last && !f.f32;
+    g.cin = master, g.cin_ld = ld, g.cin_batch = f.rows * ld;
     g.alpha = 1.0f / (sp * sx), g.beta = (float)f.a, g.pair_scale = last ? 0.f : sn;
-    TpOut &o = g.out[2];
-    if (last) {
-      const int bytes = f.f32 ? 4 : 2;
-      o.ptr = f.out, o.ld = f.cols, o.batch = n;
-      o.use_map = aligned16(f.out) && (int64_t)f.cols * bytes % 16 == 0;
-      g.out_bf16 = !f.f32;
-      if (!rc && o.use_map) rc = encode_tile_map(&o.map, f.out, bytes, !f.f32, f.cols, f.rows, f.count, f.cols, n, 32, 32, f.what);
-    } else {
-      o.use_map = 1;
-      if (!rc) rc = encode_tile_map(&o.map, master, 4, false, f.cols, f.rows, f.count, now.ld, f.rows * now.ld, 32, 32, f.what);
-    }
     if (!rc) rc = launch_ns<TP_APPLY>(f.f32, t_x, g, f.st, f.what);
     most = most_next;
     sx = sn;

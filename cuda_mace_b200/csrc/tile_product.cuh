@@ -26,6 +26,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cstring>
 
 #include "common.cuh"
@@ -45,11 +46,11 @@ enum TpKind { TP_PLAIN, TP_GATED, TP_BACK, TP_GRAM, TP_POLY, TP_APPLY };
 enum TpAct { TP_SILU = 0, TP_GELU = 1 };
 
 struct TpOperand {
-  CUtensorMap map[2];      // 16-bit values, or hi and lo
+  CUtensorMap map;         // [z][rows][columns] in boxes of 64 x 64: one map whichever index is contracted
   const float *scale;      // PAIR: inverse scales of the blocks (1 / scale), null where there are none
   int64_t sc_i, sc_k, sc_b;  // their strides over blocks of the free index, of k, and over batches
   int mn_major;            // the contracted index is the outer one
-  int batched;             // coordinates take the batch index
+  int z0, zstep;           // hi (or the values) of batch b is matrix z0 + b zstep, lo the one behind it
 };
 
 struct TpOut {
@@ -61,11 +62,11 @@ struct TpOut {
 
 struct TpArgs {
   TpOperand a[2], b[3];
-  TpOut out[4];
+  TpOut out[2];                  // 16-bit values, hi and lo; results (and APPLY's float32)
   float *out_scale[3];           // PAIR outputs with block scales: inverse scale of every 64 x 64 block
   int64_t out_scale_ld, out_scale_batch;
-  const void *cin[2];            // POLY: the Gram matrix (16-bit, or hi and lo); APPLY: X in float32
-  int64_t cin_ld, cin_batch;
+  const void *cin;               // POLY: S (hi, and cin_lo elements behind it lo); APPLY: X in float32
+  int64_t cin_ld, cin_batch, cin_lo;
   float alpha, beta, cin_scale, pair_scale;   // D = alpha * product + beta * cin / ..., see the epilogues
   int32_t *status;
   int64_t rows, cols;            // of the output
@@ -289,7 +290,6 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         for (int seg = 0; ok && seg < g.segments; seg++) {
           const bool last = g.a_of_last && T.batch == g.batches - 1;
           const TpOperand &A = g.a[last ? 1 : seg];
-          const int a_batch = A.batched ? T.batch : 0;
           int k0, k1;
           tp_range(g, T.split, seg, k0, k1);
           constexpr int PARTS0 = KIND == TP_GATED || KIND == TP_BACK ? 2 : 1;
@@ -305,27 +305,20 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             }
             const uint32_t bar = full + 8 * stage, sA = smem + (uint32_t)(stage * S::STAGE);
             const uint32_t sB = sA + TERMS * S::A_BYTES;
+            const int k = kb * 64;
             mbar_arrive_expect_tx(bar, bytes);
+            // a box is 64 rows of 128 bytes, of the free index (K-major) or of k (MN-major)
+            const auto copy = [&](const TpOperand &o, uint32_t to, int at, int term) {
+              tma_load_3d(to, &o.map, o.mn_major ? at : k, o.mn_major ? k : at, o.z0 + T.batch * o.zstep + term, bar);
+            };
 #pragma unroll
             for (int term = 0; term < TERMS; term++) {
-              const uint32_t dA = sA + term * S::A_BYTES;
-              if (A.mn_major) {
-                tma_load_3d(dA, &A.map[term], (int)T.row0, kb * 64, a_batch, bar);
-                tma_load_3d(dA + 8192, &A.map[term], (int)T.row0 + 64, kb * 64, a_batch, bar);
-              } else {
-                tma_load_3d(dA, &A.map[term], kb * 64, (int)T.row0, a_batch, bar);
-              }
+              copy(A, sA + term * S::A_BYTES, (int)T.row0, term);
+              copy(A, sA + term * S::A_BYTES + 8192, (int)T.row0 + 64, term);
               for (int p = 0; p < parts; p++) {
-                const TpOperand &B = g.b[first + p];
-                const int b_batch = B.batched ? T.batch : 0;
-                const uint32_t dB = sB + term * S::B_BYTES + (uint32_t)(p * PART_ROWS * 128);
-                if (B.mn_major) {
 #pragma unroll
-                  for (int i = 0; i < PART_ROWS / 64; i++)
-                    tma_load_3d(dB + 8192u * i, &B.map[term], T.n0 + 64 * i, kb * 64, b_batch, bar);
-                } else {
-                  tma_load_3d(dB, &B.map[term], kb * 64, T.n0, b_batch, bar);
-                }
+                for (int i = 0; i < PART_ROWS / 64; i++)
+                  copy(g.b[first + p], sB + term * S::B_BYTES + (uint32_t)(p * PART_ROWS * 128 + 8192 * i), T.n0 + 64 * i, term);
               }
             }
             used |= 1u << stage;
@@ -451,8 +444,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           const bool in_rows = row + lane < g.rows;
 #pragma unroll
           for (int c = 0; c < 8; c++) {
-            const uint4 *p = KIND == TP_APPLY ? reinterpret_cast<const uint4 *>(static_cast<const float *>(g.cin[0]) + from) + c
-                                              : reinterpret_cast<const uint4 *>(static_cast<const __half *>(g.cin[c >> 2]) + from) + (c & 3);
+            const uint4 *p = KIND == TP_APPLY ? reinterpret_cast<const uint4 *>(static_cast<const float *>(g.cin) + from) + c
+                                              : reinterpret_cast<const uint4 *>(static_cast<const __half *>(g.cin) + from + (c >> 2) * g.cin_lo) + (c & 3);
             cin[c] = in_rows ? __ldcg(p) : make_uint4(0, 0, 0, 0);
           }
         }
@@ -477,11 +470,11 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           const TpOperand &B1 = g.b[KIND == TP_GATED || (KIND == TP_BACK && seg == 0) ? 1 : (KIND == TP_BACK ? 2 : seg)];
           // scales: one block of rows a warp; two blocks of columns at most: of both projections (GATED, BACK), or side by side
           const int cb = T.n0 / 64 + (KIND == TP_GATED ? half : (KIND == TP_BACK ? 0 : half * (TN / 128)));
-          const float *pa = A.scale ? A.scale + (A.batched ? T.batch * A.sc_b : 0) + (row >> 6) * A.sc_i : nullptr;
-          const float *pb0 = B0.scale ? B0.scale + (B0.batched ? T.batch * B0.sc_b : 0) + cb * B0.sc_i : nullptr;
+          const float *pa = A.scale ? A.scale + T.batch * A.sc_b + (row >> 6) * A.sc_i : nullptr;
+          const float *pb0 = B0.scale ? B0.scale + T.batch * B0.sc_b + cb * B0.sc_i : nullptr;
           const bool two = KIND == TP_GATED || (KIND == TP_BACK && seg == 0) || TN == 256;
           const float *pb1 = !two ? pb0 : (KIND == TP_GATED || KIND == TP_BACK
-                                 ? (B1.scale ? B1.scale + (B1.batched ? T.batch * B1.sc_b : 0) + cb * B1.sc_i : nullptr)
+                                 ? (B1.scale ? B1.scale + T.batch * B1.sc_b + cb * B1.sc_i : nullptr)
                                  : (pb0 && (cb + 1) * 64 < g.cols ? pb0 + B0.sc_i : pb0));   // past the last block: zeros in any scale
           const bool a_rows = row < g.rows;   // a warp of rows past the end has zeros and no scale
           const bool b_cols = (int64_t)cb * 64 < g.cols;
@@ -565,7 +558,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           st.send(&g.out[0].map, 0, col, row, 0);
           st.begin();
           st.put(0, lo);
-          st.send(&g.out[1].map, 0, col, row, 0);
+          st.send(&g.out[0].map, 0, col, row, 1);
         } else {
           uint32_t w[32];
 #pragma unroll
@@ -633,8 +626,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           const uint32_t where = PAIR ? 0u : (p == 1 ? 2048u : 0u);
           st.put(where, w);
           if (PAIR) st.put(2048, lo);
-          st.send(&g.out[0].map, where, col, row, p);
-          if (PAIR) st.send(&g.out[1].map, 2048, col, row, p);
+          st.send(&g.out[0].map, where, col, row, TERMS * p);
+          if (PAIR) st.send(&g.out[0].map, 2048, col, row, TERMS * p + 1);
         }
       } else if constexpr (KIND == TP_PLAIN) {
         const int batch = T.split * g.batches + T.batch;
@@ -652,8 +645,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             }
             st.begin();
             st.put(0, w);
-            if (g.out[0].use_map) st.send(&g.out[0].map, 0, col0 + 32 * i, row, batch);
-            else st.send_rows(g.out[0], true, col0 + 32 * i, row, batch);
+            if (g.out[1].use_map) st.send(&g.out[1].map, 0, col0 + 32 * i, row, batch);
+            else st.send_rows(g.out[1], true, col0 + 32 * i, row, batch);
           }
         } else {
 #pragma unroll
@@ -666,8 +659,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             for (int j = 0; j < 32; j++) w[j] = __float_as_uint(v[j]);
             st.begin();
             st.put(0, w);
-            if (g.out[0].use_map) st.send(&g.out[0].map, 0, col0 + 32 * i, row, batch);
-            else st.send_rows(g.out[0], false, col0 + 32 * i, row, batch);
+            if (g.out[1].use_map) st.send(&g.out[1].map, 0, col0 + 32 * i, row, batch);
+            else st.send_rows(g.out[1], false, col0 + 32 * i, row, batch);
           }
         }
       } else {
@@ -703,7 +696,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           }
           if (i + 1 < GROUPS && col + 32 < g.cols) fetch_cin(col + 32);   // on its way while this group is put down
           if (KIND == TP_APPLY) {
-            // out[2]: float32, the X of the next step or the result
+            // out[1]: float32, the X of the next step or the result
             if (!g.out_bf16) {
               uint32_t w[32];
 #pragma unroll
@@ -711,18 +704,18 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               if (PAIR) st.begin();
               else st.begin_but_last();   // the pairs' piece may still be read
               st.put(0, w);
-              if (g.out[2].use_map) st.send(&g.out[2].map, 0, col, row, T.batch);
-              else st.send_rows(g.out[2], false, col, row, T.batch);
-            } else if (g.out[2].use_map) {
+              if (g.out[1].use_map) st.send(&g.out[1].map, 0, col, row, T.batch);
+              else st.send_rows(g.out[1], false, col, row, T.batch);
+            } else if (g.out[1].use_map) {
               uint32_t w[16];
 #pragma unroll
               for (int j = 0; j < 16; j++) w[j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
               st.begin();
               st.put(0, w);
-              st.send(&g.out[2].map, 0, col, row, T.batch);
+              st.send(&g.out[1].map, 0, col, row, T.batch);
             } else {
               __nv_bfloat16 *o =
-                  static_cast<__nv_bfloat16 *>(g.out[2].ptr) + (int64_t)T.batch * g.out[2].batch + (row + lane) * g.out[2].ld + col;
+                  static_cast<__nv_bfloat16 *>(g.out[1].ptr) + (int64_t)T.batch * g.out[1].batch + (row + lane) * g.out[1].ld + col;
 #pragma unroll
               for (int j = 0; j < 32; j++)
                 if (row + lane < g.rows && col + j < g.cols) o[j] = __float2bfloat16_rn(v[j]);
@@ -741,8 +734,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             else st.begin_but_last();   // this group's float32 piece may still be read
             st.put(where, w);
             if (LOW) st.put(where + 2048, lo);
-            st.send(&g.out[0].map, where, col, row, T.batch);
-            if (LOW) st.send(&g.out[1].map, where + 2048, col, row, T.batch);
+            st.send(&g.out[0].map, where, col, row, (LOW ? 2 : 1) * T.batch);
+            if (LOW) st.send(&g.out[0].map, where + 2048, col, row, 2 * T.batch + 1);
           }
         }
       }
@@ -767,6 +760,19 @@ int encode_tile_map(CUtensorMap *map, const void *base, int bytes, bool bf16, in
                     int64_t batch_stride, int box_cols, int box_rows, const char *what);
 
 // ---- layout of a call's workspace -------------------------------------------------------------------------------------------
+// Dynamic shared memory a kernel may ask for: said once a device, to at least `bytes`
+template <auto KERNEL>
+int allow_smem(int bytes, const char *what) {
+  static std::atomic<int> allowed[64];
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && (device < 0 || device >= 64 || allowed[device].load(std::memory_order_relaxed) < bytes)) {
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && device >= 0 && device < 64) allowed[device].store(bytes, std::memory_order_relaxed);
+  }
+  return e == cudaSuccess ? CMACE_OK : fail(CMACE_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 struct Carve {   // consecutive pieces of the workspace; without a base it only counts
@@ -780,43 +786,45 @@ struct Carve {   // consecutive pieces of the workspace; without a base it only 
   }
 };
 
-// a matrix [batches][rows][cols] as an operand of the products
+// Matrices [batches][rows][cols] as operands of the products, rows ld elements apart; pairs as [batches][hi, lo][rows][cols].
 struct Matrix {
-  void *hi = nullptr, *lo = nullptr;
-  float *scale = nullptr;
+  CUtensorMap map;         // read in boxes of 64 x 64
+  uint16_t *at = nullptr;
+  float *scale = nullptr;  // inverse scales of the pairs' blocks, [batches][blocks_m][blocks_n]
   int64_t rows = 0, ld = 0, batches = 1;
-  int cols = 0;
+  int cols = 0, terms = 1, z0 = 0;
   int64_t blocks_m() const { return (rows + 63) / 64; }
   int64_t blocks_n() const { return (cols + 63) / 64; }
+  int64_t plane() const { return rows * ld; }   // elements of a matrix
+  Matrix part(int p) const {                    // one of the batches
+    Matrix m = *this;
+    m.batches = 1, m.z0 = z0 + p * terms;
+    if (scale) m.scale = scale + p * blocks_m() * blocks_n();
+    return m;
+  }
 };
-
-// values apart by rows of a multiple of `align` elements; PAIR values with or without scales of their blocks
+inline int encode_matrix(CUtensorMap *map, const Matrix &m, int box_cols, int box_rows, bool bf16, const char *what) {
+  return encode_tile_map(map, m.at, 2, bf16, m.cols, m.rows, m.batches * m.terms, m.ld, m.plane(), box_cols, box_rows, what);
+}
+// in the workspace, rows of a multiple of `align` elements; pairs with or without scales of their blocks
 inline Matrix new_matrix(Carve &w, bool pair, int64_t rows, int cols, int64_t batches, int align = 8, bool scales = true) {
   Matrix m;
-  m.rows = rows, m.cols = cols, m.batches = batches, m.ld = up(cols, align);
-  m.hi = w.take<uint16_t>(batches * rows * m.ld);
-  if (pair) {
-    m.lo = w.take<uint16_t>(batches * rows * m.ld);
-    if (scales) m.scale = w.take<float>(batches * m.blocks_m() * m.blocks_n());
-  }
+  m.rows = rows, m.cols = cols, m.batches = batches, m.ld = up(cols, align), m.terms = pair ? 2 : 1;
+  m.at = w.take<uint16_t>(batches * m.terms * m.plane());
+  if (pair && scales) m.scale = w.take<float>(batches * m.blocks_m() * m.blocks_n());
   return m;
 }
-
-// m as an operand: k_inner: the contracted index runs along a row; box_rows: rows (of the free index) a copy takes then
-inline int set_operand(TpOperand &o, const Matrix &m, bool k_inner, int box_rows, bool bf16, const char *what) {
+// k_inner: the contracted index runs along a row
+inline void set_operand(TpOperand &o, const Matrix &m, bool k_inner) {
+  o.map = m.map;
   o.mn_major = !k_inner;
-  o.batched = m.batches > 1;
+  o.z0 = m.z0, o.zstep = m.batches > 1 ? m.terms : 0;
   o.scale = m.scale;
   o.sc_i = k_inner ? m.blocks_n() : 1;
   o.sc_k = k_inner ? 1 : m.blocks_n();
-  o.sc_b = m.blocks_m() * m.blocks_n();
-  const void *base[2] = {m.hi, m.lo};
-  for (int t = 0; t < (m.lo ? 2 : 1); t++) {
-    const int rc = encode_tile_map(&o.map[t], base[t], 2, bf16, m.cols, m.rows, m.batches, m.ld, m.rows * m.ld, 64, k_inner ? box_rows : 64, what);
-    if (rc) return rc;
-  }
-  return CMACE_OK;
+  o.sc_b = m.batches > 1 ? m.blocks_m() * m.blocks_n() : 0;
 }
+
 inline TpArgs new_args(int64_t rows, int64_t cols, int32_t *status) {
   TpArgs g;
   memset(&g, 0, sizeof(g));
@@ -837,8 +845,7 @@ int tp_launch(TpArgs &g, cudaStream_t st, const char *what) {
   g.total = (int64_t)g.mt * g.nt * g.batches * g.splits;
   if (g.total >= (int64_t)1 << 31) return fail(CMACE_ERR_UNSUPPORTED, "%s: too many tiles", what);
   const auto kernel = tile_product_kernel<KIND, PAIR, TN, ACT>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-  if (e != cudaSuccess) return fail(CMACE_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  if (const int rc = allow_smem<tile_product_kernel<KIND, PAIR, TN, ACT>>(S::SMEM, what)) return rc;
   const int grid = (int)(g.total < 148 ? g.total : 148);
   launch_chained(kernel, dim3(grid), dim3(TP_THREADS), (size_t)S::SMEM, st, g);
   return check_launch(what);

@@ -280,39 +280,40 @@ def _workspace(device, nbytes):
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
+def _gated_ff_forward(x, w_gate, w_up, w_down, activation):
+    C, H = w_gate.shape
+    M = x.numel() // C
+    y = torch.empty_like(x)
+    f32 = x.dtype == torch.float32
+    nbytes = _abi.call("cmace_gated_ff_workspace_bytes", f32, M, C, H, 0)
+    ws = _workspace(x.device, nbytes)
+    _abi.call("cmace_gated_ff_fwd_f32" if f32 else "cmace_gated_ff_fwd_bf16", x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+              w_down.data_ptr(), M, C, H, activation, y.data_ptr(), ws.data_ptr(), nbytes, _ptr(_status_tensor(x.device)),
+              _stream())
+    return y
+
+
 class _GatedFeedForwardFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation):
-        rows = x.reshape(-1, x.shape[-1]).contiguous()
-        weights = tuple(w.contiguous() for w in (w_gate, w_up, w_down))
-        M, C = rows.shape
-        H = weights[0].shape[1]
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        f32 = x.dtype == torch.float32
-        nbytes = _abi.call("cmace_gated_ff_workspace_bytes", int(f32), M, C, H, 0)
-        ws = _workspace(x.device, nbytes)
-        _abi.call("cmace_gated_ff_fwd_" + ("f32" if f32 else "bf16"), _ptr(rows), *map(_ptr, weights), M, C, H, activation,
-                  _ptr(y), _ptr(ws), nbytes, _ptr(_status_tensor(x.device)), _stream())
-        ctx.save_for_backward(rows, *weights)
+        ctx.save_for_backward(x, w_gate, w_up, w_down)
         ctx.activation = activation
-        return y
+        return _gated_ff_forward(x, w_gate, w_up, w_down, activation)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y):
-        rows, w_gate, w_up, w_down = ctx.saved_tensors
-        M, C = rows.shape
-        H = w_gate.shape[1]
+        saved = ctx.saved_tensors
+        x, w_gate = saved[:2]
+        C, H = w_gate.shape
+        M = x.numel() // C
         gy = grad_y.contiguous()
-        f32 = rows.dtype == torch.float32
-        need = ctx.needs_input_grad
-        grads = [torch.empty(grad_y.shape, dtype=rows.dtype, device=rows.device) if need[0] else None]
-        grads += [torch.empty_like(w) if n else None for w, n in zip((w_gate, w_up, w_down), need[1:4])]
-        nbytes = _abi.call("cmace_gated_ff_workspace_bytes", int(f32), M, C, H, 1)
-        ws = _workspace(rows.device, nbytes)
-        _abi.call("cmace_gated_ff_bwd_" + ("f32" if f32 else "bf16"), _ptr(rows), _ptr(w_gate), _ptr(w_up), _ptr(w_down),
-                  _ptr(gy), M, C, H, ctx.activation, *map(_ptr, grads), _ptr(ws), nbytes,
-                  _ptr(_status_tensor(rows.device)), _stream())
+        f32 = x.dtype == torch.float32
+        grads = [torch.empty_like(t) if need else None for t, need in zip(saved, ctx.needs_input_grad)]
+        nbytes = _abi.call("cmace_gated_ff_workspace_bytes", f32, M, C, H, 1)
+        ws = _workspace(x.device, nbytes)
+        _abi.call("cmace_gated_ff_bwd_f32" if f32 else "cmace_gated_ff_bwd_bf16", *map(_ptr, saved), gy.data_ptr(), M, C, H,
+                  ctx.activation, *map(_ptr, grads), ws.data_ptr(), nbytes, _ptr(_status_tensor(x.device)), _stream())
         return (*grads, None)
 
 
@@ -332,7 +333,10 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
     if x.shape[-1] != C or w_up.shape != (C, H) or w_down.shape != (H, C) or C < 1 or H < 1:
         raise RuntimeError(f"shape mismatch: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, "
                            f"w_down {tuple(w_down.shape)}")
-    return _GatedFeedForwardFunction.apply(x, w_gate, w_up, w_down, _ACTIVATIONS[activation])
+    operands = (x.contiguous(), w_gate.contiguous(), w_up.contiguous(), w_down.contiguous())
+    if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
+        return _GatedFeedForwardFunction.apply(*operands, _ACTIVATIONS[activation])
+    return _gated_ff_forward(*operands, _ACTIVATIONS[activation])
 
 
 class GatedFeedForward(torch.nn.Module):

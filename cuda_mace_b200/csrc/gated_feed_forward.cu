@@ -198,17 +198,23 @@ static int set_user_out(TpArgs &g, void *ptr, bool f32, int64_t rows, int cols, 
   return CMACE_OK;
 }
 
-template <int KIND, int ACT>
-static int launch_kind(bool pair, TpArgs &g, cudaStream_t st, const char *what) {
-  return pair ? tp_launch<KIND, true, 128, ACT>(g, st, what) : tp_launch<KIND, false, 128, ACT>(g, st, what);
+template <int ACT>
+static int launch_gated(const FeedForward &f, TpArgs &g) {
+  const bool pairs = pairs_fill(g.rows, g.cols, 1, 128);
+  if (f.f32) return pairs ? tp_launch<TP_GATED, true, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_GATED, true, 128, 1, ACT>(g, f.st, f.what);
+  return pairs ? tp_launch<TP_GATED, false, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_GATED, false, 128, 1, ACT>(g, f.st, f.what);
 }
-template <int KIND>
-static int launch_hidden(const FeedForward &f, TpArgs &g) {
-  return f.act == TP_SILU ? launch_kind<KIND, TP_SILU>(f.f32, g, f.st, f.what) : launch_kind<KIND, TP_GELU>(f.f32, g, f.st, f.what);
+template <int ACT>
+static int launch_back(const FeedForward &f, TpArgs &g) {
+  if (f.f32)
+    return pairs_fill(g.rows, g.cols, 1, 64) ? tp_launch<TP_BACK, true, 64, 2, ACT>(g, f.st, f.what) : tp_launch<TP_BACK, true, 64, 1, ACT>(g, f.st, f.what);
+  return pairs_fill(g.rows, g.cols, 1, 128) ? tp_launch<TP_BACK, false, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_BACK, false, 64, 1, ACT>(g, f.st, f.what);
 }
-static int launch_plain(bool pair, int tn, TpArgs &g, cudaStream_t st, const char *what) {
-  if (tn == 256) return pair ? tp_launch<TP_PLAIN, true, 256>(g, st, what) : tp_launch<TP_PLAIN, false, 256>(g, st, what);
-  return pair ? tp_launch<TP_PLAIN, true, 128>(g, st, what) : tp_launch<TP_PLAIN, false, 128>(g, st, what);
+static int launch_plain(bool pair, TpArgs &g, cudaStream_t st, const char *what) {
+  const int64_t times = (int64_t)g.batches * g.splits;
+  if (pair) return pairs_fill(g.rows, g.cols, times, 128) ? tp_launch<TP_PLAIN, true, 128, 2>(g, st, what) : tp_launch<TP_PLAIN, true, 128, 1>(g, st, what);
+  if (g.cols > 128 && pairs_fill(g.rows, g.cols, times, 256)) return tp_launch<TP_PLAIN, false, 256, 2>(g, st, what);
+  return pairs_fill(g.rows, g.cols, times, 128) ? tp_launch<TP_PLAIN, false, 128, 2>(g, st, what) : tp_launch<TP_PLAIN, false, 128, 1>(g, st, what);
 }
 
 static int run_prep(const PrepArgs &p, int64_t blocks, cudaStream_t st, const char *what) {
@@ -218,10 +224,10 @@ static int run_prep(const PrepArgs &p, int64_t blocks, cudaStream_t st, const ch
   return check_launch(what);
 }
 
-// Splits of the weight gradients' sum over M: rounds of tiles times the length of one, a few blocks of 64 rows for filling the ring
-// and handing over the sums, and the traffic of the partial sums.
-static int weight_splits(int64_t M, int C, int H, int tn) {
-  const int64_t tiles = 3 * ((C + 127) / 128) * (int64_t)((H + tn - 1) / tn), kb = blocks64(M);
+// Splits of the weight gradients' sum over M, by what a number costs in units of a block of 64 rows of one tile (0.3 to 0.5 us): rounds
+// of tiles, a few blocks each for filling the ring and putting the sums down, and the traffic of the partial sums.
+static int weight_splits(int64_t M, int C, int H) {
+  const int64_t tiles = 3 * ((C + 127) / 128) * (int64_t)((H + 127) / 128), kb = blocks64(M);
   int best = 1;
   double least = 0;
   for (int s = 1; s <= 64 && s <= kb; s++) {
@@ -250,13 +256,13 @@ static int forward(const FeedForward &f, void *y, Carve &w) {
   set_operand(g.b[1], wu, false);
   g.kblocks[0] = blocks64(f.C);
   if (!rc) rc = set_hidden_out(g, h, 64, bf16, f.what);
-  if (!rc) rc = launch_hidden<TP_GATED>(f, g);
+  if (!rc) rc = f.act == TP_SILU ? launch_gated<TP_SILU>(f, g) : launch_gated<TP_GELU>(f, g);
   g = new_args(f.M, f.C, f.status);
   set_operand(g.a[0], h, true);
   set_operand(g.b[0], wd, false);
   g.kblocks[0] = blocks64(f.H);
   if (!rc) rc = set_user_out(g, y, f.f32, f.M, f.C, f.what);
-  if (!rc) rc = launch_plain(f.f32, tile_columns(f.M, f.C, 1), g, f.st, f.what);
+  if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
   return rc;
 }
 
@@ -271,8 +277,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   Matrix gy = take_matrix(w, prep, blocks, f.f32, f.gy, f.M, f.C);
   Matrix hidden = new_matrix(w, f.f32, f.M, f.H, 3);   // dg, du, h
   const int64_t ld = up(f.H, 4);
-  const int tn = f.H > 128 ? 256 : 128;
-  const int splits = weight_splits(f.M, f.C, f.H, tn);
+  const int splits = weight_splits(f.M, f.C, f.H);
   float *partial = want_w ? w.take<float>((int64_t)splits * 3 * f.C * ld) : nullptr;
   if (!w.base) return CMACE_OK;
   const bool bf16 = !f.f32;
@@ -287,7 +292,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   g.segments = 2;
   g.kblocks[0] = g.kblocks[1] = blocks64(f.C);
   if (!rc) rc = set_hidden_out(g, hidden, 32, bf16, f.what);
-  if (!rc) rc = launch_hidden<TP_BACK>(f, g);
+  if (!rc) rc = f.act == TP_SILU ? launch_back<TP_SILU>(f, g) : launch_back<TP_GELU>(f, g);
   if (want_x) {
     g = new_args(f.M, f.C, f.status);
     set_operand(g.a[0], hidden.part(0), true);
@@ -297,7 +302,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
     g.segments = 2;
     g.kblocks[0] = g.kblocks[1] = blocks64(f.H);
     if (!rc) rc = set_user_out(g, gx, f.f32, f.M, f.C, f.what);
-    if (!rc) rc = launch_plain(f.f32, tile_columns(f.M, f.C, 1), g, f.st, f.what);
+    if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
   }
   if (want_w) {
     // batches dg, du and h: x^T dg, x^T du and, as its transpose, dy^T h
@@ -311,7 +316,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
     g.kblocks[0] = blocks64(f.M);
     g.out[1].use_map = 1;
     if (!rc) rc = encode_tile_map(&g.out[1].map, partial, 4, false, f.H, f.C, (int64_t)splits * 3, ld, (int64_t)f.C * ld, 32, 32, f.what);
-    if (!rc) rc = launch_plain(f.f32, tn, g, f.st, f.what);
+    if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
     WeightReduce r{partial, {gw[0], gw[1], gw[2]}, ld, splits, f.C, f.H};
     const dim3 grid((unsigned)((f.H + 31) / 32), (unsigned)((f.C + 31) / 32), 3);
     if (!rc) {

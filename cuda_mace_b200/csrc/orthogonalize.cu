@@ -112,20 +112,6 @@ struct NsFused {
   float sx[NSF_MAX_STEPS + 1], ss[NSF_MAX_STEPS], sp[NSF_MAX_STEPS];   // powers of two of X, S and P of every step
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
 __device__ __forceinline__ float4 peer_load4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
@@ -436,9 +422,11 @@ struct NsCall {
 };
 
 template <int KIND>
-static int launch_ns(bool pair, int tn, TpArgs &g, cudaStream_t st, const char *what) {
-  if (tn == 256) return tp_launch<KIND, false, 256>(g, st, what);   // pairs: the sums and their handling do not fit 168 registers
-  return pair ? tp_launch<KIND, true, 128>(g, st, what) : tp_launch<KIND, false, 128>(g, st, what);
+static int launch_ns(bool pair, TpArgs &g, cudaStream_t st, const char *what) {
+  const bool wide = !pair && g.cols > 128 && pairs_fill(g.rows, g.cols, g.batches, 256);
+  if (wide) return tp_launch<KIND, false, 256, 2>(g, st, what);
+  if (pairs_fill(g.rows, g.cols, g.batches, 128)) return pair ? tp_launch<KIND, true, 128, 2>(g, st, what) : tp_launch<KIND, false, 128, 2>(g, st, what);
+  return pair ? tp_launch<KIND, true, 128, 1>(g, st, what) : tp_launch<KIND, false, 128, 1>(g, st, what);
 }
 
 // CTAs a matrix for the kernel above, 0: it does not fit
@@ -534,7 +522,6 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   to_out.use_map = aligned16(f.out) && (int64_t)f.cols * bytes % 16 == 0;
   if (!rc && to_out.use_map) rc = encode_tile_map(&to_out.map, f.out, bytes, !f.f32, f.cols, f.rows, f.count, f.cols, n, 32, 32, f.what);
 
-  const int t_s = f.f32 ? 128 : tile_columns(side, side, f.count), t_x = f.f32 ? 128 : tile_columns(f.rows, f.cols, f.count);
   for (int step = 0; step < f.steps && !rc; step++) {
     const Matrix &now = x[step & 1];
     const double most_s = most * most, most_next = most_odd(f.a, f.b, f.c, most);
@@ -549,7 +536,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     g.out[0].map = to_s;
     g.alpha = 1.0f / (sx * sx);
     g.pair_scale = ss;
-    rc = launch_ns<TP_GRAM>(f.f32, t_s, g, f.st, f.what);
+    rc = launch_ns<TP_GRAM>(f.f32, g, f.st, f.what);
 
     g.kblocks[0] = blocks64(side);
     set_operand(g.a[0], s, true);
@@ -557,7 +544,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     g.out[0].map = to_poly;
     g.cin = s.at, g.cin_ld = s.ld, g.cin_batch = 2 * s.plane(), g.cin_lo = s.plane();
     g.alpha = (float)f.c / (ss * ss), g.beta = (float)f.b / ss, g.pair_scale = sp;
-    if (!rc) rc = launch_ns<TP_POLY>(f.f32, t_s, g, f.st, f.what);
+    if (!rc) rc = launch_ns<TP_POLY>(f.f32, g, f.st, f.what);
 
     g.rows = f.rows, g.cols = f.cols;
     set_operand(g.a[0], wide ? poly : now, true);
@@ -565,9 +552,10 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     g.out[0].map = to_x[(step + 1) & 1];
     g.out[1] = last ? to_out : to_master;
     g.out_bf16 = last && !f.f32;
+    g.cin_map = to_master.map;
     g.cin = master, g.cin_ld = ld, g.cin_batch = f.rows * ld;
     g.alpha = 1.0f / (sp * sx), g.beta = (float)f.a, g.pair_scale = last ? 0.f : sn;
-    if (!rc) rc = launch_ns<TP_APPLY>(f.f32, t_x, g, f.st, f.what);
+    if (!rc) rc = launch_ns<TP_APPLY>(f.f32, g, f.st, f.what);
     most = most_next;
     sx = sn;
   }

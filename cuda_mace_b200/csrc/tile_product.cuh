@@ -66,6 +66,7 @@ struct TpArgs {
   float *out_scale[3];           // PAIR outputs with block scales: inverse scale of every 64 x 64 block
   int64_t out_scale_ld, out_scale_batch;
   const void *cin;               // POLY: S (hi, and cin_lo elements behind it lo); APPLY: X in float32
+  CUtensorMap cin_map;           // APPLY of 16-bit operands: the same X in boxes of 32 x 32
   int64_t cin_ld, cin_batch, cin_lo;
   float alpha, beta, cin_scale, pair_scale;   // D = alpha * product + beta * cin / ..., see the epilogues
   int32_t *status;
@@ -87,6 +88,50 @@ __device__ __forceinline__ void umma_16(uint32_t d, uint64_t a, uint64_t b, uint
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+__device__ __forceinline__ void umma_16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// a pair's copies count on the first CTA's barrier, its products on both CTAs' (the same place in each)
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"((uint16_t)3)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 // Operand image of rows of 128 bytes with the 128-byte swizzle.  K-major: a row is 64 k of one i, groups of eight rows 1 024 bytes
 // apart.  MN-major: a row is 64 i of one k, groups of eight k 1 024 bytes apart (stride offset), runs of 64 i 8 192 (leading offset).
 __device__ __forceinline__ uint64_t tp_desc(uint32_t smem, int mn_major) {
@@ -94,19 +139,27 @@ __device__ __forceinline__ uint64_t tp_desc(uint32_t smem, int mn_major) {
          ((uint64_t)2 << 61);
 }
 // kind::f16: D float32, A and B fp16 (0) or bf16 (1) at bits 7 and 10, MN-major operands at bits 15 and 16
-__device__ __forceinline__ uint32_t tp_idesc(int n, int bf16, int a_mn, int b_mn) {
+__device__ __forceinline__ uint32_t tp_idesc(int n, int bf16, int a_mn, int b_mn, int m = 128) {
   return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-template <int KIND, bool PAIR, int TN>
+// TN: output columns of a tile.  CTAS = 2: a pair of CTAs works on one tile of 256 rows, each with its 128 rows of A and of the sum and
+// with half of B's columns in its shared memory, which the pair's MMAs read from both.
+template <int KIND, bool PAIR, int TN, int CTAS>
 struct TpShape {
-  static constexpr int B_ROWS = KIND == TP_BACK ? 128 : (KIND == TP_GATED ? 256 : TN);   // rows of B in a stage
-  static constexpr int OUT_N = KIND == TP_BACK ? 64 : (KIND == TP_GATED ? 128 : TN);     // output columns of a tile
+  // columns of B a segment: both projections' side by side; BACK's second segment has one's
+  static constexpr int N0 = KIND == TP_GATED || KIND == TP_BACK ? 2 * TN : TN, N1 = KIND == TP_BACK ? TN : N0;
+  static constexpr int B_ROWS = N0 / CTAS;                  // of a stage of a CTA
   static constexpr int A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128;
   static constexpr int STAGE = (A_BYTES + B_BYTES) * (PAIR ? 2 : 1);
-  // bytes an epilogue warp stages its output in: one piece of 32 rows of 128 bytes, or two where the stages leave room
-  static constexpr int STAGING = KIND >= TP_GRAM && !PAIR ? 8192 : 4096;
+  // BACK's sums of 128 columns do not fit twice: the second segment goes first, into columns that alternate, and the first waits
+  // for the epilogue of the tile before.
+  static constexpr bool LATE = KIND == TP_BACK && !PAIR && TN == 128;
+  static constexpr bool CIN_TMA = KIND == TP_APPLY && !PAIR;
+  // Bytes an epilogue warp stages its output in, pieces of 32 rows of 128 bytes; CIN_TMA: two for float32 values, which arrive, change and
+  // leave there, and half a piece for the 16-bit ones.
+  static constexpr int STAGING = CIN_TMA ? 2 * 4096 + 2048 : 4096;
   static constexpr int FIT = (TP_SMEM_BUDGET - 1024 - TP_EPILOGUE_WARPS * STAGING) / STAGE;
   static constexpr int STAGES = FIT < TP_MAX_STAGES ? FIT : TP_MAX_STAGES;
   static constexpr int SMEM = STAGE * STAGES + TP_EPILOGUE_WARPS * STAGING + 1024;
@@ -116,13 +169,13 @@ struct TpTile {
   int64_t row0;
   int n0, batch, split;
 };
-__device__ __forceinline__ TpTile tp_tile(const TpArgs &g, int64_t t, int out_n) {
+__device__ __forceinline__ TpTile tp_tile(const TpArgs &g, int64_t t, int out_n, int out_m) {
   TpTile T;
   const uint32_t u = (uint32_t)t, nt = (uint32_t)g.nt, mt = (uint32_t)g.mt;
   const uint32_t v = u / nt;
   T.n0 = (int)(u - v * nt) * out_n;
   const uint32_t w = v / mt;
-  T.row0 = (int64_t)(v - w * mt) * 128;
+  T.row0 = (int64_t)(v - w * mt) * out_m;
   T.split = (int)(w / (uint32_t)g.batches);
   T.batch = (int)(w - (uint32_t)T.split * (uint32_t)g.batches);
   return T;
@@ -218,18 +271,18 @@ struct TpStager {
     __syncwarp();
     if (row < rows && col < cols && elect_one()) tma_store_3d(map, col, (int)row, batch, smem + at);
   }
-  __device__ __forceinline__ uint32_t word(int row, int w) const {
+  __device__ __forceinline__ uint32_t word(uint32_t piece, int row, int w) const {
     uint32_t v;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(smem + (uint32_t)sw128_offset(row, w >> 2) + 4u * (uint32_t)(w & 3)) : "memory");
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(smem + piece + (uint32_t)sw128_offset(row, w >> 2) + 4u * (uint32_t)(w & 3)) : "memory");
     return v;
   }
   // rows that TMA cannot address: 32 float32 columns (one a lane) or 64 16-bit ones (two a lane)
-  __device__ __forceinline__ void send_rows(const TpOut &o, bool sixteen, int col, int64_t row, int batch) const {
+  __device__ __forceinline__ void send_rows(const TpOut &o, bool sixteen, uint32_t piece, int col, int64_t row, int batch) const {
     __syncwarp();
     const int64_t base = (int64_t)batch * o.batch;
     const int n = rows - row < 32 ? (int)(rows - row) : 32;
     for (int r = 0; r < n; r++) {
-      const uint32_t v = word(r, lane);
+      const uint32_t v = word(piece, r, lane);
       const int64_t at = base + (row + r) * o.ld + col;
       if (!sixteen) {
         if (col + lane < cols) static_cast<uint32_t *>(o.ptr)[at + lane] = v;
@@ -243,13 +296,13 @@ struct TpStager {
   }
 };
 
-template <int KIND, bool PAIR, int TN, int ACT>
+template <int KIND, bool PAIR, int TN, int CTAS, int ACT>
 __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __grid_constant__ TpArgs g) {
-  using S = TpShape<KIND, PAIR, TN>;
+  using S = TpShape<KIND, PAIR, TN, CTAS>;
   constexpr int TERMS = PAIR ? 2 : 1;
-  constexpr int STAGES = S::STAGES;
+  constexpr int STAGES = S::STAGES, ROWS = 128 * CTAS;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 5];
+  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 5 + TP_EPILOGUE_WARPS];
   __shared__ uint32_t tmem_base_slot;
   __shared__ float block_most[3][TP_EPILOGUE_WARPS];   // GATED: of alternating tiles; BACK: of the three outputs
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -258,6 +311,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
   const uint32_t acc_full = smem_u32(&bars[2 * TP_MAX_STAGES]), acc_empty = smem_u32(&bars[2 * TP_MAX_STAGES + 2]);
   const uint32_t drain = smem_u32(&bars[2 * TP_MAX_STAGES + 4]);
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int rank = CTAS == 2 ? (int)cluster_rank() : 0;
+  const int64_t first_tile = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) {
@@ -265,15 +320,21 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       mbar_init(empty + 8 * s, 1);   // one commit
     }
     for (int b = 0; b < 2; b++) {
-      mbar_init(acc_full + 8 * b, 1);                    // one commit
-      mbar_init(acc_empty + 8 * b, TP_EPILOGUE_WARPS);   // one arrival a warp
+      mbar_init(acc_full + 8 * b, 1);                           // one commit
+      mbar_init(acc_empty + 8 * b, CTAS * TP_EPILOGUE_WARPS);   // one arrival a warp
     }
     mbar_init(drain, 1);
+    for (int w = 0; w < TP_EPILOGUE_WARPS; w++) mbar_init(drain + 8 + 8 * w, 1);   // a warp's own copies
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == TP_EPILOGUE_WARPS) tmem_alloc(smem_u32(&tmem_base_slot), 512);
+  if (warp == TP_EPILOGUE_WARPS) {
+    if (CTAS == 2) tmem_alloc_pair(smem_u32(&tmem_base_slot), 512);
+    else tmem_alloc(smem_u32(&tmem_base_slot), 512);
+  }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  if (CTAS == 2) cluster_sync();   // the other CTA's barriers
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = (uint32_t)uniform((int)tmem_base_slot);
   grid_wait();
@@ -285,40 +346,47 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       int stage = 0;
       uint32_t phase = 0, used = 0;   // used: bit per stage that has been filled at least once
       bool ok = true;
-      for (int64_t t = blockIdx.x; ok && t < g.total; t += gridDim.x) {
-        const TpTile T = tp_tile(g, t, S::OUT_N);
-        for (int seg = 0; ok && seg < g.segments; seg++) {
+      const uint32_t first_full = CTAS == 2 ? peer_smem(full, 0) : full;
+      for (int64_t t = first_tile; ok && t < g.total; t += tile_step) {
+        const TpTile T = tp_tile(g, t, TN, ROWS);
+        for (int i = 0; ok && i < g.segments; i++) {
+          const int seg = S::LATE ? 1 - i : i;
           const bool last = g.a_of_last && T.batch == g.batches - 1;
           const TpOperand &A = g.a[last ? 1 : seg];
           int k0, k1;
           tp_range(g, T.split, seg, k0, k1);
-          constexpr int PARTS0 = KIND == TP_GATED || KIND == TP_BACK ? 2 : 1;
-          const int parts = KIND == TP_BACK && seg == 1 ? 1 : PARTS0;
-          const int first = KIND == TP_BACK ? 2 * seg : (KIND == TP_GATED ? 0 : seg);
-          constexpr int PART_ROWS = KIND == TP_BACK ? 64 : (KIND == TP_GATED ? 128 : TN);
-          const uint32_t bytes = (uint32_t)(TERMS * (S::A_BYTES + parts * PART_ROWS * 128));
+          const int rows = (seg == 0 ? S::N0 : S::N1) / CTAS;   // of B; 32 are copied as 64
+          const int boxes = (rows + 63) / 64;
+          const uint32_t bytes = (uint32_t)(CTAS * TERMS * (S::A_BYTES + boxes * 8192));
+          const int row0 = (int)T.row0 + 128 * rank;
           for (int kb = k0; kb < k1; kb++) {
             if (!mbar_wait(empty + 8 * stage, phase ^ 1)) {
               tp_report(g, 40);
               ok = false;
               break;
             }
-            const uint32_t bar = full + 8 * stage, sA = smem + (uint32_t)(stage * S::STAGE);
+            const uint32_t bar = first_full + 8 * stage, sA = smem + (uint32_t)(stage * S::STAGE);
             const uint32_t sB = sA + TERMS * S::A_BYTES;
             const int k = kb * 64;
-            mbar_arrive_expect_tx(bar, bytes);
+            if (rank == 0) mbar_arrive_expect_tx(full + 8 * stage, bytes);
             // a box is 64 rows of 128 bytes, of the free index (K-major) or of k (MN-major)
             const auto copy = [&](const TpOperand &o, uint32_t to, int at, int term) {
-              tma_load_3d(to, &o.map, o.mn_major ? at : k, o.mn_major ? k : at, o.z0 + T.batch * o.zstep + term, bar);
+              const int x = o.mn_major ? at : k, y = o.mn_major ? k : at, z = o.z0 + T.batch * o.zstep + term;
+              if (CTAS == 2) tma_load_3d_pair(to, &o.map, x, y, z, bar);
+              else tma_load_3d(to, &o.map, x, y, z, bar);
             };
 #pragma unroll
             for (int term = 0; term < TERMS; term++) {
-              copy(A, sA + term * S::A_BYTES, (int)T.row0, term);
-              copy(A, sA + term * S::A_BYTES + 8192, (int)T.row0 + 64, term);
-              for (int p = 0; p < parts; p++) {
-#pragma unroll
-                for (int i = 0; i < PART_ROWS / 64; i++)
-                  copy(g.b[first + p], sB + term * S::B_BYTES + (uint32_t)(p * PART_ROWS * 128 + 8192 * i), T.n0 + 64 * i, term);
+              copy(A, sA + term * S::A_BYTES, row0, term);
+              copy(A, sA + term * S::A_BYTES + 8192, row0 + 64, term);
+              for (int b = 0; b < boxes; b++) {
+                const int n = rank * rows + 64 * b;   // column of the segment's B
+                int which = seg, at = n;
+                if (KIND == TP_GATED || KIND == TP_BACK) {
+                  which = seg == 1 ? 2 : n / TN;
+                  at = seg == 1 ? n : n - which * TN;
+                }
+                copy(g.b[which], sB + term * S::B_BYTES + (uint32_t)(8192 * b), T.n0 + at, term);
               }
             }
             used |= 1u << stage;
@@ -329,20 +397,28 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           }
         }
       }
-      if (!ok) {   // no copy outlives the block: the fills that nobody took
+      if (!ok && rank == 0) {   // no copy outlives the block: the fills that nobody took
         for (int s = 0; s < STAGES; s++)
           if (used >> s & 1) mbar_wait(full + 8 * s, s < stage ? phase : phase ^ 1);
       }
     }
   } else if (warp == TP_EPILOGUE_WARPS + 1) {
     // ================================ products ================================
-    if (elect_one()) {
+    if (rank == 0 && elect_one()) {
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase[2] = {0, 0};
       bool ok = true;
       const int bf16 = g.in_f16 || PAIR ? 0 : 1;
-      for (int64_t t = blockIdx.x; ok && t < g.total; t += gridDim.x) {
-        const TpTile T = tp_tile(g, t, S::OUT_N);
+      const auto product = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+        if (CTAS == 2) umma_16_pair(d, a, b, idesc, accumulate);
+        else umma_16(d, a, b, idesc, accumulate);
+      };
+      const auto commit = [&](uint32_t bar) {
+        if (CTAS == 2) umma_commit_pair(bar);
+        else umma_commit(bar);
+      };
+      for (int64_t t = first_tile; ok && t < g.total; t += tile_step) {
+        const TpTile T = tp_tile(g, t, TN, ROWS);
         if (!PAIR) {
           if (!mbar_wait(acc_empty + 8 * buf, buf_phase[buf] ^ 1)) {
             tp_report(g, 41);
@@ -351,16 +427,22 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           tc_fence_after();
         }
         uint32_t begun = 0;
-        for (int seg = 0; ok && seg < g.segments; seg++) {
+        for (int i = 0; ok && i < g.segments; i++) {
+          const int seg = S::LATE ? 1 - i : i;
           int k0, k1;
           tp_range(g, T.split, seg, k0, k1);
           const bool last = g.a_of_last && T.batch == g.batches - 1;
           const int a_mn = g.a[last ? 1 : seg].mn_major;
           const int b_mn = g.b[KIND == TP_BACK ? 2 * seg : (KIND == TP_GATED ? 0 : seg)].mn_major;
-          const int n = KIND == TP_BACK ? (seg == 0 ? 128 : 64) : S::B_ROWS;
-          const uint32_t idesc = tp_idesc(n, bf16, a_mn, b_mn);
+          const uint32_t idesc = tp_idesc(seg == 0 ? S::N0 : S::N1, bf16, a_mn, b_mn, ROWS);
           const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;   // 16 k, in units of 16 bytes
-          if (KIND == TP_BACK && seg == 1) begun = 0;
+          if (KIND == TP_BACK) begun = 0;
+          if (S::LATE && seg == 0 && !mbar_wait(acc_empty + 8 * (buf ^ 1), buf_phase[buf ^ 1] ^ 1)) {
+            tp_report(g, 48);
+            ok = false;
+            break;
+          }
+          if (S::LATE) tc_fence_after();
           for (int kb = k0; kb < k1; kb++) {
             if (PAIR) {
               if (!mbar_wait(acc_empty + 8 * buf, buf_phase[buf] ^ 1)) {
@@ -376,40 +458,41 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               break;
             }
             tc_fence_after();
-            const uint32_t d = tmem + (uint32_t)(buf * TP_BUFFER_COLS) + (KIND == TP_BACK && !PAIR && seg == 1 ? 128u : 0u);
+            uint32_t d = tmem + (uint32_t)(buf * TP_BUFFER_COLS);
+            if (KIND == TP_BACK && !PAIR) d = S::LATE ? tmem + (seg == 0 ? 0u : 256u + 128u * (uint32_t)buf) : d + (seg == 0 ? 0u : 2u * TN);
             const uint32_t sA = smem + (uint32_t)(stage * S::STAGE), sB = sA + TERMS * S::A_BYTES;
             const uint64_t a_hi = tp_desc(sA, a_mn), b_hi = tp_desc(sB, b_mn);
 #pragma unroll
             for (int ks = 0; ks < 4; ks++) {
               if (PAIR) {
                 const uint64_t a_lo = tp_desc(sA + S::A_BYTES, a_mn), b_lo = tp_desc(sB + S::B_BYTES, b_mn);
-                umma_16(d, a_lo + ks * a_step, b_hi + ks * b_step, idesc, begun);
-                umma_16(d, a_hi + ks * a_step, b_lo + ks * b_step, idesc, 1);
-                umma_16(d, a_hi + ks * a_step, b_hi + ks * b_step, idesc, 1);
+                product(d, a_lo + ks * a_step, b_hi + ks * b_step, idesc, begun);
+                product(d, a_hi + ks * a_step, b_lo + ks * b_step, idesc, 1);
+                product(d, a_hi + ks * a_step, b_hi + ks * b_step, idesc, 1);
               } else {
-                umma_16(d, a_hi + ks * a_step, b_hi + ks * b_step, idesc, begun);
+                product(d, a_hi + ks * a_step, b_hi + ks * b_step, idesc, begun);
               }
               begun = 1;
             }
-            umma_commit(empty + 8 * stage);
+            commit(empty + 8 * stage);
             if (++stage == STAGES) {
               stage = 0;
               phase ^= 1;
             }
             if (PAIR) {
-              umma_commit(acc_full + 8 * buf);
+              commit(acc_full + 8 * buf);
               buf_phase[buf] ^= 1;
               buf ^= 1;
             }
           }
         }
         if (!PAIR && ok) {
-          umma_commit(acc_full + 8 * buf);
+          commit(acc_full + 8 * buf);
           buf_phase[buf] ^= 1;
           buf ^= 1;
         }
       }
-      umma_commit(drain);   // nothing of this block's products is in flight when the columns are given back
+      commit(drain);   // nothing of this block's products is in flight when the columns are given back
       if (!mbar_wait(drain, 0)) tp_report(g, 44);
     }
   } else {
@@ -417,23 +500,37 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
     const int q = warp & 3, half = warp >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
     const TpStager st{staging + (uint32_t)(warp * S::STAGING), lane, g.rows, g.cols};
+    const uint32_t cin_bar = drain + 8 + 8 * (uint32_t)warp;
+    uint32_t cin_phase = 0;
     int buf = 0;
     uint32_t buf_phase[2] = {0, 0};
     bool ok = true;
     // groups of 32 columns of the sum that this warp owns
-    constexpr int GROUPS = KIND == TP_BACK ? 3 : (KIND == TP_GATED ? 4 : TN / 64);
-    constexpr int SEG0_GROUPS = KIND == TP_BACK ? 2 : GROUPS;
+    constexpr int EACH = TN / 64;   // of each of the sums
+    constexpr int GROUPS = KIND == TP_BACK ? 3 * EACH : (KIND == TP_GATED ? 2 * EACH : EACH);
+    constexpr int SEG0_GROUPS = KIND == TP_BACK ? 2 * EACH : GROUPS;
+    static_assert(KIND != TP_GATED || TN == 128, "blocks of 64 columns a warp");
+    const uint32_t first_empty = CTAS == 2 ? peer_smem(acc_empty, 0) : acc_empty;
+    const auto release = [&](int b) {   // this warp has read the sums
+      tc_fence_before();
+      __syncwarp();
+      if (ok && lane == 0) {
+        if (CTAS == 2) mbar_arrive_cluster(first_empty + 8 * b);
+        else mbar_arrive(acc_empty + 8 * b);
+      }
+    };
     // first column of group i inside the accumulator (BACK: the third group has an accumulator, or columns, of its own)
     const auto column = [&](int i) -> uint32_t {
-      if (KIND == TP_GATED) return (uint32_t)((i >> 1) * 128 + 64 * half + 32 * (i & 1));
-      if (KIND == TP_BACK) return (uint32_t)(i < 2 ? 64 * i + 32 * half : (PAIR ? 32 * half : 128 + 32 * half));
-      return (uint32_t)(half * (TN / 2) + 32 * i);
+      const uint32_t in = (uint32_t)(half * (TN / 2) + 32 * (i % EACH));   // this warp's half of each sum
+      if (KIND == TP_GATED) return (uint32_t)(i / EACH * TN) + in;
+      if (KIND == TP_BACK) return i < 2 * EACH ? (uint32_t)(i / EACH * TN) + in : (PAIR ? in : (uint32_t)(2 * TN) + in);
+      return in;
     };
     // A warp whose wait gave up goes through the rest of its tiles without waiting: others meet it at the named barriers.
     int odd = 0;
-    for (int64_t t = blockIdx.x; t < g.total; t += gridDim.x, odd ^= 1) {
-      const TpTile T = tp_tile(g, t, S::OUT_N);
-      const int64_t row = T.row0 + 32 * q;   // first row of this warp
+    for (int64_t t = first_tile; t < g.total; t += tile_step, odd ^= 1) {
+      const TpTile T = tp_tile(g, t, TN, ROWS);
+      const int64_t row = T.row0 + 128 * rank + 32 * q;   // first row of this warp
       // What a Newton-Schulz epilogue adds to the product, a group of 32 columns ahead: S (hi and lo; rows of a multiple of 64 elements,
       // so that a group never runs over one's end) or X in float32.
       const int col0 = T.n0 + half * (TN / 2);
@@ -450,7 +547,19 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           }
         }
       };
-      if (col0 < g.cols) fetch_cin(col0);
+      // ... of 16-bit operands by the copy engine, into the piece that the group leaves by: two alternate
+      const auto copy_cin = [&](int col, int piece) {
+        if (elect_one()) {
+          tma_store_wait_read();
+          mbar_arrive_expect_tx(cin_bar, 4096);
+          tma_load_3d(st.smem + 4096u * (uint32_t)piece, &g.cin_map, col, (int)row, T.batch, cin_bar);
+        }
+        __syncwarp();
+      };
+      if (col0 < g.cols) {
+        if (S::CIN_TMA) copy_cin(col0, 0);
+        else fetch_cin(col0);
+      }
       float acc[PAIR ? GROUPS : 1][32];
       if (PAIR) {
 #pragma unroll
@@ -469,10 +578,11 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           const TpOperand &B0 = g.b[KIND == TP_BACK ? 2 * seg : (KIND == TP_GATED ? 0 : seg)];
           const TpOperand &B1 = g.b[KIND == TP_GATED || (KIND == TP_BACK && seg == 0) ? 1 : (KIND == TP_BACK ? 2 : seg)];
           // scales: one block of rows a warp; two blocks of columns at most: of both projections (GATED, BACK), or side by side
-          const int cb = T.n0 / 64 + (KIND == TP_GATED ? half : (KIND == TP_BACK ? 0 : half * (TN / 128)));
+          const int cb = T.n0 / 64 + (KIND == TP_BACK && TN == 64 ? 0 : half * (TN / 128));
           const float *pa = A.scale ? A.scale + T.batch * A.sc_b + (row >> 6) * A.sc_i : nullptr;
           const float *pb0 = B0.scale ? B0.scale + T.batch * B0.sc_b + cb * B0.sc_i : nullptr;
-          const bool two = KIND == TP_GATED || (KIND == TP_BACK && seg == 0) || TN == 256;
+          constexpr bool SIDE = KIND != TP_GATED && KIND != TP_BACK && TN == 256;
+          const bool two = KIND == TP_GATED || (KIND == TP_BACK && seg == 0) || SIDE;
           const float *pb1 = !two ? pb0 : (KIND == TP_GATED || KIND == TP_BACK
                                  ? (B1.scale ? B1.scale + T.batch * B1.sc_b + cb * B1.sc_i : nullptr)
                                  : (pb0 && (cb + 1) * 64 < g.cols ? pb0 + B0.sc_i : pb0));   // past the last block: zeros in any scale
@@ -499,13 +609,11 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               if (i < i0 || i >= i1) continue;
               uint32_t v[32];
               tmem_ld32(at + column(i), v);
-              const float s = (KIND == TP_GATED ? i >= 2 : (KIND == TP_BACK ? i == 1 : i >= 2)) ? s1 : s0;
+              const float s = (KIND == TP_BACK ? i == 1 : i >= 2) ? s1 : s0;
 #pragma unroll
               for (int j = 0; j < 32; j++) acc[i][j] = fmaf(__uint_as_float(v[j]), s, acc[i][j]);
             }
-            tc_fence_before();
-            __syncwarp();
-            if (ok && lane == 0) mbar_arrive(acc_empty + 8 * buf);
+            release(buf);
             buf_phase[buf] ^= 1;
             buf ^= 1;
           }
@@ -517,7 +625,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         }
         tc_fence_after();
       }
-      const uint32_t at = lanes + (uint32_t)(buf * TP_BUFFER_COLS);
+      const uint32_t at = lanes + (S::LATE ? 0u : (uint32_t)(buf * TP_BUFFER_COLS));
       // group i of the finished sums
       const auto take = [&](int i, float (&v)[32]) {
         if (PAIR) {
@@ -525,7 +633,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           for (int j = 0; j < 32; j++) v[j] = acc[PAIR ? i : 0][j];
         } else {
           uint32_t u[32];
-          tmem_ld32(at + column(i), u);
+          tmem_ld32(at + column(i) + (S::LATE && i >= SEG0_GROUPS ? 128u * (uint32_t)buf : 0u), u);
 #pragma unroll
           for (int j = 0; j < 32; j++) v[j] = __uint_as_float(u[j]);
         }
@@ -575,59 +683,63 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         }
       } else if constexpr (KIND == TP_BACK) {
         // h = act(g) u, dL/dg = dL/dh u act'(g), dL/du = dL/dh act(g)
-        const int col = T.n0 + 32 * half;
-        float a[32], u[32], dh[32];
-        take(0, a);
-        take(1, u);
-        take(2, dh);
-        float most[3] = {0.f, 0.f, 0.f};
+        static_assert(!PAIR || TN == 64, "a block of 64 columns a tile");
+#pragma unroll 1
+        for (int e = 0; e < EACH; e++) {
+          const int col = col0 + 32 * e;
+          float a[32], u[32], dh[32];
+          take(e, a);
+          take(EACH + e, u);
+          take(2 * EACH + e, dh);
+          float most[3] = {0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 32; j++) {
-          float d;
-          const float act = tp_act<ACT>(a[j], d);
-          const float h = act * u[j], dg = dh[j] * (u[j] * d), du = dh[j] * act;
-          a[j] = h;
-          u[j] = dg;
-          dh[j] = du;
+          for (int j = 0; j < 32; j++) {
+            float d;
+            const float act = tp_act<ACT>(a[j], d);
+            const float h = act * u[j], dg = dh[j] * (u[j] * d), du = dh[j] * act;
+            a[j] = h;
+            u[j] = dg;
+            dh[j] = du;
+            if (PAIR) {
+              most[0] = fmaxf(most[0], tp_finite_abs(dg));
+              most[1] = fmaxf(most[1], tp_finite_abs(du));
+              most[2] = fmaxf(most[2], tp_finite_abs(h));
+            }
+          }
+          float scale[3] = {1.f, 1.f, 1.f};
           if (PAIR) {
-            most[0] = fmaxf(most[0], tp_finite_abs(dg));
-            most[1] = fmaxf(most[1], tp_finite_abs(du));
-            most[2] = fmaxf(most[2], tp_finite_abs(h));
+#pragma unroll
+            for (int p = 0; p < 3; p++) {
+              most[p] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most[p])));
+              if (lane == 0) block_most[p][warp] = most[p];
+            }
+            tp_bar(1 + (q >> 1), 128);   // 64 rows x 64 columns: two quarters, both halves
+#pragma unroll
+            for (int p = 0; p < 3; p++) {
+              const float m = fmaxf(fmaxf(block_most[p][warp], block_most[p][warp ^ 1]), fmaxf(block_most[p][warp ^ 4], block_most[p][warp ^ 5]));
+              scale[p] = tp_scale(m);
+              if (lane == 0 && (q & 1) == 0 && half == 0 && row < g.rows && T.n0 < g.cols)
+                g.out_scale[p][(row >> 6) * g.out_scale_ld + (T.n0 >> 6)] = 1.0f / scale[p];
+            }
+            tp_bar(1 + (q >> 1), 128);   // read by all before the next tile's are written
           }
-        }
-        float scale[3] = {1.f, 1.f, 1.f};
-        if (PAIR) {
 #pragma unroll
           for (int p = 0; p < 3; p++) {
-            most[p] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most[p])));
-            if (lane == 0) block_most[p][warp] = most[p];
-          }
-          tp_bar(1 + (q >> 1), 128);   // 64 rows x 64 columns: two quarters, both halves
+            uint32_t w[16], lo[16];
 #pragma unroll
-          for (int p = 0; p < 3; p++) {
-            const float m = fmaxf(fmaxf(block_most[p][warp], block_most[p][warp ^ 1]), fmaxf(block_most[p][warp ^ 4], block_most[p][warp ^ 5]));
-            scale[p] = tp_scale(m);
-            if (lane == 0 && (q & 1) == 0 && half == 0 && row < g.rows && T.n0 < g.cols)
-              g.out_scale[p][(row >> 6) * g.out_scale_ld + (T.n0 >> 6)] = 1.0f / scale[p];
+            for (int j = 0; j < 16; j++) {
+              const float x = p == 0 ? u[2 * j] : (p == 1 ? dh[2 * j] : a[2 * j]);
+              const float y = p == 0 ? u[2 * j + 1] : (p == 1 ? dh[2 * j + 1] : a[2 * j + 1]);
+              if (PAIR) tp_split2(x * scale[p], y * scale[p], w[j], lo[j]);
+              else w[j] = tp_bf16x2(x, y);
+            }
+            if (PAIR || p != 1) st.begin();
+            const uint32_t where = PAIR ? 0u : (p == 1 ? 2048u : 0u);
+            st.put(where, w);
+            if (PAIR) st.put(2048, lo);
+            st.send(&g.out[0].map, where, col, row, TERMS * p);
+            if (PAIR) st.send(&g.out[0].map, 2048, col, row, TERMS * p + 1);
           }
-          tp_bar(1 + (q >> 1), 128);   // read by all before the next tile's are written
-        }
-#pragma unroll
-        for (int p = 0; p < 3; p++) {
-          uint32_t w[16], lo[16];
-#pragma unroll
-          for (int j = 0; j < 16; j++) {
-            const float x = p == 0 ? u[2 * j] : (p == 1 ? dh[2 * j] : a[2 * j]);
-            const float y = p == 0 ? u[2 * j + 1] : (p == 1 ? dh[2 * j + 1] : a[2 * j + 1]);
-            if (PAIR) tp_split2(x * scale[p], y * scale[p], w[j], lo[j]);
-            else w[j] = tp_bf16x2(x, y);
-          }
-          if (PAIR || p != 1) st.begin();
-          const uint32_t where = PAIR ? 0u : (p == 1 ? 2048u : 0u);
-          st.put(where, w);
-          if (PAIR) st.put(2048, lo);
-          st.send(&g.out[0].map, where, col, row, TERMS * p);
-          if (PAIR) st.send(&g.out[0].map, 2048, col, row, TERMS * p + 1);
         }
       } else if constexpr (KIND == TP_PLAIN) {
         const int batch = T.split * g.batches + T.batch;
@@ -646,7 +758,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             st.begin();
             st.put(0, w);
             if (g.out[1].use_map) st.send(&g.out[1].map, 0, col0 + 32 * i, row, batch);
-            else st.send_rows(g.out[1], true, col0 + 32 * i, row, batch);
+            else st.send_rows(g.out[1], true, 0, col0 + 32 * i, row, batch);
           }
         } else {
 #pragma unroll
@@ -660,7 +772,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             st.begin();
             st.put(0, w);
             if (g.out[1].use_map) st.send(&g.out[1].map, 0, col0 + 32 * i, row, batch);
-            else st.send_rows(g.out[1], false, col0 + 32 * i, row, batch);
+            else st.send_rows(g.out[1], false, 0, col0 + 32 * i, row, batch);
           }
         }
       } else {
@@ -685,6 +797,27 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
                 v[8 * c + 2 * k + 1] = g.alpha * v[8 * c + 2 * k + 1] + g.beta * (a.y + e.y);
               }
             }
+          } else if constexpr (S::CIN_TMA) {
+            const uint32_t piece = 4096u * (uint32_t)(i & 1);
+            if (ok && !warp_wait(cin_bar, cin_phase, lane)) {
+              if (lane == 0) tp_report(g, 49);
+              ok = false;
+            }
+            cin_phase ^= 1;
+#pragma unroll
+            for (int c = 0; c < 8; c++) {
+              float4 x;
+              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                           : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                           : "r"(st.smem + piece + (uint32_t)sw128_offset(lane, c))
+                           : "memory");
+              v[4 * c] = g.alpha * v[4 * c] + g.beta * x.x;
+              v[4 * c + 1] = g.alpha * v[4 * c + 1] + g.beta * x.y;
+              v[4 * c + 2] = g.alpha * v[4 * c + 2] + g.beta * x.z;
+              v[4 * c + 3] = g.alpha * v[4 * c + 3] + g.beta * x.w;
+            }
+            __syncwarp();
+            if (i + 1 < GROUPS && col + 32 < g.cols) copy_cin(col + 32, (i + 1) & 1);   // on its way while this group is put down
           } else {
 #pragma unroll
             for (int c = 0; c < 8; c++) {
@@ -694,25 +827,25 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               v[4 * c + 3] = g.alpha * v[4 * c + 3] + g.beta * __uint_as_float(cin[c].w);
             }
           }
-          if (i + 1 < GROUPS && col + 32 < g.cols) fetch_cin(col + 32);   // on its way while this group is put down
+          if (!S::CIN_TMA && i + 1 < GROUPS && col + 32 < g.cols) fetch_cin(col + 32);   // on its way while this group is put down
+          const uint32_t piece = S::CIN_TMA ? 4096u * (uint32_t)(i & 1) : 0u;   // copy_cin() or begin() has waited for it
           if (KIND == TP_APPLY) {
             // out[1]: float32, the X of the next step or the result
             if (!g.out_bf16) {
               uint32_t w[32];
 #pragma unroll
               for (int j = 0; j < 32; j++) w[j] = __float_as_uint(v[j]);
-              if (PAIR) st.begin();
-              else st.begin_but_last();   // the pairs' piece may still be read
-              st.put(0, w);
-              if (g.out[1].use_map) st.send(&g.out[1].map, 0, col, row, T.batch);
-              else st.send_rows(g.out[1], false, col, row, T.batch);
+              if (!S::CIN_TMA) st.begin();
+              st.put(piece, w);
+              if (g.out[1].use_map) st.send(&g.out[1].map, piece, col, row, T.batch);
+              else st.send_rows(g.out[1], false, piece, col, row, T.batch);
             } else if (g.out[1].use_map) {
               uint32_t w[16];
 #pragma unroll
               for (int j = 0; j < 16; j++) w[j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
-              st.begin();
-              st.put(0, w);
-              st.send(&g.out[1].map, 0, col, row, T.batch);
+              if (!S::CIN_TMA) st.begin();
+              st.put(piece, w);
+              st.send(&g.out[1].map, piece, col, row, T.batch);
             } else {
               __nv_bfloat16 *o =
                   static_cast<__nv_bfloat16 *>(g.out[1].ptr) + (int64_t)T.batch * g.out[1].batch + (row + lane) * g.out[1].ld + col;
@@ -722,16 +855,19 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             }
           }
           if (KIND != TP_APPLY || g.pair_scale != 0.f) {
-            constexpr uint32_t where = PAIR ? 0u : 4096u;
             constexpr bool LOW = PAIR || KIND == TP_GRAM;   // S is also added as it is: with its low part
+            constexpr uint32_t where = S::CIN_TMA ? 8192u : 0u;
             uint32_t w[16], lo[16];
 #pragma unroll
             for (int j = 0; j < 16; j++) {
               if (LOW) tp_split2(v[2 * j] * g.pair_scale, v[2 * j + 1] * g.pair_scale, w[j], lo[j]);
               else w[j] = tp_f16x2(v[2 * j] * g.pair_scale, v[2 * j + 1] * g.pair_scale);
             }
-            if (PAIR || KIND != TP_APPLY) st.begin();
-            else st.begin_but_last();   // this group's float32 piece may still be read
+            if (S::CIN_TMA) {
+              if (i + 1 == GROUPS || col + 32 >= g.cols) st.begin_but_last();   // else copy_cin() has waited for the group before
+            } else {
+              st.begin();
+            }
             st.put(where, w);
             if (LOW) st.put(where + 2048, lo);
             st.send(&g.out[0].map, where, col, row, (LOW ? 2 : 1) * T.batch);
@@ -740,9 +876,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         }
       }
       if (!PAIR) {
-        tc_fence_before();
-        __syncwarp();
-        if (ok && lane == 0) mbar_arrive(acc_empty + 8 * buf);
+        release(buf);
         buf_phase[buf] ^= 1;
         buf ^= 1;
       }
@@ -750,8 +884,15 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
     if (elect_one()) tma_store_wait_all();   // the copy engine reads this warp's staging buffer
   }
   tc_fence_before();
-  __syncthreads();
-  if (warp == TP_EPILOGUE_WARPS) tmem_dealloc(tmem, 512);
+  if (CTAS == 2) {
+    __syncthreads();
+    __syncwarp();
+    cluster_sync();   // the other CTA's products have read this one's operands, its warps have arrived here
+    if (warp == TP_EPILOGUE_WARPS) tmem_dealloc_pair(tmem, 512);
+  } else {
+    __syncthreads();
+    if (warp == TP_EPILOGUE_WARPS) tmem_dealloc(tmem, 512);
+  }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -834,20 +975,34 @@ inline TpArgs new_args(int64_t rows, int64_t cols, int32_t *status) {
 }
 inline int blocks64(int64_t n) { return (int)((n + 63) / 64); }
 
-// 256 columns a tile where that fills the SMs, 128 otherwise
-inline int tile_columns(int64_t rows, int cols, int64_t times) { return cols > 128 && (rows + 127) / 128 * ((cols + 255) / 256) * times >= 148 ? 256 : 128; }
-template <int KIND, bool PAIR, int TN, int ACT = TP_SILU>
+// Pairs of CTAs where their tiles of 256 rows fill the SMs
+inline bool pairs_fill(int64_t rows, int64_t cols, int64_t times, int tn) { return (rows + 255) / 256 * ((cols + tn - 1) / tn) * times >= 74; }
+
+template <int KIND, bool PAIR, int TN, int CTAS, int ACT = TP_SILU>
 int tp_launch(TpArgs &g, cudaStream_t st, const char *what) {
-  using S = TpShape<KIND, PAIR, TN>;
+  using S = TpShape<KIND, PAIR, TN, CTAS>;
   static_assert(S::STAGES >= 2, "a ring of two stages at least");
-  g.mt = (int)((g.rows + 127) / 128);
-  g.nt = (int)((g.cols + S::OUT_N - 1) / S::OUT_N);
+  g.mt = (int)((g.rows + 128 * CTAS - 1) / (128 * CTAS));
+  g.nt = (int)((g.cols + TN - 1) / TN);
   g.total = (int64_t)g.mt * g.nt * g.batches * g.splits;
   if (g.total >= (int64_t)1 << 31) return fail(CMACE_ERR_UNSUPPORTED, "%s: too many tiles", what);
-  const auto kernel = tile_product_kernel<KIND, PAIR, TN, ACT>;
-  if (const int rc = allow_smem<tile_product_kernel<KIND, PAIR, TN, ACT>>(S::SMEM, what)) return rc;
-  const int grid = (int)(g.total < 148 ? g.total : 148);
-  launch_chained(kernel, dim3(grid), dim3(TP_THREADS), (size_t)S::SMEM, st, g);
+  const auto kernel = tile_product_kernel<KIND, PAIR, TN, CTAS, ACT>;
+  if (const int rc = allow_smem<tile_product_kernel<KIND, PAIR, TN, CTAS, ACT>>(S::SMEM, what)) return rc;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CTAS, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  const bool chained = chain_launches() == Chain::on;   // as launch_chained()
+  if (chain_launches() == Chain::from_second) chain_launches() = Chain::on;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(CTAS * (g.total < 148 / CTAS ? g.total : 148 / CTAS)));
+  cfg.blockDim = dim3(TP_THREADS);
+  cfg.dynamicSmemBytes = (size_t)S::SMEM;
+  cfg.stream = st;
+  cfg.attrs = CTAS == 2 ? attr : attr + 1;
+  cfg.numAttrs = (CTAS == 2 ? 1 : 0) + (chained ? 1 : 0);
+  cudaLaunchKernelEx(&cfg, kernel, g);
   return check_launch(what);
 }
 

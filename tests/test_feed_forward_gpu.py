@@ -103,6 +103,7 @@ def inside(got, want):
 SIZES = [
     (1, 128, 512), (2, 1, 1), (3, 7, 5), (63, 64, 64), (64, 32, 128), (65, 96, 192), (127, 130, 66), (128, 128, 256), (129, 100, 129),
     (200, 8, 1001), (5, 250, 40), (257, 257, 65), (1000, 128, 512), (300, 512, 130),
+    (20001, 40, 136), (9999, 264, 300),   # enough rows for pairs of CTAs, 128 and 256 columns a tile
 ]
 
 

@@ -84,7 +84,7 @@ def check(out, U, steps=5, coefficients=USUAL, eps=1e-7):
 
 
 SHAPES = [(1, 1, 1), (3, 1, 40), (2, 40, 1), (4, 64, 64), (2, 16, 23), (3, 100, 64), (2, 128, 128), (2, 128, 512), (1, 512, 96), (1, 129, 130),
-          (1, 130, 129), (2, 250, 70), (1, 257, 640), (3, 5, 200), (1, 600, 300)]
+          (1, 130, 129), (2, 250, 70), (1, 257, 640), (3, 5, 200), (1, 600, 300), (40, 140, 300), (40, 300, 140)]
 
 
 @pytest.mark.parametrize("kind", ["even", "normal", "low rank"])

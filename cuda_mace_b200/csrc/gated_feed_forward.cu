@@ -74,8 +74,7 @@ __global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const __grid_constan
       v[i] = r < J.rows && col < J.cols ? __ldg(s + r * J.cols + col) : 0.f;
     }
   }
-#pragma unroll
-  for (int i = 0; i < 16; i++) most = fmaxf(most, tp_finite_abs(v[i]));
+  most = tp_most(v);
   most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
   if ((t & 31) == 0) most_of[t >> 5] = most;
   __syncthreads();
@@ -92,8 +91,8 @@ __global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const __grid_constan
       const int64_t r = row0 + (t >> 4) + 16 * i;
       if (r >= J.rows) break;
       uint2 h, l;
-      tp_split2(v[4 * i] * scale, v[4 * i + 1] * scale, h.x, l.x);
-      tp_split2(v[4 * i + 2] * scale, v[4 * i + 3] * scale, h.y, l.y);
+      tp_split2(v[4 * i], v[4 * i + 1], scale, h.x, l.x);
+      tp_split2(v[4 * i + 2], v[4 * i + 3], scale, h.y, l.y);
       *reinterpret_cast<uint2 *>(hi + r * J.ld + col) = h;
       *reinterpret_cast<uint2 *>(lo + r * J.ld + col) = l;
     }
@@ -105,7 +104,7 @@ __global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const __grid_constan
       const int64_t r = row0 + (t >> 6) + 4 * i;
       if (r >= J.rows) break;
       uint32_t h, l;
-      tp_split2(v[i] * scale, 0.f, h, l);
+      tp_split2(v[i], 0.f, scale, h, l);
       hi[r * J.ld + col] = __ushort_as_half((unsigned short)h);
       lo[r * J.ld + col] = __ushort_as_half((unsigned short)l);
     }
@@ -198,21 +197,25 @@ static int set_user_out(TpArgs &g, void *ptr, bool f32, int64_t rows, int cols, 
   return CMACE_OK;
 }
 
+static bool long_enough(bool f32, const TpArgs &g) {
+  static const int least = getenv("TP_LEAST") ? atoi(getenv("TP_LEAST")) : 8;
+  return !f32 || g.kblocks[0] + (g.segments > 1 ? g.kblocks[1] : 0) >= least * g.splits;
+}
 template <int ACT>
 static int launch_gated(const FeedForward &f, TpArgs &g) {
-  const bool pairs = pairs_fill(g.rows, g.cols, 1, 128);
+  const bool pairs = pairs_fill(g.rows, g.cols, 1, 128) && long_enough(f.f32, g);
   if (f.f32) return pairs ? tp_launch<TP_GATED, true, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_GATED, true, 128, 1, ACT>(g, f.st, f.what);
   return pairs ? tp_launch<TP_GATED, false, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_GATED, false, 128, 1, ACT>(g, f.st, f.what);
 }
 template <int ACT>
 static int launch_back(const FeedForward &f, TpArgs &g) {
   if (f.f32)
-    return pairs_fill(g.rows, g.cols, 1, 64) ? tp_launch<TP_BACK, true, 64, 2, ACT>(g, f.st, f.what) : tp_launch<TP_BACK, true, 64, 1, ACT>(g, f.st, f.what);
+    return pairs_fill(g.rows, g.cols, 1, 64) && long_enough(true, g) ? tp_launch<TP_BACK, true, 64, 2, ACT>(g, f.st, f.what) : tp_launch<TP_BACK, true, 64, 1, ACT>(g, f.st, f.what);
   return pairs_fill(g.rows, g.cols, 1, 128) ? tp_launch<TP_BACK, false, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_BACK, false, 64, 1, ACT>(g, f.st, f.what);
 }
 static int launch_plain(bool pair, TpArgs &g, cudaStream_t st, const char *what) {
   const int64_t times = (int64_t)g.batches * g.splits;
-  if (pair) return pairs_fill(g.rows, g.cols, times, 128) ? tp_launch<TP_PLAIN, true, 128, 2>(g, st, what) : tp_launch<TP_PLAIN, true, 128, 1>(g, st, what);
+  if (pair) return pairs_fill(g.rows, g.cols, times, 128) && long_enough(true, g) ? tp_launch<TP_PLAIN, true, 128, 2>(g, st, what) : tp_launch<TP_PLAIN, true, 128, 1>(g, st, what);
   if (g.cols > 128 && pairs_fill(g.rows, g.cols, times, 256)) return tp_launch<TP_PLAIN, false, 256, 2>(g, st, what);
   return pairs_fill(g.rows, g.cols, times, 128) ? tp_launch<TP_PLAIN, false, 128, 2>(g, st, what) : tp_launch<TP_PLAIN, false, 128, 1>(g, st, what);
 }

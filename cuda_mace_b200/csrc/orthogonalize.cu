@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(NS_THREADS) ns_prep_kernel(const NsPrep p) {
     p.x[at] = v;
     const int64_t plane = p.rows * p.ld, to = m * p.terms * plane + row * p.ld + col;
     uint32_t h, l;
-    tp_split2(v * p.scale, 0.f, h, l);
+    tp_split2(v, 0.f, p.scale, h, l);
     p.h[to] = __ushort_as_half((unsigned short)h);
     if (p.terms == 2) p.h[to + plane] = __ushort_as_half((unsigned short)l);
   }
@@ -135,7 +135,7 @@ __device__ __forceinline__ void put_pairs(uint32_t hi, uint32_t lo, int row, int
   for (int c = 0; c < COLS / 8; c++) {
     uint32_t h[4], l[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) tp_split2(v[8 * c + 2 * k] * scale, v[8 * c + 2 * k + 1] * scale, h[k], l[k]);
+    for (int k = 0; k < 4; k++) tp_split2(v[8 * c + 2 * k], v[8 * c + 2 * k + 1], scale, h[k], l[k]);
     const uint32_t at = (uint32_t)sw128_offset(row, piece + c);
     smem_store4(hi + at, h[0], h[1], h[2], h[3]);
     smem_store4(lo + at, l[0], l[1], l[2], l[3]);
@@ -306,8 +306,8 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
           sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
         }
         uint32_t h0, h1, l0, l1;
-        tp_split2(sum.x * ss, sum.y * ss, h0, l0);
-        tp_split2(sum.z * ss, sum.w * ss, h1, l1);
+        tp_split2(sum.x, sum.y, ss, h0, l0);
+        tp_split2(sum.z, sum.w, ss, h1, l1);
         const uint32_t to = (uint32_t)((piece >> 4) * NSF_IMAGE + sw128_offset(r, (piece & 15) >> 1) + (piece & 1) * 8);
         for (int p = 0; p < g.cluster; p++) {
           peer_store2(peer_smem(s_hi + to, (uint32_t)p), h0, h1);

@@ -129,8 +129,9 @@ __device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
+// Says that tensor memory has been read, which tcgen05.fence orders: a release here would wait for all of the warp's stores.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // Operand image of rows of 128 bytes with the 128-byte swizzle.  K-major: a row is 64 k of one i, groups of eight rows 1 024 bytes
 // apart.  MN-major: a row is 64 i of one k, groups of eight k 1 024 bytes apart (stride offset), runs of 64 i 8 192 (leading offset).
@@ -204,16 +205,41 @@ __device__ __forceinline__ float tp_finite_abs(float x) {
   const float a = fabsf(x);
   return a < CUDART_INF_F ? a : 0.f;   // infinities and NaN do not set a block's scale
 }
-// two values as (hi, lo) pairs of fp16; what is not finite goes to hi alone
-__device__ __forceinline__ void tp_split2(float x, float y, uint32_t &hi, uint32_t &lo) {
-  const __half2 h = __floats2half2_rn(x, y);
+// Largest finite magnitude of a thread's values.  Without an infinity that is a maximum with the sign left out, which drops NaN by
+// itself: one instruction a value.
+template <int N>
+__device__ __forceinline__ float tp_most(const float (&v)[N], float most = 0.f) {
+#pragma unroll
+  for (int j = 0; j < N; j++) most = fmaxf(most, fabsf(v[j]));
+  if (most < CUDART_INF_F) return most;
+  most = 0.f;
+#pragma unroll 1
+  for (int j = 0; j < N; j++) {
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; k++) x = k == j ? v[k] : x;
+    most = fmaxf(most, tp_finite_abs(x));
+  }
+  return most;
+}
+// Two values times a power of two as (hi, lo) pairs of fp16.  What is not finite has NaN for lo, and products with it come out NaN.
+__device__ __forceinline__ void tp_split2(float x, float y, float scale, uint32_t &hi, uint32_t &lo) {
+  const unsigned long long v = mul2(pack2(x, y), pack2(scale, scale));
+  float a, b;
+  unpack2(v, a, b);
+  const __half2 h = __floats2half2_rn(a, b);
   const float2 f = __half22float2(h);
-  float dx = x - f.x, dy = y - f.y;
-  dx = fabsf(f.x) < CUDART_INF_F ? dx : 0.f;
-  dy = fabsf(f.y) < CUDART_INF_F ? dy : 0.f;
-  const __half2 l = __floats2half2_rn(dx, dy);
+  unpack2(sub2(v, pack2(f.x, f.y)), a, b);
+  const __half2 l = __floats2half2_rn(a, b);
   hi = *reinterpret_cast<const uint32_t *>(&h);
   lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+// sums += scale * 32 accumulator columns
+__device__ __forceinline__ void tp_add(float (&sum)[32], const uint32_t (&v)[32], float scale) {
+  const unsigned long long s2 = pack2(scale, scale);
+#pragma unroll
+  for (int j = 0; j < 32; j += 2)
+    unpack2(fma2(pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), s2, pack2(sum[j], sum[j + 1])), sum[j], sum[j + 1]);
 }
 __device__ __forceinline__ uint32_t tp_bf16x2(float x, float y) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
@@ -610,8 +636,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               uint32_t v[32];
               tmem_ld32(at + column(i), v);
               const float s = (KIND == TP_BACK ? i == 1 : i >= 2) ? s1 : s0;
-#pragma unroll
-              for (int j = 0; j < 32; j++) acc[i][j] = fmaf(__uint_as_float(v[j]), s, acc[i][j]);
+              tp_add(acc[i], v, s);
             }
             release(buf);
             buf_phase[buf] ^= 1;
@@ -644,12 +669,11 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         if constexpr (PAIR) {
           float most = 0.f;
 #pragma unroll
-          for (int i = 0; i < 2; i++)
+          for (int i = 0; i < 2; i++) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-              acc[i][j] = tp_act<ACT>(acc[i][j]) * acc[PAIR ? 2 + i : 0][j];
-              most = fmaxf(most, tp_finite_abs(acc[i][j]));
-            }
+            for (int j = 0; j < 32; j++) acc[i][j] = tp_act<ACT>(acc[i][j]) * acc[PAIR ? 2 + i : 0][j];
+            most = tp_most(acc[i], most);
+          }
           // the block of 64 rows is this warp's and the next (or previous) quarter's of the same columns
           most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
           if (lane == 0) block_most[odd][warp] = most;
@@ -660,7 +684,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           uint32_t w[32], lo[32];
 #pragma unroll
           for (int j = 0; j < 32; j++)
-            tp_split2(acc[j >> 4][2 * (j & 15)] * scale, acc[j >> 4][2 * (j & 15) + 1] * scale, w[j], lo[j]);
+            tp_split2(acc[j >> 4][2 * (j & 15)], acc[j >> 4][2 * (j & 15) + 1], scale, w[j], lo[j]);
           st.begin();
           st.put(0, w);
           st.send(&g.out[0].map, 0, col, row, 0);
@@ -700,11 +724,11 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             a[j] = h;
             u[j] = dg;
             dh[j] = du;
-            if (PAIR) {
-              most[0] = fmaxf(most[0], tp_finite_abs(dg));
-              most[1] = fmaxf(most[1], tp_finite_abs(du));
-              most[2] = fmaxf(most[2], tp_finite_abs(h));
-            }
+          }
+          if (PAIR) {
+            most[0] = tp_most(u);
+            most[1] = tp_most(dh);
+            most[2] = tp_most(a);
           }
           float scale[3] = {1.f, 1.f, 1.f};
           if (PAIR) {
@@ -730,7 +754,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             for (int j = 0; j < 16; j++) {
               const float x = p == 0 ? u[2 * j] : (p == 1 ? dh[2 * j] : a[2 * j]);
               const float y = p == 0 ? u[2 * j + 1] : (p == 1 ? dh[2 * j + 1] : a[2 * j + 1]);
-              if (PAIR) tp_split2(x * scale[p], y * scale[p], w[j], lo[j]);
+              if (PAIR) tp_split2(x, y, scale[p], w[j], lo[j]);
               else w[j] = tp_bf16x2(x, y);
             }
             if (PAIR || p != 1) st.begin();
@@ -860,7 +884,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             uint32_t w[16], lo[16];
 #pragma unroll
             for (int j = 0; j < 16; j++) {
-              if (LOW) tp_split2(v[2 * j] * g.pair_scale, v[2 * j + 1] * g.pair_scale, w[j], lo[j]);
+              if (LOW) tp_split2(v[2 * j], v[2 * j + 1], g.pair_scale, w[j], lo[j]);
               else w[j] = tp_f16x2(v[2 * j] * g.pair_scale, v[2 * j + 1] * g.pair_scale);
             }
             if (S::CIN_TMA) {

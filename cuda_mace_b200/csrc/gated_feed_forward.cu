@@ -193,7 +193,7 @@ static int set_user_out(TpArgs &g, void *ptr, bool f32, int64_t rows, int cols, 
   g.out_bf16 = !f32;
   const int bytes = f32 ? 4 : 2;
   o.use_map = aligned16(ptr) && (int64_t)cols * bytes % 16 == 0;
-  if (o.use_map) return encode_tile_map(&o.map, ptr, bytes, !f32, cols, rows, 1, cols, rows * (int64_t)cols, f32 ? 32 : 64, 32, what);
+  if (o.use_map) return encode_tile_map(&o.map, ptr, bytes, !f32, cols, rows, 1, cols, rows * (int64_t)cols, f32 ? 16 : 32, 32, what);
   return CMACE_OK;
 }
 
@@ -208,10 +208,11 @@ static int launch_gated(const FeedForward &f, TpArgs &g) {
   return pairs ? tp_launch<TP_GATED, false, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_GATED, false, 128, 1, ACT>(g, f.st, f.what);
 }
 template <int ACT>
-static int launch_back(const FeedForward &f, TpArgs &g) {
-  if (f.f32)
-    return pairs_fill(g.rows, g.cols, 1, 64) && long_enough(true, g) ? tp_launch<TP_BACK, true, 64, 2, ACT>(g, f.st, f.what) : tp_launch<TP_BACK, true, 64, 1, ACT>(g, f.st, f.what);
-  return pairs_fill(g.rows, g.cols, 1, 128) ? tp_launch<TP_BACK, false, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_BACK, false, 64, 1, ACT>(g, f.st, f.what);
+static int launch_back(const FeedForward &f, bool wide, TpArgs &g) {
+  if (wide) return tp_launch<TP_BACK, false, 128, 2, ACT>(g, f.st, f.what);
+  if (!f.f32) return tp_launch<TP_BACK, false, 64, 1, ACT>(g, f.st, f.what);
+  return pairs_fill(g.rows, g.cols, 1, 64) && long_enough(true, g) ? tp_launch<TP_BACK, true, 64, 2, ACT>(g, f.st, f.what)
+                                                                  : tp_launch<TP_BACK, true, 64, 1, ACT>(g, f.st, f.what);
 }
 static int launch_plain(bool pair, TpArgs &g, cudaStream_t st, const char *what) {
   const int64_t times = (int64_t)g.batches * g.splits;
@@ -258,7 +259,7 @@ static int forward(const FeedForward &f, void *y, Carve &w) {
   set_operand(g.b[0], wg, false);
   set_operand(g.b[1], wu, false);
   g.kblocks[0] = blocks64(f.C);
-  if (!rc) rc = set_hidden_out(g, h, 64, bf16, f.what);
+  if (!rc) rc = set_hidden_out(g, h, 32, bf16, f.what);
   if (!rc) rc = f.act == TP_SILU ? launch_gated<TP_SILU>(f, g) : launch_gated<TP_GELU>(f, g);
   g = new_args(f.M, f.C, f.status);
   set_operand(g.a[0], h, true);
@@ -294,8 +295,9 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   set_operand(g.b[2], wd, true);
   g.segments = 2;
   g.kblocks[0] = g.kblocks[1] = blocks64(f.C);
-  if (!rc) rc = set_hidden_out(g, hidden, 32, bf16, f.what);
-  if (!rc) rc = f.act == TP_SILU ? launch_back<TP_SILU>(f, g) : launch_back<TP_GELU>(f, g);
+  const bool wide = !f.f32 && pairs_fill(f.M, f.H, 1, 128);   // tiles of 128 columns, 32 a warp
+  if (!rc) rc = set_hidden_out(g, hidden, wide ? 32 : 16, bf16, f.what);
+  if (!rc) rc = f.act == TP_SILU ? launch_back<TP_SILU>(f, wide, g) : launch_back<TP_GELU>(f, wide, g);
   if (want_x) {
     g = new_args(f.M, f.C, f.status);
     set_operand(g.a[0], hidden.part(0), true);
@@ -318,7 +320,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
     g.a_of_last = 1;
     g.kblocks[0] = blocks64(f.M);
     g.out[1].use_map = 1;
-    if (!rc) rc = encode_tile_map(&g.out[1].map, partial, 4, false, f.H, f.C, (int64_t)splits * 3, ld, (int64_t)f.C * ld, 32, 32, f.what);
+    if (!rc) rc = encode_tile_map(&g.out[1].map, partial, 4, false, f.H, f.C, (int64_t)splits * 3, ld, (int64_t)f.C * ld, 16, 32, f.what);
     if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
     WeightReduce r{partial, {gw[0], gw[1], gw[2]}, ld, splits, f.C, f.H};
     const dim3 grid((unsigned)((f.H + 31) / 32), (unsigned)((f.C + 31) / 32), 3);

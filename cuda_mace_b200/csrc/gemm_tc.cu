@@ -1303,7 +1303,7 @@ int encode_half_rows_tensor_map(CUtensorMap *tmap, const void *base, int64_t row
 }
 
 // [batches, rows, cols] of 16-bit or float32 values, rows ld elements apart, as boxes of box_cols x box_rows of one batch; the swizzle
-// spans a box's row of 64 or 128 bytes
+// spans a box's row of 32, 64 or 128 bytes
 int encode_tile_map(CUtensorMap *map, const void *base, int bytes, bool bf16, int64_t cols, int64_t rows, int64_t batches, int64_t ld,
                     int64_t batch_stride, int box_cols, int box_rows, const char *what) {
   EncodeTiledFn enc = encode_tiled_fn();
@@ -1315,7 +1315,10 @@ int encode_tile_map(CUtensorMap *map, const void *base, int bytes, bool bf16, in
   const CUtensorMapDataType type =
       bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : (bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
   const CUresult r = enc(map, type, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         box_cols * bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                         box_cols * bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                         : box_cols * bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                  : CU_TENSOR_MAP_SWIZZLE_32B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(CMACE_ERR_CUDA, "%s: cuTensorMapEncodeTiled (tile) failed (%d)", what, (int)r);
   return CMACE_OK;

@@ -512,15 +512,15 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   memset(&to_out, 0, sizeof(to_out));
   for (Matrix *m : {&x[0], &x[1], &s, &poly})
     if (!rc) rc = encode_matrix(&m->map, *m, 64, 64, false, f.what);
-  for (int k = 0; k < 2 && !rc; k++) rc = encode_matrix(&to_x[k], x[k], 32, 32, false, f.what);
-  if (!rc) rc = encode_matrix(&to_s, s, 32, 32, false, f.what);
-  if (!rc) rc = encode_matrix(&to_poly, poly, 32, 32, false, f.what);
+  for (int k = 0; k < 2 && !rc; k++) rc = encode_matrix(&to_x[k], x[k], 16, 32, false, f.what);
+  if (!rc) rc = encode_matrix(&to_s, s, 16, 32, false, f.what);
+  if (!rc) rc = encode_matrix(&to_poly, poly, 16, 32, false, f.what);
   to_master.use_map = 1;
-  if (!rc) rc = encode_tile_map(&to_master.map, master, 4, false, f.cols, f.rows, f.count, ld, f.rows * ld, 32, 32, f.what);
+  if (!rc) rc = encode_tile_map(&to_master.map, master, 4, false, f.cols, f.rows, f.count, ld, f.rows * ld, 16, 32, f.what);
   const int bytes = f.f32 ? 4 : 2;
   to_out.ptr = f.out, to_out.ld = f.cols, to_out.batch = n;
   to_out.use_map = aligned16(f.out) && (int64_t)f.cols * bytes % 16 == 0;
-  if (!rc && to_out.use_map) rc = encode_tile_map(&to_out.map, f.out, bytes, !f.f32, f.cols, f.rows, f.count, f.cols, n, 32, 32, f.what);
+  if (!rc && to_out.use_map) rc = encode_tile_map(&to_out.map, f.out, bytes, !f.f32, f.cols, f.rows, f.count, f.cols, n, 16, 32, f.what);
 
   for (int step = 0; step < f.steps && !rc; step++) {
     const Matrix &now = x[step & 1];

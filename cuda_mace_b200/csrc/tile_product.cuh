@@ -19,8 +19,9 @@
 //    memory over K = 512, three terms of it are off by 4e-6 of the largest value; in chunks by 3e-7.
 //    Compared with TF32 in three terms the operands are half as large and the instructions twice as fast.
 //
-// One persistent CTA an SM, ten warps: eight for the epilogue (two a quarter of the 128 tensor-memory lanes, each half of
-// the columns), one thread that issues the copies, one that issues the MMAs.  Two sets of accumulator columns: the
+// One persistent CTA an SM, 18 warps: 16 for the epilogue (four a quarter of the 128 tensor-memory lanes, each a quarter of
+// the columns; with eight, two a scheduler, they waited for each other's barriers, copies and special functions most of the time), one
+// thread that issues the copies, one that issues the MMAs.  Two sets of accumulator columns: the
 // products of the next chunk or tile run while the epilogue reads this one's.
 #pragma once
 #include <cuda_bf16.h>
@@ -34,10 +35,9 @@
 
 namespace cmace {
 
-constexpr int TP_EPILOGUE_WARPS = 8;
-constexpr int TP_THREADS = (TP_EPILOGUE_WARPS + 2) * 32;   // 204 registers a thread: 128 sums of a PAIR tile and their handling
+constexpr int TP_EPILOGUE_WARPS = 16;
+constexpr int TP_THREADS = (TP_EPILOGUE_WARPS + 2) * 32;   // 96 registers a thread: 64 sums of a PAIR tile and their handling
 constexpr int TP_SMEM_BUDGET = 227 * 1024 - 1024;          // without the static barriers
-constexpr int TP_BUFFER_COLS = 256;                        // one set of accumulator columns
 constexpr int TP_MAX_STAGES = 8;
 
 // GATED: D = act(x Wg) * (x Wu).  BACK: what the block's backward needs of a hidden value: h, and the gradients of both
@@ -60,6 +60,18 @@ struct TpOut {
   int use_map;
 };
 
+// Division of u < 2^31 by a number that the host knows (Granlund and Montgomery).  Every role finds its tiles by itself, and one thread issues
+// the MMAs: with divisions there, two thirds of the instructions of a short tile were these.
+struct TpDiv {
+  uint32_t mul, shift;
+};
+inline TpDiv tp_div(uint32_t d) {
+  uint32_t shift = 0;
+  while (((uint64_t)1 << shift) < d) shift++;
+  return {(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1), shift};
+}
+__device__ __forceinline__ uint32_t operator/(uint32_t u, const TpDiv &d) { return (__umulhi(d.mul, u) + u) >> d.shift; }
+
 struct TpArgs {
   TpOperand a[2], b[3];
   TpOut out[2];                  // 16-bit values, hi and lo; results (and APPLY's float32)
@@ -73,6 +85,7 @@ struct TpArgs {
   int64_t rows, cols;            // of the output
   int kblocks[2], segments;      // blocks of 64 k a segment
   int batches, splits, mt, nt;
+  TpDiv by_nt, by_mt, by_batches, by_splits;
   int64_t total;                 // tiles
   int stages;
   int a_of_last;                 // the last batch takes a[1] (its own, unbatched operand) in place of a[0]
@@ -158,9 +171,14 @@ struct TpShape {
   // for the epilogue of the tile before.
   static constexpr bool LATE = KIND == TP_BACK && !PAIR && TN == 128;
   static constexpr bool CIN_TMA = KIND == TP_APPLY && !PAIR;
-  // Bytes an epilogue warp stages its output in, pieces of 32 rows of 128 bytes; CIN_TMA: two for float32 values, which arrive, change and
-  // leave there, and half a piece for the 16-bit ones.
-  static constexpr int STAGING = CIN_TMA ? 2 * 4096 + 2048 : 4096;
+  // sets of accumulator columns, of a chunk (PAIR) or a tile; LATE: of the second segment
+  static constexpr int ACC_COLS = KIND == TP_BACK && !PAIR ? N0 + N1 : N0;
+  static constexpr int BUFFERS = LATE ? 2 : (ACC_COLS <= 128 ? 4 : 2), BUFFER_COLS = 512 / BUFFERS;
+  static_assert(LATE || ACC_COLS <= BUFFER_COLS, "accumulators");
+  static constexpr int PART = TN / 4, EACH = PART / 16;   // a warp's columns of a sum, and in groups of 16
+  // Bytes an epilogue warp stages its output in.  A piece is 32 rows of 64 bytes: 16 float32 or 32 16-bit columns; 16 of those are half a
+  // piece.  CIN_TMA: two pieces of float32, which arrive, change and leave there, and half a piece.  BACK: three arrays at once.
+  static constexpr int STAGING = CIN_TMA ? 2 * 2048 + 1024 : (KIND == TP_BACK && !PAIR ? 3 * 64 * EACH * 16 : 2048);
   static constexpr int FIT = (TP_SMEM_BUDGET - 1024 - TP_EPILOGUE_WARPS * STAGING) / STAGE;
   static constexpr int STAGES = FIT < TP_MAX_STAGES ? FIT : TP_MAX_STAGES;
   static constexpr int SMEM = STAGE * STAGES + TP_EPILOGUE_WARPS * STAGING + 1024;
@@ -172,20 +190,18 @@ struct TpTile {
 };
 __device__ __forceinline__ TpTile tp_tile(const TpArgs &g, int64_t t, int out_n, int out_m) {
   TpTile T;
-  const uint32_t u = (uint32_t)t, nt = (uint32_t)g.nt, mt = (uint32_t)g.mt;
-  const uint32_t v = u / nt;
-  T.n0 = (int)(u - v * nt) * out_n;
-  const uint32_t w = v / mt;
-  T.row0 = (int64_t)(v - w * mt) * out_m;
-  T.split = (int)(w / (uint32_t)g.batches);
+  const uint32_t u = (uint32_t)t, v = u / g.by_nt, w = v / g.by_mt;
+  T.n0 = (int)(u - v * (uint32_t)g.nt) * out_n;
+  T.row0 = (int64_t)(v - w * (uint32_t)g.mt) * out_m;
+  T.split = (int)(w / g.by_batches);
   T.batch = (int)(w - (uint32_t)T.split * (uint32_t)g.batches);
   return T;
 }
-// k blocks of a split
+// k blocks of a split (fewer than 2^25 of them, 64 splits at most)
 __device__ __forceinline__ void tp_range(const TpArgs &g, int split, int seg, int &k0, int &k1) {
-  const int n = g.kblocks[seg];
-  k0 = (int)((int64_t)n * split / g.splits);
-  k1 = (int)((int64_t)n * (split + 1) / g.splits);
+  const uint32_t n = (uint32_t)g.kblocks[seg];
+  k0 = (int)(n * (uint32_t)split / g.by_splits);
+  k1 = (int)(n * (uint32_t)(split + 1) / g.by_splits);
 }
 
 __device__ __forceinline__ void tp_report(const TpArgs &g, int code) {
@@ -234,11 +250,11 @@ __device__ __forceinline__ void tp_split2(float x, float y, float scale, uint32_
   hi = *reinterpret_cast<const uint32_t *>(&h);
   lo = *reinterpret_cast<const uint32_t *>(&l);
 }
-// sums += scale * 32 accumulator columns
-__device__ __forceinline__ void tp_add(float (&sum)[32], const uint32_t (&v)[32], float scale) {
+// sums += scale * 16 accumulator columns
+__device__ __forceinline__ void tp_add(float (&sum)[16], const uint32_t (&v)[16], float scale) {
   const unsigned long long s2 = pack2(scale, scale);
 #pragma unroll
-  for (int j = 0; j < 32; j += 2)
+  for (int j = 0; j < 16; j += 2)
     unpack2(fma2(pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), s2, pack2(sum[j], sum[j + 1])), sum[j], sum[j + 1]);
 }
 __device__ __forceinline__ uint32_t tp_bf16x2(float x, float y) {
@@ -250,22 +266,33 @@ __device__ __forceinline__ uint32_t tp_f16x2(float x, float y) {
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
+// Special-function unit without the library functions' care for subnormal results, which are zeros here: two ulp each
+__device__ __forceinline__ float tp_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float tp_sigmoid(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + tp_ex2(-1.4426950408889634f * x)));
+  return y;
+}
 // act(g); with the derivative
 template <int ACT>
 __device__ __forceinline__ float tp_act(float g) {
-  if (ACT == TP_SILU) return g * sigmoid_fast(g);
+  if (ACT == TP_SILU) return g * tp_sigmoid(g);
   return g * (0.5f * (1.0f + erff(g * 0.70710678118654752f)));
 }
 template <int ACT>
 __device__ __forceinline__ float tp_act(float g, float &d) {
   if (ACT == TP_SILU) {
-    const float s = sigmoid_fast(g);
+    const float s = tp_sigmoid(g);
     const float a = g * s;
     d = s * (1.0f + (g - a));
     return a;
   }
   const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-  d = cdf + g * (0.39894228040143268f * exp2f(-0.72134752044448170f * g * g));
+  d = cdf + g * (0.39894228040143268f * tp_ex2(-0.72134752044448170f * g * g));
   return g * cdf;
 }
 
@@ -282,40 +309,40 @@ struct TpStager {
     if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
     __syncwarp();
   }
-  // COLS 32-bit words of this lane's row at `at` (bytes into the staging buffer): rows of 128 bytes (32 words) or 64 (16)
-  template <int WORDS>
-  __device__ __forceinline__ void put(uint32_t at, const uint32_t (&w)[WORDS]) const {
+  // 16-byte chunks chunk, chunk + 1, ... of this lane's row of a piece at `at` (rows of 64 bytes) or half a piece (32 bytes)
+  template <int ROW_BYTES, int WORDS>
+  __device__ __forceinline__ void put(uint32_t at, int chunk, const uint32_t (&w)[WORDS]) const {
 #pragma unroll
     for (int c = 0; c < WORDS / 4; c++)
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                       smem + at + (uint32_t)(WORDS == 32 ? sw128_offset(lane, c) : sw64_offset(lane, c))),
-                   "r"(w[4 * c]), "r"(w[4 * c + 1]), "r"(w[4 * c + 2]), "r"(w[4 * c + 3])
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem + at + offset<ROW_BYTES>(lane, chunk + c)), "r"(w[4 * c]),
+                   "r"(w[4 * c + 1]), "r"(w[4 * c + 2]), "r"(w[4 * c + 3])
                    : "memory");
+  }
+  // the copy engine's swizzles of rows of 64 and of 32 bytes
+  template <int ROW_BYTES>
+  static __device__ __forceinline__ uint32_t offset(int row, int chunk) {
+    return ROW_BYTES == 64 ? (uint32_t)sw64_offset(row, chunk) : (uint32_t)(row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4));
   }
   __device__ __forceinline__ void send(const CUtensorMap *map, uint32_t at, int col, int64_t row, int batch) const {
     fence_proxy_async();
     __syncwarp();
     if (row < rows && col < cols && elect_one()) tma_store_3d(map, col, (int)row, batch, smem + at);
   }
-  __device__ __forceinline__ uint32_t word(uint32_t piece, int row, int w) const {
-    uint32_t v;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(smem + piece + (uint32_t)sw128_offset(row, w >> 2) + 4u * (uint32_t)(w & 3)) : "memory");
-    return v;
-  }
-  // rows that TMA cannot address: 32 float32 columns (one a lane) or 64 16-bit ones (two a lane)
+  // rows that TMA cannot address, from a piece: two rows an instruction, a lane has one float32 or two 16-bit columns
   __device__ __forceinline__ void send_rows(const TpOut &o, bool sixteen, uint32_t piece, int col, int64_t row, int batch) const {
     __syncwarp();
     const int64_t base = (int64_t)batch * o.batch;
-    const int n = rows - row < 32 ? (int)(rows - row) : 32;
-    for (int r = 0; r < n; r++) {
-      const uint32_t v = word(piece, r, lane);
+    const int w = lane & 15;
+    for (int r = lane >> 4; r < 32 && row + r < rows; r += 2) {
+      uint32_t v;
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(smem + piece + (uint32_t)sw64_offset(r, w >> 2) + 4u * (uint32_t)(w & 3)) : "memory");
       const int64_t at = base + (row + r) * o.ld + col;
       if (!sixteen) {
-        if (col + lane < cols) static_cast<uint32_t *>(o.ptr)[at + lane] = v;
+        if (col + w < cols) static_cast<uint32_t *>(o.ptr)[at + w] = v;
       } else {
-        uint16_t *p = static_cast<uint16_t *>(o.ptr) + at + 2 * lane;
-        if (col + 2 * lane < cols) p[0] = (uint16_t)v;
-        if (col + 2 * lane + 1 < cols) p[1] = (uint16_t)(v >> 16);
+        uint16_t *p = static_cast<uint16_t *>(o.ptr) + at + 2 * w;
+        if (col + 2 * w < cols) p[0] = (uint16_t)v;
+        if (col + 2 * w + 1 < cols) p[1] = (uint16_t)(v >> 16);
       }
     }
     __syncwarp();
@@ -328,14 +355,14 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
   constexpr int TERMS = PAIR ? 2 : 1;
   constexpr int STAGES = S::STAGES, ROWS = 128 * CTAS;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 5 + TP_EPILOGUE_WARPS];
+  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 9 + TP_EPILOGUE_WARPS];
   __shared__ uint32_t tmem_base_slot;
   __shared__ float block_most[3][TP_EPILOGUE_WARPS];   // GATED: of alternating tiles; BACK: of the three outputs
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t staging = smem + (uint32_t)(STAGES * S::STAGE);
   const uint32_t full = smem_u32(&bars[0]), empty = smem_u32(&bars[TP_MAX_STAGES]);
-  const uint32_t acc_full = smem_u32(&bars[2 * TP_MAX_STAGES]), acc_empty = smem_u32(&bars[2 * TP_MAX_STAGES + 2]);
-  const uint32_t drain = smem_u32(&bars[2 * TP_MAX_STAGES + 4]);
+  const uint32_t acc_full = smem_u32(&bars[2 * TP_MAX_STAGES]), acc_empty = smem_u32(&bars[2 * TP_MAX_STAGES + 4]);
+  const uint32_t drain = smem_u32(&bars[2 * TP_MAX_STAGES + 8]);
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int rank = CTAS == 2 ? (int)cluster_rank() : 0;
   const int64_t first_tile = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
@@ -345,7 +372,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       mbar_init(full + 8 * s, 1);    // the copies' expect_tx
       mbar_init(empty + 8 * s, 1);   // one commit
     }
-    for (int b = 0; b < 2; b++) {
+    for (int b = 0; b < S::BUFFERS; b++) {
       mbar_init(acc_full + 8 * b, 1);                           // one commit
       mbar_init(acc_empty + 8 * b, CTAS * TP_EPILOGUE_WARPS);   // one arrival a warp
     }
@@ -432,7 +459,11 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
     // ================================ products ================================
     if (rank == 0 && elect_one()) {
       int stage = 0, buf = 0;
-      uint32_t phase = 0, buf_phase[2] = {0, 0};
+      uint32_t phase = 0, uses = 0;   // uses: bit per set of columns, the parity of its uses
+      const auto next_buffer = [&] {
+        uses ^= 1u << buf;
+        buf = buf + 1 == S::BUFFERS ? 0 : buf + 1;
+      };
       bool ok = true;
       const int bf16 = g.in_f16 || PAIR ? 0 : 1;
       const auto product = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -446,7 +477,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       for (int64_t t = first_tile; ok && t < g.total; t += tile_step) {
         const TpTile T = tp_tile(g, t, TN, ROWS);
         if (!PAIR) {
-          if (!mbar_wait(acc_empty + 8 * buf, buf_phase[buf] ^ 1)) {
+          if (!mbar_wait(acc_empty + 8 * buf, (uses >> buf & 1) ^ 1)) {
             tp_report(g, 41);
             break;
           }
@@ -463,7 +494,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           const uint32_t idesc = tp_idesc(seg == 0 ? S::N0 : S::N1, bf16, a_mn, b_mn, ROWS);
           const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;   // 16 k, in units of 16 bytes
           if (KIND == TP_BACK) begun = 0;
-          if (S::LATE && seg == 0 && !mbar_wait(acc_empty + 8 * (buf ^ 1), buf_phase[buf ^ 1] ^ 1)) {
+          if (S::LATE && seg == 0 && !mbar_wait(acc_empty + 8 * (buf ^ 1), (uses >> (buf ^ 1) & 1) ^ 1)) {
             tp_report(g, 48);
             ok = false;
             break;
@@ -471,7 +502,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           if (S::LATE) tc_fence_after();
           for (int kb = k0; kb < k1; kb++) {
             if (PAIR) {
-              if (!mbar_wait(acc_empty + 8 * buf, buf_phase[buf] ^ 1)) {
+              if (!mbar_wait(acc_empty + 8 * buf, (uses >> buf & 1) ^ 1)) {
                 tp_report(g, 42);
                 ok = false;
                 break;
@@ -484,7 +515,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               break;
             }
             tc_fence_after();
-            uint32_t d = tmem + (uint32_t)(buf * TP_BUFFER_COLS);
+            uint32_t d = tmem + (uint32_t)(buf * S::BUFFER_COLS);
             if (KIND == TP_BACK && !PAIR) d = S::LATE ? tmem + (seg == 0 ? 0u : 256u + 128u * (uint32_t)buf) : d + (seg == 0 ? 0u : 2u * TN);
             const uint32_t sA = smem + (uint32_t)(stage * S::STAGE), sB = sA + TERMS * S::A_BYTES;
             const uint64_t a_hi = tp_desc(sA, a_mn), b_hi = tp_desc(sB, b_mn);
@@ -507,15 +538,13 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             }
             if (PAIR) {
               commit(acc_full + 8 * buf);
-              buf_phase[buf] ^= 1;
-              buf ^= 1;
+              next_buffer();
             }
           }
         }
         if (!PAIR && ok) {
           commit(acc_full + 8 * buf);
-          buf_phase[buf] ^= 1;
-          buf ^= 1;
+          next_buffer();
         }
       }
       commit(drain);   // nothing of this block's products is in flight when the columns are given back
@@ -523,19 +552,24 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
     }
   } else {
     // ================================ epilogue ================================
-    const int q = warp & 3, half = warp >> 2;
+    const int q = warp & 3, part = warp >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
     const TpStager st{staging + (uint32_t)(warp * S::STAGING), lane, g.rows, g.cols};
     const uint32_t cin_bar = drain + 8 + 8 * (uint32_t)warp;
     uint32_t cin_phase = 0;
     int buf = 0;
-    uint32_t buf_phase[2] = {0, 0};
+    uint32_t uses = 0;
+    const auto next_buffer = [&] {
+      uses ^= 1u << buf;
+      buf = buf + 1 == S::BUFFERS ? 0 : buf + 1;
+    };
     bool ok = true;
-    // groups of 32 columns of the sum that this warp owns
-    constexpr int EACH = TN / 64;   // of each of the sums
+    // groups of 16 columns of the sums that this warp owns
+    constexpr int EACH = S::EACH;
     constexpr int GROUPS = KIND == TP_BACK ? 3 * EACH : (KIND == TP_GATED ? 2 * EACH : EACH);
     constexpr int SEG0_GROUPS = KIND == TP_BACK ? 2 * EACH : GROUPS;
-    static_assert(KIND != TP_GATED || TN == 128, "blocks of 64 columns a warp");
+    static_assert(KIND != TP_GATED || TN == 128, "32 columns of both projections a warp");
+    static_assert(!PAIR || TN <= 128, "a warp's columns are of one block of 64");
     const uint32_t first_empty = CTAS == 2 ? peer_smem(acc_empty, 0) : acc_empty;
     const auto release = [&](int b) {   // this warp has read the sums
       tc_fence_before();
@@ -545,9 +579,9 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         else mbar_arrive(acc_empty + 8 * b);
       }
     };
-    // first column of group i inside the accumulator (BACK: the third group has an accumulator, or columns, of its own)
+    // first column of group i inside the accumulator (BACK: the last sum has an accumulator, or columns, of its own)
     const auto column = [&](int i) -> uint32_t {
-      const uint32_t in = (uint32_t)(half * (TN / 2) + 32 * (i % EACH));   // this warp's half of each sum
+      const uint32_t in = (uint32_t)(part * S::PART + 16 * (i % EACH));
       if (KIND == TP_GATED) return (uint32_t)(i / EACH * TN) + in;
       if (KIND == TP_BACK) return i < 2 * EACH ? (uint32_t)(i / EACH * TN) + in : (PAIR ? in : (uint32_t)(2 * TN) + in);
       return in;
@@ -557,18 +591,18 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
     for (int64_t t = first_tile; t < g.total; t += tile_step, odd ^= 1) {
       const TpTile T = tp_tile(g, t, TN, ROWS);
       const int64_t row = T.row0 + 128 * rank + 32 * q;   // first row of this warp
-      // What a Newton-Schulz epilogue adds to the product, a group of 32 columns ahead: S (hi and lo; rows of a multiple of 64 elements,
+      const int col0 = T.n0 + part * S::PART;             // first column
+      // What a Newton-Schulz epilogue adds to the product, a group of 16 columns ahead: S (hi and lo; rows of a multiple of 64 elements,
       // so that a group never runs over one's end) or X in float32.
-      const int col0 = T.n0 + half * (TN / 2);
-      uint4 cin[KIND == TP_POLY || KIND == TP_APPLY ? 8 : 1];
+      uint4 cin[KIND == TP_POLY || KIND == TP_APPLY ? 4 : 1];
       const auto fetch_cin = [&](int col) {
         if constexpr (KIND == TP_POLY || KIND == TP_APPLY) {
           const int64_t from = (int64_t)T.batch * g.cin_batch + (row + lane) * g.cin_ld + col;
           const bool in_rows = row + lane < g.rows;
 #pragma unroll
-          for (int c = 0; c < 8; c++) {
+          for (int c = 0; c < 4; c++) {
             const uint4 *p = KIND == TP_APPLY ? reinterpret_cast<const uint4 *>(static_cast<const float *>(g.cin) + from) + c
-                                              : reinterpret_cast<const uint4 *>(static_cast<const __half *>(g.cin) + from + (c >> 2) * g.cin_lo) + (c & 3);
+                                              : reinterpret_cast<const uint4 *>(static_cast<const __half *>(g.cin) + from + (c >> 1) * g.cin_lo) + (c & 1);
             cin[c] = in_rows ? __ldcg(p) : make_uint4(0, 0, 0, 0);
           }
         }
@@ -577,8 +611,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       const auto copy_cin = [&](int col, int piece) {
         if (elect_one()) {
           tma_store_wait_read();
-          mbar_arrive_expect_tx(cin_bar, 4096);
-          tma_load_3d(st.smem + 4096u * (uint32_t)piece, &g.cin_map, col, (int)row, T.batch, cin_bar);
+          mbar_arrive_expect_tx(cin_bar, 2048);
+          tma_load_3d(st.smem + 2048u * (uint32_t)piece, &g.cin_map, col, (int)row, T.batch, cin_bar);
         }
         __syncwarp();
       };
@@ -586,12 +620,12 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         if (S::CIN_TMA) copy_cin(col0, 0);
         else fetch_cin(col0);
       }
-      float acc[PAIR ? GROUPS : 1][32];
+      float acc[PAIR ? GROUPS : 1][16];
       if (PAIR) {
 #pragma unroll
         for (int i = 0; i < (PAIR ? GROUPS : 1); i++)
 #pragma unroll
-          for (int j = 0; j < 32; j++) acc[i][j] = 0.f;
+          for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
 #pragma unroll
         for (int seg = 0; seg < 2; seg++) {
           if (seg >= g.segments) break;
@@ -600,124 +634,117 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           int k0, k1;
           tp_range(g, T.split, seg, k0, k1);
           const bool last = g.a_of_last && T.batch == g.batches - 1;
+          constexpr bool TWO = KIND == TP_GATED || KIND == TP_BACK;   // both projections in the first segment
           const TpOperand &A = g.a[last ? 1 : seg];
-          const TpOperand &B0 = g.b[KIND == TP_BACK ? 2 * seg : (KIND == TP_GATED ? 0 : seg)];
-          const TpOperand &B1 = g.b[KIND == TP_GATED || (KIND == TP_BACK && seg == 0) ? 1 : (KIND == TP_BACK ? 2 : seg)];
-          // scales: one block of rows a warp; two blocks of columns at most: of both projections (GATED, BACK), or side by side
-          const int cb = T.n0 / 64 + (KIND == TP_BACK && TN == 64 ? 0 : half * (TN / 128));
-          const float *pa = A.scale ? A.scale + T.batch * A.sc_b + (row >> 6) * A.sc_i : nullptr;
-          const float *pb0 = B0.scale ? B0.scale + T.batch * B0.sc_b + cb * B0.sc_i : nullptr;
-          constexpr bool SIDE = KIND != TP_GATED && KIND != TP_BACK && TN == 256;
-          const bool two = KIND == TP_GATED || (KIND == TP_BACK && seg == 0) || SIDE;
-          const float *pb1 = !two ? pb0 : (KIND == TP_GATED || KIND == TP_BACK
-                                 ? (B1.scale ? B1.scale + T.batch * B1.sc_b + cb * B1.sc_i : nullptr)
-                                 : (pb0 && (cb + 1) * 64 < g.cols ? pb0 + B0.sc_i : pb0));   // past the last block: zeros in any scale
-          const bool a_rows = row < g.rows;   // a warp of rows past the end has zeros and no scale
-          const bool b_cols = (int64_t)cb * 64 < g.cols;
+          const TpOperand &B0 = g.b[TWO ? 2 * seg : seg];
+          // inverse scales, one block of rows a warp, one of columns (of each projection)
+          const int cb = (TWO && TN == 64 ? T.n0 : col0) >> 6;
+          const bool a_rows = row < g.rows, b_cols = (int64_t)cb * 64 < g.cols;   // past the end: zeros in any scale
+          const float *pa = A.scale && a_rows ? A.scale + T.batch * A.sc_b + (row >> 6) * A.sc_i : nullptr;
+          const float *pb0 = B0.scale && b_cols ? B0.scale + T.batch * B0.sc_b + cb * B0.sc_i : nullptr;
+          const float *pb1 = TWO && seg == 0 && g.b[1].scale && b_cols ? g.b[1].scale + cb * g.b[1].sc_i : nullptr;
           float na = 1.f, nb0 = 1.f, nb1 = 1.f;
           const auto fetch = [&](int kb) {
-            if (pa && a_rows) na = __ldcg(pa + kb * A.sc_k);
-            if (pb0 && b_cols) nb0 = __ldcg(pb0 + kb * B0.sc_k);
-            if (pb1 && b_cols) nb1 = __ldcg(pb1 + kb * B1.sc_k);
+            if (pa) na = __ldcg(pa + kb * A.sc_k);
+            if (pb0) nb0 = __ldcg(pb0 + kb * B0.sc_k);
+            if (TWO && seg == 0 && pb1) nb1 = __ldcg(pb1 + kb * B0.sc_k);   // both projections' weights are of one size
           };
           fetch(k0);
           for (int kb = k0; kb < k1; kb++) {
             const float s0 = na * nb0, s1 = na * nb1;
             if (kb + 1 < k1) fetch(kb + 1);
-            if (ok && !warp_wait(acc_full + 8 * buf, buf_phase[buf], lane)) {
+            if (ok && !warp_wait(acc_full + 8 * buf, uses >> buf & 1, lane)) {
               if (lane == 0) tp_report(g, 45);
               ok = false;
             }
             tc_fence_after();
-            const uint32_t at = lanes + (uint32_t)(buf * TP_BUFFER_COLS);
+            const uint32_t at = lanes + (uint32_t)(buf * S::BUFFER_COLS);
 #pragma unroll
             for (int i = 0; i < (PAIR ? GROUPS : 1); i++) {
               if (i < i0 || i >= i1) continue;
-              uint32_t v[32];
-              tmem_ld32(at + column(i), v);
-              const float s = (KIND == TP_BACK ? i == 1 : i >= 2) ? s1 : s0;
-              tp_add(acc[i], v, s);
+              uint32_t v[16];
+              tmem_ld16_nowait(at + column(i), v);
+              tmem_ld_wait();
+              tp_add(acc[i], v, TWO && i / EACH == 1 ? s1 : s0);
             }
             release(buf);
-            buf_phase[buf] ^= 1;
-            buf ^= 1;
+            next_buffer();
           }
         }
       } else {
-        if (ok && !warp_wait(acc_full + 8 * buf, buf_phase[buf], lane)) {
+        if (ok && !warp_wait(acc_full + 8 * buf, uses >> buf & 1, lane)) {
           if (lane == 0) tp_report(g, 46);
           ok = false;
         }
         tc_fence_after();
       }
-      const uint32_t at = lanes + (S::LATE ? 0u : (uint32_t)(buf * TP_BUFFER_COLS));
+      const uint32_t at = lanes + (S::LATE ? 0u : (uint32_t)(buf * S::BUFFER_COLS));
       // group i of the finished sums
-      const auto take = [&](int i, float (&v)[32]) {
+      const auto take = [&](int i, float (&v)[16]) {
         if (PAIR) {
 #pragma unroll
-          for (int j = 0; j < 32; j++) v[j] = acc[PAIR ? i : 0][j];
+          for (int j = 0; j < 16; j++) v[j] = acc[PAIR ? i : 0][j];
         } else {
-          uint32_t u[32];
-          tmem_ld32(at + column(i) + (S::LATE && i >= SEG0_GROUPS ? 128u * (uint32_t)buf : 0u), u);
+          uint32_t u[16];
+          tmem_ld16_nowait(at + column(i) + (S::LATE && i >= SEG0_GROUPS ? 128u * (uint32_t)buf : 0u), u);
+          tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; j++) v[j] = __uint_as_float(u[j]);
+          for (int j = 0; j < 16; j++) v[j] = __uint_as_float(u[j]);
         }
       };
 
       if constexpr (KIND == TP_GATED) {
-        const int col = T.n0 + 64 * half;
         if constexpr (PAIR) {
           float most = 0.f;
 #pragma unroll
-          for (int i = 0; i < 2; i++) {
+          for (int i = 0; i < EACH; i++) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) acc[i][j] = tp_act<ACT>(acc[i][j]) * acc[PAIR ? 2 + i : 0][j];
+            for (int j = 0; j < 16; j++) acc[i][j] = tp_act<ACT>(acc[i][j]) * acc[PAIR ? EACH + i : 0][j];
             most = tp_most(acc[i], most);
           }
-          // the block of 64 rows is this warp's and the next (or previous) quarter's of the same columns
+          // a block of 64 x 64 values is two quarters' and two parts' warps'
           most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
           if (lane == 0) block_most[odd][warp] = most;
-          tp_bar(1 + 2 * half + (q >> 1), 64);
-          const float scale = tp_scale(fmaxf(most, block_most[odd][warp ^ 1]));
-          if (lane == 0 && (q & 1) == 0 && row < g.rows && col < g.cols)
-            g.out_scale[0][(row >> 6) * g.out_scale_ld + (col >> 6)] = 1.0f / scale;
-          uint32_t w[32], lo[32];
+          tp_bar(1 + 2 * (part >> 1) + (q >> 1), 128);
+          const float scale = tp_scale(fmaxf(fmaxf(most, block_most[odd][warp ^ 1]), fmaxf(block_most[odd][warp ^ 4], block_most[odd][warp ^ 5])));
+          if (lane == 0 && (q & 1) == 0 && (part & 1) == 0 && row < g.rows && col0 < g.cols)
+            g.out_scale[0][(row >> 6) * g.out_scale_ld + (col0 >> 6)] = 1.0f / scale;
+          uint32_t w[16], lo[16];
 #pragma unroll
-          for (int j = 0; j < 32; j++)
-            tp_split2(acc[j >> 4][2 * (j & 15)], acc[j >> 4][2 * (j & 15) + 1], scale, w[j], lo[j]);
+          for (int j = 0; j < 16; j++) tp_split2(acc[j >> 3][2 * (j & 7)], acc[j >> 3][2 * (j & 7) + 1], scale, w[j], lo[j]);
           st.begin();
-          st.put(0, w);
-          st.send(&g.out[0].map, 0, col, row, 0);
+          st.put<64>(0, 0, w);
+          st.send(&g.out[0].map, 0, col0, row, 0);
           st.begin();
-          st.put(0, lo);
-          st.send(&g.out[0].map, 0, col, row, 1);
+          st.put<64>(0, 0, lo);
+          st.send(&g.out[0].map, 0, col0, row, 1);
         } else {
-          uint32_t w[32];
+          uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 2; i++) {
-            float a[32], u[32];
+          for (int i = 0; i < EACH; i++) {
+            float a[16], u[16];
             take(i, a);
-            take(2 + i, u);
+            take(EACH + i, u);
 #pragma unroll
-            for (int j = 0; j < 16; j++) w[16 * i + j] = tp_bf16x2(tp_act<ACT>(a[2 * j]) * u[2 * j], tp_act<ACT>(a[2 * j + 1]) * u[2 * j + 1]);
+            for (int j = 0; j < 8; j++) w[8 * i + j] = tp_bf16x2(tp_act<ACT>(a[2 * j]) * u[2 * j], tp_act<ACT>(a[2 * j + 1]) * u[2 * j + 1]);
           }
           st.begin();
-          st.put(0, w);
-          st.send(&g.out[0].map, 0, col, row, 0);
+          st.put<64>(0, 0, w);
+          st.send(&g.out[0].map, 0, col0, row, 0);
         }
       } else if constexpr (KIND == TP_BACK) {
         // h = act(g) u, dL/dg = dL/dh u act'(g), dL/du = dL/dh act(g)
         static_assert(!PAIR || TN == 64, "a block of 64 columns a tile");
-#pragma unroll 1
+        constexpr int ROW = 32 * EACH, PIECE = 32 * ROW;   // bytes a row, and of one array's piece
+        if (!PAIR) st.begin();
+#pragma unroll
         for (int e = 0; e < EACH; e++) {
-          const int col = col0 + 32 * e;
-          float a[32], u[32], dh[32];
+          float a[16], u[16], dh[16];
           take(e, a);
           take(EACH + e, u);
           take(2 * EACH + e, dh);
-          float most[3] = {0.f, 0.f, 0.f};
 #pragma unroll
-          for (int j = 0; j < 32; j++) {
+          for (int j = 0; j < 16; j++) {
             float d;
             const float act = tp_act<ACT>(a[j], d);
             const float h = act * u[j], dg = dh[j] * (u[j] * d), du = dh[j] * act;
@@ -725,44 +752,46 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             u[j] = dg;
             dh[j] = du;
           }
-          if (PAIR) {
-            most[0] = tp_most(u);
-            most[1] = tp_most(dh);
-            most[2] = tp_most(a);
-          }
           float scale[3] = {1.f, 1.f, 1.f};
           if (PAIR) {
+            float most[3] = {tp_most(u), tp_most(dh), tp_most(a)};
 #pragma unroll
             for (int p = 0; p < 3; p++) {
               most[p] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most[p])));
               if (lane == 0) block_most[p][warp] = most[p];
             }
-            tp_bar(1 + (q >> 1), 128);   // 64 rows x 64 columns: two quarters, both halves
+            tp_bar(1 + (q >> 1), 256);   // 64 rows x 64 columns: two quarters, all parts
 #pragma unroll
             for (int p = 0; p < 3; p++) {
-              const float m = fmaxf(fmaxf(block_most[p][warp], block_most[p][warp ^ 1]), fmaxf(block_most[p][warp ^ 4], block_most[p][warp ^ 5]));
+              float m = 0.f;
+#pragma unroll
+              for (int k = 0; k < 4; k++) m = fmaxf(m, fmaxf(block_most[p][(q & 2) + 4 * k], block_most[p][(q & 2) + 1 + 4 * k]));
               scale[p] = tp_scale(m);
-              if (lane == 0 && (q & 1) == 0 && half == 0 && row < g.rows && T.n0 < g.cols)
+              if (lane == 0 && (q & 1) == 0 && part == 0 && row < g.rows && T.n0 < g.cols)
                 g.out_scale[p][(row >> 6) * g.out_scale_ld + (T.n0 >> 6)] = 1.0f / scale[p];
             }
-            tp_bar(1 + (q >> 1), 128);   // read by all before the next tile's are written
+            tp_bar(1 + (q >> 1), 256);   // read by all before the next tile's are written
           }
 #pragma unroll
           for (int p = 0; p < 3; p++) {
-            uint32_t w[16], lo[16];
+            uint32_t w[8], lo[8];
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
+            for (int j = 0; j < 8; j++) {
               const float x = p == 0 ? u[2 * j] : (p == 1 ? dh[2 * j] : a[2 * j]);
               const float y = p == 0 ? u[2 * j + 1] : (p == 1 ? dh[2 * j + 1] : a[2 * j + 1]);
               if (PAIR) tp_split2(x, y, scale[p], w[j], lo[j]);
               else w[j] = tp_bf16x2(x, y);
             }
-            if (PAIR || p != 1) st.begin();
-            const uint32_t where = PAIR ? 0u : (p == 1 ? 2048u : 0u);
-            st.put(where, w);
-            if (PAIR) st.put(2048, lo);
-            st.send(&g.out[0].map, where, col, row, TERMS * p);
-            if (PAIR) st.send(&g.out[0].map, 2048, col, row, TERMS * p + 1);
+            if (PAIR) {
+              st.begin();
+              st.put<32>(0, 0, w);
+              st.put<32>(1024, 0, lo);
+              st.send(&g.out[0].map, 0, col0, row, 2 * p);
+              st.send(&g.out[0].map, 1024, col0, row, 2 * p + 1);
+            } else {
+              st.put<ROW>(PIECE * p, 2 * e, w);
+              if (e + 1 == EACH) st.send(&g.out[0].map, PIECE * p, col0, row, p);
+            }
           }
         }
       } else if constexpr (KIND == TP_PLAIN) {
@@ -770,70 +799,72 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         if (g.out_bf16) {
 #pragma unroll
           for (int i = 0; i < GROUPS; i += 2) {
-            if (col0 + 32 * i >= g.cols) break;
-            uint32_t w[32];
+            const int col = col0 + 16 * i;
+            if (col >= g.cols) break;
+            uint32_t w[16];
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-              float v[32];
+              float v[16];
               take(i + k, v);
 #pragma unroll
-              for (int j = 0; j < 16; j++) w[16 * k + j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
+              for (int j = 0; j < 8; j++) w[8 * k + j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
             }
             st.begin();
-            st.put(0, w);
-            if (g.out[1].use_map) st.send(&g.out[1].map, 0, col0 + 32 * i, row, batch);
-            else st.send_rows(g.out[1], true, 0, col0 + 32 * i, row, batch);
+            st.put<64>(0, 0, w);
+            if (g.out[1].use_map) st.send(&g.out[1].map, 0, col, row, batch);
+            else st.send_rows(g.out[1], true, 0, col, row, batch);
           }
         } else {
 #pragma unroll
           for (int i = 0; i < GROUPS; i++) {
-            if (col0 + 32 * i >= g.cols) break;
-            float v[32];
+            const int col = col0 + 16 * i;
+            if (col >= g.cols) break;
+            float v[16];
             take(i, v);
-            uint32_t w[32];
+            uint32_t w[16];
 #pragma unroll
-            for (int j = 0; j < 32; j++) w[j] = __float_as_uint(v[j]);
+            for (int j = 0; j < 16; j++) w[j] = __float_as_uint(v[j]);
             st.begin();
-            st.put(0, w);
-            if (g.out[1].use_map) st.send(&g.out[1].map, 0, col0 + 32 * i, row, batch);
-            else st.send_rows(g.out[1], false, 0, col0 + 32 * i, row, batch);
+            st.put<64>(0, 0, w);
+            if (g.out[1].use_map) st.send(&g.out[1].map, 0, col, row, batch);
+            else st.send_rows(g.out[1], false, 0, col, row, batch);
           }
         }
       } else {
         // Newton-Schulz: values in float32, then hi and lo (or one fp16) at a power of two that the caller has from its bounds
 #pragma unroll
         for (int i = 0; i < GROUPS; i++) {
-          const int col = col0 + 32 * i;
+          const int col = col0 + 16 * i;
           if (col >= g.cols) break;
-          float v[32];
+          const bool more = i + 1 < GROUPS && col + 16 < g.cols;
+          const uint32_t piece = S::CIN_TMA ? 2048u * (uint32_t)(i & 1) : 0u;
+          float v[16];
           take(i, v);
           if constexpr (KIND == TP_GRAM) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] *= g.alpha;
+            for (int j = 0; j < 16; j++) v[j] *= g.alpha;
           } else if constexpr (KIND == TP_POLY) {
+            const uint32_t hw[8] = {cin[0].x, cin[0].y, cin[0].z, cin[0].w, cin[1].x, cin[1].y, cin[1].z, cin[1].w};
+            const uint32_t lw[8] = {cin[2].x, cin[2].y, cin[2].z, cin[2].w, cin[3].x, cin[3].y, cin[3].z, cin[3].w};
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-              const uint32_t hw[4] = {cin[c].x, cin[c].y, cin[c].z, cin[c].w}, lw[4] = {cin[4 + c].x, cin[4 + c].y, cin[4 + c].z, cin[4 + c].w};
-#pragma unroll
-              for (int k = 0; k < 4; k++) {
-                const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&hw[k])), e = __half22float2(*reinterpret_cast<const __half2 *>(&lw[k]));
-                v[8 * c + 2 * k] = g.alpha * v[8 * c + 2 * k] + g.beta * (a.x + e.x);
-                v[8 * c + 2 * k + 1] = g.alpha * v[8 * c + 2 * k + 1] + g.beta * (a.y + e.y);
-              }
+            for (int k = 0; k < 8; k++) {
+              const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&hw[k])), e = __half22float2(*reinterpret_cast<const __half2 *>(&lw[k]));
+              v[2 * k] = g.alpha * v[2 * k] + g.beta * (a.x + e.x);
+              v[2 * k + 1] = g.alpha * v[2 * k + 1] + g.beta * (a.y + e.y);
             }
+            if (more) fetch_cin(col + 16);   // on its way while this group is put down
           } else if constexpr (S::CIN_TMA) {
-            const uint32_t piece = 4096u * (uint32_t)(i & 1);
             if (ok && !warp_wait(cin_bar, cin_phase, lane)) {
               if (lane == 0) tp_report(g, 49);
               ok = false;
             }
             cin_phase ^= 1;
 #pragma unroll
-            for (int c = 0; c < 8; c++) {
+            for (int c = 0; c < 4; c++) {
               float4 x;
               asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
                            : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
-                           : "r"(st.smem + piece + (uint32_t)sw128_offset(lane, c))
+                           : "r"(st.smem + piece + (uint32_t)sw64_offset(lane, c))
                            : "memory");
               v[4 * c] = g.alpha * v[4 * c] + g.beta * x.x;
               v[4 * c + 1] = g.alpha * v[4 * c + 1] + g.beta * x.y;
@@ -841,68 +872,62 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               v[4 * c + 3] = g.alpha * v[4 * c + 3] + g.beta * x.w;
             }
             __syncwarp();
-            if (i + 1 < GROUPS && col + 32 < g.cols) copy_cin(col + 32, (i + 1) & 1);   // on its way while this group is put down
+            if (more) copy_cin(col + 16, (i + 1) & 1);
           } else {
 #pragma unroll
-            for (int c = 0; c < 8; c++) {
+            for (int c = 0; c < 4; c++) {
               v[4 * c] = g.alpha * v[4 * c] + g.beta * __uint_as_float(cin[c].x);
               v[4 * c + 1] = g.alpha * v[4 * c + 1] + g.beta * __uint_as_float(cin[c].y);
               v[4 * c + 2] = g.alpha * v[4 * c + 2] + g.beta * __uint_as_float(cin[c].z);
               v[4 * c + 3] = g.alpha * v[4 * c + 3] + g.beta * __uint_as_float(cin[c].w);
             }
+            if (more) fetch_cin(col + 16);
           }
-          if (!S::CIN_TMA && i + 1 < GROUPS && col + 32 < g.cols) fetch_cin(col + 32);   // on its way while this group is put down
-          const uint32_t piece = S::CIN_TMA ? 4096u * (uint32_t)(i & 1) : 0u;   // copy_cin() or begin() has waited for it
           if (KIND == TP_APPLY) {
-            // out[1]: float32, the X of the next step or the result
+            // out[1]: float32, the X of the next step or the result.  CIN_TMA: copy_cin() has waited until the piece was free.
+            if (!S::CIN_TMA) st.begin();
             if (!g.out_bf16) {
-              uint32_t w[32];
+              uint32_t w[16];
 #pragma unroll
-              for (int j = 0; j < 32; j++) w[j] = __float_as_uint(v[j]);
-              if (!S::CIN_TMA) st.begin();
-              st.put(piece, w);
+              for (int j = 0; j < 16; j++) w[j] = __float_as_uint(v[j]);
+              st.put<64>(piece, 0, w);
               if (g.out[1].use_map) st.send(&g.out[1].map, piece, col, row, T.batch);
               else st.send_rows(g.out[1], false, piece, col, row, T.batch);
             } else if (g.out[1].use_map) {
-              uint32_t w[16];
+              uint32_t w[8];
 #pragma unroll
-              for (int j = 0; j < 16; j++) w[j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
-              if (!S::CIN_TMA) st.begin();
-              st.put(piece, w);
+              for (int j = 0; j < 8; j++) w[j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
+              st.put<32>(piece, 0, w);
               st.send(&g.out[1].map, piece, col, row, T.batch);
             } else {
               __nv_bfloat16 *o =
                   static_cast<__nv_bfloat16 *>(g.out[1].ptr) + (int64_t)T.batch * g.out[1].batch + (row + lane) * g.out[1].ld + col;
 #pragma unroll
-              for (int j = 0; j < 32; j++)
+              for (int j = 0; j < 16; j++)
                 if (row + lane < g.rows && col + j < g.cols) o[j] = __float2bfloat16_rn(v[j]);
             }
           }
           if (KIND != TP_APPLY || g.pair_scale != 0.f) {
             constexpr bool LOW = PAIR || KIND == TP_GRAM;   // S is also added as it is: with its low part
-            constexpr uint32_t where = S::CIN_TMA ? 8192u : 0u;
-            uint32_t w[16], lo[16];
+            constexpr uint32_t where = S::CIN_TMA ? 4096u : 0u;
+            uint32_t w[8], lo[8];
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
+            for (int j = 0; j < 8; j++) {
               if (LOW) tp_split2(v[2 * j], v[2 * j + 1], g.pair_scale, w[j], lo[j]);
               else w[j] = tp_f16x2(v[2 * j] * g.pair_scale, v[2 * j + 1] * g.pair_scale);
             }
-            if (S::CIN_TMA) {
-              if (i + 1 == GROUPS || col + 32 >= g.cols) st.begin_but_last();   // else copy_cin() has waited for the group before
-            } else {
-              st.begin();
-            }
-            st.put(where, w);
-            if (LOW) st.put(where + 2048, lo);
+            if (!S::CIN_TMA) st.begin();
+            else if (!more) st.begin_but_last();   // else copy_cin() has waited for the group before
+            st.put<32>(where, 0, w);
+            if (LOW) st.put<32>(where + 1024, 0, lo);
             st.send(&g.out[0].map, where, col, row, (LOW ? 2 : 1) * T.batch);
-            if (LOW) st.send(&g.out[0].map, where + 2048, col, row, 2 * T.batch + 1);
+            if (LOW) st.send(&g.out[0].map, where + 1024, col, row, 2 * T.batch + 1);
           }
         }
       }
       if (!PAIR) {
         release(buf);
-        buf_phase[buf] ^= 1;
-        buf ^= 1;
+        next_buffer();
       }
     }
     if (elect_one()) tma_store_wait_all();   // the copy engine reads this warp's staging buffer
@@ -1010,6 +1035,7 @@ int tp_launch(TpArgs &g, cudaStream_t st, const char *what) {
   g.nt = (int)((g.cols + TN - 1) / TN);
   g.total = (int64_t)g.mt * g.nt * g.batches * g.splits;
   if (g.total >= (int64_t)1 << 31) return fail(CMACE_ERR_UNSUPPORTED, "%s: too many tiles", what);
+  g.by_nt = tp_div((uint32_t)g.nt), g.by_mt = tp_div((uint32_t)g.mt), g.by_batches = tp_div((uint32_t)g.batches), g.by_splits = tp_div((uint32_t)g.splits);
   const auto kernel = tile_product_kernel<KIND, PAIR, TN, CTAS, ACT>;
   if (const int rc = allow_smem<tile_product_kernel<KIND, PAIR, TN, CTAS, ACT>>(S::SMEM, what)) return rc;
   cudaLaunchAttribute attr[2];

@@ -128,16 +128,21 @@ __global__ void __launch_bounds__(256) weight_reduce_kernel(const WeightReduce p
   if (out == nullptr) return;
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int64_t matrix = (int64_t)p.C * p.ld;
+  const int h = h0 + x;
+  const float *v = p.partial + which * matrix + (int64_t)(c0 + y) * p.ld + h;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (h < p.H) {
+#pragma unroll 4
+    for (int s = 0; s < p.splits; s++, v += 3 * matrix)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (c0 + y + 8 * i < p.C) sum[i] += __ldcg(v + (int64_t)(8 * i) * p.ld);
+  }
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const int c = c0 + y + 8 * i, h = h0 + x;
-    float sum = 0.f;
-    if (c < p.C && h < p.H) {
-      const float *v = p.partial + which * matrix + (int64_t)c * p.ld + h;
-      for (int s = 0; s < p.splits; s++) sum += __ldcg(v + (int64_t)s * 3 * matrix);
-      if (which < 2) out[(int64_t)c * p.H + h] = (T)sum;
-    }
-    tile[y + 8 * i][x] = sum;
+    const int c = c0 + y + 8 * i;
+    if (which < 2 && c < p.C && h < p.H) out[(int64_t)c * p.H + h] = (T)sum[i];
+    tile[y + 8 * i][x] = sum[i];
   }
   if (which < 2) return;
   __syncthreads();
@@ -185,8 +190,8 @@ static int set_hidden_out(TpArgs &g, const Matrix &m, int box_cols, bool bf16, c
   return encode_matrix(&g.out[0].map, m, box_cols, 32, bf16, what);
 }
 // rows of a caller's array: by TMA where it can address them
-static int set_user_out(TpArgs &g, void *ptr, bool f32, int64_t rows, int cols, const char *what) {
-  TpOut &o = g.out[1];
+static int set_user_out(TpArgs &g, void *ptr, bool f32, int64_t rows, int cols, const char *what, int which = 1) {
+  TpOut &o = g.out[which];
   o.ptr = ptr;
   o.ld = cols;
   o.batch = rows * (int64_t)cols;
@@ -229,13 +234,14 @@ static int run_prep(const PrepArgs &p, int64_t blocks, cudaStream_t st, const ch
 }
 
 // Splits of the weight gradients' sum over M, by what a number costs in units of a block of 64 rows of one tile (0.3 to 0.5 us): rounds
-// of tiles, a few blocks each for filling the ring and putting the sums down, and the traffic of the partial sums.
+// of tiles, a few blocks each for filling the ring and putting the sums down, the kernel that adds the splits and its traffic.
 static int weight_splits(int64_t M, int C, int H) {
   const int64_t tiles = 3 * ((C + 127) / 128) * (int64_t)((H + 127) / 128), kb = blocks64(M);
   int best = 1;
   double least = 0;
   for (int s = 1; s <= 64 && s <= kb; s++) {
-    const double cost = (double)((tiles * s + 147) / 148) * ((double)((kb + s - 1) / s) + 6.0) + s * 3.0 * C * H * 6e-6;
+    double cost = (double)((tiles * s + 147) / 148) * ((double)((kb + s - 1) / s) + 6.0);
+    if (s > 1) cost += 10.0 + s * 3.0 * C * H * 6e-6;
     if (s == 1 || cost < least) best = s, least = cost;
   }
   return best;
@@ -282,7 +288,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   Matrix hidden = new_matrix(w, f.f32, f.M, f.H, 3);   // dg, du, h
   const int64_t ld = up(f.H, 4);
   const int splits = weight_splits(f.M, f.C, f.H);
-  float *partial = want_w ? w.take<float>((int64_t)splits * 3 * f.C * ld) : nullptr;
+  float *partial = want_w && splits > 1 ? w.take<float>((int64_t)splits * 3 * f.C * ld) : nullptr;
   if (!w.base) return CMACE_OK;
   const bool bf16 = !f.f32;
   int rc = run_prep(prep, blocks, f.st, f.what);
@@ -295,8 +301,8 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   set_operand(g.b[2], wd, true);
   g.segments = 2;
   g.kblocks[0] = g.kblocks[1] = blocks64(f.C);
-  const bool wide = !f.f32 && pairs_fill(f.M, f.H, 1, 128);   // tiles of 128 columns, 32 a warp
-  if (!rc) rc = set_hidden_out(g, hidden, wide ? 32 : 16, bf16, f.what);
+  const bool wide = !f.f32 && pairs_fill(f.M, f.H, 1, 128);   // tiles of 128 columns
+  if (!rc) rc = set_hidden_out(g, hidden, 16, bf16, f.what);
   if (!rc) rc = f.act == TP_SILU ? launch_back<TP_SILU>(f, wide, g) : launch_back<TP_GELU>(f, wide, g);
   if (want_x) {
     g = new_args(f.M, f.C, f.status);
@@ -309,7 +315,27 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
     if (!rc) rc = set_user_out(g, gx, f.f32, f.M, f.C, f.what);
     if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
   }
-  if (want_w) {
+  if (want_w && splits == 1) {
+    if (gw[0] || gw[1]) {
+      g = new_args(f.C, f.H, f.status);
+      set_operand(g.a[0], x, false);
+      set_operand(g.b[0], gw[0] && gw[1] ? hidden : hidden.part(gw[0] ? 0 : 1), false);
+      g.batches = gw[0] && gw[1] ? 2 : 1;
+      g.out_of_batch = 1;
+      g.kblocks[0] = blocks64(f.M);
+      if (!rc) rc = set_user_out(g, gw[0] ? gw[0] : gw[1], f.f32, f.C, f.H, f.what, 0);
+      if (!rc && g.batches == 2) rc = set_user_out(g, gw[1], f.f32, f.C, f.H, f.what, 1);
+      if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
+    }
+    if (gw[2]) {
+      g = new_args(f.H, f.C, f.status);
+      set_operand(g.a[0], hidden.part(2), false);
+      set_operand(g.b[0], gy, false);
+      g.kblocks[0] = blocks64(f.M);
+      if (!rc) rc = set_user_out(g, gw[2], f.f32, f.H, f.C, f.what);
+      if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
+    }
+  } else if (want_w) {
     // batches dg, du and h: x^T dg, x^T du and, as its transpose, dy^T h
     g = new_args(f.C, f.H, f.status);
     set_operand(g.a[0], x, false);

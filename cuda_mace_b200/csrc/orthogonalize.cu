@@ -10,6 +10,7 @@
 // every step, and the host makes powers of two of the bounds.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "tile_product.cuh"
 
@@ -87,13 +88,16 @@ __global__ void __launch_bounds__(NS_THREADS) ns_prep_kernel(const NsPrep p) {
 // ---- all steps in one kernel, for matrices whose shorter side fits a tile ------------------------------------------------------
 // X [side <= 128, columns] (a tall matrix is read and written transposed) stays on the SM: as fp16 pairs in shared memory, which
 // serve S = X X^T (contracted index inside a row) and P X (contracted index over the rows) from the same image, and in float32 in
-// tensor memory, 128 lanes x 256 columns.  S, then P = b S + c S S in its place, are a second image.  A matrix of more than 256 columns
-// (128 in a cluster) is spread over the CTAs of a cluster: each has its columns of X and a part of S, which they sum
-// through distributed shared memory (each its share of the rows, in the order of the ranks) and hand to all.
+// tensor memory.  S, then P = b S + c S S, go the same way.  A matrix of more than 128 columns is spread over the CTAs of a cluster: each
+// has its columns of X and a part of S; every CTA adds up the parts' rows that are its own, in the order of the ranks, and hands their pairs
+// to all.  (A stack that fills the SMs keeps up to 256 columns in one CTA.)
 //
 // The three products of a step and what stands between them form a chain, so the block works on one thing at a time: 16 warps for the
 // elementwise phases (a warp of each quarter of the lanes has a quarter of the columns), one thread issues MMAs.  Terms with a low part come
 // first: the sum is small while they are added, and the truncating additions that count are the 4 a 64 k of hi hi.
+//
+// A_TMEM (up to 128 columns a CTA): the A operands are in tensor memory too, since an MMA of 128 columns with both operands in shared
+// memory takes 85 to 100 cycles instead of 64.  Columns: sum 128, X 128, hi and lo of S or P 128, of X 128.  With 256 columns: sum, X.
 constexpr int NSF_THREADS = 512;
 constexpr int NSF_STAGE_LD = 65;          // floats a row of the transposing buffer
 constexpr int NSF_IMAGE = 128 * 128;      // 128 rows of 64 fp16
@@ -112,13 +116,13 @@ struct NsFused {
   float sx[NSF_MAX_STEPS + 1], ss[NSF_MAX_STEPS], sp[NSF_MAX_STEPS];   // powers of two of X, S and P of every step
 };
 
+__device__ __forceinline__ void peer_store2(uint32_t addr, uint32_t x, uint32_t y) {
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ float4 peer_load4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
-}
-__device__ __forceinline__ void peer_store2(uint32_t addr, uint32_t x, uint32_t y) {
-  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
 }
 __device__ __forceinline__ void smem_store4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -128,38 +132,64 @@ __device__ __forceinline__ uint4 smem_load4(uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
-// hi and lo of COLS values of one row (16-byte pieces `piece`, ... of its 128 bytes) into the images at hi and lo
-template <int COLS>
-__device__ __forceinline__ void put_pairs(uint32_t hi, uint32_t lo, int row, int piece, const float (&v)[COLS], float scale) {
-#pragma unroll
-  for (int c = 0; c < COLS / 8; c++) {
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) tp_split2(v[8 * c + 2 * k], v[8 * c + 2 * k + 1], scale, h[k], l[k]);
-    const uint32_t at = (uint32_t)sw128_offset(row, piece + c);
-    smem_store4(hi + at, h[0], h[1], h[2], h[3]);
-    smem_store4(lo + at, l[0], l[1], l[2], l[3]);
+// One thread of every CTA of a cluster arrives on the barrier of each, for its block (which has met at bar.sync before), and all threads
+// wait on their own CTA's: some 700 cycles where barrier.cluster of 512 threads takes 2 000.
+__device__ __forceinline__ void peer_arrive(uint32_t bar, uint32_t rank) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(peer_smem(bar, rank)) : "memory");
+}
+__device__ __forceinline__ bool peer_wait(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (clock64() - t0 > GT_TIMEOUT_CYCLES) return false;
   }
 }
+// two packed fp16 of each part as the floats that they stand for, times their power of two
+__device__ __forceinline__ float2 pair_value(uint32_t hi, uint32_t lo) {
+  const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&hi)), y = __half22float2(*reinterpret_cast<const __half2 *>(&lo));
+  return make_float2(x.x + y.x, x.y + y.y);
+}
+// WORDS packed values of one row (16-byte pieces `piece`, ... of its 128 bytes) into an image
+template <int WORDS>
+__device__ __forceinline__ void put_row(uint32_t image, int row, int piece, const uint32_t (&w)[WORDS]) {
+#pragma unroll
+  for (int c = 0; c < WORDS / 4; c++) smem_store4(image + (uint32_t)sw128_offset(row, piece + c), w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+}
+template <int N>
+__device__ __forceinline__ void split_row(const float (&v)[N], float scale, uint32_t (&hi)[N / 2], uint32_t (&lo)[N / 2]) {
+#pragma unroll
+  for (int k = 0; k < N / 2; k++) tp_split2(v[2 * k], v[2 * k + 1], scale, hi[k], lo[k]);
+}
 
-template <bool CLUSTER>
+template <int CLUSTER, bool A_TMEM>
 __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_constant__ NsFused g) {
+  static_assert(CLUSTER == 1 || A_TMEM, "up to 128 columns a CTA of a cluster");
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t done_bar;
+  __shared__ __align__(8) uint64_t done_bar, peer_bars[2];
   __shared__ uint32_t tmem_base_slot;
   __shared__ double sums[NSF_THREADS / 32 + 1];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char *const generic = smem_raw + (base - raw);
   const uint32_t x_hi = base, x_lo = base + (uint32_t)(g.chunks * NSF_IMAGE), s_hi = base + (uint32_t)(2 * g.chunks * NSF_IMAGE);
-  const uint32_t s_lo = s_hi + 2 * NSF_IMAGE, part = s_hi + NSF_S_BYTES;   // part: CLUSTER, this CTA's S in float32
+  const uint32_t s_lo = s_hi + 2 * NSF_IMAGE, part = s_hi + NSF_S_BYTES;   // part: this CTA's part of S
   float *const stage = reinterpret_cast<float *>(generic + (s_hi - base));   // before and after the steps
   const uint32_t bar = smem_u32(&done_bar);
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31, q = warp & 3, group = warp >> 2;
   const int row = 32 * q + lane;
-  const uint32_t rank = CLUSTER ? cluster_rank() : 0;
+  const uint32_t rank = CLUSTER > 1 ? cluster_rank() : 0;
 
   if (tid == 0) {
     mbar_init(bar, 1);
+    mbar_init(smem_u32(&peer_bars[0]), CLUSTER);
+    mbar_init(smem_u32(&peer_bars[1]), CLUSTER);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) tmem_alloc(smem_u32(&tmem_base_slot), 512);
@@ -167,9 +197,10 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = (uint32_t)uniform((int)tmem_base_slot);
-  const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16), master = acc + 256;
+  const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16), master = acc + (A_TMEM ? 128 : 256);
+  const uint32_t s_tmem = acc + 256, x_tmem = acc + 384;   // A_TMEM: hi in 64 columns, lo in the next 64
   grid_begin();
-  const int64_t matrix = blockIdx.x / (unsigned)g.cluster;
+  const int64_t matrix = blockIdx.x / (unsigned)CLUSTER;
   const int64_t size = (int64_t)g.side * g.length;
   const int col0 = (int)rank * g.columns;
   uint32_t phase = 0;
@@ -177,92 +208,135 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
 
   // ---- the update into tensor memory, and its norm -----------------------------------------------------------------------
   double square = 0;
-  for (int ch = 0; ch < g.chunks; ch++) {
-    float v[16];
-    if (!g.tall) {
+  constexpr int AHEAD = A_TMEM ? 2 : 1;   // chunks on their way at once
+  float v[AHEAD][16];
+  // a thread's 16 values of a chunk: of one column and every eighth row, or (tall) of one row and every fourth column
+  struct Mine {
+    int64_t first, step;
+    int n;   // of them in the matrix
+  };
+  const auto mine_of = [&](int ch) {
+    Mine m;
+    const int r0 = g.tall ? tid & 127 : tid >> 6, in = 64 * ch + (g.tall ? tid >> 7 : tid & 63), end = min(g.columns, g.length - col0);
+    m.n = g.tall ? (r0 < g.side ? (end - in + 3) / 4 : 0) : (in < end ? (g.side - r0 + 7) / 8 : 0);
+    m.first = matrix * size + (g.tall ? (int64_t)(col0 + in) * g.side + r0 : (int64_t)r0 * g.length + col0 + in);
+    m.step = g.tall ? 4 * (int64_t)g.side : 8 * (int64_t)g.length;
+    return m;
+  };
+  const auto fetch = [&](int ch, float (&to)[16]) {
+    const Mine m = mine_of(ch);
+    if (g.bf16) {
+      const __nv_bfloat16 *from = static_cast<const __nv_bfloat16 *>(g.src) + m.first;
 #pragma unroll
-      for (int k = 0; k < 16; k++) {
-        const int e = tid + NSF_THREADS * k, r = e >> 6, cc = 64 * ch + (e & 63), c = col0 + cc;
-        v[k] = r < g.side && cc < g.columns && c < g.length ? ns_load(g.src, matrix * size + (int64_t)r * g.length + c, g.bf16) : 0.f;
-      }
+      for (int k = 0; k < 16; k++, from += m.step) to[k] = k < m.n ? __bfloat162float(*from) : 0.f;
     } else {
+      const float *from = static_cast<const float *>(g.src) + m.first;
+#pragma unroll
+      for (int k = 0; k < 16; k++, from += m.step) to[k] = k < m.n ? *from : 0.f;
+    }
+  };
+#pragma unroll
+  for (int a = 0; a < AHEAD; a++)
+    if (a < g.chunks) fetch(a, v[a]);
+  for (int first = 0; first < g.chunks; first += AHEAD) {
+#pragma unroll
+    for (int a = 0; a < AHEAD; a++) {
+      const int ch = first + a;
+      if (ch >= g.chunks) break;
+      __syncthreads();
 #pragma unroll
       for (int k = 0; k < 16; k++) {
-        const int e = tid + NSF_THREADS * k, r = e & 127, cc = 64 * ch + (e >> 7), c = col0 + cc;
-        v[k] = r < g.side && cc < g.columns && c < g.length ? ns_load(g.src, matrix * size + (int64_t)c * g.side + r, g.bf16) : 0.f;
+        const int e = tid + NSF_THREADS * k;
+        stage[g.tall ? (e & 127) * NSF_STAGE_LD + (e >> 7) : (e >> 6) * NSF_STAGE_LD + (e & 63)] = v[a][k];
+        square = fma((double)v[a][k], (double)v[a][k], square);
       }
-    }
-    __syncthreads();
+      if (ch + AHEAD < g.chunks) fetch(ch + AHEAD, v[a]);
+      __syncthreads();
+      uint32_t w[16];
 #pragma unroll
-    for (int k = 0; k < 16; k++) {
-      const int e = tid + NSF_THREADS * k;
-      if (!g.tall) stage[(e >> 6) * NSF_STAGE_LD + (e & 63)] = v[k];
-      else stage[(e & 127) * NSF_STAGE_LD + (e >> 7)] = v[k];
-      square = fma((double)v[k], (double)v[k], square);
+      for (int k = 0; k < 16; k++) w[k] = __float_as_uint(stage[row * NSF_STAGE_LD + 16 * group + k]);
+      tmem_st16(master + (uint32_t)(64 * ch + 16 * group), w);
     }
-    __syncthreads();
-    uint32_t w[16];
-#pragma unroll
-    for (int k = 0; k < 16; k++) w[k] = __float_as_uint(stage[row * NSF_STAGE_LD + 16 * group + k]);
-    tmem_st16(master + (uint32_t)(64 * ch + 16 * group), w);
   }
   tmem_st_wait();
+  // sums in the same order everywhere: of a warp's lanes, of the warps, of the CTAs of a cluster
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
   if (lane == 0) sums[warp] = square;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < NSF_THREADS / 32; w++) square += sums[w];
-    sums[NSF_THREADS / 32] = square;
-  }
-  if (CLUSTER) {
+  square = sums[lane & 15];
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
+  if (CLUSTER > 1) {
+    if (tid == 0) sums[NSF_THREADS / 32] = square;
     cluster_sync();
     square = 0;
-    for (int r = 0; r < g.cluster; r++) {
-      double v;
-      asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(peer_smem(smem_u32(&sums[NSF_THREADS / 32]), (uint32_t)r)) : "memory");
-      square += v;
+#pragma unroll
+    for (int r = 0; r < CLUSTER; r++) {
+      double other;
+      asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(other) : "r"(peer_smem(smem_u32(&sums[NSF_THREADS / 32]), (uint32_t)r)) : "memory");
+      square += other;
     }
-  } else {
-    __syncthreads();
-    square = sums[NSF_THREADS / 32];
   }
   const float inv = (float)(1.0 / (sqrt(square) + g.eps));
+  // a chunk's pairs of X: shared memory, and tensor memory where it has room
+  const auto put_x = [&](int ch, const float (&x)[16], float scale) {
+    uint32_t hi[8], lo[8];
+    split_row(x, scale, hi, lo);
+    put_row(x_hi + (uint32_t)(ch * NSF_IMAGE), row, 2 * group, hi);
+    put_row(x_lo + (uint32_t)(ch * NSF_IMAGE), row, 2 * group, lo);
+    if (A_TMEM) {
+      tmem_st8(x_tmem + (uint32_t)(32 * ch + 8 * group), hi);
+      tmem_st8(x_tmem + (uint32_t)(64 + 32 * ch + 8 * group), lo);
+    }
+  };
   for (int ch = 0; ch < g.chunks; ch++) {
     const uint32_t at = master + (uint32_t)(64 * ch + 16 * group);
     uint32_t w[16];
-    float v[16];
+    float x[16];
     tmem_ld16_nowait(at, w);
     tmem_ld_wait();
 #pragma unroll
-    for (int k = 0; k < 16; k++) v[k] = __uint_as_float(w[k]) * inv;
+    for (int k = 0; k < 16; k++) x[k] = __uint_as_float(w[k]) * inv;
 #pragma unroll
-    for (int k = 0; k < 16; k++) w[k] = __float_as_uint(v[k]);
+    for (int k = 0; k < 16; k++) w[k] = __float_as_uint(x[k]);
     tmem_st16(at, w);
-    put_pairs(x_hi + (uint32_t)(ch * NSF_IMAGE), x_lo + (uint32_t)(ch * NSF_IMAGE), row, 2 * group, v, g.sx[0]);
+    put_x(ch, x, g.sx[0]);
   }
   tmem_st_wait();
 
-  const int side16 = (g.side + 15) & ~15, n_x = 64 * g.chunks;
-  const uint32_t idesc_s = tp_idesc(side16, 0, 0, 0), idesc_x = tp_idesc(n_x, 0, 0, 1);
-  // operands are written, sums are read: products a*b of `steps16` times 16 k, three terms, the ones with a low part first
-  const auto products = [&](uint32_t a_hi, uint32_t a_lo, uint32_t b_hi, uint32_t b_lo, int steps16, bool b_mn, uint32_t idesc) {
+  const int side16 = (g.side + 15) & ~15;
+  const uint32_t idesc_s = tp_idesc(side16, 0, 0, 0), idesc_x = tp_idesc(64 * g.chunks, 0, 0, 1);
+  // Operands are written, sums are read: products of A and B over `steps16` times 16 k, three terms, the ones with a low part first.
+  // Descriptors of an image's steps differ by constants: one thread issues all MMAs, at some ten cycles an instruction.
+  const uint64_t lo_of_x = (uint64_t)(g.chunks * (NSF_IMAGE >> 4)), lo_of_s = 2 * (NSF_IMAGE >> 4);
+  const uint64_t x_desc = tp_desc(x_hi, 0), s_desc = tp_desc(s_hi, 0);
+  // X with its rows as k: runs of 64 columns an image apart
+  const uint64_t x_rows = (tp_desc(x_hi, 1) & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(NSF_IMAGE >> 4) << 16);
+  const auto products = [&](uint32_t a_tmem, uint64_t A, uint64_t a_lo, uint64_t B, uint64_t b_lo, int steps16, auto b_mn, uint32_t idesc) {
+    constexpr bool B_MN = decltype(b_mn)::value;
+    constexpr int MOST = B_MN || A_TMEM ? 8 : 16;   // 128 rows, 128 or 256 columns
     fence_proxy_async();
     tc_fence_before();
     __syncthreads();
     if (warp == 0 && elect_one()) {
       tc_fence_after();
-      const auto A = [&](uint32_t image, int k) { return tp_desc(image + (uint32_t)((k >> 2) * NSF_IMAGE + (k & 3) * 32), 0); };
-      const auto B = [&](uint32_t image, int k) {
-        // MN-major: 16 rows of the image a step, runs of 64 columns an image apart
-        if (b_mn) return (tp_desc(image + (uint32_t)(k * 2048), 1) & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(NSF_IMAGE >> 4) << 16);
-        return tp_desc(image + (uint32_t)((k >> 2) * NSF_IMAGE + (k & 3) * 32), 0);
+      const auto product = [&](int k, uint64_t al, uint64_t bl, uint32_t accumulate) {
+        const uint64_t b = B + bl + (uint64_t)(B_MN ? k * 128 : (k >> 2) * (NSF_IMAGE >> 4) + (k & 3) * 2);
+        if (A_TMEM) umma_f16_ts(tmem, a_tmem + (uint32_t)(8 * k) + (al ? 64u : 0u), b, idesc, accumulate);
+        else umma_16(tmem, A + al + (uint64_t)((k >> 2) * (NSF_IMAGE >> 4) + (k & 3) * 2), b, idesc, accumulate);
       };
-      for (int k = 0; k < steps16; k++) {
-        umma_16(tmem, A(a_lo, k), B(b_hi, k), idesc, k > 0);
-        umma_16(tmem, A(a_hi, k), B(b_lo, k), idesc, 1);
+#pragma unroll
+      for (int k = 0; k < MOST; k++) {
+        if (k >= steps16) break;
+        product(k, a_lo, 0, k > 0);
+        product(k, 0, b_lo, 1);
       }
-      for (int k = 0; k < steps16; k++) umma_16(tmem, A(a_hi, k), B(b_hi, k), idesc, 1);
+#pragma unroll
+      for (int k = 0; k < MOST; k++) {
+        if (k >= steps16) break;
+        product(k, 0, 0, 1);
+      }
       umma_commit(bar);
     }
     if (ok && !warp_wait(bar, phase, lane)) {   // a block that gave up goes on: the others of its cluster meet it at the barriers
@@ -272,73 +346,110 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
     phase ^= 1;
     tc_fence_after();
   };
-  const int s_chunk = group >> 1, s_piece = 4 * (group & 1);   // this thread's 32 columns of S
-  const uint32_t s_at = (uint32_t)(s_chunk * NSF_IMAGE);
+  const uint32_t s_first = tmem + 256, x_first = tmem + 384;   // lane 0 of the A operands
+  const int s_piece = 4 * (group & 1);                          // this thread's 32 columns of S
+  const uint32_t s_at = (uint32_t)((group >> 1) * NSF_IMAGE);
+  const bool mine = 32 * group < side16;   // columns from side16 on are not written by a product, and none reads what is made of them
   const int x_steps = (min(g.columns, g.length - col0 > 0 ? g.length - col0 : 1) + 15) / 16;
 
+  uint32_t peer_phase = 0;
+  const auto meet = [&](int which) {
+    const uint32_t peer_bar = smem_u32(&peer_bars[which]);
+    __syncthreads();
+    if (tid < CLUSTER) peer_arrive(peer_bar, (uint32_t)tid);
+    if (ok && !peer_wait(peer_bar, peer_phase)) {
+      if (lane == 0 && g.status) atomicCAS(g.status, 0, 50);
+      ok = false;
+    }
+  };
   for (int step = 0; step < g.steps; step++) {
     const float sx = g.sx[step], ss = g.ss[step], sp = g.sp[step];
-    uint32_t u[32];
-    float v[32];
+    uint32_t u[32] = {}, hi[16] = {}, lo[16] = {};
+    float s[32];
     // S = X X^T
-    products(x_hi, x_lo, x_hi, x_lo, x_steps, false, idesc_s);
-    tmem_ld32(acc + (uint32_t)(32 * group), u);
+    products(x_first, x_desc, lo_of_x, x_desc, lo_of_x, x_steps, std::false_type{}, idesc_s);
+    if (mine) tmem_ld32(acc + (uint32_t)(32 * group), u);
     const float to_s = 1.0f / (sx * sx);
-    const bool mine = 32 * group < side16;   // columns that the product has written
 #pragma unroll
-    for (int j = 0; j < 32; j++) v[j] = mine && 32 * group + j < side16 ? __uint_as_float(u[j]) * to_s : 0.f;
-    if (!CLUSTER) {
-      put_pairs(s_hi + s_at, s_lo + s_at, row, s_piece, v, ss);
+    for (int j = 0; j < 32; j++) s[j] = __uint_as_float(u[j]) * to_s;
+    if (CLUSTER == 1) {
+      if (mine) {
+        split_row(s, ss, hi, lo);
+        put_row(s_hi + s_at, row, s_piece, hi);
+        put_row(s_lo + s_at, row, s_piece, lo);
+      }
     } else {
-      // part: [128 rows][32 pieces of four columns], the piece changed by the row so that a warp's stores and loads meet all banks
+      // part: [128 rows][32 pieces of four columns], the piece changed by the row: a warp's accesses meet all banks.  Between SMs it is bytes
+      // that count, 11 to 12 a cycle here whichever side moves them: each CTA fetches its share of the rows and sends pairs.
+      constexpr int SHARE = 128 / CLUSTER;
 #pragma unroll
       for (int c = 0; c < 8; c++)
-        smem_store4(part + (uint32_t)(row * 512 + (((8 * group + c) ^ (row & 31)) << 4)), __float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]),
-                    __float_as_uint(v[4 * c + 2]), __float_as_uint(v[4 * c + 3]));
-      cluster_sync();
-      const int rows_each = 128 / g.cluster;
-      for (int e = tid; e < rows_each * 32; e += NSF_THREADS) {
-        const int r = (int)rank * rows_each + (e >> 5), piece = e & 31;
-        const uint32_t at = part + (uint32_t)(r * 512 + ((piece ^ (r & 31)) << 4));
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p = 0; p < g.cluster; p++) {
-          const float4 x = peer_load4(peer_smem(at, (uint32_t)p));
-          sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
-        }
-        uint32_t h0, h1, l0, l1;
-        tp_split2(sum.x, sum.y, ss, h0, l0);
-        tp_split2(sum.z, sum.w, ss, h1, l1);
+        smem_store4(part + (uint32_t)(row * 512 + (((8 * group + c) ^ (row & 31)) << 4)), __float_as_uint(s[4 * c]), __float_as_uint(s[4 * c + 1]),
+                    __float_as_uint(s[4 * c + 2]), __float_as_uint(s[4 * c + 3]));
+      meet(0);
+#pragma unroll
+      for (int e = tid; e < SHARE * 32; e += NSF_THREADS) {   // four columns of a row: a warp's loads are 512 bytes on end
+        const int r = (int)rank * SHARE + (e >> 5), piece = e & 31;
+        const uint32_t from = part + (uint32_t)(r * 512 + ((piece ^ (r & 31)) << 4));
+        float4 x[CLUSTER];
+#pragma unroll
+        for (int p = 0; p < CLUSTER; p++) x[p] = peer_load4(peer_smem(from, (uint32_t)p));
+        float sum[4] = {};
+#pragma unroll
+        for (int p = 0; p < CLUSTER; p++) sum[0] += x[p].x, sum[1] += x[p].y, sum[2] += x[p].z, sum[3] += x[p].w;
+        uint32_t h[2], l[2];
+        split_row(sum, ss, h, l);
         const uint32_t to = (uint32_t)((piece >> 4) * NSF_IMAGE + sw128_offset(r, (piece & 15) >> 1) + (piece & 1) * 8);
-        for (int p = 0; p < g.cluster; p++) {
-          peer_store2(peer_smem(s_hi + to, (uint32_t)p), h0, h1);
-          peer_store2(peer_smem(s_lo + to, (uint32_t)p), l0, l1);
+#pragma unroll
+        for (int p = 0; p < CLUSTER; p++) {
+          peer_store2(peer_smem(s_hi + to, (uint32_t)p), h[0], h[1]);
+          peer_store2(peer_smem(s_lo + to, (uint32_t)p), l[0], l[1]);
         }
       }
-      asm volatile("fence.proxy.async;" ::: "memory");   // the images are read by tensor cores of all CTAs
-      cluster_sync();
-    }
-    // P = b S + c S S, in the place of S
-    products(s_hi, s_lo, s_hi, s_lo, side16 / 16, false, idesc_s);
-    tmem_ld32(acc + (uint32_t)(32 * group), u);
-    const float from_ss = g.c / (ss * ss), from_s = g.b / ss;
+      meet(1);   // products() fences the images for the tensor cores
+      peer_phase ^= 1;
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-      const uint32_t at = s_at + (uint32_t)sw128_offset(row, s_piece + c);
-      const uint4 h = smem_load4(s_hi + at), l = smem_load4(s_lo + at);
-      const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
+      for (int c = 0; c < 4; c++) {
+        const uint32_t at = s_at + (uint32_t)sw128_offset(row, s_piece + c);
+        const uint4 h = smem_load4(s_hi + at), l = smem_load4(s_lo + at);
+        hi[4 * c] = h.x, hi[4 * c + 1] = h.y, hi[4 * c + 2] = h.z, hi[4 * c + 3] = h.w;
+        lo[4 * c] = l.x, lo[4 * c + 1] = l.y, lo[4 * c + 2] = l.z, lo[4 * c + 3] = l.w;
+      }
+      const float from = 1.0f / ss;
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&hw[k])), y = __half22float2(*reinterpret_cast<const __half2 *>(&lw[k]));
-        const int j = 8 * c + 2 * k;
-        v[j] = mine && 32 * group + j < side16 ? __uint_as_float(u[j]) * from_ss + from_s * (x.x + y.x) : 0.f;
-        v[j + 1] = mine && 32 * group + j < side16 ? __uint_as_float(u[j + 1]) * from_ss + from_s * (x.y + y.y) : 0.f;
+      for (int k = 0; k < 16; k++) {
+        const float2 x = pair_value(hi[k], lo[k]);
+        s[2 * k] = x.x * from, s[2 * k + 1] = x.y * from;
       }
     }
-    put_pairs(s_hi + s_at, s_lo + s_at, row, s_piece, v, sp);
+    if (A_TMEM) {
+      tmem_st16(s_tmem + (uint32_t)(16 * group), hi);
+      tmem_st16(s_tmem + (uint32_t)(64 + 16 * group), lo);
+      tmem_st_wait();
+    }
+    // P = b S + c S S
+    products(s_first, s_desc, lo_of_s, s_desc, lo_of_s, side16 / 16, std::false_type{}, idesc_s);
+    if (mine) {
+      tmem_ld32(acc + (uint32_t)(32 * group), u);
+      const float from_ss = g.c / (ss * ss);
+#pragma unroll
+      for (int j = 0; j < 32; j++) s[j] = g.b * s[j] + from_ss * __uint_as_float(u[j]);
+      split_row(s, sp, hi, lo);
+      if (!A_TMEM) {
+        put_row(s_hi + s_at, row, s_piece, hi);
+        put_row(s_lo + s_at, row, s_piece, lo);
+      }
+    }
+    if (A_TMEM) {
+      tmem_st16(s_tmem + (uint32_t)(16 * group), hi);
+      tmem_st16(s_tmem + (uint32_t)(64 + 16 * group), lo);
+      tmem_st_wait();
+    }
     // X = a X + P X
-    products(s_hi, s_lo, x_hi, x_lo, side16 / 16, true, idesc_x);
+    products(s_first, s_desc, lo_of_s, x_rows, lo_of_x, side16 / 16, std::true_type{}, idesc_x);
     const float from_p = 1.0f / (sp * sx);
     const bool last = step + 1 == g.steps;
+#pragma unroll(A_TMEM ? 2 : 1)
     for (int ch = 0; ch < g.chunks; ch++) {
       const uint32_t col = (uint32_t)(64 * ch + 16 * group);
       uint32_t w[16], m[16];
@@ -352,22 +463,25 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
 #pragma unroll
         for (int k = 0; k < 16; k++) m[k] = __float_as_uint(x[k]);
         tmem_st16(master + col, m);
-        put_pairs(x_hi + (uint32_t)(ch * NSF_IMAGE), x_lo + (uint32_t)(ch * NSF_IMAGE), row, 2 * group, x, g.sx[step + 1]);
+        put_x(ch, x, g.sx[step + 1]);
       } else {
-        __syncthreads();   // every warp has its sums: the image of P is free; and the stores of the chunk before are done
+        __syncthreads();   // every warp has its sums: the image of S is free; and the stores of the chunk before are done
 #pragma unroll
         for (int k = 0; k < 16; k++) stage[row * NSF_STAGE_LD + 16 * group + k] = x[k];
         __syncthreads();
-#pragma unroll 4
-        for (int k = 0; k < 16; k++) {
-          const int e = tid + NSF_THREADS * k;
-          const int r = g.tall ? e & 127 : e >> 6, in = g.tall ? e >> 7 : e & 63, c = col0 + 64 * ch + in;
-          if (r < g.side && 64 * ch + in < g.columns && c < g.length) {
-            const int64_t at = matrix * size + (g.tall ? (int64_t)c * g.side + r : (int64_t)r * g.length + c);
-            const float y = stage[r * NSF_STAGE_LD + in];
-            if (g.bf16) static_cast<__nv_bfloat16 *>(g.out)[at] = __float2bfloat16_rn(y);
-            else static_cast<float *>(g.out)[at] = y;
-          }
+        const Mine m = mine_of(ch);
+        const float *from = stage + (g.tall ? (tid & 127) * NSF_STAGE_LD + (tid >> 7) : (tid >> 6) * NSF_STAGE_LD + (tid & 63));
+        const int next = g.tall ? 4 : 8 * NSF_STAGE_LD;
+        if (g.bf16) {
+          __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(g.out) + m.first;
+#pragma unroll
+          for (int k = 0; k < 16; k++, to += m.step)
+            if (k < m.n) *to = __float2bfloat16_rn(from[k * next]);
+        } else {
+          float *to = static_cast<float *>(g.out) + m.first;
+#pragma unroll
+          for (int k = 0; k < 16; k++, to += m.step)
+            if (k < m.n) *to = from[k * next];
         }
       }
     }
@@ -375,6 +489,10 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
   }
   tc_fence_before();
   __syncthreads();
+  if (CLUSTER > 1) {   // nobody reads or writes a block's shared memory after it has left
+    __syncwarp();
+    cluster_sync();
+  }
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
@@ -439,6 +557,24 @@ static int fused_cluster(int64_t count, int64_t rows, int cols) {
   return p;
 }
 
+template <int CLUSTER, bool A_TMEM>
+static int launch_fused(const NsCall &f, const NsFused &g, int smem) {
+  if (const int rc = allow_smem<ns_fused_kernel<CLUSTER, A_TMEM>>(smem, f.what)) return rc;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CLUSTER, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(f.count * CLUSTER));
+  cfg.blockDim = dim3(NSF_THREADS);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = f.st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = CLUSTER > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_fused_kernel<CLUSTER, A_TMEM>, g);
+  if (e != cudaSuccess) return fail(CMACE_ERR_CUDA, "%s: %s", f.what, cudaGetErrorString(e));
+  return check_launch(f.what);
+}
+
 static int run_fused(const NsCall &f, int cluster) {
   NsFused g;
   memset(&g, 0, sizeof(g));
@@ -457,21 +593,12 @@ static int run_fused(const NsCall &f, int cluster) {
     most = most_odd(f.a, f.b, f.c, most);
   }
   const int smem = 2 * g.chunks * NSF_IMAGE + NSF_S_BYTES + (cluster > 1 ? 128 * 512 : 0) + 1024;
-  const auto kernel = cluster > 1 ? ns_fused_kernel<true> : ns_fused_kernel<false>;
-  if (const int rc = cluster > 1 ? allow_smem<ns_fused_kernel<true>>(smem, f.what) : allow_smem<ns_fused_kernel<false>>(smem, f.what)) return rc;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)cluster, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(f.count * cluster));
-  cfg.blockDim = dim3(NSF_THREADS);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = f.st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, g);
-  if (e != cudaSuccess) return fail(CMACE_ERR_CUDA, "%s: %s", f.what, cudaGetErrorString(e));
-  return check_launch(f.what);
+  switch (cluster) {
+    case 2: return launch_fused<2, true>(f, g, smem);
+    case 4: return launch_fused<4, true>(f, g, smem);
+    case 8: return launch_fused<8, true>(f, g, smem);
+    default: return g.chunks <= 2 ? launch_fused<1, true>(f, g, smem) : launch_fused<1, false>(f, g, smem);
+  }
 }
 // how far singular values can grow is what fp16 operands and float32 sums have to hold
 static int check_growth(const NsCall &f) {
@@ -578,7 +705,7 @@ static int run_orthogonalize(bool f32, const void *update, int64_t count, int64_
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(CMACE_ERR_ARG, "%s: the workspace has to be aligned to 256 bytes", what);
   if (!(std::isfinite(a) && std::isfinite(b) && std::isfinite(c)) || !(eps >= 0)) return fail(CMACE_ERR_ARG, "%s: bad coefficients or eps", what);
   NsCall f{f32, update, out, count, rows, cols, steps, a, b, c, eps, status, (cudaStream_t)stream, what};
-  if (int rc = check_growth(f)) return rc;
+  if (const int rc = check_growth(f)) return rc;
   Carve need{nullptr};
   orthogonalize(f, need);
   if (bytes < need.used) return fail(CMACE_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes, (long long)need.used);

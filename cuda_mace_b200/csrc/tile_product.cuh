@@ -89,6 +89,7 @@ struct TpArgs {
   int64_t total;                 // tiles
   int stages;
   int a_of_last;                 // the last batch takes a[1] (its own, unbatched operand) in place of a[0]
+  int out_of_batch;              // PLAIN: batch b goes to out[b], an array of its own
   int out_bf16;                  // PLAIN, APPLY's result: 16-bit output
   int in_f16;                    // 16-bit operands are fp16, not bf16
 };
@@ -178,7 +179,7 @@ struct TpShape {
   static constexpr int PART = TN / 4, EACH = PART / 16;   // a warp's columns of a sum, and in groups of 16
   // Bytes an epilogue warp stages its output in.  A piece is 32 rows of 64 bytes: 16 float32 or 32 16-bit columns; 16 of those are half a
   // piece.  CIN_TMA: two pieces of float32, which arrive, change and leave there, and half a piece.  BACK: three arrays at once.
-  static constexpr int STAGING = CIN_TMA ? 2 * 2048 + 1024 : (KIND == TP_BACK && !PAIR ? 3 * 64 * EACH * 16 : 2048);
+  static constexpr int STAGING = CIN_TMA ? 2 * 2048 + 1024 : (KIND == TP_BACK && !PAIR ? 3 * 1024 : 2048);
   static constexpr int FIT = (TP_SMEM_BUDGET - 1024 - TP_EPILOGUE_WARPS * STAGING) / STAGE;
   static constexpr int STAGES = FIT < TP_MAX_STAGES ? FIT : TP_MAX_STAGES;
   static constexpr int SMEM = STAGE * STAGES + TP_EPILOGUE_WARPS * STAGING + 1024;
@@ -735,8 +736,6 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       } else if constexpr (KIND == TP_BACK) {
         // h = act(g) u, dL/dg = dL/dh u act'(g), dL/du = dL/dh act(g)
         static_assert(!PAIR || TN == 64, "a block of 64 columns a tile");
-        constexpr int ROW = 32 * EACH, PIECE = 32 * ROW;   // bytes a row, and of one array's piece
-        if (!PAIR) st.begin();
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
           float a[16], u[16], dh[16];
@@ -789,13 +788,15 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               st.send(&g.out[0].map, 0, col0, row, 2 * p);
               st.send(&g.out[0].map, 1024, col0, row, 2 * p + 1);
             } else {
-              st.put<ROW>(PIECE * p, 2 * e, w);
-              if (e + 1 == EACH) st.send(&g.out[0].map, PIECE * p, col0, row, p);
+              if (p == 0) st.begin();
+              st.put<32>(1024 * p, 0, w);
+              st.send(&g.out[0].map, 1024 * p, col0 + 16 * e, row, p);
             }
           }
         }
       } else if constexpr (KIND == TP_PLAIN) {
-        const int batch = T.split * g.batches + T.batch;
+        const TpOut &out = g.out[g.out_of_batch ? T.batch : 1];
+        const int batch = g.out_of_batch ? 0 : T.split * g.batches + T.batch;
         if (g.out_bf16) {
 #pragma unroll
           for (int i = 0; i < GROUPS; i += 2) {
@@ -811,8 +812,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             }
             st.begin();
             st.put<64>(0, 0, w);
-            if (g.out[1].use_map) st.send(&g.out[1].map, 0, col, row, batch);
-            else st.send_rows(g.out[1], true, 0, col, row, batch);
+            if (out.use_map) st.send(&out.map, 0, col, row, batch);
+            else st.send_rows(out, true, 0, col, row, batch);
           }
         } else {
 #pragma unroll
@@ -826,8 +827,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             for (int j = 0; j < 16; j++) w[j] = __float_as_uint(v[j]);
             st.begin();
             st.put<64>(0, 0, w);
-            if (g.out[1].use_map) st.send(&g.out[1].map, 0, col, row, batch);
-            else st.send_rows(g.out[1], false, 0, col, row, batch);
+            if (out.use_map) st.send(&out.map, 0, col, row, batch);
+            else st.send_rows(out, false, 0, col, row, batch);
           }
         }
       } else {
@@ -1024,8 +1025,11 @@ inline TpArgs new_args(int64_t rows, int64_t cols, int32_t *status) {
 }
 inline int blocks64(int64_t n) { return (int)((n + 63) / 64); }
 
-// Pairs of CTAs where their tiles of 256 rows fill the SMs
-inline bool pairs_fill(int64_t rows, int64_t cols, int64_t times, int tn) { return (rows + 255) / 256 * ((cols + tn - 1) / tn) * times >= 74; }
+// Pairs of CTAs where their tiles of 256 rows fill the SMs and the last of them is not mostly empty
+inline bool pairs_fill(int64_t rows, int64_t cols, int64_t times, int tn) {
+  const int64_t mt = (rows + 255) / 256;
+  return mt * ((cols + tn - 1) / tn) * times >= 74 && 9 * mt * 256 <= 10 * up(rows, 128);
+}
 
 template <int KIND, bool PAIR, int TN, int CTAS, int ACT = TP_SILU>
 int tp_launch(TpArgs &g, cudaStream_t st, const char *what) {

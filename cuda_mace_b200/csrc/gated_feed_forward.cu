@@ -202,28 +202,30 @@ static int set_user_out(TpArgs &g, void *ptr, bool f32, int64_t rows, int cols, 
   return CMACE_OK;
 }
 
-static bool long_enough(bool f32, const TpArgs &g) {
-  static const int least = getenv("TP_LEAST") ? atoi(getenv("TP_LEAST")) : 8;
-  return !f32 || g.kblocks[0] + (g.segments > 1 ? g.kblocks[1] : 0) >= least * g.splits;
+static TpCost cost_of(const TpArgs &g, bool pair) {
+  return {g.rows, g.cols, (g.kblocks[0] + (g.segments > 1 ? g.kblocks[1] : 0)) / g.splits + 1, (int64_t)g.batches * g.splits, pair};
 }
 template <int ACT>
 static int launch_gated(const FeedForward &f, TpArgs &g) {
-  const bool pairs = pairs_fill(g.rows, g.cols, 1, 128) && long_enough(f.f32, g);
+  const TpCost cost = cost_of(g, f.f32);
+  const bool pairs = cost(2, 128, 256) < cost(1, 128, 256);
   if (f.f32) return pairs ? tp_launch<TP_GATED, true, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_GATED, true, 128, 1, ACT>(g, f.st, f.what);
   return pairs ? tp_launch<TP_GATED, false, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_GATED, false, 128, 1, ACT>(g, f.st, f.what);
 }
 template <int ACT>
-static int launch_back(const FeedForward &f, bool wide, TpArgs &g) {
-  if (wide) return tp_launch<TP_BACK, false, 128, 2, ACT>(g, f.st, f.what);
-  if (!f.f32) return tp_launch<TP_BACK, false, 64, 1, ACT>(g, f.st, f.what);
-  return pairs_fill(g.rows, g.cols, 1, 64) && long_enough(true, g) ? tp_launch<TP_BACK, true, 64, 2, ACT>(g, f.st, f.what)
-                                                                  : tp_launch<TP_BACK, true, 64, 1, ACT>(g, f.st, f.what);
+static int launch_back(const FeedForward &f, TpArgs &g) {
+  const TpCost cost = cost_of(g, f.f32);   // half of its blocks have two projections' columns, half one's
+  if (f.f32)
+    return cost(2, 64, 96) < cost(1, 64, 96) ? tp_launch<TP_BACK, true, 64, 2, ACT>(g, f.st, f.what) : tp_launch<TP_BACK, true, 64, 1, ACT>(g, f.st, f.what);
+  return cost(2, 128, 192) < cost(1, 64, 96) ? tp_launch<TP_BACK, false, 128, 2, ACT>(g, f.st, f.what)
+                                             : tp_launch<TP_BACK, false, 64, 1, ACT>(g, f.st, f.what);
 }
 static int launch_plain(bool pair, TpArgs &g, cudaStream_t st, const char *what) {
-  const int64_t times = (int64_t)g.batches * g.splits;
-  if (pair) return pairs_fill(g.rows, g.cols, times, 128) && long_enough(true, g) ? tp_launch<TP_PLAIN, true, 128, 2>(g, st, what) : tp_launch<TP_PLAIN, true, 128, 1>(g, st, what);
-  if (g.cols > 128 && pairs_fill(g.rows, g.cols, times, 256)) return tp_launch<TP_PLAIN, false, 256, 2>(g, st, what);
-  return pairs_fill(g.rows, g.cols, times, 128) ? tp_launch<TP_PLAIN, false, 128, 2>(g, st, what) : tp_launch<TP_PLAIN, false, 128, 1>(g, st, what);
+  const TpCost cost = cost_of(g, pair);
+  const int64_t one = cost(1, 128, 128), two = cost(2, 128, 128);
+  if (pair) return two < one ? tp_launch<TP_PLAIN, true, 128, 2>(g, st, what) : tp_launch<TP_PLAIN, true, 128, 1>(g, st, what);
+  if (cost(2, 256, 256) < std::min(one, two)) return tp_launch<TP_PLAIN, false, 256, 2>(g, st, what);
+  return two < one ? tp_launch<TP_PLAIN, false, 128, 2>(g, st, what) : tp_launch<TP_PLAIN, false, 128, 1>(g, st, what);
 }
 
 static int run_prep(const PrepArgs &p, int64_t blocks, cudaStream_t st, const char *what) {
@@ -301,9 +303,8 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   set_operand(g.b[2], wd, true);
   g.segments = 2;
   g.kblocks[0] = g.kblocks[1] = blocks64(f.C);
-  const bool wide = !f.f32 && pairs_fill(f.M, f.H, 1, 128);   // tiles of 128 columns
   if (!rc) rc = set_hidden_out(g, hidden, 16, bf16, f.what);
-  if (!rc) rc = f.act == TP_SILU ? launch_back<TP_SILU>(f, wide, g) : launch_back<TP_GELU>(f, wide, g);
+  if (!rc) rc = f.act == TP_SILU ? launch_back<TP_SILU>(f, g) : launch_back<TP_GELU>(f, g);
   if (want_x) {
     g = new_args(f.M, f.C, f.status);
     set_operand(g.a[0], hidden.part(0), true);

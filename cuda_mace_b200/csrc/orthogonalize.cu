@@ -3,10 +3,10 @@
 // value s goes to a s + b s^3 + c s^5, so all of them meet near 1.
 //
 // What the precision asks for: a small singular value is multiplied by a up to `steps` times (485 with the usual coefficients), and so is
-// what rounding adds along its direction.  X itself is therefore kept in float32 and a X formed from that; the operands of the
-// products may be rounded further, since what that adds lies in the rows or in the columns of the large values, turns their
-// vectors by the rounding and is not multiplied.  float32 takes pairs of fp16 values (tile_product.cuh), bf16 single fp16 values (2^-12 instead of
-// the result's 2^-9).  fp16's range suffices without looking at the values: |X|_2 <= 1 bounds every entry of X, S and b S + c S S in
+// what rounding adds along its direction.  X itself is therefore kept to 22 bits or more, as a pair of fp16 values (tile_product.cuh), and
+// a X formed from both; the operands of the products may be rounded further, since what that adds lies in the rows or in the columns of the large values, turns their
+// vectors by the rounding and is not multiplied.  float32 takes pairs there too, bf16 the high values alone (2^-12 instead of the
+// result's 2^-9).  fp16's range suffices without looking at the values: |X|_2 <= 1 bounds every entry of X, S and b S + c S S in
 // every step, and the host makes powers of two of the bounds.
 #include <algorithm>
 #include <cmath>
@@ -22,11 +22,9 @@ constexpr int NS_CHUNKS = 64;   // partial sums of a matrix at most
 struct NsPrep {
   const void *src;
   double *partial;   // [count][chunks]
-  float *x;          // [count][rows][ld]
-  __half *h;         // [count][terms][rows][ld]
-  int terms;
+  __half *h;         // [count][hi, lo][rows][ld]
   int64_t count, rows;
-  int cols, ld, chunks, bf16;
+  int cols, ld, chunks, bf16, blocks;   // blocks of ns_prep_kernel a matrix
   double eps;
   float scale;
 };
@@ -34,17 +32,44 @@ struct NsPrep {
 __device__ __forceinline__ float ns_load(const void *p, int64_t i, int bf16) {
   return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]) : static_cast<const float *>(p)[i];
 }
+// values i .. i + n - 1 (n <= 8) of an array; wide: i is a multiple of eight of an array aligned to 16 bytes, and all eight are there
+__device__ __forceinline__ void ns_load8(float (&v)[8], const void *p, int64_t i, int n, int bf16, bool wide) {
+  if (!wide) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = k < n ? ns_load(p, i + k, bf16) : 0.f;
+  } else if (bf16) {
+    const uint4 x = __ldg(reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p) + i));
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[2 * k] = __uint_as_float(w[k] << 16), v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+  } else {
+    const float4 *f = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+    const float4 x = __ldg(f), y = __ldg(f + 1);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+  }
+}
 
-// Squares in float64: neither large nor small updates leave the range, and the sum of a matrix is one value whatever its size.
+// Squares of eight values in float32 where those neither leave its range nor fall below it, in float64 otherwise and from there on: neither
+// large nor small updates are lost, and the sum of a matrix is one value whatever its size.
 __global__ void __launch_bounds__(NS_THREADS) ns_norm_kernel(const NsPrep p) {
   __shared__ double sums[NS_THREADS / 32];
   grid_begin();
-  const int64_t n = p.rows * p.cols, m = blockIdx.x / p.chunks, c = blockIdx.x - m * p.chunks;
-  const int64_t i0 = n * c / p.chunks, i1 = n * (c + 1) / p.chunks;
+  const int64_t n = p.rows * p.cols, m = blockIdx.x / (unsigned)p.chunks, c = blockIdx.x - m * p.chunks, n8 = (n + 7) / 8;
+  const int64_t i0 = n8 * c / p.chunks, i1 = n8 * (c + 1) / p.chunks;
+  const bool wide = n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.src) & 15) == 0;
   double s = 0;
+#pragma unroll 4
   for (int64_t i = i0 + threadIdx.x; i < i1; i += NS_THREADS) {
-    const double v = ns_load(p.src, m * n + i, p.bf16);
-    s = fma(v, v, s);
+    float v[8], t = 0.f;
+    ns_load8(v, p.src, m * n + 8 * i, (int)min((int64_t)8, n - 8 * i), p.bf16, wide);
+#pragma unroll
+    for (int k = 0; k < 8; k++) t = fmaf(v[k], v[k], t);
+    if (t > 1e-30f && t < 1e30f) {
+      s += t;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; k++) s = fma((double)v[k], (double)v[k], s);
+    }
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
@@ -56,32 +81,33 @@ __global__ void __launch_bounds__(NS_THREADS) ns_norm_kernel(const NsPrep p) {
   }
 }
 
-// A block of 32 rows x 32 columns of a matrix a CTA of 256 threads.
+// X of the first step as pairs; a thread takes eight columns of a row, four times.
 __global__ void __launch_bounds__(NS_THREADS) ns_prep_kernel(const NsPrep p) {
   grid_begin();
-  const int64_t per = (p.rows + 31) / 32 * ((p.cols + 31) / 32);
-  const int64_t m = blockIdx.x / per, b = blockIdx.x - m * per;
-  const int nb = (p.cols + 31) / 32;
-  const int64_t row0 = b / nb * 32;
-  const int col = (int)(b - b / nb * nb) * 32 + (threadIdx.x & 31);
+  const int64_t m = blockIdx.x / (unsigned)p.blocks, b = blockIdx.x - m * p.blocks;
   double s = 0;   // every warp sums the partial sums, in the same order
   for (int c = threadIdx.x & 31; c < p.chunks; c += 32) s += __ldcg(p.partial + m * p.chunks + c);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
   const float inv = (float)(1.0 / (sqrt(s) + p.eps));
-  if (col >= p.cols) return;
+  const int per_row = (p.cols + 7) / 8;
+  const int64_t items = p.rows * per_row, plane = p.rows * p.ld;
+  const bool wide = p.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(p.src) & 15) == 0;
+  __half *hi = p.h + m * 2 * plane;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const int64_t row = row0 + (threadIdx.x >> 5) + 8 * i;
-    if (row >= p.rows) break;
-    const float v = ns_load(p.src, (m * p.rows + row) * p.cols + col, p.bf16) * inv;
-    const int64_t at = (m * p.rows + row) * p.ld + col;
-    p.x[at] = v;
-    const int64_t plane = p.rows * p.ld, to = m * p.terms * plane + row * p.ld + col;
-    uint32_t h, l;
-    tp_split2(v, 0.f, p.scale, h, l);
-    p.h[to] = __ushort_as_half((unsigned short)h);
-    if (p.terms == 2) p.h[to + plane] = __ushort_as_half((unsigned short)l);
+    const int64_t item = (b * 4 + i) * NS_THREADS + threadIdx.x;
+    if (item >= items) break;
+    const int64_t row = item / per_row;
+    const int col = (int)(item - row * per_row) * 8;
+    float v[8];
+    ns_load8(v, p.src, (m * p.rows + row) * p.cols + col, p.cols - col < 8 ? p.cols - col : 8, p.bf16, wide);
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) tp_split2(v[2 * k] * inv, v[2 * k + 1] * inv, p.scale, h[k], l[k]);
+    __half *to = hi + row * p.ld + col;   // rows have a multiple of 64 elements
+    *reinterpret_cast<uint4 *>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4 *>(to + plane) = make_uint4(l[0], l[1], l[2], l[3]);
   }
 }
 
@@ -541,10 +567,11 @@ struct NsCall {
 
 template <int KIND>
 static int launch_ns(bool pair, TpArgs &g, cudaStream_t st, const char *what) {
-  const bool wide = !pair && g.cols > 128 && pairs_fill(g.rows, g.cols, g.batches, 256);
-  if (wide) return tp_launch<KIND, false, 256, 2>(g, st, what);
-  if (pairs_fill(g.rows, g.cols, g.batches, 128)) return pair ? tp_launch<KIND, true, 128, 2>(g, st, what) : tp_launch<KIND, false, 128, 2>(g, st, what);
-  return pair ? tp_launch<KIND, true, 128, 1>(g, st, what) : tp_launch<KIND, false, 128, 1>(g, st, what);
+  const TpCost cost{g.rows, g.cols, g.kblocks[0], g.batches, pair};
+  const int64_t one = cost(1, 128, 128), two = cost(2, 128, 128);
+  if (pair) return two < one ? tp_launch<KIND, true, 128, 2>(g, st, what) : tp_launch<KIND, true, 128, 1>(g, st, what);
+  if (cost(2, 256, 256) < std::min(one, two)) return tp_launch<KIND, false, 256, 2>(g, st, what);
+  return two < one ? tp_launch<KIND, false, 128, 2>(g, st, what) : tp_launch<KIND, false, 128, 1>(g, st, what);
 }
 
 // CTAs a matrix for the kernel above, 0: it does not fit
@@ -620,30 +647,26 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   const int chunks = (int)std::min<int64_t>(NS_CHUNKS, (n + 8191) / 8192);
   double *partial = w.take<double>(f.count * chunks);
   Matrix x[2];
-  for (Matrix &m : x) m = new_matrix(w, f.f32, f.rows, f.cols, f.count, 64, false);
+  for (Matrix &m : x) m = new_matrix(w, true, f.rows, f.cols, f.count, 64, false);
   Matrix s = new_matrix(w, true, side, side, f.count, 64, false), poly = new_matrix(w, f.f32, side, side, f.count, 64, false);
-  const int64_t ld = x[0].ld;
-  float *master = w.take<float>(f.count * f.rows * ld);
   if (!w.base) return CMACE_OK;
 
   double most = 1.0;   // bound of the singular values
   float sx = fp16_scale(most);
-  NsPrep p{f.src, partial, master, reinterpret_cast<__half *>(x[0].at), x[0].terms, f.count, f.rows, f.cols, (int)ld, chunks, f.f32 ? 0 : 1, f.eps, sx};
+  const int blocks = (int)((f.rows * ((f.cols + 7) / 8) + 4 * NS_THREADS - 1) / (4 * NS_THREADS));
+  NsPrep p{f.src, partial, reinterpret_cast<__half *>(x[0].at), f.count, f.rows, f.cols, (int)x[0].ld, chunks, f.f32 ? 0 : 1, blocks, f.eps, sx};
   launch_chained(ns_norm_kernel, dim3((unsigned)(f.count * chunks)), dim3(NS_THREADS), (size_t)0, f.st, p);
-  launch_chained(ns_prep_kernel, dim3((unsigned)(f.count * ((f.rows + 31) / 32) * ((f.cols + 31) / 32))), dim3(NS_THREADS), (size_t)0, f.st, p);
+  launch_chained(ns_prep_kernel, dim3((unsigned)(f.count * blocks)), dim3(NS_THREADS), (size_t)0, f.st, p);
   int rc = check_launch(f.what);
-  // maps, read and written: of X twice, S, P, the float32 X and the result
+  // maps, read and written: of X twice, S, P and the result
   CUtensorMap to_x[2], to_s, to_poly;
-  TpOut to_master, to_out;
-  memset(&to_master, 0, sizeof(to_master));
+  TpOut to_out;
   memset(&to_out, 0, sizeof(to_out));
   for (Matrix *m : {&x[0], &x[1], &s, &poly})
     if (!rc) rc = encode_matrix(&m->map, *m, 64, 64, false, f.what);
   for (int k = 0; k < 2 && !rc; k++) rc = encode_matrix(&to_x[k], x[k], 16, 32, false, f.what);
   if (!rc) rc = encode_matrix(&to_s, s, 16, 32, false, f.what);
   if (!rc) rc = encode_matrix(&to_poly, poly, 16, 32, false, f.what);
-  to_master.use_map = 1;
-  if (!rc) rc = encode_tile_map(&to_master.map, master, 4, false, f.cols, f.rows, f.count, ld, f.rows * ld, 16, 32, f.what);
   const int bytes = f.f32 ? 4 : 2;
   to_out.ptr = f.out, to_out.ld = f.cols, to_out.batch = n;
   to_out.use_map = aligned16(f.out) && (int64_t)f.cols * bytes % 16 == 0;
@@ -677,11 +700,10 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     set_operand(g.a[0], wide ? poly : now, true);
     set_operand(g.b[0], wide ? now : poly, !wide);
     g.out[0].map = to_x[(step + 1) & 1];
-    g.out[1] = last ? to_out : to_master;
-    g.out_bf16 = last && !f.f32;
-    g.cin_map = to_master.map;
-    g.cin = master, g.cin_ld = ld, g.cin_batch = f.rows * ld;
-    g.alpha = 1.0f / (sp * sx), g.beta = (float)f.a, g.pair_scale = last ? 0.f : sn;
+    g.out[1] = to_out;
+    g.out_bf16 = !f.f32;
+    g.cin = now.at, g.cin_ld = now.ld, g.cin_batch = 2 * now.plane(), g.cin_lo = now.plane();
+    g.alpha = 1.0f / (sp * sx), g.beta = (float)f.a / sx, g.pair_scale = last ? 0.f : sn;
     if (!rc) rc = launch_ns<TP_APPLY>(f.f32, g, f.st, f.what);
     most = most_next;
     sx = sn;
@@ -692,7 +714,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
 static int check_ns(const char *what, int64_t count, int64_t rows, int cols, int steps) {
   if (count < 0 || rows < 1 || cols < 1 || steps < 1 || steps > 100)
     return fail(CMACE_ERR_ARG, "%s: bad sizes: %lld matrices of %lld x %d, %d steps", what, (long long)count, (long long)rows, cols, steps);
-  if (rows > 1 << 20 || cols > 1 << 20 || count * ((rows + 31) / 32) * ((cols + 31) / 32) >= (int64_t)1 << 31)
+  if (rows > 1 << 20 || cols > 1 << 20 || count * ((rows + 31) / 32) * ((cols + 31) / 32) >= (int64_t)1 << 30)
     return fail(CMACE_ERR_UNSUPPORTED, "%s: sides up to 2^20 and 2^31 blocks of 32 x 32", what);
   return CMACE_OK;
 }

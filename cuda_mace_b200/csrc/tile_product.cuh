@@ -74,11 +74,10 @@ __device__ __forceinline__ uint32_t operator/(uint32_t u, const TpDiv &d) { retu
 
 struct TpArgs {
   TpOperand a[2], b[3];
-  TpOut out[2];                  // 16-bit values, hi and lo; results (and APPLY's float32)
+  TpOut out[2];                  // 16-bit values, hi and lo; results
   float *out_scale[3];           // PAIR outputs with block scales: inverse scale of every 64 x 64 block
   int64_t out_scale_ld, out_scale_batch;
-  const void *cin;               // POLY: S (hi, and cin_lo elements behind it lo); APPLY: X in float32
-  CUtensorMap cin_map;           // APPLY of 16-bit operands: the same X in boxes of 32 x 32
+  const void *cin;               // POLY: S, APPLY: X: hi, and cin_lo elements behind it lo
   int64_t cin_ld, cin_batch, cin_lo;
   float alpha, beta, cin_scale, pair_scale;   // D = alpha * product + beta * cin / ..., see the epilogues
   int32_t *status;
@@ -171,15 +170,14 @@ struct TpShape {
   // BACK's sums of 128 columns do not fit twice: the second segment goes first, into columns that alternate, and the first waits
   // for the epilogue of the tile before.
   static constexpr bool LATE = KIND == TP_BACK && !PAIR && TN == 128;
-  static constexpr bool CIN_TMA = KIND == TP_APPLY && !PAIR;
   // sets of accumulator columns, of a chunk (PAIR) or a tile; LATE: of the second segment
   static constexpr int ACC_COLS = KIND == TP_BACK && !PAIR ? N0 + N1 : N0;
   static constexpr int BUFFERS = LATE ? 2 : (ACC_COLS <= 128 ? 4 : 2), BUFFER_COLS = 512 / BUFFERS;
   static_assert(LATE || ACC_COLS <= BUFFER_COLS, "accumulators");
   static constexpr int PART = TN / 4, EACH = PART / 16;   // a warp's columns of a sum, and in groups of 16
   // Bytes an epilogue warp stages its output in.  A piece is 32 rows of 64 bytes: 16 float32 or 32 16-bit columns; 16 of those are half a
-  // piece.  CIN_TMA: two pieces of float32, which arrive, change and leave there, and half a piece.  BACK: three arrays at once.
-  static constexpr int STAGING = CIN_TMA ? 2 * 2048 + 1024 : (KIND == TP_BACK && !PAIR ? 3 * 1024 : 2048);
+  // piece.  BACK of 16-bit operands: three arrays at once; Newton-Schulz of those: two pieces that alternate.
+  static constexpr int STAGING = PAIR ? 2048 : (KIND == TP_BACK ? 3 * 1024 : (KIND >= TP_GRAM ? 2 * 2048 : 2048));
   static constexpr int FIT = (TP_SMEM_BUDGET - 1024 - TP_EPILOGUE_WARPS * STAGING) / STAGE;
   static constexpr int STAGES = FIT < TP_MAX_STAGES ? FIT : TP_MAX_STAGES;
   static constexpr int SMEM = STAGE * STAGES + TP_EPILOGUE_WARPS * STAGING + 1024;
@@ -306,8 +304,8 @@ struct TpStager {
     if (elect_one()) tma_store_wait_read();
     __syncwarp();
   }
-  __device__ __forceinline__ void begin_but_last() const {   // ... all but the last store's piece
-    if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+  __device__ __forceinline__ void begin_but_two() const {   // ... all but the last two stores' pieces
+    if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");
     __syncwarp();
   }
   // 16-byte chunks chunk, chunk + 1, ... of this lane's row of a piece at `at` (rows of 64 bytes) or half a piece (32 bytes)
@@ -356,7 +354,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
   constexpr int TERMS = PAIR ? 2 : 1;
   constexpr int STAGES = S::STAGES, ROWS = 128 * CTAS;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 9 + TP_EPILOGUE_WARPS];
+  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 9];
   __shared__ uint32_t tmem_base_slot;
   __shared__ float block_most[3][TP_EPILOGUE_WARPS];   // GATED: of alternating tiles; BACK: of the three outputs
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -378,7 +376,6 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       mbar_init(acc_empty + 8 * b, CTAS * TP_EPILOGUE_WARPS);   // one arrival a warp
     }
     mbar_init(drain, 1);
-    for (int w = 0; w < TP_EPILOGUE_WARPS; w++) mbar_init(drain + 8 + 8 * w, 1);   // a warp's own copies
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == TP_EPILOGUE_WARPS) {
@@ -391,6 +388,11 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = (uint32_t)uniform((int)tmem_base_slot);
+  if (threadIdx.x < 5) {   // the maps are arguments: fetched before the wait
+    const CUtensorMap *map = threadIdx.x < 2 ? &g.a[threadIdx.x].map : &g.b[threadIdx.x - 2].map;
+    if (threadIdx.x == 0 || threadIdx.x == 2 || (threadIdx.x == 4 ? KIND == TP_BACK : g.segments > 1 || KIND == TP_GATED || KIND == TP_BACK || g.a_of_last))
+      asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+  }
   grid_wait();
   grid_release();   // after the allocation
 
@@ -556,8 +558,6 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
     const int q = warp & 3, part = warp >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
     const TpStager st{staging + (uint32_t)(warp * S::STAGING), lane, g.rows, g.cols};
-    const uint32_t cin_bar = drain + 8 + 8 * (uint32_t)warp;
-    uint32_t cin_phase = 0;
     int buf = 0;
     uint32_t uses = 0;
     const auto next_buffer = [&] {
@@ -593,34 +593,23 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       const TpTile T = tp_tile(g, t, TN, ROWS);
       const int64_t row = T.row0 + 128 * rank + 32 * q;   // first row of this warp
       const int col0 = T.n0 + part * S::PART;             // first column
-      // What a Newton-Schulz epilogue adds to the product, a group of 16 columns ahead: S (hi and lo; rows of a multiple of 64 elements,
-      // so that a group never runs over one's end) or X in float32.
-      uint4 cin[KIND == TP_POLY || KIND == TP_APPLY ? 4 : 1];
-      const auto fetch_cin = [&](int col) {
-        if constexpr (KIND == TP_POLY || KIND == TP_APPLY) {
-          const int64_t from = (int64_t)T.batch * g.cin_batch + (row + lane) * g.cin_ld + col;
+      // What a Newton-Schulz epilogue adds to the product: S or X, hi and lo of 16 columns a group (rows of a multiple of 64 elements, so that
+      // a group never runs over one's end).  Two groups are on their way at a time, from before the sums are there.
+      constexpr bool CIN = KIND == TP_POLY || KIND == TP_APPLY;
+      uint4 cin[CIN ? 2 : 1][CIN ? 4 : 1];
+      const auto fetch_cin = [&](int i) {
+        if constexpr (CIN) {
+          const int col = col0 + 16 * i;
+          if (i >= GROUPS || col >= g.cols) return;
+          const __half *from = static_cast<const __half *>(g.cin) + (int64_t)T.batch * g.cin_batch + (row + lane) * g.cin_ld + col;
           const bool in_rows = row + lane < g.rows;
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
-            const uint4 *p = KIND == TP_APPLY ? reinterpret_cast<const uint4 *>(static_cast<const float *>(g.cin) + from) + c
-                                              : reinterpret_cast<const uint4 *>(static_cast<const __half *>(g.cin) + from + (c >> 1) * g.cin_lo) + (c & 1);
-            cin[c] = in_rows ? __ldcg(p) : make_uint4(0, 0, 0, 0);
-          }
+          for (int c = 0; c < 4; c++)
+            cin[i & 1][c] = in_rows ? __ldcg(reinterpret_cast<const uint4 *>(from + (c >> 1) * g.cin_lo) + (c & 1)) : make_uint4(0, 0, 0, 0);
         }
       };
-      // ... of 16-bit operands by the copy engine, into the piece that the group leaves by: two alternate
-      const auto copy_cin = [&](int col, int piece) {
-        if (elect_one()) {
-          tma_store_wait_read();
-          mbar_arrive_expect_tx(cin_bar, 2048);
-          tma_load_3d(st.smem + 2048u * (uint32_t)piece, &g.cin_map, col, (int)row, T.batch, cin_bar);
-        }
-        __syncwarp();
-      };
-      if (col0 < g.cols) {
-        if (S::CIN_TMA) copy_cin(col0, 0);
-        else fetch_cin(col0);
-      }
+      fetch_cin(0);
+      fetch_cin(1);
       float acc[PAIR ? GROUPS : 1][16];
       if (PAIR) {
 #pragma unroll
@@ -832,97 +821,64 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           }
         }
       } else {
-        // Newton-Schulz: values in float32, then hi and lo (or one fp16) at a power of two that the caller has from its bounds
+        // Newton-Schulz: values in float32, then hi and lo at a power of two that the caller has from its bounds
 #pragma unroll
         for (int i = 0; i < GROUPS; i++) {
           const int col = col0 + 16 * i;
           if (col >= g.cols) break;
-          const bool more = i + 1 < GROUPS && col + 16 < g.cols;
-          const uint32_t piece = S::CIN_TMA ? 2048u * (uint32_t)(i & 1) : 0u;
+          const uint32_t piece = S::STAGING > 2048 ? 2048u * (uint32_t)(i & 1) : 0u;
+          const auto begin = [&] {
+            if (S::STAGING > 2048) st.begin_but_two();   // hi and lo of the group before may still be read
+            else st.begin();
+          };
           float v[16];
           take(i, v);
-          if constexpr (KIND == TP_GRAM) {
-#pragma unroll
-            for (int j = 0; j < 16; j++) v[j] *= g.alpha;
-          } else if constexpr (KIND == TP_POLY) {
-            const uint32_t hw[8] = {cin[0].x, cin[0].y, cin[0].z, cin[0].w, cin[1].x, cin[1].y, cin[1].z, cin[1].w};
-            const uint32_t lw[8] = {cin[2].x, cin[2].y, cin[2].z, cin[2].w, cin[3].x, cin[3].y, cin[3].z, cin[3].w};
+          if constexpr (CIN) {
+            const uint4 (&x)[4] = cin[i & 1];
+            const uint32_t hw[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+            const uint32_t lw[8] = {x[2].x, x[2].y, x[2].z, x[2].w, x[3].x, x[3].y, x[3].z, x[3].w};
 #pragma unroll
             for (int k = 0; k < 8; k++) {
               const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&hw[k])), e = __half22float2(*reinterpret_cast<const __half2 *>(&lw[k]));
               v[2 * k] = g.alpha * v[2 * k] + g.beta * (a.x + e.x);
               v[2 * k + 1] = g.alpha * v[2 * k + 1] + g.beta * (a.y + e.y);
             }
-            if (more) fetch_cin(col + 16);   // on its way while this group is put down
-          } else if constexpr (S::CIN_TMA) {
-            if (ok && !warp_wait(cin_bar, cin_phase, lane)) {
-              if (lane == 0) tp_report(g, 49);
-              ok = false;
-            }
-            cin_phase ^= 1;
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-              float4 x;
-              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                           : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
-                           : "r"(st.smem + piece + (uint32_t)sw64_offset(lane, c))
-                           : "memory");
-              v[4 * c] = g.alpha * v[4 * c] + g.beta * x.x;
-              v[4 * c + 1] = g.alpha * v[4 * c + 1] + g.beta * x.y;
-              v[4 * c + 2] = g.alpha * v[4 * c + 2] + g.beta * x.z;
-              v[4 * c + 3] = g.alpha * v[4 * c + 3] + g.beta * x.w;
-            }
-            __syncwarp();
-            if (more) copy_cin(col + 16, (i + 1) & 1);
+            fetch_cin(i + 2);
           } else {
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-              v[4 * c] = g.alpha * v[4 * c] + g.beta * __uint_as_float(cin[c].x);
-              v[4 * c + 1] = g.alpha * v[4 * c + 1] + g.beta * __uint_as_float(cin[c].y);
-              v[4 * c + 2] = g.alpha * v[4 * c + 2] + g.beta * __uint_as_float(cin[c].z);
-              v[4 * c + 3] = g.alpha * v[4 * c + 3] + g.beta * __uint_as_float(cin[c].w);
-            }
-            if (more) fetch_cin(col + 16);
-          }
-          if (KIND == TP_APPLY) {
-            // out[1]: float32, the X of the next step or the result.  CIN_TMA: copy_cin() has waited until the piece was free.
-            if (!S::CIN_TMA) st.begin();
-            if (!g.out_bf16) {
-              uint32_t w[16];
-#pragma unroll
-              for (int j = 0; j < 16; j++) w[j] = __float_as_uint(v[j]);
-              st.put<64>(piece, 0, w);
-              if (g.out[1].use_map) st.send(&g.out[1].map, piece, col, row, T.batch);
-              else st.send_rows(g.out[1], false, piece, col, row, T.batch);
-            } else if (g.out[1].use_map) {
-              uint32_t w[8];
-#pragma unroll
-              for (int j = 0; j < 8; j++) w[j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
-              st.put<32>(piece, 0, w);
-              st.send(&g.out[1].map, piece, col, row, T.batch);
-            } else {
-              __nv_bfloat16 *o =
-                  static_cast<__nv_bfloat16 *>(g.out[1].ptr) + (int64_t)T.batch * g.out[1].batch + (row + lane) * g.out[1].ld + col;
-#pragma unroll
-              for (int j = 0; j < 16; j++)
-                if (row + lane < g.rows && col + j < g.cols) o[j] = __float2bfloat16_rn(v[j]);
-            }
+            for (int j = 0; j < 16; j++) v[j] *= g.alpha;
           }
           if (KIND != TP_APPLY || g.pair_scale != 0.f) {
-            constexpr bool LOW = PAIR || KIND == TP_GRAM;   // S is also added as it is: with its low part
-            constexpr uint32_t where = S::CIN_TMA ? 4096u : 0u;
             uint32_t w[8], lo[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-              if (LOW) tp_split2(v[2 * j], v[2 * j + 1], g.pair_scale, w[j], lo[j]);
-              else w[j] = tp_f16x2(v[2 * j] * g.pair_scale, v[2 * j + 1] * g.pair_scale);
-            }
-            if (!S::CIN_TMA) st.begin();
-            else if (!more) st.begin_but_last();   // else copy_cin() has waited for the group before
-            st.put<32>(where, 0, w);
-            if (LOW) st.put<32>(where + 1024, 0, lo);
-            st.send(&g.out[0].map, where, col, row, (LOW ? 2 : 1) * T.batch);
-            if (LOW) st.send(&g.out[0].map, where + 1024, col, row, 2 * T.batch + 1);
+            for (int j = 0; j < 8; j++) tp_split2(v[2 * j], v[2 * j + 1], g.pair_scale, w[j], lo[j]);
+            begin();
+            st.put<32>(piece, 0, w);
+            if (PAIR || KIND != TP_POLY) st.put<32>(piece + 1024, 0, lo);   // S and X are also added as they are: with their low part
+            constexpr int Z = PAIR || KIND != TP_POLY ? 2 : 1;
+            st.send(&g.out[0].map, piece, col, row, Z * T.batch);
+            if (Z == 2) st.send(&g.out[0].map, piece + 1024, col, row, 2 * T.batch + 1);
+          } else if (!g.out_bf16) {   // APPLY's result
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) w[j] = __float_as_uint(v[j]);
+            st.begin();
+            st.put<64>(piece, 0, w);
+            if (g.out[1].use_map) st.send(&g.out[1].map, piece, col, row, T.batch);
+            else st.send_rows(g.out[1], false, piece, col, row, T.batch);
+          } else if (g.out[1].use_map) {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
+            st.begin();
+            st.put<32>(piece, 0, w);
+            st.send(&g.out[1].map, piece, col, row, T.batch);
+          } else {
+            __nv_bfloat16 *o =
+                static_cast<__nv_bfloat16 *>(g.out[1].ptr) + (int64_t)T.batch * g.out[1].batch + (row + lane) * g.out[1].ld + col;
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+              if (row + lane < g.rows && col + j < g.cols) o[j] = __float2bfloat16_rn(v[j]);
           }
         }
       }
@@ -931,7 +887,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         next_buffer();
       }
     }
-    if (elect_one()) tma_store_wait_all();   // the copy engine reads this warp's staging buffer
+    if (elect_one()) tma_store_wait_read();   // the copy engine reads this warp's staging buffer; what it writes, the grid's end waits for
   }
   tc_fence_before();
   if (CTAS == 2) {
@@ -1025,11 +981,20 @@ inline TpArgs new_args(int64_t rows, int64_t cols, int32_t *status) {
 }
 inline int blocks64(int64_t n) { return (int)((n + 63) / 64); }
 
-// Pairs of CTAs where their tiles of 256 rows fill the SMs and the last of them is not mostly empty
-inline bool pairs_fill(int64_t rows, int64_t cols, int64_t times, int tn) {
-  const int64_t mt = (rows + 255) / 256;
-  return mt * ((cols + tn - 1) / tn) * times >= 74 && 9 * mt * 256 <= 10 * up(rows, 128);
-}
+// What a variant costs in cycles: rounds of its tiles over the SMs, each as long as its products or, at 64 bytes a cycle and SM, its copies,
+// and something for the epilogue and the chain at a tile's ends.  n: columns of B, out: of the output, tn: of a tile.
+struct TpCost {
+  int64_t rows, out;
+  int kblocks;
+  int64_t times;
+  bool pair;
+  int64_t operator()(int ctas, int tn, int n) const {
+    const int64_t tiles = (rows + 128 * ctas - 1) / (128 * ctas) * ((out + tn - 1) / tn) * times;
+    const int64_t rounds = (tiles + 148 / ctas - 1) / (148 / ctas);
+    const int64_t products = (pair ? 3 : 1) * 2 * n, copies = (pair ? 2 : 1) * (128 + n / ctas) * 2;   // a block of 64 k
+    return rounds * (kblocks * (products > copies ? products : copies) + 2000 + 16 * n);
+  }
+};
 
 template <int KIND, bool PAIR, int TN, int CTAS, int ACT = TP_SILU>
 int tp_launch(TpArgs &g, cudaStream_t st, const char *what) {

@@ -17,7 +17,7 @@
 namespace cmace {
 
 constexpr int NS_THREADS = 256;
-constexpr int NS_CHUNKS = 64;   // partial sums of a matrix at most
+constexpr int NS_CHUNKS = 512;   // partial sums of a matrix at most
 
 struct NsPrep {
   const void *src;
@@ -565,13 +565,20 @@ struct NsCall {
   const char *what;
 };
 
-template <int KIND>
-static int launch_ns(bool pair, TpArgs &g, cudaStream_t st, const char *what) {
-  const TpCost cost{g.rows, g.cols, g.kblocks[0], g.batches, pair};
+struct NsVariant {
+  int ctas, tn;
+};
+static NsVariant ns_variant(bool pair, int64_t rows, int cols, int kblocks, int64_t count) {
+  const TpCost cost{rows, cols, kblocks, count, pair};
   const int64_t one = cost(1, 128, 128), two = cost(2, 128, 128);
-  if (pair) return two < one ? tp_launch<KIND, true, 128, 2>(g, st, what) : tp_launch<KIND, true, 128, 1>(g, st, what);
-  if (cost(2, 256, 256) < std::min(one, two)) return tp_launch<KIND, false, 256, 2>(g, st, what);
-  return two < one ? tp_launch<KIND, false, 128, 2>(g, st, what) : tp_launch<KIND, false, 128, 1>(g, st, what);
+  if (!pair && cost(2, 256, 256) < std::min(one, two)) return {2, 256};
+  return {two < one ? 2 : 1, 128};
+}
+template <int KIND>
+static int launch_ns(bool pair, NsVariant v, TpArgs &g, cudaStream_t st, const char *what) {
+  if (v.tn == 256) return tp_launch<KIND, false, 256, 2>(g, st, what);
+  if (v.ctas == 2) return pair ? tp_launch<KIND, true, 128, 2>(g, st, what) : tp_launch<KIND, false, 128, 2>(g, st, what);
+  return pair ? tp_launch<KIND, true, 128, 1>(g, st, what) : tp_launch<KIND, false, 128, 1>(g, st, what);
 }
 
 // CTAs a matrix for the kernel above, 0: it does not fit
@@ -658,15 +665,19 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   launch_chained(ns_norm_kernel, dim3((unsigned)(f.count * chunks)), dim3(NS_THREADS), (size_t)0, f.st, p);
   launch_chained(ns_prep_kernel, dim3((unsigned)(f.count * blocks)), dim3(NS_THREADS), (size_t)0, f.st, p);
   int rc = check_launch(f.what);
-  // maps, read and written: of X twice, S, P and the result
-  CUtensorMap to_x[2], to_s, to_poly;
+  // maps: operands; what is added and written, in boxes of the variants' columns a warp
+  const int kb_s = blocks64(wide ? f.cols : f.rows), kb = blocks64(side);
+  const NsVariant v_gram = ns_variant(f.f32, side, side, kb_s, f.count), v_poly = ns_variant(f.f32, side, side, kb, f.count),
+                  v_apply = ns_variant(f.f32, f.rows, f.cols, kb, f.count);
+  CUtensorMap part_x[2], to_s, from_s, to_poly;
   TpOut to_out;
   memset(&to_out, 0, sizeof(to_out));
   for (Matrix *m : {&x[0], &x[1], &s, &poly})
     if (!rc) rc = encode_matrix(&m->map, *m, 64, 64, false, f.what);
-  for (int k = 0; k < 2 && !rc; k++) rc = encode_matrix(&to_x[k], x[k], 16, 32, false, f.what);
-  if (!rc) rc = encode_matrix(&to_s, s, 16, 32, false, f.what);
-  if (!rc) rc = encode_matrix(&to_poly, poly, 16, 32, false, f.what);
+  for (int k = 0; k < 2 && !rc; k++) rc = encode_matrix(&part_x[k], x[k], v_apply.tn / 4, 32, false, f.what);
+  if (!rc) rc = encode_matrix(&to_s, s, v_gram.tn / 4, 32, false, f.what);
+  if (!rc) rc = encode_matrix(&from_s, s, v_poly.tn / 4, 32, false, f.what);
+  if (!rc) rc = encode_matrix(&to_poly, poly, v_poly.tn / 4, 32, false, f.what);
   const int bytes = f.f32 ? 4 : 2;
   to_out.ptr = f.out, to_out.ld = f.cols, to_out.batch = n;
   to_out.use_map = aligned16(f.out) && (int64_t)f.cols * bytes % 16 == 0;
@@ -680,31 +691,31 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     TpArgs g = new_args(side, side, f.status);
     g.batches = (int)f.count;
     g.in_f16 = 1;
-    g.kblocks[0] = blocks64(wide ? f.cols : f.rows);
+    g.kblocks[0] = kb_s;
     set_operand(g.a[0], now, wide);
     set_operand(g.b[0], now, wide);
     g.out[0].map = to_s;
     g.alpha = 1.0f / (sx * sx);
     g.pair_scale = ss;
-    rc = launch_ns<TP_GRAM>(f.f32, g, f.st, f.what);
+    rc = launch_ns<TP_GRAM>(f.f32, v_gram, g, f.st, f.what);
 
-    g.kblocks[0] = blocks64(side);
+    g.kblocks[0] = kb;
     set_operand(g.a[0], s, true);
     set_operand(g.b[0], s, true);
     g.out[0].map = to_poly;
-    g.cin = s.at, g.cin_ld = s.ld, g.cin_batch = 2 * s.plane(), g.cin_lo = s.plane();
+    g.cin = from_s;
     g.alpha = (float)f.c / (ss * ss), g.beta = (float)f.b / ss, g.pair_scale = sp;
-    if (!rc) rc = launch_ns<TP_POLY>(f.f32, g, f.st, f.what);
+    if (!rc) rc = launch_ns<TP_POLY>(f.f32, v_poly, g, f.st, f.what);
 
     g.rows = f.rows, g.cols = f.cols;
     set_operand(g.a[0], wide ? poly : now, true);
     set_operand(g.b[0], wide ? now : poly, !wide);
-    g.out[0].map = to_x[(step + 1) & 1];
+    g.out[0].map = part_x[(step + 1) & 1];
     g.out[1] = to_out;
     g.out_bf16 = !f.f32;
-    g.cin = now.at, g.cin_ld = now.ld, g.cin_batch = 2 * now.plane(), g.cin_lo = now.plane();
+    g.cin = part_x[step & 1];
     g.alpha = 1.0f / (sp * sx), g.beta = (float)f.a / sx, g.pair_scale = last ? 0.f : sn;
-    if (!rc) rc = launch_ns<TP_APPLY>(f.f32, g, f.st, f.what);
+    if (!rc) rc = launch_ns<TP_APPLY>(f.f32, v_apply, g, f.st, f.what);
     most = most_next;
     sx = sn;
   }

@@ -77,8 +77,7 @@ struct TpArgs {
   TpOut out[2];                  // 16-bit values, hi and lo; results
   float *out_scale[3];           // PAIR outputs with block scales: inverse scale of every 64 x 64 block
   int64_t out_scale_ld, out_scale_batch;
-  const void *cin;               // POLY: S, APPLY: X: hi, and cin_lo elements behind it lo
-  int64_t cin_ld, cin_batch, cin_lo;
+  CUtensorMap cin;               // POLY: S, APPLY: X, in boxes of 32 rows of a warp's columns; batch b is hi 2 b and lo 2 b + 1
   float alpha, beta, cin_scale, pair_scale;   // D = alpha * product + beta * cin / ..., see the epilogues
   int32_t *status;
   int64_t rows, cols;            // of the output
@@ -176,8 +175,9 @@ struct TpShape {
   static_assert(LATE || ACC_COLS <= BUFFER_COLS, "accumulators");
   static constexpr int PART = TN / 4, EACH = PART / 16;   // a warp's columns of a sum, and in groups of 16
   // Bytes an epilogue warp stages its output in.  A piece is 32 rows of 64 bytes: 16 float32 or 32 16-bit columns; 16 of those are half a
-  // piece.  BACK of 16-bit operands: three arrays at once; Newton-Schulz of those: two pieces that alternate.
-  static constexpr int STAGING = PAIR ? 2048 : (KIND == TP_BACK ? 3 * 1024 : (KIND >= TP_GRAM ? 2 * 2048 : 2048));
+  // piece.  BACK of 16-bit operands: three arrays at once.  Newton-Schulz: hi and lo of a warp's 32 x PART values,
+  // GRAM, where nothing comes in, one after the other.
+  static constexpr int STAGING = KIND >= TP_GRAM ? (KIND == TP_GRAM ? 1 : 2) * 32 * PART * 2 : (KIND == TP_BACK && !PAIR ? 3 * 1024 : 2048);
   static constexpr int FIT = (TP_SMEM_BUDGET - 1024 - TP_EPILOGUE_WARPS * STAGING) / STAGE;
   static constexpr int STAGES = FIT < TP_MAX_STAGES ? FIT : TP_MAX_STAGES;
   static constexpr int SMEM = STAGE * STAGES + TP_EPILOGUE_WARPS * STAGING + 1024;
@@ -304,11 +304,13 @@ struct TpStager {
     if (elect_one()) tma_store_wait_read();
     __syncwarp();
   }
-  __device__ __forceinline__ void begin_but_two() const {   // ... all but the last two stores' pieces
-    if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");
-    __syncwarp();
-  }
   // 16-byte chunks chunk, chunk + 1, ... of this lane's row of a piece at `at` (rows of 64 bytes) or half a piece (32 bytes)
+  template <int ROW_BYTES>
+  __device__ __forceinline__ uint4 get(uint32_t at, int chunk) const {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem + at + offset<ROW_BYTES>(lane, chunk)) : "memory");
+    return v;
+  }
   template <int ROW_BYTES, int WORDS>
   __device__ __forceinline__ void put(uint32_t at, int chunk, const uint32_t (&w)[WORDS]) const {
 #pragma unroll
@@ -317,10 +319,10 @@ struct TpStager {
                    "r"(w[4 * c + 1]), "r"(w[4 * c + 2]), "r"(w[4 * c + 3])
                    : "memory");
   }
-  // the copy engine's swizzles of rows of 64 and of 32 bytes
+  // the copy engine's swizzles of rows of 128, 64 and 32 bytes
   template <int ROW_BYTES>
   static __device__ __forceinline__ uint32_t offset(int row, int chunk) {
-    return ROW_BYTES == 64 ? (uint32_t)sw64_offset(row, chunk) : (uint32_t)(row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4));
+    return ROW_BYTES == 128 ? (uint32_t)sw128_offset(row, chunk) : ROW_BYTES == 64 ? (uint32_t)sw64_offset(row, chunk) : (uint32_t)(row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4));
   }
   __device__ __forceinline__ void send(const CUtensorMap *map, uint32_t at, int col, int64_t row, int batch) const {
     fence_proxy_async();
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
   constexpr int TERMS = PAIR ? 2 : 1;
   constexpr int STAGES = S::STAGES, ROWS = 128 * CTAS;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 9];
+  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 9 + TP_EPILOGUE_WARPS];
   __shared__ uint32_t tmem_base_slot;
   __shared__ float block_most[3][TP_EPILOGUE_WARPS];   // GATED: of alternating tiles; BACK: of the three outputs
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -376,6 +378,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       mbar_init(acc_empty + 8 * b, CTAS * TP_EPILOGUE_WARPS);   // one arrival a warp
     }
     mbar_init(drain, 1);
+    for (int w = 0; w < TP_EPILOGUE_WARPS; w++) mbar_init(drain + 8 + 8 * w, 1);   // a warp's own copies
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == TP_EPILOGUE_WARPS) {
@@ -558,6 +561,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
     const int q = warp & 3, part = warp >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
     const TpStager st{staging + (uint32_t)(warp * S::STAGING), lane, g.rows, g.cols};
+    const uint32_t cin_bar = drain + 8 + 8 * (uint32_t)warp;
+    uint32_t cin_phase = 0;
     int buf = 0;
     uint32_t uses = 0;
     const auto next_buffer = [&] {
@@ -593,23 +598,20 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       const TpTile T = tp_tile(g, t, TN, ROWS);
       const int64_t row = T.row0 + 128 * rank + 32 * q;   // first row of this warp
       const int col0 = T.n0 + part * S::PART;             // first column
-      // What a Newton-Schulz epilogue adds to the product: S or X, hi and lo of 16 columns a group (rows of a multiple of 64 elements, so that
-      // a group never runs over one's end).  Two groups are on their way at a time, from before the sums are there.
+      // What a Newton-Schulz epilogue adds to the product, S or X: on its way into the pieces that the warp's values leave by, before the sums
+      // are there.  (Loads by the lanes, each of its own row, took as long as the products.)
       constexpr bool CIN = KIND == TP_POLY || KIND == TP_APPLY;
-      uint4 cin[CIN ? 2 : 1][CIN ? 4 : 1];
-      const auto fetch_cin = [&](int i) {
-        if constexpr (CIN) {
-          const int col = col0 + 16 * i;
-          if (i >= GROUPS || col >= g.cols) return;
-          const __half *from = static_cast<const __half *>(g.cin) + (int64_t)T.batch * g.cin_batch + (row + lane) * g.cin_ld + col;
-          const bool in_rows = row + lane < g.rows;
-#pragma unroll
-          for (int c = 0; c < 4; c++)
-            cin[i & 1][c] = in_rows ? __ldcg(reinterpret_cast<const uint4 *>(from + (c >> 1) * g.cin_lo) + (c & 1)) : make_uint4(0, 0, 0, 0);
+      constexpr uint32_t LOW = 32 * S::PART * 2;   // bytes from a warp's hi to its lo
+      const bool here = row < g.rows && col0 < g.cols;
+      if (CIN && here) {
+        if (elect_one()) {
+          tma_store_wait_read();
+          mbar_arrive_expect_tx(cin_bar, 2 * LOW);
+          tma_load_3d(st.smem, &g.cin, col0, (int)row, 2 * T.batch, cin_bar);
+          tma_load_3d(st.smem + LOW, &g.cin, col0, (int)row, 2 * T.batch + 1, cin_bar);
         }
-      };
-      fetch_cin(0);
-      fetch_cin(1);
+        __syncwarp();
+      }
       float acc[PAIR ? GROUPS : 1][16];
       if (PAIR) {
 #pragma unroll
@@ -822,63 +824,88 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         }
       } else {
         // Newton-Schulz: values in float32, then hi and lo at a power of two that the caller has from its bounds
+        constexpr int ROW = 2 * S::PART;   // bytes of a row of a piece
+        if (CIN && here) {
+          if (ok && !warp_wait(cin_bar, cin_phase, lane)) {
+            if (lane == 0) tp_report(g, 49);
+            ok = false;
+          }
+          cin_phase ^= 1;
+        }
+        const bool result = KIND == TP_APPLY && g.pair_scale == 0.f;
+        if (!CIN) st.begin();
+        float all[GROUPS][16];   // of the result, which leaves in pieces of another shape
 #pragma unroll
         for (int i = 0; i < GROUPS; i++) {
-          const int col = col0 + 16 * i;
-          if (col >= g.cols) break;
-          const uint32_t piece = S::STAGING > 2048 ? 2048u * (uint32_t)(i & 1) : 0u;
-          const auto begin = [&] {
-            if (S::STAGING > 2048) st.begin_but_two();   // hi and lo of the group before may still be read
-            else st.begin();
-          };
-          float v[16];
+          float (&v)[16] = all[i];
           take(i, v);
           if constexpr (CIN) {
-            const uint4 (&x)[4] = cin[i & 1];
-            const uint32_t hw[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
-            const uint32_t lw[8] = {x[2].x, x[2].y, x[2].z, x[2].w, x[3].x, x[3].y, x[3].z, x[3].w};
+            const uint4 x = st.get<ROW>(0, 2 * i), y = st.get<ROW>(0, 2 * i + 1), xl = st.get<ROW>(LOW, 2 * i), yl = st.get<ROW>(LOW, 2 * i + 1);
+            const uint32_t hw[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w}, lw[8] = {xl.x, xl.y, xl.z, xl.w, yl.x, yl.y, yl.z, yl.w};
 #pragma unroll
             for (int k = 0; k < 8; k++) {
               const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&hw[k])), e = __half22float2(*reinterpret_cast<const __half2 *>(&lw[k]));
               v[2 * k] = g.alpha * v[2 * k] + g.beta * (a.x + e.x);
               v[2 * k + 1] = g.alpha * v[2 * k + 1] + g.beta * (a.y + e.y);
             }
-            fetch_cin(i + 2);
           } else {
 #pragma unroll
             for (int j = 0; j < 16; j++) v[j] *= g.alpha;
           }
-          if (KIND != TP_APPLY || g.pair_scale != 0.f) {
+          if (!result) {
             uint32_t w[8], lo[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) tp_split2(v[2 * j], v[2 * j + 1], g.pair_scale, w[j], lo[j]);
-            begin();
-            st.put<32>(piece, 0, w);
-            if (PAIR || KIND != TP_POLY) st.put<32>(piece + 1024, 0, lo);   // S and X are also added as they are: with their low part
-            constexpr int Z = PAIR || KIND != TP_POLY ? 2 : 1;
-            st.send(&g.out[0].map, piece, col, row, Z * T.batch);
-            if (Z == 2) st.send(&g.out[0].map, piece + 1024, col, row, 2 * T.batch + 1);
-          } else if (!g.out_bf16) {   // APPLY's result
-            uint32_t w[16];
+            st.put<ROW>(0, 2 * i, w);
+            if (CIN) st.put<ROW>(LOW, 2 * i, lo);
+            else
 #pragma unroll
-            for (int j = 0; j < 16; j++) w[j] = __float_as_uint(v[j]);
+              for (int j = 0; j < 8; j++) v[j] = __uint_as_float(lo[j]);   // GRAM: kept until hi has left
+          }
+        }
+        if (!result) {
+          constexpr int Z = PAIR || KIND != TP_POLY ? 2 : 1;   // S and X are also added as they are: with their low part
+          st.send(&g.out[0].map, 0, col0, row, Z * T.batch);
+          if (!CIN) {
             st.begin();
-            st.put<64>(piece, 0, w);
-            if (g.out[1].use_map) st.send(&g.out[1].map, piece, col, row, T.batch);
-            else st.send_rows(g.out[1], false, piece, col, row, T.batch);
-          } else if (g.out[1].use_map) {
-            uint32_t w[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) w[j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
-            st.begin();
-            st.put<32>(piece, 0, w);
-            st.send(&g.out[1].map, piece, col, row, T.batch);
-          } else {
-            __nv_bfloat16 *o =
-                static_cast<__nv_bfloat16 *>(g.out[1].ptr) + (int64_t)T.batch * g.out[1].batch + (row + lane) * g.out[1].ld + col;
+            for (int i = 0; i < GROUPS; i++) {
+              uint32_t lo[8];
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-              if (row + lane < g.rows && col + j < g.cols) o[j] = __float2bfloat16_rn(v[j]);
+              for (int j = 0; j < 8; j++) lo[j] = __float_as_uint(all[i][j]);
+              st.put<ROW>(0, 2 * i, lo);
+            }
+          }
+          if (Z == 2) st.send(&g.out[0].map, CIN ? LOW : 0u, col0, row, 2 * T.batch + 1);
+        } else {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < GROUPS; i++) {
+            const int col = col0 + 16 * i;
+            if (col >= g.cols) break;
+            const float (&v)[16] = all[i];
+            if (!g.out_bf16) {
+              uint32_t w[16];
+#pragma unroll
+              for (int j = 0; j < 16; j++) w[j] = __float_as_uint(v[j]);
+              st.begin();
+              st.put<64>(0, 0, w);
+              if (g.out[1].use_map) st.send(&g.out[1].map, 0, col, row, T.batch);
+              else st.send_rows(g.out[1], false, 0, col, row, T.batch);
+            } else if (g.out[1].use_map) {
+              uint32_t w[8];
+#pragma unroll
+              for (int j = 0; j < 8; j++) w[j] = tp_bf16x2(v[2 * j], v[2 * j + 1]);
+              st.begin();
+              st.put<32>(0, 0, w);
+              st.send(&g.out[1].map, 0, col, row, T.batch);
+            } else {
+              __nv_bfloat16 *o =
+                  static_cast<__nv_bfloat16 *>(g.out[1].ptr) + (int64_t)T.batch * g.out[1].batch + (row + lane) * g.out[1].ld + col;
+#pragma unroll
+              for (int j = 0; j < 16; j++)
+                if (row + lane < g.rows && col + j < g.cols) o[j] = __float2bfloat16_rn(v[j]);
+            }
           }
         }
       }

@@ -111,6 +111,140 @@ __global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const __grid_constan
   }
 }
 
+// ---- few rows: a pass over the weights -------------------------------------------------------------------------------------------
+// With up to eight rows the block is as long as its weights take to arrive, and a tensor core's tile would be 1/16 full at most: plain
+// float32 FMA, a weight read once for all rows.  A CTA has 32 columns (segments of 64 or 128 bytes of a row), its 16 warps every 64th group
+// of rows of W, and the CTAs of a cluster share the rows where columns alone do not fill the SMs.  h stays float32 in the workspace.
+// (Width 1 024, hidden width 4 096, both kernels in a recorded graph: one row 10.4 us in bf16 and 10.7 in float32, against 26 and 65 by tiles; eight
+// rows 21.6 and 20.3 against 24 and 66.  128 and 512: 6.8 and 6.1 against 10.4 and 15.7; eight rows 9.8 and 9.2 against 10.5 and 15.8.)
+constexpr int FEW_ROWS = 8, FEW_THREADS = 512, FEW_COLS = 32, FEW_K = 1024;   // FEW_K: rows of W whose x is in shared memory
+
+struct FewArgs {
+  const void *x;       // [M, K]: T, or h in float32
+  const void *w[2];    // [K, N]
+  void *out;           // [M, N]: h in float32, or T
+  int M, K, N, cluster, wide;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void few_load(float (&v)[V], const T *p, int n, bool wide) {
+  if (!wide) {
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = i < n ? (float)p[i] : 0.f;
+  } else if constexpr (sizeof(T) == 4) {
+    const float4 x = __ldg(reinterpret_cast<const float4 *>(p));
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  } else {
+    uint32_t w[V / 2];
+    if constexpr (V == 8) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else {
+      const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
+      w[0] = x.x, w[1] = x.y;
+    }
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+// columns a thread: 16 bytes, 8 where the sums of eight rows would not fit the registers
+template <typename T, int M>
+constexpr int few_cols() { return sizeof(T) == 2 && M <= 4 ? 8 : 4; }
+
+// GATED: h = act(x Wg) * (x Wu), otherwise y = h Wd.  M: rows, or up to seven more.
+template <typename T, int M, bool GATED, int ACT>
+__global__ void __launch_bounds__(FEW_THREADS, 1) few_rows_kernel(const FewArgs g) {
+  constexpr int W = GATED ? 2 : 1, WARPS = FEW_THREADS / 32, V = few_cols<T, M>(), LANES = FEW_COLS / V, ROWS = 32 / LANES;   // of a warp's load
+  extern __shared__ float few_smem[];   // x [FEW_K][M]; then the warps' sums [WARPS][W][M][32]
+  __shared__ float total[W][M][FEW_COLS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane % LANES, row = lane / LANES;
+  const int rank = blockIdx.x % g.cluster, col = (int)(blockIdx.x / g.cluster) * FEW_COLS + V * part;
+  const int k0 = (int)((int64_t)g.K * rank / g.cluster), k1 = (int)((int64_t)g.K * (rank + 1) / g.cluster);
+  const int n = g.N - col;
+  grid_begin();
+  float acc[W][M][V] = {};
+  for (int from = k0; from < k1; from += FEW_K) {
+    const int len = min(FEW_K, k1 - from);
+    __syncthreads();
+    for (int i = threadIdx.x; i < len * M; i += FEW_THREADS) {
+      const int m = i / len, k = i - m * len;
+      float v = 0.f;
+      if (m < g.M) {
+        const int64_t at = (int64_t)m * g.K + from + k;
+        v = GATED ? (float)static_cast<const T *>(g.x)[at] : __ldcg(static_cast<const float *>(g.x) + at);   // h: of the kernel before
+      }
+      few_smem[k * M + m] = v;
+    }
+    __syncthreads();
+    if (n > 0) {
+#pragma unroll(M <= 2 ? 8 : 4)
+      for (int k = ROWS * warp + row; k < len; k += ROWS * WARPS) {
+        float w[W][V], x[M];
+#pragma unroll
+        for (int i = 0; i < W; i++) few_load<T, V>(w[i], static_cast<const T *>(g.w[i]) + (int64_t)(from + k) * g.N + col, n, g.wide);
+#pragma unroll
+        for (int m = 0; m < M; m++) x[m] = few_smem[k * M + m];
+#pragma unroll
+        for (int i = 0; i < W; i++)
+#pragma unroll
+          for (int m = 0; m < M; m++)
+#pragma unroll
+            for (int j = 0; j < V; j++) acc[i][m][j] = fmaf(x[m], w[i][j], acc[i][m][j]);
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < W; i++)
+#pragma unroll
+    for (int m = 0; m < M; m++)
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        float v = acc[i][m][j];
+#pragma unroll
+        for (int d = LANES; d < 32; d *= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+        if (row == 0) few_smem[((warp * W + i) * M + m) * FEW_COLS + V * part + j] = v;
+      }
+  __syncthreads();
+  for (int e = threadIdx.x; e < W * M * FEW_COLS; e += FEW_THREADS) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < WARPS; k++) v += few_smem[k * (W * M * FEW_COLS) + e];
+    (&total[0][0][0])[e] = v;
+  }
+  if (g.cluster > 1) {
+    __syncwarp();
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
+  if (rank == 0) {
+    for (int e = threadIdx.x; e < M * FEW_COLS; e += FEW_THREADS) {
+      const int m = e / FEW_COLS, c = (int)(blockIdx.x / g.cluster) * FEW_COLS + e % FEW_COLS;
+      float v[W];
+#pragma unroll
+      for (int i = 0; i < W; i++) {
+        v[i] = 0.f;
+        const uint32_t at = smem_u32(&total[i][m][e % FEW_COLS]);
+        for (int r = 0; r < g.cluster; r++) {
+          float part_sum;
+          if (g.cluster > 1) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part_sum) : "r"(peer_smem(at, (uint32_t)r)) : "memory");
+          else part_sum = total[i][m][e % FEW_COLS];
+          v[i] += part_sum;
+        }
+      }
+      if (m < g.M && c < g.N) {
+        if (GATED) static_cast<float *>(g.out)[(int64_t)m * g.N + c] = tp_act<ACT>(v[0]) * v[W - 1];
+        else static_cast<T *>(g.out)[(int64_t)m * g.N + c] = (T)v[0];
+      }
+    }
+  }
+  if (g.cluster > 1) {   // nobody leaves while its sums are read
+    __syncwarp();
+    cluster_sync();
+  }
+}
+
 // ---- weight gradients: the splits' sums, the third transposed ------------------------------------------------------------------
 struct WeightReduce {
   const float *partial;   // [splits][3][C][ld]
@@ -249,7 +383,39 @@ static int weight_splits(int64_t M, int C, int H) {
   return best;
 }
 
+template <typename T, int M, bool GATED, int ACT>
+static int launch_few(FewArgs g, cudaStream_t st, const char *what) {
+  const int blocks = (g.N + FEW_COLS - 1) / FEW_COLS;
+  g.cluster = 1;
+  while (g.cluster < 8 && 2 * g.cluster * blocks <= 148 && g.K >= 128 * g.cluster) g.cluster *= 2;
+  constexpr int V = few_cols<T, M>();
+  g.wide = g.N % V == 0;
+  for (int i = 0; i < (GATED ? 2 : 1); i++) g.wide = g.wide && reinterpret_cast<uintptr_t>(g.w[i]) % (V * sizeof(T)) == 0;
+  constexpr int SUMS = FEW_THREADS / 32 * (GATED ? 2 : 1) * FEW_COLS, SMEM = M * (FEW_K > SUMS ? FEW_K : SUMS) * 4;
+  if (const int rc = allow_smem<few_rows_kernel<T, M, GATED, ACT>>(SMEM, what)) return rc;
+  return launch_cluster(few_rows_kernel<T, M, GATED, ACT>, g.cluster, blocks * g.cluster, FEW_THREADS, SMEM, st, what, g);
+}
+template <typename T, int M, int ACT>
+static int few_rows(const FeedForward &f, void *y, float *h) {
+  FewArgs g{f.x, {f.wg, f.wu}, h, (int)f.M, f.C, f.H, 1, 0};
+  if (const int rc = launch_few<T, M, true, ACT>(g, f.st, f.what)) return rc;
+  g.x = h, g.w[0] = f.wd, g.out = y, g.K = f.H, g.N = f.C;
+  return launch_few<T, M, false, ACT>(g, f.st, f.what);
+}
+template <typename T, int ACT>
+static int few_rows(const FeedForward &f, void *y, float *h) {
+  return f.M == 1 ? few_rows<T, 1, ACT>(f, y, h) : f.M == 2 ? few_rows<T, 2, ACT>(f, y, h) : f.M <= 4 ? few_rows<T, 4, ACT>(f, y, h) : few_rows<T, 8, ACT>(f, y, h);
+}
+template <typename T>
+static int few_rows(const FeedForward &f, void *y, float *h) {
+  return f.act == TP_SILU ? few_rows<T, TP_SILU>(f, y, h) : few_rows<T, TP_GELU>(f, y, h);
+}
+
 static int forward(const FeedForward &f, void *y, Carve &w) {
+  if (f.M <= FEW_ROWS) {
+    float *h = w.take<float>(f.M * f.H);
+    return !w.base ? CMACE_OK : (f.f32 ? few_rows<float>(f, y, h) : few_rows<__nv_bfloat16>(f, y, h));
+  }
   PrepArgs prep;
   memset(&prep, 0, sizeof(prep));
   int64_t blocks = 0;

@@ -594,19 +594,7 @@ static int fused_cluster(int64_t count, int64_t rows, int cols) {
 template <int CLUSTER, bool A_TMEM>
 static int launch_fused(const NsCall &f, const NsFused &g, int smem) {
   if (const int rc = allow_smem<ns_fused_kernel<CLUSTER, A_TMEM>>(smem, f.what)) return rc;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = CLUSTER, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(f.count * CLUSTER));
-  cfg.blockDim = dim3(NSF_THREADS);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = f.st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = CLUSTER > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_fused_kernel<CLUSTER, A_TMEM>, g);
-  if (e != cudaSuccess) return fail(CMACE_ERR_CUDA, "%s: %s", f.what, cudaGetErrorString(e));
-  return check_launch(f.what);
+  return launch_cluster(ns_fused_kernel<CLUSTER, A_TMEM>, CLUSTER, f.count * CLUSTER, NSF_THREADS, smem, f.st, f.what, g);
 }
 
 static int run_fused(const NsCall &f, int cluster) {

@@ -1023,6 +1023,27 @@ struct TpCost {
   }
 };
 
+// launch_chained() with clusters of `ctas`
+template <typename Args>
+int launch_cluster(void (*kernel)(Args), int ctas, int64_t blocks, int threads, int smem, cudaStream_t st, const char *what, const Args &args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  const bool chained = chain_launches() == Chain::on;
+  if (chain_launches() == Chain::from_second) chain_launches() = Chain::on;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cfg.attrs = ctas > 1 ? attr : attr + 1;
+  cfg.numAttrs = (ctas > 1 ? 1 : 0) + (chained ? 1 : 0);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
+  return e == cudaSuccess ? check_launch(what) : fail(CMACE_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
 template <int KIND, bool PAIR, int TN, int CTAS, int ACT = TP_SILU>
 int tp_launch(TpArgs &g, cudaStream_t st, const char *what) {
   using S = TpShape<KIND, PAIR, TN, CTAS>;
@@ -1034,22 +1055,7 @@ int tp_launch(TpArgs &g, cudaStream_t st, const char *what) {
   g.by_nt = tp_div((uint32_t)g.nt), g.by_mt = tp_div((uint32_t)g.mt), g.by_batches = tp_div((uint32_t)g.batches), g.by_splits = tp_div((uint32_t)g.splits);
   const auto kernel = tile_product_kernel<KIND, PAIR, TN, CTAS, ACT>;
   if (const int rc = allow_smem<tile_product_kernel<KIND, PAIR, TN, CTAS, ACT>>(S::SMEM, what)) return rc;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CTAS, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  const bool chained = chain_launches() == Chain::on;   // as launch_chained()
-  if (chain_launches() == Chain::from_second) chain_launches() = Chain::on;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(CTAS * (g.total < 148 / CTAS ? g.total : 148 / CTAS)));
-  cfg.blockDim = dim3(TP_THREADS);
-  cfg.dynamicSmemBytes = (size_t)S::SMEM;
-  cfg.stream = st;
-  cfg.attrs = CTAS == 2 ? attr : attr + 1;
-  cfg.numAttrs = (CTAS == 2 ? 1 : 0) + (chained ? 1 : 0);
-  cudaLaunchKernelEx(&cfg, kernel, g);
-  return check_launch(what);
+  return launch_cluster(kernel, CTAS, (int)(CTAS * (g.total < 148 / CTAS ? g.total : 148 / CTAS)), TP_THREADS, S::SMEM, st, what, g);
 }
 
 }  // namespace cmace

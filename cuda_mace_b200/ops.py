@@ -16,6 +16,7 @@ All tensors must live on a CUDA device; float32 and float64 are supported everyw
 reference's Linear is float32 only).  Kernels run on torch's current stream.  There is no
 fallback: a CPU tensor raises.
 """
+import functools
 import math
 from collections import OrderedDict
 
@@ -280,15 +281,24 @@ def _workspace(device, nbytes):
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
+@functools.lru_cache(4096)
+def _gated_ff_bytes(f32, M, C, H, backward):
+    nbytes = _abi.call("cmace_gated_ff_workspace_bytes", f32, M, C, H, backward)
+    if nbytes < 0:
+        raise RuntimeError(_abi.load().cmace_last_error().decode())
+    return nbytes
+
+
 def _gated_ff_forward(x, w_gate, w_up, w_down, activation):
     C, H = w_gate.shape
     M = x.numel() // C
     y = torch.empty_like(x)
-    f32 = x.dtype == torch.float32
-    nbytes = _abi.call("cmace_gated_ff_workspace_bytes", f32, M, C, H, 0)
-    ws = _workspace(x.device, nbytes)
+    f32 = x.dtype is torch.float32
+    device = x.device
+    nbytes = _gated_ff_bytes(f32, M, C, H, 0)
+    ws = _workspace(device, nbytes)
     _abi.call("cmace_gated_ff_fwd_f32" if f32 else "cmace_gated_ff_fwd_bf16", x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
-              w_down.data_ptr(), M, C, H, activation, y.data_ptr(), ws.data_ptr(), nbytes, _ptr(_status_tensor(x.device)),
+              w_down.data_ptr(), M, C, H, activation, y.data_ptr(), ws.data_ptr(), nbytes, _status_tensor(device).data_ptr(),
               _stream())
     return y
 
@@ -308,9 +318,9 @@ class _GatedFeedForwardFunction(torch.autograd.Function):
         C, H = w_gate.shape
         M = x.numel() // C
         gy = grad_y.contiguous()
-        f32 = x.dtype == torch.float32
+        f32 = x.dtype is torch.float32
         grads = [torch.empty_like(t) if need else None for t, need in zip(saved, ctx.needs_input_grad)]
-        nbytes = _abi.call("cmace_gated_ff_workspace_bytes", f32, M, C, H, 1)
+        nbytes = _gated_ff_bytes(f32, M, C, H, 1)
         ws = _workspace(x.device, nbytes)
         _abi.call("cmace_gated_ff_bwd_f32" if f32 else "cmace_gated_ff_bwd_bf16", *map(_ptr, saved), gy.data_ptr(), M, C, H,
                   ctx.activation, *map(_ptr, grads), ws.data_ptr(), nbytes, _ptr(_status_tensor(x.device)), _stream())
@@ -325,7 +335,8 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
     if activation not in _ACTIVATIONS:
         raise ValueError(f"gated_feed_forward: activation {activation!r} is none of {sorted(_ACTIVATIONS)}")
     _check_cuda(x, w_gate, w_up, w_down)
-    if x.dtype not in (torch.float32, torch.bfloat16) or any(w.dtype != x.dtype for w in (w_gate, w_up, w_down)):
+    dtype = x.dtype
+    if dtype not in (torch.float32, torch.bfloat16) or w_gate.dtype != dtype or w_up.dtype != dtype or w_down.dtype != dtype:
         raise TypeError("gated_feed_forward needs float32 or bfloat16 operands of one type")
     if x.dim() < 1 or w_gate.dim() != 2:
         raise RuntimeError("gated_feed_forward needs rows and weight matrices")
@@ -333,10 +344,10 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
     if x.shape[-1] != C or w_up.shape != (C, H) or w_down.shape != (H, C) or C < 1 or H < 1:
         raise RuntimeError(f"shape mismatch: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, "
                            f"w_down {tuple(w_down.shape)}")
-    operands = (x.contiguous(), w_gate.contiguous(), w_up.contiguous(), w_down.contiguous())
-    if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
-        return _GatedFeedForwardFunction.apply(*operands, _ACTIVATIONS[activation])
-    return _gated_ff_forward(*operands, _ACTIVATIONS[activation])
+    x, w_gate, w_up, w_down = x.contiguous(), w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
+        return _GatedFeedForwardFunction.apply(x, w_gate, w_up, w_down, _ACTIVATIONS[activation])
+    return _gated_ff_forward(x, w_gate, w_up, w_down, _ACTIVATIONS[activation])
 
 
 class GatedFeedForward(torch.nn.Module):
@@ -354,6 +365,14 @@ class GatedFeedForward(torch.nn.Module):
 # --------------------------------------------------------------------------------------
 # orthogonalised updates
 # --------------------------------------------------------------------------------------
+@functools.lru_cache(4096)
+def _orthogonalize_bytes(f32, count, m, n):
+    nbytes = _abi.call("cmace_orthogonalize_workspace_bytes", f32, count, m, n)
+    if nbytes < 0:
+        raise RuntimeError(_abi.load().cmace_last_error().decode())
+    return nbytes
+
+
 def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
     """Matrices of `update` [..., m, n] brought near their orthogonal factors by Newton-Schulz products: X = U / (|U| + eps)
     with the Frobenius norm of each matrix, then `steps` times X <- a X + (b S + c S S) X with S = X X^T and
@@ -372,10 +391,9 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
     out = torch.empty_like(u)
     count = u.numel() // (m * n)
     f32 = u.dtype == torch.float32
-    nbytes = _abi.call("cmace_orthogonalize_workspace_bytes", int(f32), count, m, n)
-    ws = _workspace(u.device, max(nbytes, 0))
-    name = "cmace_orthogonalize_" + ("f32" if f32 else "bf16")
-    _abi.call(name, _ptr(u), count, m, n, int(steps), a, b, c, float(eps), _ptr(out), _ptr(ws), nbytes,
+    nbytes = _orthogonalize_bytes(f32, count, m, n)
+    ws = _workspace(u.device, nbytes)
+    _abi.call("cmace_orthogonalize_f32" if f32 else "cmace_orthogonalize_bf16", _ptr(u), count, m, n, int(steps), a, b, c, float(eps), _ptr(out), _ptr(ws), nbytes,
               _ptr(_status_tensor(u.device)), _stream())
     _abi.launch_count += 2 + 3 * int(steps)
     return out

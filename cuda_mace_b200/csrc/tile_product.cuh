@@ -19,9 +19,10 @@
 //    memory over K = 512, three terms of it are off by 4e-6 of the largest value; in chunks by 3e-7.
 //    Compared with TF32 in three terms the operands are half as large and the instructions twice as fast.
 //
-// One persistent CTA an SM, 18 warps: 16 for the epilogue (four a quarter of the 128 tensor-memory lanes, each a quarter of
+// One persistent CTA an SM, 19 warps: 16 for the epilogue (four a quarter of the 128 tensor-memory lanes, each a quarter of
 // the columns; with eight, two a scheduler, they waited for each other's barriers, copies and special functions most of the time), one
-// thread that issues the copies, one that issues the MMAs.  Two sets of accumulator columns: the
+// thread that issues the copies, one that issues the MMAs, and a warp that fetches the blocks' scales ahead (the epilogue warps waited
+// 700 cycles a segment for them: 47 of the 180 us of the backward's hidden values at 64 000 rows, widths 128 and 512).  Two sets of accumulator columns: the
 // products of the next chunk or tile run while the epilogue reads this one's.
 #pragma once
 #include <cuda_bf16.h>
@@ -36,9 +37,10 @@
 namespace cmace {
 
 constexpr int TP_EPILOGUE_WARPS = 16;
-constexpr int TP_THREADS = (TP_EPILOGUE_WARPS + 2) * 32;   // 96 registers a thread: 64 sums of a PAIR tile and their handling
+constexpr int TP_THREADS = (TP_EPILOGUE_WARPS + 3) * 32;   // 96 registers a thread: 64 sums of a PAIR tile and their handling
 constexpr int TP_SMEM_BUDGET = 227 * 1024 - 1024;          // without the static barriers
 constexpr int TP_MAX_STAGES = 8;
+constexpr int TP_SCALES = 8;                               // chunks whose scales are ahead
 
 // GATED: D = act(x Wg) * (x Wu).  BACK: what the block's backward needs of a hidden value: h, and the gradients of both
 // projections.  GRAM, POLY, APPLY: the three products of a Newton-Schulz step.
@@ -356,14 +358,16 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
   constexpr int TERMS = PAIR ? 2 : 1;
   constexpr int STAGES = S::STAGES, ROWS = 128 * CTAS;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 9 + TP_EPILOGUE_WARPS];
+  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 9 + TP_EPILOGUE_WARPS + 2 * TP_SCALES];
   __shared__ uint32_t tmem_base_slot;
-  __shared__ float block_most[3][TP_EPILOGUE_WARPS];   // GATED: of alternating tiles; BACK: of the three outputs
+  __shared__ float block_most[2][3][TP_EPILOGUE_WARPS];   // of alternating tiles, of BACK's three outputs
+  __shared__ float scales[TP_SCALES][8];   // of a chunk: products of the inverse scales, [block of rows][of columns][projection]
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t staging = smem + (uint32_t)(STAGES * S::STAGE);
   const uint32_t full = smem_u32(&bars[0]), empty = smem_u32(&bars[TP_MAX_STAGES]);
   const uint32_t acc_full = smem_u32(&bars[2 * TP_MAX_STAGES]), acc_empty = smem_u32(&bars[2 * TP_MAX_STAGES + 4]);
   const uint32_t drain = smem_u32(&bars[2 * TP_MAX_STAGES + 8]);
+  const uint32_t scale_full = drain + 8 + 8 * TP_EPILOGUE_WARPS, scale_empty = scale_full + 8 * TP_SCALES;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int rank = CTAS == 2 ? (int)cluster_rank() : 0;
   const int64_t first_tile = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
@@ -378,6 +382,10 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       mbar_init(acc_empty + 8 * b, CTAS * TP_EPILOGUE_WARPS);   // one arrival a warp
     }
     mbar_init(drain, 1);
+    for (int s = 0; s < TP_SCALES; s++) {
+      mbar_init(scale_full + 8 * s, 1);
+      mbar_init(scale_empty + 8 * s, TP_EPILOGUE_WARPS);
+    }
     for (int w = 0; w < TP_EPILOGUE_WARPS; w++) mbar_init(drain + 8 + 8 * w, 1);   // a warp's own copies
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -556,6 +564,48 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       commit(drain);   // nothing of this block's products is in flight when the columns are given back
       if (!mbar_wait(drain, 0)) tp_report(g, 44);
     }
+  } else if (warp == TP_EPILOGUE_WARPS + 2) {
+    // ================================ scales ================================
+    // four chunks at a time, eight lanes each
+    if (PAIR) {
+      uint32_t chunk = 0;   // of this block
+      bool ok = true;
+      const int block_row = (lane >> 2) & 1, block_col = (lane >> 1) & 1, projection = lane & 1;
+      constexpr bool TWO = KIND == TP_GATED || KIND == TP_BACK;   // both projections in the first segment
+      for (int64_t t = first_tile; ok && t < g.total; t += tile_step) {
+        const TpTile T = tp_tile(g, t, TN, ROWS);
+        const int64_t row = T.row0 + 128 * rank + 64 * block_row;
+        const int col = T.n0 + (TN == 64 ? 0 : 64 * block_col);
+        for (int seg = 0; ok && seg < g.segments; seg++) {
+          const bool last = g.a_of_last && T.batch == g.batches - 1;
+          const TpOperand &A = g.a[last ? 1 : seg], &B = g.b[TWO ? (seg == 0 ? projection : 2) : seg];
+          int k0, k1;
+          tp_range(g, T.split, seg, k0, k1);
+          // past the end there are zeros, in any scale
+          const float *pa = A.scale && row < g.rows ? A.scale + T.batch * A.sc_b + (row >> 6) * A.sc_i : nullptr;
+          const float *pb = B.scale && col < g.cols ? B.scale + T.batch * B.sc_b + (col >> 6) * B.sc_i : nullptr;
+          for (int kb = k0; ok && kb < k1; kb += 4) {
+            const int mine = kb + (lane >> 3), n = k1 - kb < 4 ? k1 - kb : 4;
+            float a = 1.f, b = 1.f;
+            if (mine < k1) {
+              if (pa) a = __ldcg(pa + mine * A.sc_k);
+              if (pb) b = __ldcg(pb + mine * B.sc_k);
+            }
+            for (int i = 0; ok && i < n; i++) {
+              const uint32_t slot = (chunk + i) % TP_SCALES;
+              if (!warp_wait(scale_empty + 8 * slot, ((chunk + i) / TP_SCALES & 1) ^ 1, lane)) {
+                if (lane == 0) tp_report(g, 51);
+                ok = false;
+              }
+            }
+            if (mine < k1) scales[(chunk + (lane >> 3)) % TP_SCALES][lane & 7] = a * b;
+            __syncwarp();
+            if (ok && lane < n) mbar_arrive(scale_full + 8 * ((chunk + lane) % TP_SCALES));
+            chunk += n;
+          }
+        }
+      }
+    }
   } else {
     // ================================ epilogue ================================
     const int q = warp & 3, part = warp >> 2;
@@ -594,6 +644,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
     };
     // A warp whose wait gave up goes through the rest of its tiles without waiting: others meet it at the named barriers.
     int odd = 0;
+    uint32_t chunk = 0;
     for (int64_t t = first_tile; t < g.total; t += tile_step, odd ^= 1) {
       const TpTile T = tp_tile(g, t, TN, ROWS);
       const int64_t row = T.row0 + 128 * rank + 32 * q;   // first row of this warp
@@ -625,30 +676,15 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           const int i1 = KIND == TP_BACK && seg == 0 ? SEG0_GROUPS : GROUPS;
           int k0, k1;
           tp_range(g, T.split, seg, k0, k1);
-          const bool last = g.a_of_last && T.batch == g.batches - 1;
-          constexpr bool TWO = KIND == TP_GATED || KIND == TP_BACK;   // both projections in the first segment
-          const TpOperand &A = g.a[last ? 1 : seg];
-          const TpOperand &B0 = g.b[TWO ? 2 * seg : seg];
-          // inverse scales, one block of rows a warp, one of columns (of each projection)
-          const int cb = (TWO && TN == 64 ? T.n0 : col0) >> 6;
-          const bool a_rows = row < g.rows, b_cols = (int64_t)cb * 64 < g.cols;   // past the end: zeros in any scale
-          const float *pa = A.scale && a_rows ? A.scale + T.batch * A.sc_b + (row >> 6) * A.sc_i : nullptr;
-          const float *pb0 = B0.scale && b_cols ? B0.scale + T.batch * B0.sc_b + cb * B0.sc_i : nullptr;
-          const float *pb1 = TWO && seg == 0 && g.b[1].scale && b_cols ? g.b[1].scale + cb * g.b[1].sc_i : nullptr;
-          float na = 1.f, nb0 = 1.f, nb1 = 1.f;
-          const auto fetch = [&](int kb) {
-            if (pa) na = __ldcg(pa + kb * A.sc_k);
-            if (pb0) nb0 = __ldcg(pb0 + kb * B0.sc_k);
-            if (TWO && seg == 0 && pb1) nb1 = __ldcg(pb1 + kb * B0.sc_k);   // both projections' weights are of one size
-          };
-          fetch(k0);
-          for (int kb = k0; kb < k1; kb++) {
-            const float s0 = na * nb0, s1 = na * nb1;
-            if (kb + 1 < k1) fetch(kb + 1);
-            if (ok && !warp_wait(acc_full + 8 * buf, uses >> buf & 1, lane)) {
+          constexpr bool TWO = KIND == TP_GATED || KIND == TP_BACK;
+          for (int kb = k0; kb < k1; kb++, chunk++) {
+            const uint32_t slot = chunk % TP_SCALES;
+            if (ok && !(warp_wait(scale_full + 8 * slot, chunk / TP_SCALES & 1, lane) && warp_wait(acc_full + 8 * buf, uses >> buf & 1, lane))) {
               if (lane == 0) tp_report(g, 45);
               ok = false;
             }
+            const float *scale = scales[slot] + 4 * (q >> 1) + 2 * (part >> 1);   // TN = 64: both blocks of columns are the one
+            const float s0 = scale[0], s1 = scale[1];
             tc_fence_after();
             const uint32_t at = lanes + (uint32_t)(buf * S::BUFFER_COLS);
 #pragma unroll
@@ -660,6 +696,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               tp_add(acc[i], v, TWO && i / EACH == 1 ? s1 : s0);
             }
             release(buf);
+            if (ok && lane == 0) mbar_arrive(scale_empty + 8 * slot);   // after the warp has met in release()
             next_buffer();
           }
         }
@@ -696,9 +733,9 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           }
           // a block of 64 x 64 values is two quarters' and two parts' warps'
           most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-          if (lane == 0) block_most[odd][warp] = most;
+          if (lane == 0) block_most[odd][0][warp] = most;
           tp_bar(1 + 2 * (part >> 1) + (q >> 1), 128);
-          const float scale = tp_scale(fmaxf(fmaxf(most, block_most[odd][warp ^ 1]), fmaxf(block_most[odd][warp ^ 4], block_most[odd][warp ^ 5])));
+          const float scale = tp_scale(fmaxf(fmaxf(most, block_most[odd][0][warp ^ 1]), fmaxf(block_most[odd][0][warp ^ 4], block_most[odd][0][warp ^ 5])));
           if (lane == 0 && (q & 1) == 0 && (part & 1) == 0 && row < g.rows && col0 < g.cols)
             g.out_scale[0][(row >> 6) * g.out_scale_ld + (col0 >> 6)] = 1.0f / scale;
           uint32_t w[16], lo[16];
@@ -748,19 +785,18 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
 #pragma unroll
             for (int p = 0; p < 3; p++) {
               most[p] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most[p])));
-              if (lane == 0) block_most[p][warp] = most[p];
+              if (lane == 0) block_most[odd][p][warp] = most[p];
             }
             tp_bar(1 + (q >> 1), 256);   // 64 rows x 64 columns: two quarters, all parts
 #pragma unroll
             for (int p = 0; p < 3; p++) {
               float m = 0.f;
 #pragma unroll
-              for (int k = 0; k < 4; k++) m = fmaxf(m, fmaxf(block_most[p][(q & 2) + 4 * k], block_most[p][(q & 2) + 1 + 4 * k]));
+              for (int k = 0; k < 4; k++) m = fmaxf(m, fmaxf(block_most[odd][p][(q & 2) + 4 * k], block_most[odd][p][(q & 2) + 1 + 4 * k]));
               scale[p] = tp_scale(m);
               if (lane == 0 && (q & 1) == 0 && part == 0 && row < g.rows && T.n0 < g.cols)
                 g.out_scale[p][(row >> 6) * g.out_scale_ld + (T.n0 >> 6)] = 1.0f / scale[p];
             }
-            tp_bar(1 + (q >> 1), 256);   // read by all before the next tile's are written
           }
 #pragma unroll
           for (int p = 0; p < 3; p++) {

@@ -5,8 +5,9 @@
 // What the precision asks for: a small singular value is multiplied by a up to `steps` times (485 with the usual coefficients), and so is
 // what rounding adds along its direction.  X itself is therefore kept to 22 bits or more, as a pair of fp16 values (tile_product.cuh), and
 // a X formed from both; the operands of the products may be rounded further, since what that adds lies in the rows or in the columns of the large values, turns their
-// vectors by the rounding and is not multiplied.  float32 takes pairs there too, bf16 the high values alone (2^-12 instead of the
-// result's 2^-9).  fp16's range suffices without looking at the values: |X|_2 <= 1 bounds every entry of X, S and b S + c S S in
+// vectors by the rounding and is not multiplied.  float32 takes pairs there too.  bf16 takes the high values alone (2^-12 instead of the
+// result's 2^-9) but for S S, the smallest of the products, whose rounding weighs most: with pairs there the error of a result is 1.2 to
+// 1.4 times that of its own rounding, without 1.6 to 1.8.  fp16's range suffices without looking at the values: |X|_2 <= 1 bounds every entry of X, S and b S + c S S in
 // every step, and the host makes powers of two of the bounds.
 #include <algorithm>
 #include <cmath>
@@ -575,10 +576,13 @@ static NsVariant ns_variant(bool pair, int64_t rows, int cols, int kblocks, int6
   return {two < one ? 2 : 1, 128};
 }
 template <int KIND>
-static int launch_ns(bool pair, NsVariant v, TpArgs &g, cudaStream_t st, const char *what) {
+static int launch_ns(NsVariant v, TpArgs &g, cudaStream_t st, const char *what) {
+  return v.ctas == 2 ? tp_launch<KIND, true, 128, 2>(g, st, what) : tp_launch<KIND, true, 128, 1>(g, st, what);
+}
+template <int KIND>
+static int launch_ns_single(NsVariant v, TpArgs &g, cudaStream_t st, const char *what) {
   if (v.tn == 256) return tp_launch<KIND, false, 256, 2>(g, st, what);
-  if (v.ctas == 2) return pair ? tp_launch<KIND, true, 128, 2>(g, st, what) : tp_launch<KIND, false, 128, 2>(g, st, what);
-  return pair ? tp_launch<KIND, true, 128, 1>(g, st, what) : tp_launch<KIND, false, 128, 1>(g, st, what);
+  return v.ctas == 2 ? tp_launch<KIND, false, 128, 2>(g, st, what) : tp_launch<KIND, false, 128, 1>(g, st, what);
 }
 
 // CTAs a matrix for the kernel above, 0: it does not fit
@@ -643,7 +647,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   double *partial = w.take<double>(f.count * chunks);
   Matrix x[2];
   for (Matrix &m : x) m = new_matrix(w, true, f.rows, f.cols, f.count, 64, false);
-  Matrix s = new_matrix(w, true, side, side, f.count, 64, false), poly = new_matrix(w, f.f32, side, side, f.count, 64, false);
+  Matrix s = new_matrix(w, true, side, side, f.count, 64, false), poly = new_matrix(w, true, side, side, f.count, 64, false);
   if (!w.base) return CMACE_OK;
 
   double most = 1.0;   // bound of the singular values
@@ -655,7 +659,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   int rc = check_launch(f.what);
   // maps: operands; what is added and written, in boxes of the variants' columns a warp
   const int kb_s = blocks64(wide ? f.cols : f.rows), kb = blocks64(side);
-  const NsVariant v_gram = ns_variant(f.f32, side, side, kb_s, f.count), v_poly = ns_variant(f.f32, side, side, kb, f.count),
+  const NsVariant v_gram = ns_variant(f.f32, side, side, kb_s, f.count), v_poly = ns_variant(true, side, side, kb, f.count),
                   v_apply = ns_variant(f.f32, f.rows, f.cols, kb, f.count);
   CUtensorMap part_x[2], to_s, from_s, to_poly;
   TpOut to_out;
@@ -685,7 +689,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     g.out[0].map = to_s;
     g.alpha = 1.0f / (sx * sx);
     g.pair_scale = ss;
-    rc = launch_ns<TP_GRAM>(f.f32, v_gram, g, f.st, f.what);
+    rc = f.f32 ? launch_ns<TP_GRAM>(v_gram, g, f.st, f.what) : launch_ns_single<TP_GRAM>(v_gram, g, f.st, f.what);
 
     g.kblocks[0] = kb;
     set_operand(g.a[0], s, true);
@@ -693,7 +697,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     g.out[0].map = to_poly;
     g.cin = from_s;
     g.alpha = (float)f.c / (ss * ss), g.beta = (float)f.b / ss, g.pair_scale = sp;
-    if (!rc) rc = launch_ns<TP_POLY>(f.f32, v_poly, g, f.st, f.what);
+    if (!rc) rc = launch_ns<TP_POLY>(v_poly, g, f.st, f.what);
 
     g.rows = f.rows, g.cols = f.cols;
     set_operand(g.a[0], wide ? poly : now, true);
@@ -703,7 +707,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     g.out_bf16 = !f.f32;
     g.cin = part_x[step & 1];
     g.alpha = 1.0f / (sp * sx), g.beta = (float)f.a / sx, g.pair_scale = last ? 0.f : sn;
-    if (!rc) rc = launch_ns<TP_APPLY>(f.f32, v_apply, g, f.st, f.what);
+    if (!rc) rc = f.f32 ? launch_ns<TP_APPLY>(v_apply, g, f.st, f.what) : launch_ns_single<TP_APPLY>(v_apply, g, f.st, f.what);
     most = most_next;
     sx = sn;
   }

@@ -900,8 +900,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           }
         }
         if (!result) {
-          constexpr int Z = PAIR || KIND != TP_POLY ? 2 : 1;   // S and X are also added as they are: with their low part
-          st.send(&g.out[0].map, 0, col0, row, Z * T.batch);
+          st.send(&g.out[0].map, 0, col0, row, 2 * T.batch);
           if (!CIN) {
             st.begin();
 #pragma unroll
@@ -912,7 +911,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               st.put<ROW>(0, 2 * i, lo);
             }
           }
-          if (Z == 2) st.send(&g.out[0].map, CIN ? LOW : 0u, col0, row, 2 * T.batch + 1);
+          st.send(&g.out[0].map, CIN ? LOW : 0u, col0, row, 2 * T.batch + 1);
         } else {
           __syncwarp();
 #pragma unroll

@@ -18,6 +18,7 @@ fallback: a CPU tensor raises.
 """
 import functools
 import math
+import os
 from collections import OrderedDict
 
 import torch
@@ -275,56 +276,21 @@ def tensor_core_ok(dtype, K, N):
 # gated feed-forward block
 # --------------------------------------------------------------------------------------
 _ACTIVATIONS = {"silu": 0, "gelu": 1}
+_DENSE_LIB_PATH = os.path.join(os.path.dirname(_abi.LIB_PATH), "libcuda_mace_b200_dense.so")
+_gated_feed_forward = None   # the torch operator of csrc/dense_ops.cpp, once it is loaded
+
+
+def _load_dense():
+    global _gated_feed_forward
+    _abi.load()   # the operators link against the C-ABI library
+    if not os.path.isfile(_DENSE_LIB_PATH):
+        raise ImportError(f"{_DENSE_LIB_PATH} is missing: build it with `python -m cuda_mace_b200.build`")
+    torch.ops.load_library(_DENSE_LIB_PATH)
+    _gated_feed_forward = torch.ops.cmace_b200.gated_feed_forward.default
 
 
 def _workspace(device, nbytes):
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
-
-
-@functools.lru_cache(4096)
-def _gated_ff_bytes(f32, M, C, H, backward):
-    nbytes = _abi.call("cmace_gated_ff_workspace_bytes", f32, M, C, H, backward)
-    if nbytes < 0:
-        raise RuntimeError(_abi.load().cmace_last_error().decode())
-    return nbytes
-
-
-def _gated_ff_forward(x, w_gate, w_up, w_down, activation):
-    C, H = w_gate.shape
-    M = x.numel() // C
-    y = torch.empty_like(x)
-    f32 = x.dtype is torch.float32
-    device = x.device
-    nbytes = _gated_ff_bytes(f32, M, C, H, 0)
-    ws = _workspace(device, nbytes)
-    _abi.call("cmace_gated_ff_fwd_f32" if f32 else "cmace_gated_ff_fwd_bf16", x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
-              w_down.data_ptr(), M, C, H, activation, y.data_ptr(), ws.data_ptr(), nbytes, _status_tensor(device).data_ptr(),
-              _stream())
-    return y
-
-
-class _GatedFeedForwardFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, activation):
-        ctx.save_for_backward(x, w_gate, w_up, w_down)
-        ctx.activation = activation
-        return _gated_ff_forward(x, w_gate, w_up, w_down, activation)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_y):
-        saved = ctx.saved_tensors
-        x, w_gate = saved[:2]
-        C, H = w_gate.shape
-        M = x.numel() // C
-        gy = grad_y.contiguous()
-        f32 = x.dtype is torch.float32
-        grads = [torch.empty_like(t) if need else None for t, need in zip(saved, ctx.needs_input_grad)]
-        nbytes = _gated_ff_bytes(f32, M, C, H, 1)
-        ws = _workspace(x.device, nbytes)
-        _abi.call("cmace_gated_ff_bwd_f32" if f32 else "cmace_gated_ff_bwd_bf16", *map(_ptr, saved), gy.data_ptr(), M, C, H,
-                  ctx.activation, *map(_ptr, grads), ws.data_ptr(), nbytes, _ptr(_status_tensor(x.device)), _stream())
-        return (*grads, None)
 
 
 def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
@@ -332,22 +298,15 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
     float32 or all bfloat16; `activation` is "silu" or "gelu" (with erf).  Differentiable (once) in x and the three weights.
     Sums are float32 in both types; float32 runs on the tensor cores in three terms (cmace_gated_ff_fwd_f32), bfloat16 rounds the hidden
     values to bfloat16 between the products.  The backward keeps x and the weights only and forms the hidden values again."""
-    if activation not in _ACTIVATIONS:
+    code = _ACTIVATIONS.get(activation)
+    if code is None:
         raise ValueError(f"gated_feed_forward: activation {activation!r} is none of {sorted(_ACTIVATIONS)}")
-    _check_cuda(x, w_gate, w_up, w_down)
-    dtype = x.dtype
-    if dtype not in (torch.float32, torch.bfloat16) or w_gate.dtype != dtype or w_up.dtype != dtype or w_down.dtype != dtype:
-        raise TypeError("gated_feed_forward needs float32 or bfloat16 operands of one type")
-    if x.dim() < 1 or w_gate.dim() != 2:
-        raise RuntimeError("gated_feed_forward needs rows and weight matrices")
-    C, H = w_gate.shape
-    if x.shape[-1] != C or w_up.shape != (C, H) or w_down.shape != (H, C) or C < 1 or H < 1:
-        raise RuntimeError(f"shape mismatch: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, "
-                           f"w_down {tuple(w_down.shape)}")
-    x, w_gate, w_up, w_down = x.contiguous(), w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
-        return _GatedFeedForwardFunction.apply(x, w_gate, w_up, w_down, _ACTIVATIONS[activation])
-    return _gated_ff_forward(x, w_gate, w_up, w_down, _ACTIVATIONS[activation])
+    if not x.is_cuda:
+        raise RuntimeError("cuda_mace_b200 operators need CUDA tensors (there is no CPU path)")
+    if _gated_feed_forward is None:
+        _load_dense()
+    _abi.launch_count += 3 if x.dtype is torch.float32 else 2
+    return _gated_feed_forward(x, w_gate, w_up, w_down, code, _status_tensor(x.device))
 
 
 class GatedFeedForward(torch.nn.Module):

@@ -96,3 +96,138 @@ def test_values(shape, dtype, kind, dev):
     U = update(sum(shape), shape, dtype, dev, kind)
     check(ops.orthogonalize(U), U)
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shape", [(2, 48, 80), (1, 200, 150)])
+@pytest.mark.parametrize("steps,coefficients,eps", [(1, USUAL, 1e-7), (3, (2.0, -1.5, 0.5), 0.0), (8, (1.5, -0.5, 0.0), 1e-3), (2, (0.0, 1.0, 0.0), 1e-7),
+                                                    (2, (1.0, 0.0, 0.0), 1e-7)])
+def test_coefficients(shape, steps, coefficients, eps, dtype, dev):
+    from cuda_mace_b200 import ops
+
+    U = update(5, shape, dtype, dev)
+    check(ops.orthogonalize(U, steps=steps, coefficients=coefficients, eps=eps), U, steps, coefficients, eps)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shape", [(3, 40, 56), (3, 200, 150), (2, 30, 700)])
+def test_zeros_and_what_is_not_finite(shape, dtype, dev):
+    """A matrix of zeros stays one; an infinity or a NaN spoils its own matrix."""
+    from cuda_mace_b200 import ops
+
+    U = update(6, shape, dtype, dev)
+    want = ops.orthogonalize(U)
+    for bad in (0.0, float("inf"), float("nan")):
+        V = U.clone()
+        if bad == 0.0:
+            V[1] = 0
+        else:
+            V[1, 3, 5] = bad
+        out = ops.orthogonalize(V)
+        assert torch.equal(out[0], want[0]) and (len(U) < 3 or torch.equal(out[2], want[2]))
+        assert not out[1].any() if bad == 0.0 else not torch.isfinite(out[1]).all()
+
+
+@pytest.mark.parametrize("shape", [(2, 33, 90), (1, 150, 200)])
+@pytest.mark.parametrize("size", [1e-25, 1e-12, 1e9, 1e25])
+def test_sizes_of_updates(shape, size, dev):
+    """With eps = 0 the result does not depend on the update's size."""
+    from cuda_mace_b200 import ops
+
+    U = update(7, shape, F32, dev)
+    V = U * size
+    check(ops.orthogonalize(V, eps=0.0), V, eps=0.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shape", [(2, 3, 40, 56), (2, 2, 150, 200)])
+def test_layouts(shape, dtype, dev):
+    """Stacks of stacks (ElementalLinear's [Z, 4, K, N]), transposed and odd addresses, single matrices, empty stacks."""
+    from cuda_mace_b200 import ops
+
+    U = update(8, shape, dtype, dev)
+    want = ops.orthogonalize(U)
+    assert want.shape == U.shape
+    assert torch.equal(ops.orthogonalize(U.view(-1, *shape[-2:])), want.view(-1, *shape[-2:]))
+    assert torch.equal(ops.orthogonalize(U[1, 1]), want[1, 1])
+    assert torch.equal(ops.orthogonalize(U.transpose(-1, -2).contiguous().transpose(-1, -2)), want)
+    room = torch.zeros(U.numel() + 1, dtype=dtype, device=dev)
+    room[1:].copy_(U.reshape(-1))
+    check(ops.orthogonalize(room[1:].view(shape)), U)
+    assert ops.orthogonalize(U[:0]).shape == (0, *shape[1:])
+    t = ops.orthogonalize(U.transpose(-1, -2))
+    check(t, U.transpose(-1, -2))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shape", [(5, 64, 64), (2, 100, 500), (1, 200, 300)])
+def test_same_bits_streams_and_graphs(shape, dtype, dev):
+    from cuda_mace_b200 import ops
+
+    sets = [update(20 + k, shape, dtype, dev) for k in range(3)]
+    want = [ops.orthogonalize(U) for U in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got.append(ops.orthogonalize(sets[k]))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    static = sets[0].clone()
+    graphs, outs, pool = [], [], None
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(ops.orthogonalize(static))
+        pool = g.pool()
+        graphs.append(g)
+    for k in (1, 2, 0):
+        static.copy_(sets[k])
+        for g, out in zip(graphs, outs):
+            g.replay()
+            assert torch.equal(out, want[k])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shape", [(2, 50, 60), (1, 150, 260), (2, 40, 600)])
+def test_in_place(shape, dtype, dev):
+    """The C entry takes its input as its output."""
+    from cuda_mace_b200 import _abi, ops
+
+    U = update(9, shape, dtype, dev)
+    want = ops.orthogonalize(U)
+    f32 = dtype == F32
+    n = _abi.call("cmace_orthogonalize_workspace_bytes", f32, *shape)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    _abi.call("cmace_orthogonalize_" + ("f32" if f32 else "bf16"), U.data_ptr(), *shape, 5, *USUAL, 1e-7, U.data_ptr(), ws.data_ptr(), n, 0,
+              torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(U, want)
+
+
+def test_refusals_on_the_device(dev):
+    from cuda_mace_b200 import _abi, ops
+
+    U = update(10, (2, 20, 30), F32, dev)
+    with pytest.raises(RuntimeError, match="may grow"):
+        ops.orthogonalize(U, steps=20, coefficients=(10.0, 0.0, 0.0))
+    with pytest.raises(RuntimeError, match="bad sizes"):
+        ops.orthogonalize(U, steps=0)
+    with pytest.raises(RuntimeError, match="bad coefficients"):
+        ops.orthogonalize(U, coefficients=(float("nan"), 0.0, 0.0))
+    with pytest.raises(RuntimeError, match="bad coefficients"):
+        ops.orthogonalize(U, eps=-1.0)
+    with pytest.raises(TypeError):
+        ops.orthogonalize(U.double())
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.orthogonalize(U.clone().requires_grad_(True))
+    with torch.no_grad():
+        ops.orthogonalize(U.clone().requires_grad_(True))
+    out = torch.full_like(U, 3.0)
+    V = update(10, (2, 200, 300), F32, dev)
+    with pytest.raises(RuntimeError, match="needed"):
+        _abi.call("cmace_orthogonalize_f32", V.data_ptr(), 2, 200, 300, 5, *USUAL, 1e-7, out.data_ptr(), V.data_ptr() & ~255, 16, 0, 0)
+    torch.cuda.synchronize()
+    assert (out == 3.0).all()

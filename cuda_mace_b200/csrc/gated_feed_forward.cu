@@ -432,13 +432,13 @@ static int forward(const FeedForward &f, void *y, Carve &w) {
   set_operand(g.a[0], x, true);
   set_operand(g.b[0], wg, false);
   set_operand(g.b[1], wu, false);
-  g.kblocks[0] = blocks64(f.C);
+  set_k(g, 0, f.C);
   if (!rc) rc = set_hidden_out(g, h, 32, bf16, f.what);
   if (!rc) rc = f.act == TP_SILU ? launch_gated<TP_SILU>(f, g) : launch_gated<TP_GELU>(f, g);
   g = new_args(f.M, f.C, f.status);
   set_operand(g.a[0], h, true);
   set_operand(g.b[0], wd, false);
-  g.kblocks[0] = blocks64(f.H);
+  set_k(g, 0, f.H);
   if (!rc) rc = set_user_out(g, y, f.f32, f.M, f.C, f.what);
   if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
   return rc;
@@ -468,7 +468,8 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   set_operand(g.b[1], wu, false);
   set_operand(g.b[2], wd, true);
   g.segments = 2;
-  g.kblocks[0] = g.kblocks[1] = blocks64(f.C);
+  set_k(g, 0, f.C);
+    set_k(g, 1, f.C);
   if (!rc) rc = set_hidden_out(g, hidden, 16, bf16, f.what);
   if (!rc) rc = f.act == TP_SILU ? launch_back<TP_SILU>(f, g) : launch_back<TP_GELU>(f, g);
   if (want_x) {
@@ -478,7 +479,8 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
     set_operand(g.b[0], wg, true);
     set_operand(g.b[1], wu, true);
     g.segments = 2;
-    g.kblocks[0] = g.kblocks[1] = blocks64(f.H);
+    set_k(g, 0, f.H);
+    set_k(g, 1, f.H);
     if (!rc) rc = set_user_out(g, gx, f.f32, f.M, f.C, f.what);
     if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
   }
@@ -489,7 +491,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
       set_operand(g.b[0], gw[0] && gw[1] ? hidden : hidden.part(gw[0] ? 0 : 1), false);
       g.batches = gw[0] && gw[1] ? 2 : 1;
       g.out_of_batch = 1;
-      g.kblocks[0] = blocks64(f.M);
+      set_k(g, 0, f.M);
       if (!rc) rc = set_user_out(g, gw[0] ? gw[0] : gw[1], f.f32, f.C, f.H, f.what, 0);
       if (!rc && g.batches == 2) rc = set_user_out(g, gw[1], f.f32, f.C, f.H, f.what, 1);
       if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
@@ -498,7 +500,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
       g = new_args(f.H, f.C, f.status);
       set_operand(g.a[0], hidden.part(2), false);
       set_operand(g.b[0], gy, false);
-      g.kblocks[0] = blocks64(f.M);
+      set_k(g, 0, f.M);
       if (!rc) rc = set_user_out(g, gw[2], f.f32, f.H, f.C, f.what);
       if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
     }
@@ -511,7 +513,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
     g.batches = 3;
     g.splits = splits;
     g.a_of_last = 1;
-    g.kblocks[0] = blocks64(f.M);
+    set_k(g, 0, f.M);
     g.out[1].use_map = 1;
     if (!rc) rc = encode_tile_map(&g.out[1].map, partial, 4, false, f.H, f.C, (int64_t)splits * 3, ld, (int64_t)f.C * ld, 16, 32, f.what);
     if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);

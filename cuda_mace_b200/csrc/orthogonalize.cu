@@ -683,7 +683,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     TpArgs g = new_args(side, side, f.status);
     g.batches = (int)f.count;
     g.in_f16 = 1;
-    g.kblocks[0] = kb_s;
+    set_k(g, 0, wide ? f.cols : f.rows);
     set_operand(g.a[0], now, wide);
     set_operand(g.b[0], now, wide);
     g.out[0].map = to_s;
@@ -691,7 +691,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     g.pair_scale = ss;
     rc = f.f32 ? launch_ns<TP_GRAM>(v_gram, g, f.st, f.what) : launch_ns_single<TP_GRAM>(v_gram, g, f.st, f.what);
 
-    g.kblocks[0] = kb;
+    set_k(g, 0, side);
     set_operand(g.a[0], s, true);
     set_operand(g.b[0], s, true);
     g.out[0].map = to_poly;

@@ -16,7 +16,9 @@
 //    holds over 2^18 below that value and degrades to an absolute 2^-39 of it beyond.  A block of 64 k is one chunk: its sum goes
 //    to its own accumulator columns and the epilogue warps add it, times the two blocks' scales, to float32 registers, rounding to
 //    nearest.  That also keeps the tensor core's own accumulation, which truncates, to 12 instructions: summed in tensor
-//    memory over K = 512, three terms of it are off by 4e-6 of the largest value; in chunks by 3e-7.
+//    memory over K = 512, three terms of it are off by 4e-6 of the largest value; in chunks all sums come out smaller by 2.0e-7 (terms of
+//    either sign) to 2.9e-7 (of one), which the scale that they are multiplied with anyway puts back: 1 + 2^-22.  Three products one
+//    after the other are off by 2e-7 to 4e-7 with it, by 6e-7 to 9e-7 without.
 //    Compared with TF32 in three terms the operands are half as large and the instructions twice as fast.
 //
 // One persistent CTA an SM, 19 warps: 16 for the epilogue (four a quarter of the 128 tensor-memory lanes, each a quarter of
@@ -84,6 +86,7 @@ struct TpArgs {
   int32_t *status;
   int64_t rows, cols;            // of the output
   int kblocks[2], segments;      // blocks of 64 k a segment
+  int last16[2];                 // steps of 16 k in the last of them
   int batches, splits, mt, nt;
   TpDiv by_nt, by_mt, by_batches, by_splits;
   int64_t total;                 // tiles
@@ -586,9 +589,11 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           const float *pb = B.scale && col < g.cols ? B.scale + T.batch * B.sc_b + (col >> 6) * B.sc_i : nullptr;
           for (int kb = k0; ok && kb < k1; kb += 4) {
             const int mine = kb + (lane >> 3), n = k1 - kb < 4 ? k1 - kb : 4;
-            float a = 1.f, b = 1.f;
+            // what truncation takes, by the additions that have something to add
+            const int steps = mine + 1 == g.kblocks[seg] ? g.last16[seg] : 4;
+            float a = steps == 4 ? 1.f + 0x1p-22f : (steps > 1 ? 1.f + 0x1p-23f : 1.f), b = 1.f;
             if (mine < k1) {
-              if (pa) a = __ldcg(pa + mine * A.sc_k);
+              if (pa) a *= __ldcg(pa + mine * A.sc_k);
               if (pb) b = __ldcg(pb + mine * B.sc_k);
             }
             for (int i = 0; ok && i < n; i++) {
@@ -1042,6 +1047,10 @@ inline TpArgs new_args(int64_t rows, int64_t cols, int32_t *status) {
   return g;
 }
 inline int blocks64(int64_t n) { return (int)((n + 63) / 64); }
+inline void set_k(TpArgs &g, int seg, int64_t k) {
+  g.kblocks[seg] = blocks64(k);
+  g.last16[seg] = (int)((k - 1) % 64) / 16 + 1;
+}
 
 // What a variant costs in cycles: rounds of its tiles over the SMs, each as long as its products or, at 64 bytes a cycle and SM, its copies,
 // and something for the epilogue and the chain at a tile's ends.  n: columns of B, out: of the output, tn: of a tile.

@@ -408,15 +408,17 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
     } else {
       // part: [128 rows][32 pieces of four columns], the piece changed by the row: a warp's accesses meet all banks.  Between SMs it is bytes
       // that count, 11 to 12 a cycle here whichever side moves them: each CTA fetches its share of the rows and sends pairs.
-      constexpr int SHARE = 128 / CLUSTER;
+      if (mine)
 #pragma unroll
-      for (int c = 0; c < 8; c++)
-        smem_store4(part + (uint32_t)(row * 512 + (((8 * group + c) ^ (row & 31)) << 4)), __float_as_uint(s[4 * c]), __float_as_uint(s[4 * c + 1]),
-                    __float_as_uint(s[4 * c + 2]), __float_as_uint(s[4 * c + 3]));
+        for (int c = 0; c < 8; c++)
+          smem_store4(part + (uint32_t)(row * 512 + (((8 * group + c) ^ (row & 31)) << 4)), __float_as_uint(s[4 * c]), __float_as_uint(s[4 * c + 1]),
+                      __float_as_uint(s[4 * c + 2]), __float_as_uint(s[4 * c + 3]));
       meet(0);
-#pragma unroll
-      for (int e = tid; e < SHARE * 32; e += NSF_THREADS) {   // four columns of a row: a warp's loads are 512 bytes on end
-        const int r = (int)rank * SHARE + (e >> 5), piece = e & 31;
+      // four columns a lane: a warp's loads are a row of up to 512 bytes on end
+      const int share = (side16 + CLUSTER - 1) / CLUSTER, piece = lane;
+#pragma unroll 2
+      for (int r = (int)rank * share + warp; r < min((int)(rank + 1) * share, side16); r += NSF_THREADS / 32) {
+        if (4 * piece >= side16) break;
         const uint32_t from = part + (uint32_t)(r * 512 + ((piece ^ (r & 31)) << 4));
         float4 x[CLUSTER];
 #pragma unroll
@@ -589,7 +591,8 @@ static int launch_ns_single(NsVariant v, TpArgs &g, cudaStream_t st, const char 
 static int fused_cluster(int64_t count, int64_t rows, int cols) {
   const int64_t side = std::min<int64_t>(rows, cols), length = std::max<int64_t>(rows, cols);
   if (side > 128 || length > 1024) return 0;
-  if (length <= 128 || (length <= 256 && count > 74)) return 1;
+  // one of 128 x 160: 44 us in one CTA, 49 in two; of 128 x 256: 53 and 51 (64 x 160: 33 and 35, 64 x 256: 39 and 35)
+  if (length <= 192 || (length <= 256 && count > 74)) return 1;
   int p = 2;
   while (p * 128 < length) p *= 2;
   return p;

@@ -281,11 +281,24 @@ __device__ __forceinline__ float tp_sigmoid(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + tp_ex2(-1.4426950408889634f * x)));
   return y;
 }
+// Cumulative normal distribution by formula 7.1.26 of Abramowitz and Stegun's Handbook (after Hastings): erfc(z) = e^(-z^2) times a polynomial
+// of 1 / (1 + p z), to 1.5e-7, without a branch and without the cancellation of 1 + erf far below zero.  e: e^(-g^2 / 2), which the derivative
+// takes as well.  (erff: two ways for small and large arguments, which the lanes of a warp both go.)
+__device__ __forceinline__ float tp_normal_cdf(float g, float &e) {
+  const float z = fabsf(g) * 0.70710678118654752f;
+  float t;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f, z, 1.0f)));
+  e = tp_ex2(-1.4426950408889634f * z * z);
+  const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  const float tail = 0.5f * poly * e;
+  return g < 0.f ? tail : 1.0f - tail;   // NaN stays NaN
+}
 // act(g); with the derivative
 template <int ACT>
 __device__ __forceinline__ float tp_act(float g) {
   if (ACT == TP_SILU) return g * tp_sigmoid(g);
-  return g * (0.5f * (1.0f + erff(g * 0.70710678118654752f)));
+  float e;
+  return g * tp_normal_cdf(g, e);
 }
 template <int ACT>
 __device__ __forceinline__ float tp_act(float g, float &d) {
@@ -295,8 +308,9 @@ __device__ __forceinline__ float tp_act(float g, float &d) {
     d = s * (1.0f + (g - a));
     return a;
   }
-  const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-  d = cdf + g * (0.39894228040143268f * tp_ex2(-0.72134752044448170f * g * g));
+  float e;
+  const float cdf = tp_normal_cdf(g, e);
+  d = cdf + 0.39894228040143268f * g * e;
   return g * cdf;
 }
 
@@ -337,18 +351,26 @@ struct TpStager {
   // rows that TMA cannot address, from a piece: two rows an instruction, a lane has one float32 or two 16-bit columns
   __device__ __forceinline__ void send_rows(const TpOut &o, bool sixteen, uint32_t piece, int col, int64_t row, int batch) const {
     __syncwarp();
-    const int64_t base = (int64_t)batch * o.batch;
-    const int w = lane & 15;
-    for (int r = lane >> 4; r < 32 && row + r < rows; r += 2) {
-      uint32_t v;
-      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(smem + piece + (uint32_t)sw64_offset(r, w >> 2) + 4u * (uint32_t)(w & 3)) : "memory");
-      const int64_t at = base + (row + r) * o.ld + col;
-      if (!sixteen) {
-        if (col + w < cols) static_cast<uint32_t *>(o.ptr)[at + w] = v;
-      } else {
-        uint16_t *p = static_cast<uint16_t *>(o.ptr) + at + 2 * w;
-        if (col + 2 * w < cols) p[0] = (uint16_t)v;
-        if (col + 2 * w + 1 < cols) p[1] = (uint16_t)(v >> 16);
+    const int w = lane & 15, r0 = lane >> 4, n = (int)(rows - row < 32 ? rows - row : 32);
+    uint32_t v[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+      asm volatile("ld.shared.b32 %0, [%1];"
+                   : "=r"(v[i])
+                   : "r"(smem + piece + (uint32_t)sw64_offset(r0 + 2 * i, w >> 2) + 4u * (uint32_t)(w & 3))
+                   : "memory");
+    const int64_t at = (int64_t)batch * o.batch + (row + r0) * o.ld + col + (sixteen ? 2 * w : w);
+    if (!sixteen) {
+      uint32_t *p = static_cast<uint32_t *>(o.ptr) + at;
+#pragma unroll
+      for (int i = 0; i < 16; i++, p += 2 * o.ld)
+        if (r0 + 2 * i < n && col + w < cols) *p = v[i];
+    } else {
+      uint16_t *p = static_cast<uint16_t *>(o.ptr) + at;
+#pragma unroll
+      for (int i = 0; i < 16; i++, p += 2 * o.ld) {
+        if (r0 + 2 * i < n && col + 2 * w < cols) p[0] = (uint16_t)v[i];
+        if (r0 + 2 * i < n && col + 2 * w + 1 < cols) p[1] = (uint16_t)(v[i] >> 16);
       }
     }
     __syncwarp();

@@ -1074,7 +1074,7 @@ inline void set_k(TpArgs &g, int seg, int64_t k) {
   g.last16[seg] = (int)((k - 1) % 64) / 16 + 1;
 }
 
-// What a variant costs in cycles: rounds of its tiles over the SMs, each as long as its products or, at 64 bytes a cycle and SM, its copies,
+// What a variant costs in cycles: rounds of its tiles over the SMs, each as long as its products or, at 50 bytes a cycle and SM, its copies,
 // and something for the epilogue and the chain at a tile's ends.  n: columns of B, out: of the output, tn: of a tile.
 struct TpCost {
   int64_t rows, out;
@@ -1084,7 +1084,7 @@ struct TpCost {
   int64_t operator()(int ctas, int tn, int n) const {
     const int64_t tiles = (rows + 128 * ctas - 1) / (128 * ctas) * ((out + tn - 1) / tn) * times;
     const int64_t rounds = (tiles + 148 / ctas - 1) / (148 / ctas);
-    const int64_t products = (pair ? 3 : 1) * 2 * n, copies = (pair ? 2 : 1) * (128 + n / ctas) * 2;   // a block of 64 k
+    const int64_t products = (pair ? 3 : 1) * 2 * n, copies = (pair ? 2 : 1) * (128 + n / ctas) * 128 / 50;   // a block of 64 k
     return rounds * (kblocks * (products > copies ? products : copies) + 2000 + 16 * n);
   }
 };

@@ -42,7 +42,6 @@ constexpr int TP_EPILOGUE_WARPS = 16;
 constexpr int TP_THREADS = (TP_EPILOGUE_WARPS + 3) * 32;   // 96 registers a thread: 64 sums of a PAIR tile and their handling
 constexpr int TP_SMEM_BUDGET = 227 * 1024 - 1024;          // without the static barriers
 constexpr int TP_MAX_STAGES = 8;
-constexpr int TP_SCALES = 8;                               // chunks whose scales are ahead
 
 // GATED: D = act(x Wg) * (x Wu).  BACK: what the block's backward needs of a hidden value: h, and the gradients of both
 // projections.  GRAM, POLY, APPLY: the three products of a Newton-Schulz step.
@@ -383,16 +382,16 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
   constexpr int TERMS = PAIR ? 2 : 1;
   constexpr int STAGES = S::STAGES, ROWS = 128 * CTAS;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 9 + TP_EPILOGUE_WARPS + 2 * TP_SCALES];
+  __shared__ __align__(8) uint64_t bars[2 * TP_MAX_STAGES + 13 + TP_EPILOGUE_WARPS];
   __shared__ uint32_t tmem_base_slot;
   __shared__ float block_most[2][3][TP_EPILOGUE_WARPS];   // of alternating tiles, of BACK's three outputs
-  __shared__ float scales[TP_SCALES][8];   // of a chunk: products of the inverse scales, [block of rows][of columns][projection]
+  __shared__ float scales[4][8];   // of the chunk in each set of columns: products of the inverse scales, [block of rows][of columns][projection]
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t staging = smem + (uint32_t)(STAGES * S::STAGE);
   const uint32_t full = smem_u32(&bars[0]), empty = smem_u32(&bars[TP_MAX_STAGES]);
   const uint32_t acc_full = smem_u32(&bars[2 * TP_MAX_STAGES]), acc_empty = smem_u32(&bars[2 * TP_MAX_STAGES + 4]);
   const uint32_t drain = smem_u32(&bars[2 * TP_MAX_STAGES + 8]);
-  const uint32_t scale_full = drain + 8 + 8 * TP_EPILOGUE_WARPS, scale_empty = scale_full + 8 * TP_SCALES;
+  const uint32_t scale_empty = drain + 8 + 8 * TP_EPILOGUE_WARPS;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int rank = CTAS == 2 ? (int)cluster_rank() : 0;
   const int64_t first_tile = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
@@ -403,14 +402,11 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       mbar_init(empty + 8 * s, 1);   // one commit
     }
     for (int b = 0; b < S::BUFFERS; b++) {
-      mbar_init(acc_full + 8 * b, 1);                           // one commit
+      mbar_init(acc_full + 8 * b, PAIR ? 2 : 1);                // one commit, the scales' arrival
       mbar_init(acc_empty + 8 * b, CTAS * TP_EPILOGUE_WARPS);   // one arrival a warp
     }
     mbar_init(drain, 1);
-    for (int s = 0; s < TP_SCALES; s++) {
-      mbar_init(scale_full + 8 * s, 1);
-      mbar_init(scale_empty + 8 * s, TP_EPILOGUE_WARPS);
-    }
+    for (int b = 0; b < S::BUFFERS; b++) mbar_init(scale_empty + 8 * b, TP_EPILOGUE_WARPS);
     for (int w = 0; w < TP_EPILOGUE_WARPS; w++) mbar_init(drain + 8 + 8 * w, 1);   // a warp's own copies
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -618,17 +614,17 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               if (pa) a *= __ldcg(pa + mine * A.sc_k);
               if (pb) b = __ldcg(pb + mine * B.sc_k);
             }
-            for (int i = 0; ok && i < n; i++) {
-              const uint32_t slot = (chunk + i) % TP_SCALES;
-              if (!warp_wait(scale_empty + 8 * slot, ((chunk + i) / TP_SCALES & 1) ^ 1, lane)) {
+            for (int i = 0; ok && i < n; i++, chunk++) {
+              const uint32_t set = chunk % S::BUFFERS;
+              if (!warp_wait(scale_empty + 8 * set, (chunk / S::BUFFERS & 1) ^ 1, lane)) {
                 if (lane == 0) tp_report(g, 51);
                 ok = false;
+                break;
               }
+              if (lane >> 3 == i) scales[set][lane & 7] = a * b;
+              __syncwarp();
+              if (lane == 0) mbar_arrive(acc_full + 8 * set);
             }
-            if (mine < k1) scales[(chunk + (lane >> 3)) % TP_SCALES][lane & 7] = a * b;
-            __syncwarp();
-            if (ok && lane < n) mbar_arrive(scale_full + 8 * ((chunk + lane) % TP_SCALES));
-            chunk += n;
           }
         }
       }
@@ -671,7 +667,6 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
     };
     // A warp whose wait gave up goes through the rest of its tiles without waiting: others meet it at the named barriers.
     int odd = 0;
-    uint32_t chunk = 0;
     for (int64_t t = first_tile; t < g.total; t += tile_step, odd ^= 1) {
       const TpTile T = tp_tile(g, t, TN, ROWS);
       const int64_t row = T.row0 + 128 * rank + 32 * q;   // first row of this warp
@@ -704,13 +699,12 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           int k0, k1;
           tp_range(g, T.split, seg, k0, k1);
           constexpr bool TWO = KIND == TP_GATED || KIND == TP_BACK;
-          for (int kb = k0; kb < k1; kb++, chunk++) {
-            const uint32_t slot = chunk % TP_SCALES;
-            if (ok && !(warp_wait(scale_full + 8 * slot, chunk / TP_SCALES & 1, lane) && warp_wait(acc_full + 8 * buf, uses >> buf & 1, lane))) {
+          for (int kb = k0; kb < k1; kb++) {
+            if (ok && !warp_wait_all(acc_full + 8 * buf, uses >> buf & 1, lane)) {
               if (lane == 0) tp_report(g, 45);
               ok = false;
             }
-            const float *scale = scales[slot] + 4 * (q >> 1) + 2 * (part >> 1);   // TN = 64: both blocks of columns are the one
+            const float *scale = scales[buf] + 4 * (q >> 1) + 2 * (part >> 1);   // TN = 64: both blocks of columns are the one
             const float s0 = scale[0], s1 = scale[1];
             tc_fence_after();
             const uint32_t at = lanes + (uint32_t)(buf * S::BUFFER_COLS);
@@ -723,12 +717,12 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               tp_add(acc[i], v, TWO && i / EACH == 1 ? s1 : s0);
             }
             release(buf);
-            if (ok && lane == 0) mbar_arrive(scale_empty + 8 * slot);   // after the warp has met in release()
+            if (ok && lane == 0) mbar_arrive(scale_empty + 8 * buf);   // after the warp has met in release()
             next_buffer();
           }
         }
       } else {
-        if (ok && !warp_wait(acc_full + 8 * buf, uses >> buf & 1, lane)) {
+        if (ok && !warp_wait_all(acc_full + 8 * buf, uses >> buf & 1, lane)) {
           if (lane == 0) tp_report(g, 46);
           ok = false;
         }

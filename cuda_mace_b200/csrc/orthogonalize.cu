@@ -9,6 +9,11 @@
 // result's 2^-9) but for S S, the smallest of the products, whose rounding weighs most: with pairs there the error of a result is 1.2 to
 // 1.4 times that of its own rounding, without 1.6 to 1.8.  fp16's range suffices without looking at the values: |X|_2 <= 1 bounds every entry of X, S and b S + c S S in
 // every step, and the host makes powers of two of the bounds.
+//
+// Measured (B200, us a call of five steps, launches and all): one kernel: 4 of 64 x 64 20, 40 of 128 x 128 37, 3 of 128 x 512 in four CTAs each 59;
+// a kernel a product: 1 of 1 001 x 250 149 (17 launches of 6 to 9: chains of first copies, four to 16 blocks of 64 k, an epilogue),
+// 2 of 1 024 x 4 096 in bf16 290 to 325 (X X^T 20, S S 12, P X 28 a step; at 50 to 64 bytes a cycle and SM the copies of 128 x 256 operands
+// take as long as their products).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -1,6 +1,6 @@
 """Op-level timings of the CUDA operators on the isolated-operator configurations of the benchmark spec.
 
-    python -m cuda_mace_b200.opbench [--op all|symcon|imp|fused|linear|radial|nlist] [--dtype f32|f64] [--iters 20]
+    python -m cuda_mace_b200.opbench [--op all|symcon|imp|fused|linear|radial|dense|nlist] [--dtype f32|f64] [--iters 20]
 
 symcon  SymmetricContraction, N = 4096 atoms, 128 channels, 10 species, forward and forward+backward
 imp     InvariantMessagePassing, N = 8192 receivers, Poisson(30) edges each, 128 channels, forward and backward
@@ -9,6 +9,7 @@ gradr   gradient of the last hidden radial layer from operands formed inside the
 linear  Linear, N = 3000 and N = 64000 nodes, 128 channels; ElementalLinear, N = 64000, 4 elements
 edge    spherical harmonics and the tabulated (cubic spline) radial weights, E = 157 000 and 3 331 524 edges
 radial  the three hidden radial layers in one kernel (float32), E edges
+dense   the gated feed-forward block (forward, training step) and orthogonalised updates, float32 and bfloat16
 nlist   neighbour list of the 64 000-atom slab system on the device (cell-list kernels) and on the host (numpy)
 
 One JSON line per measurement: CUDA-event time per call (after warm-up, inputs larger than L2 or L2 flushed by
@@ -163,6 +164,29 @@ def bench_linear(dtype, iters, dev):
     ops.check_status()
 
 
+def bench_dense(dtype, iters, dev):
+    """The block at a 128-channel model's widths and at wide ones, the updates of its weights and of an ElementalLinear."""
+    if dtype != torch.float32:
+        return
+    gen = torch.Generator(device=dev).manual_seed(6)
+    rand = lambda dt, *shape: torch.randn(*shape, generator=gen, device=dev).to(dt)  # noqa: E731
+    for dt, s in ((torch.float32, 4), (torch.bfloat16, 2)):
+        for M, C, H in ((1, 1024, 4096), (3000, 128, 512), (64000, 128, 512), (8192, 1024, 4096)):
+            leaves = [t.requires_grad_(True) for t in (rand(dt, M, C), rand(dt, C, H) / C ** 0.5, rand(dt, C, H) / C ** 0.5, rand(dt, H, C) / H ** 0.5)]
+            gy = rand(dt, M, C)
+            case = f"M={M} C={C} H={H} {str(dt)[6:]}"
+            with torch.no_grad():
+                t = _time(lambda: ops.gated_feed_forward(*leaves), iters)
+            _emit("feed_forward", case + " forward", t, s * (2 * M * C + 3 * C * H), gflops=round(6 * M * C * H / t / 1e6, 1))
+            t = _time(lambda: torch.autograd.grad(ops.gated_feed_forward(*leaves), leaves, gy), iters)
+            _emit("feed_forward", case + " forward and backward", t, s * (4 * M * C + 6 * C * H), gflops=round(18 * M * C * H / t / 1e6, 1))
+        for n, r, c in ((40, 128, 128), (3, 128, 512), (3, 1024, 4096)):
+            U = rand(dt, n, r, c)
+            t = _time(lambda: ops.orthogonalize(U), iters)
+            _emit("orthogonalize", f"{n} of {r} x {c} {str(dt)[6:]}", t, 2 * s * n * r * c, gflops=round(5 * n * (3 * r * r * c + r ** 3) / t / 1e6, 1))
+    ops.check_status()
+
+
 def bench_edge(dtype, iters, dev):
     """Spherical harmonics alone (the reference's operator) and the tabulated radial weights, at the edge counts of
     the 3 000-atom box and of one 64 000-atom slab."""
@@ -232,7 +256,7 @@ def bench_nlist(iters, dev, nodes):
 
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    ap.add_argument("--op", default="all", choices=["all", "symcon", "imp", "fused", "gradr", "linear", "edge", "radial", "nlist"])
+    ap.add_argument("--op", default="all", choices=["all", "symcon", "imp", "fused", "gradr", "linear", "edge", "radial", "dense", "nlist"])
     ap.add_argument("--graph", default="poisson", choices=["poisson", "symmetric"], help="edge list of the imp case")
     ap.add_argument("--dtype", default="f32", choices=["f32", "f64"])
     ap.add_argument("--iters", type=int, default=20)
@@ -253,6 +277,8 @@ def main():
         bench_edge(dtype, args.iters, dev)
     if args.op in ("all", "radial"):
         bench_radial(dtype, args.iters, dev, args.edges)
+    if args.op in ("all", "dense"):
+        bench_dense(dtype, args.iters, dev)
     if args.op in ("all", "gradr"):
         bench_gradr(dtype, args.iters, dev, args.nodes)
     if args.op in ("all", "fused"):

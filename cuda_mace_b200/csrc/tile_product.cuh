@@ -482,6 +482,19 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               stage = 0;
               phase ^= 1;
             }
+            // What the first tile's epilogue adds comes behind the first operands: in front of them it kept the products waiting for up to 7 us.
+            if constexpr (KIND == TP_POLY || KIND == TP_APPLY) {
+              if (t == first_tile && kb + 1 == (k1 - k0 < STAGES ? k1 : k0 + STAGES)) {
+                for (int w = 0; w < TP_EPILOGUE_WARPS; w++) {
+                  const int row = row0 + 32 * (w & 3), col = T.n0 + (w >> 2) * S::PART;
+                  if (row >= g.rows || col >= g.cols) continue;
+                  const uint32_t to = staging + (uint32_t)(w * S::STAGING), cin_bar = drain + 8 + 8 * (uint32_t)w;
+                  mbar_arrive_expect_tx(cin_bar, 2 * 32 * S::PART * 2);
+                  tma_load_3d(to, &g.cin, col, row, 2 * T.batch, cin_bar);
+                  tma_load_3d(to + 32 * S::PART * 2, &g.cin, col, row, 2 * T.batch + 1, cin_bar);
+                }
+              }
+            }
           }
         }
       }
@@ -676,7 +689,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       constexpr bool CIN = KIND == TP_POLY || KIND == TP_APPLY;
       constexpr uint32_t LOW = 32 * S::PART * 2;   // bytes from a warp's hi to its lo
       const bool here = row < g.rows && col0 < g.cols;
-      if (CIN && here) {
+      if (CIN && here && t != first_tile) {   // the first tile's: by the thread that issues the copies
         if (elect_one()) {
           tma_store_wait_read();
           mbar_arrive_expect_tx(cin_bar, 2 * LOW);
@@ -883,7 +896,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         // Newton-Schulz: values in float32, then hi and lo at a power of two that the caller has from its bounds
         constexpr int ROW = 2 * S::PART;   // bytes of a row of a piece
         if (CIN && here) {
-          if (ok && !warp_wait(cin_bar, cin_phase, lane)) {
+          if (!warp_wait(cin_bar, cin_phase, lane)) {   // after another wait gave up too: no copy outlives the block
             if (lane == 0) tp_report(g, 49);
             ok = false;
           }

@@ -99,6 +99,7 @@ Tensor gated_feed_forward(const Tensor &x_, const Tensor &wg_, const Tensor &wu_
     TORCH_CHECK(t->get_device() == device, "operand on cuda:", t->get_device(), " while cuda:", device, " is the current device");
     TORCH_CHECK_TYPE(t->scalar_type() == x_.scalar_type() && (x_.scalar_type() == torch::kFloat32 || x_.scalar_type() == torch::kBFloat16),
                      "gated_feed_forward needs float32 or bfloat16 operands of one type");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "gated_feed_forward has no forward-mode derivative");
   }
   TORCH_CHECK(x_.dim() >= 1 && wg_.dim() == 2 && wu_.dim() == 2 && wd_.dim() == 2, "gated_feed_forward needs rows and weight matrices");
   const int64_t width = wg_.size(0), hidden = wg_.size(1);

@@ -474,7 +474,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   set_operand(g.b[2], wd, true);
   g.segments = 2;
   set_k(g, 0, f.C);
-    set_k(g, 1, f.C);
+  set_k(g, 1, f.C);
   if (!rc) rc = set_hidden_out(g, hidden, 16, bf16, f.what);
   if (!rc) rc = f.act == TP_SILU ? launch_back<TP_SILU>(f, g) : launch_back<TP_GELU>(f, g);
   if (want_x) {

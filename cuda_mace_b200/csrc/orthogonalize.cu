@@ -55,6 +55,17 @@ __device__ __forceinline__ void ns_load8(float (&v)[8], const void *p, int64_t i
   }
 }
 
+// 1 / (|U| + eps) as two factors, the first a power of two: |U| of a matrix of float32's largest or smallest values leaves float32's range.
+struct NsInverse {
+  float first, second;
+  __device__ __forceinline__ NsInverse(double square, double eps) {
+    const double inv = 1.0 / (sqrt(square) + eps);
+    first = inv > 0x1p100 ? 0x1p100f : inv < 0x1p-100 ? 0x1p-100f : 1.0f;
+    second = (float)(inv / first);
+  }
+  __device__ __forceinline__ float operator*(float v) const { return v * first * second; }
+};
+
 // Squares of eight values in float32 where those neither leave its range nor fall below it, in float64 otherwise and from there on: neither
 // large nor small updates are lost, and the sum of a matrix is one value whatever its size.
 __global__ void __launch_bounds__(NS_THREADS) ns_norm_kernel(const NsPrep p) {
@@ -95,7 +106,7 @@ __global__ void __launch_bounds__(NS_THREADS) ns_prep_kernel(const NsPrep p) {
   for (int c = threadIdx.x & 31; c < p.chunks; c += 32) s += __ldcg(p.partial + m * p.chunks + c);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-  const float inv = (float)(1.0 / (sqrt(s) + p.eps));
+  const NsInverse inv(s, p.eps);
   const int per_row = (p.cols + 7) / 8;
   const int64_t items = p.rows * per_row, plane = p.rows * p.ld;
   const bool wide = p.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(p.src) & 15) == 0;
@@ -110,7 +121,7 @@ __global__ void __launch_bounds__(NS_THREADS) ns_prep_kernel(const NsPrep p) {
     ns_load8(v, p.src, (m * p.rows + row) * p.cols + col, p.cols - col < 8 ? p.cols - col : 8, p.bf16, wide);
     uint32_t h[4], l[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) tp_split2(v[2 * k] * inv, v[2 * k + 1] * inv, p.scale, h[k], l[k]);
+    for (int k = 0; k < 4; k++) tp_split2(inv * v[2 * k], inv * v[2 * k + 1], p.scale, h[k], l[k]);
     __half *to = hi + row * p.ld + col;   // rows have a multiple of 64 elements
     *reinterpret_cast<uint4 *>(to) = make_uint4(h[0], h[1], h[2], h[3]);
     *reinterpret_cast<uint4 *>(to + plane) = make_uint4(l[0], l[1], l[2], l[3]);
@@ -310,7 +321,7 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
       square += other;
     }
   }
-  const float inv = (float)(1.0 / (sqrt(square) + g.eps));
+  const NsInverse inv(square, g.eps);
   // a chunk's pairs of X: shared memory, and tensor memory where it has room
   const auto put_x = [&](int ch, const float (&x)[16], float scale) {
     uint32_t hi[8], lo[8];
@@ -329,7 +340,7 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
     tmem_ld16_nowait(at, w);
     tmem_ld_wait();
 #pragma unroll
-    for (int k = 0; k < 16; k++) x[k] = __uint_as_float(w[k]) * inv;
+    for (int k = 0; k < 16; k++) x[k] = inv * __uint_as_float(w[k]);
 #pragma unroll
     for (int k = 0; k < 16; k++) w[k] = __float_as_uint(x[k]);
     tmem_st16(at, w);
@@ -726,7 +737,7 @@ static int check_ns(const char *what, int64_t count, int64_t rows, int cols, int
   if (count < 0 || rows < 1 || cols < 1 || steps < 1 || steps > 100)
     return fail(CMACE_ERR_ARG, "%s: bad sizes: %lld matrices of %lld x %d, %d steps", what, (long long)count, (long long)rows, cols, steps);
   if (rows > 1 << 20 || cols > 1 << 20 || count * ((rows + 31) / 32) * ((cols + 31) / 32) >= (int64_t)1 << 30)
-    return fail(CMACE_ERR_UNSUPPORTED, "%s: sides up to 2^20 and 2^31 blocks of 32 x 32", what);
+    return fail(CMACE_ERR_UNSUPPORTED, "%s: sides up to 2^20 and fewer than 2^30 blocks of 32 x 32", what);
   return CMACE_OK;
 }
 

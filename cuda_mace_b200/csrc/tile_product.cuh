@@ -24,8 +24,8 @@
 // One persistent CTA an SM, 19 warps: 16 for the epilogue (four a quarter of the 128 tensor-memory lanes, each a quarter of
 // the columns; with eight, two a scheduler, they waited for each other's barriers, copies and special functions most of the time), one
 // thread that issues the copies, one that issues the MMAs, and a warp that fetches the blocks' scales ahead (the epilogue warps waited
-// 700 cycles a segment for them: 47 of the 180 us of the backward's hidden values at 64 000 rows, widths 128 and 512).  Two sets of accumulator columns: the
-// products of the next chunk or tile run while the epilogue reads this one's.
+// 700 cycles a segment for them: 47 of the 180 us of the backward's hidden values at 64 000 rows, widths 128 and 512).  Two to four sets of accumulator
+// columns: the products of the next chunks or tiles run while the epilogue reads this one's.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -81,7 +81,7 @@ struct TpArgs {
   float *out_scale[3];           // PAIR outputs with block scales: inverse scale of every 64 x 64 block
   int64_t out_scale_ld, out_scale_batch;
   CUtensorMap cin;               // POLY: S, APPLY: X, in boxes of 32 rows of a warp's columns; batch b is hi 2 b and lo 2 b + 1
-  float alpha, beta, cin_scale, pair_scale;   // D = alpha * product + beta * cin / ..., see the epilogues
+  float alpha, beta, pair_scale;   // D = alpha * product + beta * cin, times pair_scale where D is a pair
   int32_t *status;
   int64_t rows, cols;            // of the output
   int kblocks[2], segments;      // blocks of 64 k a segment
@@ -89,7 +89,6 @@ struct TpArgs {
   int batches, splits, mt, nt;
   TpDiv by_nt, by_mt, by_batches, by_splits;
   int64_t total;                 // tiles
-  int stages;
   int a_of_last;                 // the last batch takes a[1] (its own, unbatched operand) in place of a[0]
   int out_of_batch;              // PLAIN: batch b goes to out[b], an array of its own
   int out_bf16;                  // PLAIN, APPLY's result: 16-bit output

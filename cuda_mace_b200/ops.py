@@ -22,6 +22,7 @@ import os
 from collections import OrderedDict
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _abi
 
@@ -297,7 +298,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
     """(act(x @ w_gate) * (x @ w_up)) @ w_down for rows of node features x [..., C], w_gate and w_up [C, H], w_down [H, C], all
     float32 or all bfloat16; `activation` is "silu" or "gelu" (with erf).  Differentiable (once) in x and the three weights.
     Sums are float32 in both types; float32 runs on the tensor cores in three terms (cmace_gated_ff_fwd_f32), bfloat16 rounds the hidden
-    values to bfloat16 between the products.  The backward keeps x and the weights only and forms the hidden values again."""
+    values to bfloat16 between the products (eight rows or fewer keep them in float32).  The backward keeps x and the weights only and forms the hidden values again."""
     code = _ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"gated_feed_forward: activation {activation!r} is none of {sorted(_ACTIVATIONS)}")
@@ -342,8 +343,14 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
         raise TypeError(f"orthogonalize needs float32 or bfloat16, got {update.dtype}")
     if update.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("orthogonalize has no gradient: detach the update or call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(update).tangent is not None:
+        raise NotImplementedError("orthogonalize has no forward-mode derivative")
     if update.dim() < 2 or update.shape[-1] < 1 or update.shape[-2] < 1:
         raise RuntimeError(f"orthogonalize needs matrices [..., m, n], got {tuple(update.shape)}")
+    if max(update.shape[-2:]) > 1 << 20:   # before a size is passed as a C int
+        raise RuntimeError(f"orthogonalize: sides up to 2^20, got {tuple(update.shape)}")
+    if not 1 <= steps <= 100:
+        raise RuntimeError(f"orthogonalize: bad sizes: {steps} steps")
     a, b, c = (float(v) for v in coefficients)
     u = update.detach().contiguous()
     m, n = u.shape[-2:]
@@ -354,7 +361,7 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
     ws = _workspace(u.device, nbytes)
     _abi.call("cmace_orthogonalize_f32" if f32 else "cmace_orthogonalize_bf16", _ptr(u), count, m, n, int(steps), a, b, c, float(eps), _ptr(out), _ptr(ws), nbytes,
               _ptr(_status_tensor(u.device)), _stream())
-    _abi.launch_count += 2 + 3 * int(steps)
+    _abi.launch_count += 1 if nbytes == 256 else 2 + 3 * int(steps)   # one kernel needs no workspace
     return out
 
 

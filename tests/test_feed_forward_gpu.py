@@ -432,3 +432,18 @@ def test_block_trained_with_orthogonalised_updates(dev):
     for n, p in block.named_parameters():
         # a step moves a weight by at most 0.02 * 1.3 a singular direction; the gradients' 1e-6 are enlarged by up to 485 in the smallest
         assert rel_err(p, want[n]) < 1e-4, n
+
+
+def test_forward_mode_is_refused(dev):
+    from torch.autograd import forward_ad
+
+    from cuda_mace_b200 import ops
+
+    t = list(case(82, 20, 16, 24, F32, dev)[:4])
+    with forward_ad.dual_level():
+        for i in range(4):
+            dual = list(t)
+            dual[i] = forward_ad.make_dual(t[i], torch.ones_like(t[i]))
+            with pytest.raises(NotImplementedError):
+                ops.gated_feed_forward(*dual)
+        ops.gated_feed_forward(*t)

@@ -231,3 +231,30 @@ def test_refusals_on_the_device(dev):
         _abi.call("cmace_orthogonalize_f32", V.data_ptr(), 2, 200, 300, 5, *USUAL, 1e-7, out.data_ptr(), V.data_ptr() & ~255, 16, 0, 0)
     torch.cuda.synchronize()
     assert (out == 3.0).all()
+
+
+@pytest.mark.parametrize("shape", [(2, 33, 90), (1, 150, 200)])
+@pytest.mark.parametrize("size", [1e-40, 1e-35, 1e37])
+def test_ends_of_float32(shape, size, dev):
+    """Updates whose norm, or its inverse, is no float32 value (1e-40: the update's own values are subnormal)."""
+    from cuda_mace_b200 import ops
+
+    V = update(11, shape, F32, dev) * size
+    assert torch.isfinite(V).all()
+    check(ops.orthogonalize(V, eps=0.0), V, eps=0.0)
+
+
+def test_long_sides_and_forward_mode_are_refused(dev):
+    from torch.autograd import forward_ad
+
+    from cuda_mace_b200 import ops
+
+    with pytest.raises(RuntimeError, match="sides up to"):
+        ops.orthogonalize(torch.ones(1, 1, device=dev).expand(1, 2 ** 32 + 16))
+    with pytest.raises(RuntimeError, match="bad sizes"):
+        ops.orthogonalize(torch.ones(2, 2, device=dev), steps=2 ** 32 + 5)
+    U = update(12, (4, 5), F32, dev)
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            ops.orthogonalize(forward_ad.make_dual(U, torch.ones_like(U)))
+        ops.orthogonalize(U)

@@ -19,6 +19,7 @@
 // In bf16, h, dg and du are rounded once to bf16 between the products, as the operands of a 16-bit product have to be; with the
 // rounding of the results that makes 1.4 times the error of a result that is rounded alone.  Sums over M are float32.
 #include <algorithm>
+#include <type_traits>
 
 #include "tile_product.cuh"
 
@@ -250,6 +251,317 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_rows_kernel(const FewArgs 
   }
 }
 
+// ---- some rows: the whole block in one kernel -----------------------------------------------------------------------------------
+// Where few tiles are full, a call is as long as its chain of kernels (copies, products, an epilogue, the next kernel's start: 5 to 6 us each),
+// and a full tile's tensor-core rate counts for nothing.
+// Here a warp needs nobody until the end: it has 16 rows and a group of 16 (float32) or 32 (bf16) hidden columns, forms g and u of them
+// with warp-wide MMAs (mma.sync), and multiplies h, whose sums lie in the registers as the next product's operand has to, with its rows of Wd.
+// Weights come from L2 to registers once a block of 16 rows, four k a lane: k and the columns are dealt to lanes so that a lane's
+// loads are vectors (the order of k in a product is free).  The warps' sums of y are added at the end, in shared memory and over a
+// cluster that shares the hidden columns, in one order.  float32: three products of TF32 parts (lo hi, hi lo, hi hi) of 16 k, started at zero and
+// added to float32 registers, so that the tensor core's truncation stays at 2^-24 of a partial sum.
+// 192 rows, 128 and 512: float32 12 us against 17.7 by tiles, bf16 9.0 against 10.7; 400 rows, 32 and 512: 5.9 against 16.1, 5.3 against 10.2.  A
+// warp's chain bounds it (loads, six dependent products a step, 16 values a load to split): two rows of blocks an SM at once do not fit the
+// registers.  Groups spread over twice as many CTAs: the same (a cluster costs 1.7).
+constexpr int SOME_THREADS = 256, SOME_WARPS = SOME_THREADS / 32, SOME_ROWS = 16;
+
+struct SomeArgs {
+  const void *x, *w[2], *wd;
+  void *y;
+  int64_t M;
+  int C, H, ld, cluster, wide;   // ld: elements a row of x in shared memory
+};
+constexpr int some_group(bool f32) { return f32 ? 16 : 32; }   // hidden columns
+
+__device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// x = hi + lo to 2^-22 of x, both rounded to TF32's 11 bits
+__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+// 8 or 16 bytes of `base`, `off` bytes behind it (the matrices here are below 4 GB).  FULL: all of it is there and aligned.  Otherwise the
+// first n elements are (WIDE: all or none, aligned), zeros stand for the others, and their loads go to the matrix's first elements: loads
+// without a branch leave together.
+template <typename T, bool FULL, bool WIDE, int WORDS>
+__device__ __forceinline__ void some_load(uint32_t (&v)[WORDS], const void *base, uint32_t off, int n) {
+  const char *p = static_cast<const char *>(base);
+  if constexpr (FULL || WIDE) {
+    p += FULL || n > 0 ? off : 0u;
+    if constexpr (WORDS == 4) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+      const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
+      v[0] = x.x, v[1] = x.y;
+    }
+    if (FULL) return;
+#pragma unroll
+    for (int i = 0; i < WORDS; i++) v[i] = n > 0 ? v[i] : 0u;
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < WORDS; i++) {
+      const uint32_t x = __ldg(reinterpret_cast<const uint32_t *>(p + (i < n ? off + 4 * i : 0u)));
+      v[i] = i < n ? x : 0u;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < WORDS; i++) {
+      const uint32_t x = __ldg(reinterpret_cast<const uint16_t *>(p + (2 * i < n ? off + 4 * i : 0u)));
+      const uint32_t y = __ldg(reinterpret_cast<const uint16_t *>(p + (2 * i + 1 < n ? off + 4 * i + 2 : 0u)));
+      v[i] = (2 * i < n ? x : 0u) | (2 * i + 1 < n ? y << 16 : 0u);
+    }
+  }
+}
+// the two k of column t of a bf16 operand, from two rows' words
+__device__ __forceinline__ uint32_t k_pair(const uint32_t (&a)[2], const uint32_t (&b)[2], int t) {
+  return __byte_perm(a[t >> 1], b[t >> 1], t & 1 ? 0x7632 : 0x5410);
+}
+
+// a lane's columns col, col + 1, ... of both projections, of rows k .. k + 3 and those of the next steps of 16
+template <typename T, bool FULL, bool WIDE, int DEPTH>
+__device__ __forceinline__ void some_projections(uint32_t (&to)[DEPTH][2][4][2], const SomeArgs &g, int col, int k) {
+  const uint32_t row = (uint32_t)(g.H * (int)sizeof(T));
+  uint32_t off = (uint32_t)k * row + (uint32_t)(col * (int)sizeof(T));
+#pragma unroll
+  for (int d = 0; d < DEPTH; d++, off += 12 * row)
+#pragma unroll
+    for (int i = 0; i < 4; i++, off += row)
+#pragma unroll
+      for (int p = 0; p < 2; p++) some_load<T, FULL, WIDE>(to[d][p][i], g.w[p], off, k + 16 * d + i < g.C ? g.H - col : 0);
+}
+// columns col .. col + 3 of Wd's rows: the hidden columns k + t and k + NT + t that a lane has values of
+template <typename T, bool FULL, bool WIDE, int NT, int DW>
+__device__ __forceinline__ void some_down(uint32_t (&to)[NT][2][DW], const SomeArgs &g, int k, int col) {
+  const uint32_t row = (uint32_t)(g.C * (int)sizeof(T)), off = (uint32_t)k * row + (uint32_t)(col * (int)sizeof(T));
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int i = 0; i < 2; i++) some_load<T, FULL, WIDE>(to[t][i], g.wd, off + (uint32_t)(NT * i + t) * row, k + NT * i + t < g.H ? g.C - col : 0);
+}
+
+// CT: spans of 32 columns of y, at least C / 32
+template <typename T, int CT, int ACT>
+__global__ void __launch_bounds__(SOME_THREADS, 1) some_rows_kernel(const SomeArgs g) {
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int GROUP = some_group(F32), NT = GROUP / 8, DEPTH = 2;   // DEPTH: steps of 16 k that are loaded together
+  constexpr int COLS = 32 * CT, RED = SOME_ROWS * COLS;
+  extern __shared__ __align__(16) unsigned char some_smem[];
+  T *const xs = reinterpret_cast<T *>(some_smem);   // x [16][ld], float32: hi, then lo
+  float *const red = reinterpret_cast<float *>(some_smem + (F32 ? 2 : 1) * SOME_ROWS * g.ld * (int)sizeof(T));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = lane & 3, j = lane >> 2;
+  const int rank = g.cluster > 1 ? (int)cluster_rank() : 0;
+  const int64_t row0 = (int64_t)(blockIdx.x / (unsigned)g.cluster) * SOME_ROWS;
+  const int steps = (g.C + 15) / 16, groups = (g.H + GROUP - 1) / GROUP;
+  const auto fetch = [&](uint32_t (&to)[DEPTH][2][4][2], int group, int step) {
+    const int col = group * GROUP + NT * j, k = 16 * step + 4 * q;
+    if (g.wide && (group + 1) * GROUP <= g.H && 16 * (step + DEPTH) <= g.C) some_projections<T, true, true>(to, g, col, k);
+    else if (g.wide) some_projections<T, false, true>(to, g, col, k);
+    else some_projections<T, false, false>(to, g, col, k);
+  };
+  constexpr int DW = F32 ? 4 : 2;   // words of four columns of y
+  const auto fetch_down = [&](uint32_t (&to)[NT][2][DW], int group, int span) {
+    const int k = group * GROUP + 2 * NT * q, col = 32 * span + 4 * j;
+    if (g.wide && (group + 1) * GROUP <= g.H && 32 * span + 32 <= g.C) some_down<T, true, true>(to, g, k, col);
+    else if (g.wide) some_down<T, false, true>(to, g, k, col);
+    else some_down<T, false, false>(to, g, k, col);
+  };
+  const int first = rank * SOME_WARPS + warp;
+  uint32_t w[2][DEPTH][2][4][2];
+  fetch(w[0], first, 0);
+#pragma unroll
+  for (int r = warp; r < SOME_ROWS; r += SOME_WARPS)
+    for (int k = 4 * lane; k < 16 * steps; k += 128) {
+      constexpr int XW = F32 ? 4 : 2;
+      uint32_t v[XW];
+      const void *row = static_cast<const T *>(g.x) + (row0 + r < g.M ? row0 + r : row0) * g.C;
+      const int n = row0 + r < g.M ? g.C - k : 0;
+      if (g.wide) some_load<T, false, true>(v, row, (uint32_t)(k * (int)sizeof(T)), n);
+      else some_load<T, false, false>(v, row, (uint32_t)(k * (int)sizeof(T)), n);
+      if constexpr (F32) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) split_tf32(__uint_as_float(v[i]), hi[i], lo[i]);
+        *reinterpret_cast<uint4 *>(xs + r * g.ld + k) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4 *>(xs + (SOME_ROWS + r) * g.ld + k) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      } else {
+        *reinterpret_cast<uint2 *>(xs + r * g.ld + k) = make_uint2(v[0], v[1]);
+      }
+    }
+  __syncthreads();
+  float y[CT][4][4] = {};
+  for (int group = first; group < groups; group += g.cluster * SOME_WARPS) {
+    float sum[2][NT][4] = {};
+    const auto multiply = [&](const uint32_t (&from)[DEPTH][2][4][2], int step) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; d++) {
+        if (step + d >= steps) break;
+        const T *a = xs + j * g.ld + 16 * (step + d) + 4 * q;
+        if constexpr (F32) {
+          const float4 h0 = *reinterpret_cast<const float4 *>(a), h1 = *reinterpret_cast<const float4 *>(a + 8 * g.ld);
+          const float4 l0 = *reinterpret_cast<const float4 *>(a + 16 * g.ld), l1 = *reinterpret_cast<const float4 *>(a + 24 * g.ld);
+          const uint32_t ah[2][4] = {{__float_as_uint(h0.x), __float_as_uint(h1.x), __float_as_uint(h0.y), __float_as_uint(h1.y)},
+                                     {__float_as_uint(h0.z), __float_as_uint(h1.z), __float_as_uint(h0.w), __float_as_uint(h1.w)}};
+          const uint32_t al[2][4] = {{__float_as_uint(l0.x), __float_as_uint(l1.x), __float_as_uint(l0.y), __float_as_uint(l1.y)},
+                                     {__float_as_uint(l0.z), __float_as_uint(l1.z), __float_as_uint(l0.w), __float_as_uint(l1.w)}};
+          // six products of 2 NT sums in turn: each waits for the one before of its sum
+          uint32_t bh[2 * NT][4], bl[2 * NT][4];
+          float part[2 * NT][4] = {};
+#pragma unroll
+          for (int n = 0; n < 2 * NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) split_tf32(__uint_as_float(from[d][n / NT][i][n % NT]), bh[n][i], bl[n][i]);
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int n = 0; n < 2 * NT; n++) mma_tf32(part[n], al[e][0], al[e][1], al[e][2], al[e][3], bh[n][2 * e], bh[n][2 * e + 1]);
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int n = 0; n < 2 * NT; n++) mma_tf32(part[n], ah[e][0], ah[e][1], ah[e][2], ah[e][3], bl[n][2 * e], bl[n][2 * e + 1]);
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int n = 0; n < 2 * NT; n++) mma_tf32(part[n], ah[e][0], ah[e][1], ah[e][2], ah[e][3], bh[n][2 * e], bh[n][2 * e + 1]);
+#pragma unroll
+          for (int n = 0; n < 2 * NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) sum[n / NT][n % NT][i] += part[n][i];
+        } else {
+          const uint2 a0 = *reinterpret_cast<const uint2 *>(a), a1 = *reinterpret_cast<const uint2 *>(a + 8 * g.ld);
+#pragma unroll
+          for (int p = 0; p < 2; p++)
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+              mma_bf16(sum[p][t], a0.x, a1.x, a0.y, a1.y, k_pair(from[d][p][0], from[d][p][1], t), k_pair(from[d][p][2], from[d][p][3], t));
+        }
+      }
+    };
+    uint32_t down[2][NT][2][DW];
+    for (int step = 0; step < steps; step += 2 * DEPTH) {
+      if (step + DEPTH < steps) fetch(w[1], group, step + DEPTH);
+      multiply(w[0], step);
+      if (step + 2 * DEPTH < steps) fetch(w[0], group, step + 2 * DEPTH);
+      else fetch_down(down[0], group, 0);
+      if (step + DEPTH < steps) multiply(w[1], step + DEPTH);
+    }
+    // h of column NT (2 q + c) + t: rows j (values 0, 1) and j + 8 (2, 3) of tile t
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) sum[0][t][i] = tp_act<ACT>(sum[0][t][i]) * sum[1][t][i];
+#pragma unroll
+    for (int span = 0; span < CT; span++) {
+      if (span + 1 < CT) fetch_down(down[(span + 1) & 1], group, span + 1);   // spans behind C: of zeros
+      else if (group + g.cluster * SOME_WARPS < groups) fetch(w[0], group + g.cluster * SOME_WARPS, 0);
+      const uint32_t(&b)[NT][2][DW] = down[span & 1];
+      if constexpr (F32) {
+        float part[4][4] = {};
+        uint32_t ah[NT][4], al[NT][4];   // k of the product: q and q + 4 are columns 2 q and 2 q + 1 of the tile
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          split_tf32(sum[0][t][0], ah[t][0], al[t][0]);
+          split_tf32(sum[0][t][2], ah[t][1], al[t][1]);
+          split_tf32(sum[0][t][1], ah[t][2], al[t][2]);
+          split_tf32(sum[0][t][3], ah[t][3], al[t][3]);
+        }
+        uint32_t bh[4][NT][2], bl[4][NT][2];
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) split_tf32(__uint_as_float(b[t][i][s]), bh[s][t][i], bl[s][t][i]);
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int s = 0; s < 4; s++) mma_tf32(part[s], al[t][0], al[t][1], al[t][2], al[t][3], bh[s][t][0], bh[s][t][1]);
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int s = 0; s < 4; s++) mma_tf32(part[s], ah[t][0], ah[t][1], ah[t][2], ah[t][3], bl[s][t][0], bl[s][t][1]);
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int s = 0; s < 4; s++) mma_tf32(part[s], ah[t][0], ah[t][1], ah[t][2], ah[t][3], bh[s][t][0], bh[s][t][1]);
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) y[span][s][i] += part[s][i];
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; t += 2) {
+          const uint32_t a0 = tp_bf16x2(sum[0][t][0], sum[0][t][1]), a1 = tp_bf16x2(sum[0][t][2], sum[0][t][3]);
+          const uint32_t a2 = tp_bf16x2(sum[0][t + 1][0], sum[0][t + 1][1]), a3 = tp_bf16x2(sum[0][t + 1][2], sum[0][t + 1][3]);
+#pragma unroll
+          for (int s = 0; s < 4; s++) mma_bf16(y[span][s], a0, a1, a2, a3, k_pair(b[t][0], b[t][1], s), k_pair(b[t + 1][0], b[t + 1][1], s));
+        }
+      }
+    }
+  }
+  // columns 8 q .. 8 q + 7 of a span, of rows j and j + 8
+#pragma unroll
+  for (int span = 0; span < CT; span++)
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+      for (int c = 0; c < 2; c++)
+        *reinterpret_cast<float4 *>(red + warp * RED + (j + 8 * r) * COLS + 32 * span + 8 * q + 4 * c) =
+            make_float4(y[span][0][2 * r + c], y[span][1][2 * r + c], y[span][2][2 * r + c], y[span][3][2 * r + c]);
+  __syncthreads();
+  const auto store = [&](int e, const float4 &v) {
+    const int64_t row = row0 + e / COLS;
+    const int c = e % COLS, n = row < g.M ? g.C - c : 0;
+    T *to = static_cast<T *>(g.y) + row * g.C + c;
+    if (g.wide) {
+      if (n <= 0) return;
+      if constexpr (F32) *reinterpret_cast<float4 *>(to) = v;
+      else *reinterpret_cast<uint2 *>(to) = make_uint2(tp_bf16x2(v.x, v.y), tp_bf16x2(v.z, v.w));
+    } else {
+      if (n > 0) to[0] = (T)v.x;
+      if (n > 1) to[1] = (T)v.y;
+      if (n > 2) to[2] = (T)v.z;
+      if (n > 3) to[3] = (T)v.w;
+    }
+  };
+  for (int e = 4 * tid; e < RED; e += 4 * SOME_THREADS) {
+    float4 v = *reinterpret_cast<const float4 *>(red + e);
+#pragma unroll
+    for (int k = 1; k < SOME_WARPS; k++) {
+      const float4 o = *reinterpret_cast<const float4 *>(red + k * RED + e);
+      v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+    }
+    if (g.cluster == 1) store(e, v);
+    else *reinterpret_cast<float4 *>(red + e) = v;
+  }
+  if (g.cluster == 1) return;
+  __syncwarp();
+  cluster_sync();
+  const int per = RED / g.cluster;
+  for (int e = rank * per + 4 * tid; e < (rank + 1) * per; e += 4 * SOME_THREADS) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < g.cluster; r++) {
+      float4 o;
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w)
+                   : "r"(peer_smem(smem_u32(red + e), (uint32_t)r))
+                   : "memory");
+      v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+    }
+    store(e, v);
+  }
+  __syncwarp();
+  cluster_sync();   // nobody leaves while its sums are read
+}
+
 // ---- weight gradients: the splits' sums, the third transposed ------------------------------------------------------------------
 struct WeightReduce {
   const float *partial;   // [splits][3][C][ld]
@@ -416,7 +728,58 @@ static int few_rows(const FeedForward &f, void *y, float *h) {
   return f.act == TP_SILU ? few_rows<T, TP_SILU>(f, y, h) : few_rows<T, TP_GELU>(f, y, h);
 }
 
+// CTAs of some_rows_kernel a block of rows: the hidden columns' groups are shared while SMs are free and every warp has one.
+static int some_cluster(bool f32, int64_t M, int H) {
+  const int64_t blocks = (M + SOME_ROWS - 1) / SOME_ROWS;
+  const int groups = (H + some_group(f32) - 1) / some_group(f32);
+  int cluster = 1;
+  while (cluster < 8 && 2 * cluster * blocks <= 148 && groups > cluster * SOME_WARPS) cluster *= 2;
+  return cluster;
+}
+template <typename T, int CT, int ACT>
+static int launch_some(const FeedForward &f, void *y) {
+  SomeArgs g{f.x, {f.wg, f.wu}, f.wd, y, f.M, f.C, f.H, 0, 1, 0};
+  const int64_t blocks = (f.M + SOME_ROWS - 1) / SOME_ROWS;
+  g.cluster = some_cluster(f.f32, f.M, f.H);
+  // rows of x 64 (float32: quarters of a warp read two of them) or 32 bytes (halves read four) past a multiple of 128
+  constexpr int SIZE = sizeof(T);
+  g.ld = (int)(up(up(f.C, 16) * SIZE, 128) + (SIZE == 4 ? 64 : 32)) / SIZE;
+  g.wide = f.H % (8 / SIZE) == 0 && f.C % 4 == 0 && ((reinterpret_cast<uintptr_t>(f.wg) | reinterpret_cast<uintptr_t>(f.wu)) & 7) == 0 &&
+           ((reinterpret_cast<uintptr_t>(f.x) | reinterpret_cast<uintptr_t>(f.wd) | reinterpret_cast<uintptr_t>(y)) & (4 * SIZE - 1)) == 0;
+  const int smem = (SIZE == 4 ? 2 : 1) * SOME_ROWS * g.ld * SIZE + SOME_WARPS * SOME_ROWS * 32 * CT * 4;
+  constexpr int MOST = (SIZE == 4 ? 2 : 1) * SOME_ROWS * (32 * CT * SIZE + 128 + 64) + SOME_WARPS * SOME_ROWS * 32 * CT * 4;
+  if (const int rc = allow_smem<some_rows_kernel<T, CT, ACT>>(MOST, f.what)) return rc;
+  return launch_cluster(some_rows_kernel<T, CT, ACT>, g.cluster, blocks * g.cluster, SOME_THREADS, smem, f.st, f.what, g);
+}
+template <typename T, int ACT>
+static int some_rows(const FeedForward &f, void *y) {
+  return f.C <= 32 ? launch_some<T, 1, ACT>(f, y) : f.C <= 64 ? launch_some<T, 2, ACT>(f, y) : launch_some<T, 4, ACT>(f, y);
+}
+template <typename T>
+static int some_rows(const FeedForward &f, void *y) {
+  return f.act == TP_SILU ? some_rows<T, TP_SILU>(f, y) : some_rows<T, TP_GELU>(f, y);
+}
+// Whether the kernel above is the fastest, in ns of a recorded call, from lines through what was measured (up to 8 000 rows, widths
+// 16 to 128, hidden widths 16 to 512; in brackets: this kernel and the others; us): float32, 100 rows: 32 and 64 (3.9, 12.2), 32 and 512
+// (5.8, 15.9), 128 and 512 (12.0, 17.6), 100 and 301 (13.6, 17.6); 8 000 rows, 64 and 256: (40, 17).  bf16, 100 rows: 32 and 64 (3.4, 8.4), 128 and 512
+// (8.9, 10.7), 33 and 70 (6.1, 13.1); 8 000 rows, 64 and 256 (19, 11).  One row, 128 and 512: float32 (11.2, 6.3), bf16 (8.5, 6.7).  Beyond
+// 128 columns y takes the registers that the loads need: at 256 and 512, 22 against 19 in float32, 15 against 11 in bf16.
+// Sizes alone decide, not addresses: the workspace is asked for without them.
+static bool some_rows_pay(const FeedForward &f) {
+  if (f.C > 128) return false;
+  const int cluster = some_cluster(f.f32, f.M, f.H), group = some_group(f.f32);
+  const int64_t each = ((f.H + group - 1) / group + cluster * SOME_WARPS - 1) / (cluster * SOME_WARPS);   // groups a warp
+  const int64_t rounds = ((f.M + SOME_ROWS - 1) / SOME_ROWS * cluster + 147) / 148;
+  const bool wide = f.C % 4 == 0 && f.H % (f.f32 ? 2 : 4) == 0, tma = f.f32 || (f.C % 8 == 0 && f.H % 8 == 0);
+  const int64_t one = (f.f32 ? 53 : 34) * f.C * (wide ? 2 : f.f32 ? 3 : 6) / 2;   // a group
+  const int64_t some = rounds * ((f.f32 ? 2800 : 2400) + each * one) + (cluster > 1 ? 1700 : 0);
+  if (f.M <= FEW_ROWS) return some < 5600 + 300 * f.M + 15 * f.C + 2 * f.H;   // with 2 us of a second launch
+  const int64_t blocks = (f.C + 63) / 64 + (f.H + 63) / 64;
+  return some < (f.f32 ? 10800 + 500 * blocks : (tma ? 8000 : 12000) + 200 * blocks);
+}
+
 static int forward(const FeedForward &f, void *y, Carve &w) {
+  if (some_rows_pay(f)) return !w.base ? CMACE_OK : (f.f32 ? some_rows<float>(f, y) : some_rows<__nv_bfloat16>(f, y));
   if (f.M <= FEW_ROWS) {
     float *h = w.take<float>(f.M * f.H);
     return !w.base ? CMACE_OK : (f.f32 ? few_rows<float>(f, y, h) : few_rows<__nv_bfloat16>(f, y, h));
@@ -549,6 +912,7 @@ static int run_forward(bool f32, const void *x, const void *wg, const void *wu, 
   FeedForward f{f32, x, wg, wu, wd, nullptr, M, C, H, act, status, (cudaStream_t)stream, what};
   Carve count{nullptr};
   forward(f, y, count);
+  count.used = std::max<int64_t>(count.used, 256);   // what is asked for at least
   if (bytes < count.used) return fail(CMACE_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes, (long long)count.used);
   ChainScope chain;
   chain_launches() = Chain::from_second;
@@ -596,7 +960,7 @@ int64_t cmace_gated_ff_workspace_bytes(int is_f32, int64_t rows, int width, int 
   void *const none[3] = {nullptr, nullptr, nullptr};
   if (backward_pass) backward(f, nullptr, none, true, true, count);
   else forward(f, nullptr, count);
-  return count.used;
+  return std::max<int64_t>(count.used, 256);
 }
 
 int cmace_gated_ff_fwd_f32(const float *x, const float *w_gate, const float *w_up, const float *w_down, int64_t rows, int width, int hidden,

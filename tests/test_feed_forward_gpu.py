@@ -447,3 +447,48 @@ def test_forward_mode_is_refused(dev):
             with pytest.raises(NotImplementedError):
                 ops.gated_feed_forward(*dual)
         ops.gated_feed_forward(*t)
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,C,H", [(9, 16, 16), (16, 32, 512), (17, 40, 200), (100, 128, 512), (33, 100, 301), (40, 127, 65), (1, 20, 900), (7, 64, 64),
+                                   (700, 128, 128), (300, 8, 8), (64, 36, 1030), (3000, 33, 70), (2500, 32, 64), (400, 96, 1100), (50, 4, 2)])
+def test_some_rows(M, C, H, dtype, apart, dev):
+    """Sizes on both sides of where one kernel has the whole block; `apart`: operands one element behind an aligned address."""
+    from cuda_mace_b200 import ops
+
+    t = case(M + C + H + 1, M, C, H, dtype, dev)[:4]
+    if apart:
+        for i, v in enumerate(t):
+            buffer = torch.full((v.numel() + 1,), float("nan"), dtype=dtype, device=dev)
+            buffer[1:] = v.flatten()
+            t[i] = buffer[1:].view(v.shape)
+    y = ops.gated_feed_forward(*t)
+    inside(y, reference(*(v.double() for v in t), None, "silu", dtype)["y"])
+    assert torch.equal(y, ops.gated_feed_forward(*t))
+    # what lies behind the last row is not written: the C entry with room behind y
+    from cuda_mace_b200 import _abi
+
+    f32 = dtype == F32
+    room = torch.full((M * C + 64,), 7.0, dtype=dtype, device=dev)
+    n = _abi.call("cmace_gated_ff_workspace_bytes", int(f32), M, C, H, 0)
+    ws = torch.full((n,), 0xFF, dtype=torch.uint8, device=dev)   # NaN wherever a value that was never written is read
+    stream = torch.cuda.current_stream().cuda_stream
+    _abi.call("cmace_gated_ff_fwd_" + ("f32" if f32 else "bf16"), *(v.data_ptr() for v in t), M, C, H, 0, room.data_ptr(), ws.data_ptr(), n, 0, stream)
+    assert torch.equal(room[:M * C].view(M, C), y) and (room[M * C:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,C,H", [(40, 32, 64), (40, 120, 500)])
+def test_some_rows_that_are_not_finite(M, C, H, dtype, dev):
+    from cuda_mace_b200 import ops
+
+    t = case(93, M, C, H, dtype, dev)[:4]
+    want = ops.gated_feed_forward(*t)
+    x = t[0].clone()
+    x[0, 3], x[17, C - 1], x[39, 0] = float("nan"), float("inf"), float("-inf")
+    got = ops.gated_feed_forward(x, *t[1:])
+    bad = torch.zeros(M, dtype=torch.bool, device=dev)
+    bad[[0, 17, 39]] = True
+    assert torch.equal(got[~bad], want[~bad])
+    assert not torch.isfinite(got[bad]).all(1).any()

@@ -604,6 +604,39 @@ __global__ void __launch_bounds__(256) weight_reduce_kernel(const WeightReduce p
   }
 }
 
+// ---- rows of y or dx whose sum over the hidden columns was split: added in the order of the splits ------------------------------------
+struct RowsSum {
+  const float *partial;   // [splits][M][ld]
+  void *out;              // [M][C]
+  int64_t M;
+  int ld, C, splits, wide;
+};
+// A thread adds four columns of a row.
+template <typename T>
+__global__ void __launch_bounds__(256) rows_sum_kernel(const RowsSum p) {
+  grid_begin();
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, plane = p.M * p.ld;
+  if (at >= plane) return;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < p.splits; s++) {
+    const float4 o = __ldcg(reinterpret_cast<const float4 *>(p.partial + s * plane + at));
+    v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+  }
+  const int64_t row = at / p.ld;
+  const int c = (int)(at - row * p.ld), n = p.C - c;
+  T *to = static_cast<T *>(p.out) + row * p.C + c;
+  if (p.wide) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(to) = v;
+    else *reinterpret_cast<uint2 *>(to) = make_uint2(tp_bf16x2(v.x, v.y), tp_bf16x2(v.z, v.w));
+  } else {
+    to[0] = (T)v.x;
+    if (n > 1) to[1] = (T)v.y;
+    if (n > 2) to[2] = (T)v.z;
+    if (n > 3) to[3] = (T)v.w;
+  }
+}
+
 // ---- a call -----------------------------------------------------------------------------------------------------------------
 struct FeedForward {
   bool f32;
@@ -677,6 +710,39 @@ static int launch_plain(bool pair, TpArgs &g, cudaStream_t st, const char *what)
   if (pair) return two < one ? tp_launch<TP_PLAIN, true, 128, 2>(g, st, what) : tp_launch<TP_PLAIN, true, 128, 1>(g, st, what);
   if (cost(2, 256, 256) < std::min(one, two)) return tp_launch<TP_PLAIN, false, 256, 2>(g, st, what);
   return two < one ? tp_launch<TP_PLAIN, false, 128, 2>(g, st, what) : tp_launch<TP_PLAIN, false, 128, 1>(g, st, what);
+}
+
+// Splits of a sum over the hidden columns for [M, C] results whose tiles leave SMs idle, by what the products cost and, for a second kernel, its
+// launch and its traffic (3 600 bytes a cycle), 12 500 cycles.  (Forward, without and with, us: float32 64 rows, 512 and 4 096: 50, 30; 100 rows, 256 and
+// 2 048: 30, 22; bf16 the same 21.8, 18.3 and 14.8, 16.2.  Forward and backward, 64 rows: 140, 79; bf16 64, 47.)
+static int row_splits(bool pair, int64_t M, int C, int kblocks) {
+  int best = 1;
+  int64_t least = 0;
+  for (int s = 1; s <= 32 && 2 * s <= kblocks; s *= 2) {
+    const TpCost cost{M, C, kblocks / s + 1, s, pair};
+    int64_t c = std::min(cost(1, 128, 128), cost(2, 128, 128));
+    if (!pair) c = std::min(c, cost(2, 256, 256));
+    if (s > 1) c += 12500 + (s + 1) * M * C / 450;
+    if (s == 1 || c < least) best = s, least = c;
+  }
+  return best;
+}
+// a product whose rows go to the caller's array, by way of the splits' sums where there are any
+static int launch_rows(const FeedForward &f, TpArgs &g, void *out, int splits, float *partial) {
+  if (splits == 1) {
+    if (const int rc = set_user_out(g, out, f.f32, f.M, f.C, f.what)) return rc;
+    return launch_plain(f.f32, g, f.st, f.what);
+  }
+  const int ld = (int)up(f.C, 4);
+  g.splits = splits;
+  g.out[1].use_map = 1;
+  if (const int rc = encode_tile_map(&g.out[1].map, partial, 4, false, f.C, f.M, splits, ld, f.M * ld, 16, 32, f.what)) return rc;
+  if (const int rc = launch_plain(f.f32, g, f.st, f.what)) return rc;
+  const RowsSum r{partial, out, f.M, ld, f.C, splits, f.C % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (f.f32 ? 15 : 7)) == 0};
+  const dim3 grid((unsigned)((f.M * ld / 4 + 255) / 256));
+  if (f.f32) launch_chained(rows_sum_kernel<float>, grid, dim3(256), (size_t)0, f.st, r);
+  else launch_chained(rows_sum_kernel<__nv_bfloat16>, grid, dim3(256), (size_t)0, f.st, r);
+  return check_launch(f.what);
 }
 
 static int run_prep(const PrepArgs &p, int64_t blocks, cudaStream_t st, const char *what) {
@@ -773,7 +839,7 @@ static bool some_rows_pay(const FeedForward &f) {
   const bool wide = f.C % 4 == 0 && f.H % (f.f32 ? 2 : 4) == 0, tma = f.f32 || (f.C % 8 == 0 && f.H % 8 == 0);
   const int64_t one = (f.f32 ? 53 : 34) * f.C * (wide ? 2 : f.f32 ? 3 : 6) / 2;   // a group
   const int64_t some = rounds * ((f.f32 ? 2800 : 2400) + each * one) + (cluster > 1 ? 1700 : 0);
-  if (f.M <= FEW_ROWS) return some < 5600 + 300 * f.M + 15 * f.C + 2 * f.H;   // with 2 us of a second launch
+  if (f.M <= FEW_ROWS) return f.H <= 1024 && some < 5600 + 300 * f.M + 15 * f.C + 2 * f.H;   // with 2 us of a second launch; long weights want all SMs
   const int64_t blocks = (f.C + 63) / 64 + (f.H + 63) / 64;
   return some < (f.f32 ? 10800 + 500 * blocks : (tma ? 8000 : 12000) + 200 * blocks);
 }
@@ -792,6 +858,8 @@ static int forward(const FeedForward &f, void *y, Carve &w) {
   Matrix wu = take_matrix(w, prep, blocks, f.f32, f.wu, f.C, f.H);
   Matrix wd = take_matrix(w, prep, blocks, f.f32, f.wd, f.H, f.C);
   Matrix h = new_matrix(w, f.f32, f.M, f.H, 1);
+  const int splits = row_splits(f.f32, f.M, f.C, blocks64(f.H));
+  float *partial = splits > 1 ? w.take<float>(splits * f.M * up(f.C, 4)) : nullptr;
   if (!w.base) return CMACE_OK;
   const bool bf16 = !f.f32;
   int rc = run_prep(prep, blocks, f.st, f.what);
@@ -807,8 +875,7 @@ static int forward(const FeedForward &f, void *y, Carve &w) {
   set_operand(g.a[0], h, true);
   set_operand(g.b[0], wd, false);
   set_k(g, 0, f.H);
-  if (!rc) rc = set_user_out(g, y, f.f32, f.M, f.C, f.what);
-  if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
+  if (!rc) rc = launch_rows(f, g, y, splits, partial);
   return rc;
 }
 
@@ -825,6 +892,8 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   const int64_t ld = up(f.H, 4);
   const int splits = weight_splits(f.M, f.C, f.H);
   float *partial = want_w && splits > 1 ? w.take<float>((int64_t)splits * 3 * f.C * ld) : nullptr;
+  const int x_splits = row_splits(f.f32, f.M, f.C, 2 * blocks64(f.H));
+  float *x_partial = want_x && x_splits > 1 ? w.take<float>(x_splits * f.M * up(f.C, 4)) : nullptr;
   if (!w.base) return CMACE_OK;
   const bool bf16 = !f.f32;
   int rc = run_prep(prep, blocks, f.st, f.what);
@@ -849,8 +918,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
     g.segments = 2;
     set_k(g, 0, f.H);
     set_k(g, 1, f.H);
-    if (!rc) rc = set_user_out(g, gx, f.f32, f.M, f.C, f.what);
-    if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
+    if (!rc) rc = launch_rows(f, g, gx, x_splits, x_partial);
   }
   if (want_w && splits == 1) {
     if (gw[0] || gw[1]) {

@@ -452,7 +452,7 @@ def test_forward_mode_is_refused(dev):
 @pytest.mark.parametrize("apart", [False, True])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("M,C,H", [(9, 16, 16), (16, 32, 512), (17, 40, 200), (100, 128, 512), (33, 100, 301), (40, 127, 65), (1, 20, 900), (7, 64, 64),
-                                   (700, 128, 128), (300, 8, 8), (64, 36, 1030), (3000, 33, 70), (2500, 32, 64), (400, 96, 1100), (50, 4, 2)])
+                                   (700, 128, 128), (300, 8, 8), (64, 36, 1030), (3000, 33, 70), (2500, 32, 64), (400, 96, 1100), (50, 4, 2), (20, 24, 20000), (3, 16, 5000)])
 def test_some_rows(M, C, H, dtype, apart, dev):
     """Sizes on both sides of where one kernel has the whole block; `apart`: operands one element behind an aligned address."""
     from cuda_mace_b200 import ops
@@ -492,3 +492,15 @@ def test_some_rows_that_are_not_finite(M, C, H, dtype, dev):
     bad[[0, 17, 39]] = True
     assert torch.equal(got[~bad], want[~bad])
     assert not torch.isfinite(got[bad]).all(1).any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,C,H", [(100, 256, 2048), (64, 264, 1500), (9, 130, 4100), (300, 33, 3001), (700, 132, 1024)])
+def test_sums_over_many_hidden_columns(M, C, H, dtype, dev):
+    """Few rows and long sums, which are split, for y and the gradient of x."""
+    t = case(M + C + H + 2, M, C, H, dtype, dev)
+    got, again = run_all(*t, "silu"), run_all(*t, "silu")
+    want = reference(*(v.double() for v in t), "silu", dtype)
+    for name, a, b in zip(("y", "x", "w_gate", "w_up", "w_down"), got, again):
+        inside(a, want[name])
+        assert torch.equal(a, b)

@@ -14,6 +14,8 @@
 // Only x and the weights are kept for the backward: forming g and u again costs 4 M C H operations, keeping them in float32 16 bytes
 // a hidden value written and read (what would be as exact as the products are), which pays from C of about 1 000 only.
 //
+// Where tiles would be empty or the chain of kernels long, the forward pass goes another way: few_rows_kernel (up to eight rows) and some_rows_kernel
+// (up to 128 columns) below.
 // float32 goes as pairs of fp16 values (tile_product.cuh); a first kernel splits x and the weights.  bf16 is read where it lies;
 // rows that TMA cannot address (a width that is not a multiple of eight, an address that is not one of 16 bytes) are copied first.
 // In bf16, h, dg and du are rounded once to bf16 between the products, as the operands of a 16-bit product have to be; with the
@@ -713,7 +715,7 @@ static int launch_plain(bool pair, TpArgs &g, cudaStream_t st, const char *what)
 }
 
 // Splits of a sum over the hidden columns for [M, C] results whose tiles leave SMs idle, by what the products cost and, for a second kernel, its
-// launch and its traffic (3 600 bytes a cycle), 12 500 cycles.  (Forward, without and with, us: float32 64 rows, 512 and 4 096: 50, 30; 100 rows, 256 and
+// launch and its traffic (3 600 bytes a cycle), 10 000 cycles or, where copies hide less of them, 15 000.  (Forward, without and with, us: float32 64 rows, 512 and 4 096: 50, 30; 100 rows, 256 and
 // 2 048: 30, 22; bf16 the same 21.8, 18.3 and 14.8, 16.2.  Forward and backward, 64 rows: 140, 79; bf16 64, 47.)
 static int row_splits(bool pair, int64_t M, int C, int kblocks) {
   int best = 1;
@@ -722,7 +724,7 @@ static int row_splits(bool pair, int64_t M, int C, int kblocks) {
     const TpCost cost{M, C, kblocks / s + 1, s, pair};
     int64_t c = std::min(cost(1, 128, 128), cost(2, 128, 128));
     if (!pair) c = std::min(c, cost(2, 256, 256));
-    if (s > 1) c += 12500 + (s + 1) * M * C / 450;
+    if (s > 1) c += (pair ? 10000 : 15000) + (s + 1) * M * C / 450;
     if (s == 1 || c < least) best = s, least = c;
   }
   return best;

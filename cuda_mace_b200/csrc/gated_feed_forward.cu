@@ -134,26 +134,31 @@ struct FewArgs {
   int M, K, N, cluster, wide;
 };
 
-template <typename T, int V>
-__device__ __forceinline__ void few_load(float (&v)[V], const T *p, int n, bool wide) {
-  if (!wide) {
-#pragma unroll
-    for (int i = 0; i < V; i++) v[i] = i < n ? (float)p[i] : 0.f;
-  } else if constexpr (sizeof(T) == 4) {
-    const float4 x = __ldg(reinterpret_cast<const float4 *>(p));
-    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-  } else {
-    uint32_t w[V / 2];
-    if constexpr (V == 8) {
+// V values from p as they lie, the first n of them (wide: all, aligned), zeros for the others
+template <typename T, int V, int WORDS = V * (int)sizeof(T) / 4>
+__device__ __forceinline__ void few_load(uint32_t (&v)[WORDS], const T *p, int n, bool wide) {
+  if (wide) {
+    if constexpr (WORDS == 4) {
       const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
-      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
     } else {
       const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
-      w[0] = x.x, w[1] = x.y;
+      v[0] = x.x, v[1] = x.y;
     }
+  } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < V / 2; i++) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    for (int i = 0; i < V; i++) v[i] = i < n ? __float_as_uint(__ldg(p + i)) : 0u;
+  } else {
+    const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+    for (int i = 0; i < WORDS; i++) v[i] = (2 * i < n ? (uint32_t)__ldg(h + 2 * i) : 0u) | (2 * i + 1 < n ? (uint32_t)__ldg(h + 2 * i + 1) << 16 : 0u);
   }
+}
+template <typename T, int WORDS>
+__device__ __forceinline__ float few_value(const uint32_t (&v)[WORDS], int i) {
+  if (sizeof(T) == 4) return __uint_as_float(v[i % WORDS]);
+  const uint32_t w = v[i / 2];
+  return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
 }
 // columns a thread: 16 bytes, 8 where the sums of eight rows would not fit the registers
 template <typename T, int M>
@@ -169,6 +174,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_rows_kernel(const FewArgs 
   const int rank = blockIdx.x % g.cluster, col = (int)(blockIdx.x / g.cluster) * FEW_COLS + V * part;
   const int k0 = (int)((int64_t)g.K * rank / g.cluster), k1 = (int)((int64_t)g.K * (rank + 1) / g.cluster);
   const int n = g.N - col;
+  // Wd does not come from the kernel before: it is on its way while that one ends.
+  if (!GATED) {
+    const T *w = static_cast<const T *>(g.w[0]) + (int)(blockIdx.x / g.cluster) * FEW_COLS;
+    for (int k = k0 + (int)threadIdx.x; k < k1; k += FEW_THREADS) asm volatile("prefetch.global.L1 [%0];" ::"l"(w + (int64_t)k * g.N));
+  }
   grid_begin();
   float acc[W][M][V] = {};
   for (int from = k0; from < k1; from += FEW_K) {
@@ -185,19 +195,28 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_rows_kernel(const FewArgs 
     }
     __syncthreads();
     if (n > 0) {
-#pragma unroll(M <= 2 ? 8 : 4)
-      for (int k = ROWS * warp + row; k < len; k += ROWS * WARPS) {
-        float w[W][V], x[M];
+      // AHEAD loads leave together, however long the rest is; behind the last row they read it once more, for nothing.
+      constexpr int AHEAD = M <= 2 ? 8 : 4, STEP = ROWS * WARPS;
+      for (int first = ROWS * warp + row; first < len; first += AHEAD * STEP) {
+        uint32_t w[AHEAD][W][V * (int)sizeof(T) / 4];
 #pragma unroll
-        for (int i = 0; i < W; i++) few_load<T, V>(w[i], static_cast<const T *>(g.w[i]) + (int64_t)(from + k) * g.N + col, n, g.wide);
+        for (int a = 0; a < AHEAD; a++)
 #pragma unroll
-        for (int m = 0; m < M; m++) x[m] = few_smem[k * M + m];
+          for (int i = 0; i < W; i++)
+            few_load<T, V>(w[a][i], static_cast<const T *>(g.w[i]) + (int64_t)(from + min(first + a * STEP, len - 1)) * g.N + col, n, g.wide);
 #pragma unroll
-        for (int i = 0; i < W; i++)
+        for (int a = 0; a < AHEAD; a++) {
+          if (first + a * STEP >= len) break;
+          float x[M];
 #pragma unroll
-          for (int m = 0; m < M; m++)
+          for (int m = 0; m < M; m++) x[m] = few_smem[(first + a * STEP) * M + m];
 #pragma unroll
-            for (int j = 0; j < V; j++) acc[i][m][j] = fmaf(x[m], w[i][j], acc[i][m][j]);
+          for (int i = 0; i < W; i++)
+#pragma unroll
+            for (int m = 0; m < M; m++)
+#pragma unroll
+              for (int j = 0; j < V; j++) acc[i][m][j] = fmaf(x[m], few_value<T>(w[a][i], j), acc[i][m][j]);
+        }
       }
     }
   }

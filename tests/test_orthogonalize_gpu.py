@@ -258,3 +258,14 @@ def test_long_sides_and_forward_mode_are_refused(dev):
         with pytest.raises(NotImplementedError):
             ops.orthogonalize(forward_ad.make_dual(U, torch.ones_like(U)))
         ops.orthogonalize(U)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shape", [(2, 40, 520), (1, 520, 128), (2, 100, 193), (80, 20, 250), (1, 128, 1024), (1, 128, 1025)])
+def test_columns_over_a_cluster(shape, dtype, dev):
+    """Columns that do not divide among the CTAs (of 520 over eight of 80 the last has none), and the lines between the variants."""
+    from cuda_mace_b200 import ops
+
+    U = update(13 + sum(shape), shape, dtype, dev)
+    check(ops.orthogonalize(U), U)
+    ops.check_status()

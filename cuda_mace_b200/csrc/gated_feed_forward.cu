@@ -123,8 +123,9 @@ __global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const __grid_constan
 // With up to eight rows the block is as long as its weights take to arrive, and a tensor core's tile would be 1/16 full at most: plain
 // float32 FMA, a weight read once for all rows.  A CTA has 32 columns (segments of 64 or 128 bytes of a row), its 16 warps every 64th group
 // of rows of W, and the CTAs of a cluster share the rows where columns alone do not fill the SMs.  h stays float32 in the workspace.
-// (Width 1 024, hidden width 4 096, both kernels in a recorded graph: one row 10.4 us in bf16 and 10.7 in float32, against 26 and 65 by tiles; eight
-// rows 21.6 and 20.3 against 24 and 66.  128 and 512: 6.8 and 6.1 against 10.4 and 15.7; eight rows 9.8 and 9.2 against 10.5 and 15.8.)
+// Three sets of weights in turn, both kernels in a recorded graph, us: 1 024 and 4 096, one row 9.5 in bf16 and 14.5 in float32, eight rows 21 and 24
+// against 20.5 and 44 by tiles; 512 and 2 048, one row 10 and 9.6 (clusters), eight 15.5 and 15 against 15.5 and 27.  Eight rows are bound by
+// FMA and by their operands: x from shared memory, weights to float32.
 constexpr int FEW_ROWS = 8, FEW_THREADS = 512, FEW_COLS = 32, FEW_K = 1024;   // FEW_K: rows of W whose x is in shared memory
 
 struct FewArgs {
@@ -132,6 +133,7 @@ struct FewArgs {
   const void *w[2];    // [K, N]
   void *out;           // [M, N]: h in float32, or T
   int M, K, N, cluster, wide;
+  int32_t *status;
 };
 
 // V values from p as they lie, the first n of them (wide: all, aligned), zeros for the others
@@ -169,11 +171,20 @@ template <typename T, int M, bool GATED, int ACT>
 __global__ void __launch_bounds__(FEW_THREADS, 1) few_rows_kernel(const FewArgs g) {
   constexpr int W = GATED ? 2 : 1, WARPS = FEW_THREADS / 32, V = few_cols<T, M>(), LANES = FEW_COLS / V, ROWS = 32 / LANES;   // of a warp's load
   extern __shared__ float few_smem[];   // x [FEW_K][M]; then the warps' sums [WARPS][W][M][32]
-  __shared__ float total[W][M][FEW_COLS];
+  __shared__ float total[8][W][M][FEW_COLS];   // of the CTAs of a cluster, in the first one's
+  __shared__ __align__(8) uint64_t joined;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane % LANES, row = lane / LANES;
   const int rank = blockIdx.x % g.cluster, col = (int)(blockIdx.x / g.cluster) * FEW_COLS + V * part;
   const int k0 = (int)((int64_t)g.K * rank / g.cluster), k1 = (int)((int64_t)g.K * (rank + 1) / g.cluster);
   const int n = g.N - col;
+  if (g.cluster > 1) {
+    if (threadIdx.x == 0) {
+      mbar_init(smem_u32(&joined), (uint32_t)g.cluster - 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    cluster_arrive();
+  }
   // Wd does not come from the kernel before: it is on its way while that one ends.
   if (!GATED) {
     const T *w = static_cast<const T *>(g.w[0]) + (int)(blockIdx.x / g.cluster) * FEW_COLS;
@@ -195,15 +206,18 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_rows_kernel(const FewArgs 
     }
     __syncthreads();
     if (n > 0) {
-      // AHEAD loads leave together, however long the rest is; behind the last row they read it once more, for nothing.
+      // AHEAD loads leave together, however long the rest is; behind the last row they read it once more,
+      // for nothing.
       constexpr int AHEAD = M <= 2 ? 8 : 4, STEP = ROWS * WARPS;
       for (int first = ROWS * warp + row; first < len; first += AHEAD * STEP) {
         uint32_t w[AHEAD][W][V * (int)sizeof(T) / 4];
 #pragma unroll
-        for (int a = 0; a < AHEAD; a++)
+        for (int a = 0; a < AHEAD; a++) {
+          if (first - row + a * STEP >= len) break;   // none of the warp's rows
 #pragma unroll
           for (int i = 0; i < W; i++)
             few_load<T, V>(w[a][i], static_cast<const T *>(g.w[i]) + (int64_t)(from + min(first + a * STEP, len - 1)) * g.N + col, n, g.wide);
+        }
 #pragma unroll
         for (int a = 0; a < AHEAD; a++) {
           if (first + a * STEP >= len) break;
@@ -233,42 +247,38 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_rows_kernel(const FewArgs 
         if (row == 0) few_smem[((warp * W + i) * M + m) * FEW_COLS + V * part + j] = v;
       }
   __syncthreads();
+  // The first CTA of a cluster gets the others' sums: one arrival each instead of two barriers of all threads: 11.1 us for a row of
+  // 512 x 2 048 in bf16, 12.0 with those.
+  if (g.cluster > 1) {
+    __syncwarp();
+    cluster_wait();
+  }
   for (int e = threadIdx.x; e < W * M * FEW_COLS; e += FEW_THREADS) {
     float v = 0.f;
 #pragma unroll
     for (int k = 0; k < WARPS; k++) v += few_smem[k * (W * M * FEW_COLS) + e];
-    (&total[0][0][0])[e] = v;
+    float *const to = &total[rank][0][0][0] + e;
+    if (rank == 0) *to = v;
+    else asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer_smem(smem_u32(to), 0)), "f"(v) : "memory");
   }
-  if (g.cluster > 1) {
-    __syncwarp();
-    cluster_sync();
-  } else {
-    __syncthreads();
+  __syncthreads();
+  if (rank != 0) {
+    if (threadIdx.x == 0) peer_arrive(smem_u32(&joined), 0);
+    return;
   }
-  if (rank == 0) {
-    for (int e = threadIdx.x; e < M * FEW_COLS; e += FEW_THREADS) {
-      const int m = e / FEW_COLS, c = (int)(blockIdx.x / g.cluster) * FEW_COLS + e % FEW_COLS;
-      float v[W];
+  if (g.cluster > 1 && !peer_wait(smem_u32(&joined), 0) && g.status) atomicCAS(g.status, 0, 51);
+  for (int e = threadIdx.x; e < M * FEW_COLS; e += FEW_THREADS) {
+    const int m = e / FEW_COLS, c = (int)(blockIdx.x / g.cluster) * FEW_COLS + e % FEW_COLS;
+    float v[W];
 #pragma unroll
-      for (int i = 0; i < W; i++) {
-        v[i] = 0.f;
-        const uint32_t at = smem_u32(&total[i][m][e % FEW_COLS]);
-        for (int r = 0; r < g.cluster; r++) {
-          float part_sum;
-          if (g.cluster > 1) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part_sum) : "r"(peer_smem(at, (uint32_t)r)) : "memory");
-          else part_sum = total[i][m][e % FEW_COLS];
-          v[i] += part_sum;
-        }
-      }
-      if (m < g.M && c < g.N) {
-        if (GATED) static_cast<float *>(g.out)[(int64_t)m * g.N + c] = tp_act<ACT>(v[0]) * v[W - 1];
-        else static_cast<T *>(g.out)[(int64_t)m * g.N + c] = (T)v[0];
-      }
+    for (int i = 0; i < W; i++) {
+      v[i] = 0.f;
+      for (int r = 0; r < g.cluster; r++) v[i] += total[r][i][m][e % FEW_COLS];
     }
-  }
-  if (g.cluster > 1) {   // nobody leaves while its sums are read
-    __syncwarp();
-    cluster_sync();
+    if (m < g.M && c < g.N) {
+      if (GATED) static_cast<float *>(g.out)[(int64_t)m * g.N + c] = tp_act<ACT>(v[0]) * v[W - 1];
+      else static_cast<T *>(g.out)[(int64_t)m * g.N + c] = (T)v[0];
+    }
   }
 }
 
@@ -283,7 +293,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_rows_kernel(const FewArgs 
 // added to float32 registers, so that the tensor core's truncation stays at 2^-24 of a partial sum.
 // 192 rows, 128 and 512: float32 12 us against 17.7 by tiles, bf16 9.0 against 10.7; 400 rows, 32 and 512: 5.9 against 16.1, 5.3 against 10.2.  A
 // warp's chain bounds it (loads, six dependent products a step, 16 values a load to split): two rows of blocks an SM at once do not fit the
-// registers.  Groups spread over twice as many CTAs: the same (a cluster costs 1.7).
+// registers.  Groups spread over twice as many CTAs: the same (a cluster costs 1.7; sums pushed to the CTA that stores them, with one arrival each: the same or 1 more).
 constexpr int SOME_THREADS = 256, SOME_WARPS = SOME_THREADS / 32, SOME_ROWS = 16;
 
 struct SomeArgs {
@@ -801,7 +811,7 @@ static int launch_few(FewArgs g, cudaStream_t st, const char *what) {
 }
 template <typename T, int M, int ACT>
 static int few_rows(const FeedForward &f, void *y, float *h) {
-  FewArgs g{f.x, {f.wg, f.wu}, h, (int)f.M, f.C, f.H, 1, 0};
+  FewArgs g{f.x, {f.wg, f.wu}, h, (int)f.M, f.C, f.H, 1, 0, f.status};
   if (const int rc = launch_few<T, M, true, ACT>(g, f.st, f.what)) return rc;
   g.x = h, g.w[0] = f.wd, g.out = y, g.K = f.H, g.N = f.C;
   return launch_few<T, M, false, ACT>(g, f.st, f.what);

@@ -175,26 +175,6 @@ __device__ __forceinline__ uint4 smem_load4(uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
-// One thread of every CTA of a cluster arrives on the barrier of each, for its block (which has met at bar.sync before), and all threads
-// wait on their own CTA's: some 700 cycles where barrier.cluster of 512 threads takes 2 000.
-__device__ __forceinline__ void peer_arrive(uint32_t bar, uint32_t rank) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(peer_smem(bar, rank)) : "memory");
-}
-__device__ __forceinline__ bool peer_wait(uint32_t bar, uint32_t parity) {
-  const long long t0 = clock64();
-  while (true) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if (clock64() - t0 > GT_TIMEOUT_CYCLES) return false;
-  }
-}
 // two packed fp16 of each part as the floats that they stand for, times their power of two
 __device__ __forceinline__ float2 pair_value(uint32_t hi, uint32_t lo) {
   const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&hi)), y = __half22float2(*reinterpret_cast<const __half2 *>(&lo));

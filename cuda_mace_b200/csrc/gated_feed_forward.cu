@@ -744,16 +744,17 @@ static int launch_plain(bool pair, TpArgs &g, cudaStream_t st, const char *what)
 }
 
 // Splits of a sum over the hidden columns for [M, C] results whose tiles leave SMs idle, by what the products cost and, for a second kernel, its
-// launch and its traffic (3 600 bytes a cycle), 10 000 cycles or, where copies hide less of them, 15 000.  (Forward, without and with, us: float32 64 rows, 512 and 4 096: 50, 30; 100 rows, 256 and
-// 2 048: 30, 22; bf16 the same 21.8, 18.3 and 14.8, 16.2.  Forward and backward, 64 rows: 140, 79; bf16 64, 47.)
-static int row_splits(bool pair, int64_t M, int C, int kblocks) {
+// launch and its traffic (3 600 bytes a cycle), `second` cycles more.  Forward, without and with, us: float32 64 rows, 512 and 4 096: 50, 30; 100 rows,
+// 256 and 2 048: 30, 22; bf16 the same 21.8, 18.3 and 14.8, 16.2: from 10 000 and 15 000 cycles on.  Forward and backward, 64 rows: 140, 79;
+// bf16 64, 47; but outside a graph a call with gradients is 90 of host whatever its kernels take, and another launch 4 more: from 30 000.
+static int row_splits(bool pair, int64_t M, int C, int kblocks, int64_t second) {
   int best = 1;
   int64_t least = 0;
   for (int s = 1; s <= 32 && 2 * s <= kblocks; s *= 2) {
     const TpCost cost{M, C, kblocks / s + 1, s, pair};
     int64_t c = std::min(cost(1, 128, 128), cost(2, 128, 128));
     if (!pair) c = std::min(c, cost(2, 256, 256));
-    if (s > 1) c += (pair ? 10000 : 15000) + (s + 1) * M * C / 450;
+    if (s > 1) c += second + (s + 1) * M * C / 450;
     if (s == 1 || c < least) best = s, least = c;
   }
   return best;
@@ -889,7 +890,7 @@ static int forward(const FeedForward &f, void *y, Carve &w) {
   Matrix wu = take_matrix(w, prep, blocks, f.f32, f.wu, f.C, f.H);
   Matrix wd = take_matrix(w, prep, blocks, f.f32, f.wd, f.H, f.C);
   Matrix h = new_matrix(w, f.f32, f.M, f.H, 1);
-  const int splits = row_splits(f.f32, f.M, f.C, blocks64(f.H));
+  const int splits = row_splits(f.f32, f.M, f.C, blocks64(f.H), f.f32 ? 10000 : 15000);
   float *partial = splits > 1 ? w.take<float>(splits * f.M * up(f.C, 4)) : nullptr;
   if (!w.base) return CMACE_OK;
   const bool bf16 = !f.f32;
@@ -923,7 +924,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   const int64_t ld = up(f.H, 4);
   const int splits = weight_splits(f.M, f.C, f.H);
   float *partial = want_w && splits > 1 ? w.take<float>((int64_t)splits * 3 * f.C * ld) : nullptr;
-  const int x_splits = row_splits(f.f32, f.M, f.C, 2 * blocks64(f.H));
+  const int x_splits = row_splits(f.f32, f.M, f.C, 2 * blocks64(f.H), 30000);
   float *x_partial = want_x && x_splits > 1 ? w.take<float>(x_splits * f.M * up(f.C, 4)) : nullptr;
   if (!w.base) return CMACE_OK;
   const bool bf16 = !f.f32;

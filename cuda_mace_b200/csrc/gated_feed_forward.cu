@@ -33,7 +33,7 @@ struct PrepJob {
   void *hi, *lo;       // lo null: copy
   float *scale;        // inverse scales of the blocks
   int64_t rows, first; // first block of this job
-  int cols, ld, blocks_n;
+  int cols, ld, blocks_n, bf16;   // bf16: of the source of a pair
 };
 struct PrepArgs {
   PrepJob job[5];
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const __grid_constan
     return;
   }
   const float *s = static_cast<const float *>(J.src);
-  const bool wide = (J.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(J.src) & 15) == 0;
+  const bool wide = (J.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(J.src) & 15) == 0 && !J.bf16;
   float v[16];
   float most = 0.f;
   if (wide) {
@@ -79,7 +79,8 @@ __global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const __grid_constan
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const int64_t r = row0 + (t >> 6) + 4 * i;
-      v[i] = r < J.rows && col < J.cols ? __ldg(s + r * J.cols + col) : 0.f;
+      if (J.bf16) v[i] = r < J.rows && col < J.cols ? __bfloat162float(static_cast<const __nv_bfloat16 *>(J.src)[r * J.cols + col]) : 0.f;
+      else v[i] = r < J.rows && col < J.cols ? __ldg(s + r * J.cols + col) : 0.f;
     }
   }
   most = tp_most(v);
@@ -319,6 +320,11 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) 
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
 }
+// two values as bf16 and what that leaves: h keeps 16 bits, for half as many products again
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t &hi, uint32_t &lo) {
+  hi = tp_bf16x2(x, y);
+  lo = tp_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u));
+}
 // 8 or 16 bytes of `base`, `off` bytes behind it (the matrices here are below 4 GB).  FULL: all of it is there and aligned.  Otherwise the
 // first n elements are (WIDE: all or none, aligned), zeros stand for the others, and their loads go to the matrix's first elements: loads
 // without a branch leave together.
@@ -530,10 +536,17 @@ __global__ void __launch_bounds__(SOME_THREADS, 1) some_rows_kernel(const SomeAr
       } else {
 #pragma unroll
         for (int t = 0; t < NT; t += 2) {
-          const uint32_t a0 = tp_bf16x2(sum[0][t][0], sum[0][t][1]), a1 = tp_bf16x2(sum[0][t][2], sum[0][t][3]);
-          const uint32_t a2 = tp_bf16x2(sum[0][t + 1][0], sum[0][t + 1][1]), a3 = tp_bf16x2(sum[0][t + 1][2], sum[0][t + 1][3]);
+          uint32_t a[4], l[4];
+          split_bf16(sum[0][t][0], sum[0][t][1], a[0], l[0]);
+          split_bf16(sum[0][t][2], sum[0][t][3], a[1], l[1]);
+          split_bf16(sum[0][t + 1][0], sum[0][t + 1][1], a[2], l[2]);
+          split_bf16(sum[0][t + 1][2], sum[0][t + 1][3], a[3], l[3]);
 #pragma unroll
-          for (int s = 0; s < 4; s++) mma_bf16(y[span][s], a0, a1, a2, a3, k_pair(b[t][0], b[t][1], s), k_pair(b[t + 1][0], b[t + 1][1], s));
+          for (int s = 0; s < 4; s++) {
+            const uint32_t b0 = k_pair(b[t][0], b[t][1], s), b1 = k_pair(b[t + 1][0], b[t + 1][1], s);
+            mma_bf16(y[span][s], a[0], a[1], a[2], a[3], b0, b1);
+            mma_bf16(y[span][s], l[0], l[1], l[2], l[3], b0, b1);
+          }
         }
       }
     }
@@ -670,7 +683,7 @@ __global__ void __launch_bounds__(256) rows_sum_kernel(const RowsSum p) {
 
 // ---- a call -----------------------------------------------------------------------------------------------------------------
 struct FeedForward {
-  bool f32;
+  bool f32, pair;   // types of the arrays; products of pairs
   const void *x, *wg, *wu, *wd, *gy;
   int64_t M;
   int C, H, act;
@@ -680,16 +693,16 @@ struct FeedForward {
 };
 
 // A caller's matrix: read where it lies, or laid out in the workspace by the job that is added.
-static Matrix take_matrix(Carve &w, PrepArgs &prep, int64_t &blocks, bool f32, const void *src, int64_t rows, int cols) {
-  if (!f32 && cols % 8 == 0 && aligned16(src)) {
+static Matrix take_matrix(Carve &w, PrepArgs &prep, int64_t &blocks, const FeedForward &f, const void *src, int64_t rows, int cols) {
+  if (!f.pair && cols % 8 == 0 && aligned16(src)) {
     Matrix m;
     m.at = static_cast<uint16_t *>(const_cast<void *>(src));
     m.rows = rows, m.cols = cols, m.ld = cols;
     return m;
   }
-  const Matrix m = new_matrix(w, f32, rows, cols, 1);
+  const Matrix m = new_matrix(w, f.pair, rows, cols, 1);
   PrepJob &j = prep.job[prep.jobs++];
-  j = PrepJob{src, m.at, f32 ? m.at + m.plane() : nullptr, m.scale, rows, blocks, cols, (int)m.ld, (int)m.blocks_n()};
+  j = PrepJob{src, m.at, f.pair ? m.at + m.plane() : nullptr, m.scale, rows, blocks, cols, (int)m.ld, (int)m.blocks_n(), !f.f32};
   blocks += m.blocks_m() * m.blocks_n();
   return m;
 }
@@ -722,15 +735,15 @@ static TpCost cost_of(const TpArgs &g, bool pair) {
 }
 template <int ACT>
 static int launch_gated(const FeedForward &f, TpArgs &g) {
-  const TpCost cost = cost_of(g, f.f32);
+  const TpCost cost = cost_of(g, f.pair);
   const bool pairs = cost(2, 128, 256) < cost(1, 128, 256);
-  if (f.f32) return pairs ? tp_launch<TP_GATED, true, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_GATED, true, 128, 1, ACT>(g, f.st, f.what);
+  if (f.pair) return pairs ? tp_launch<TP_GATED, true, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_GATED, true, 128, 1, ACT>(g, f.st, f.what);
   return pairs ? tp_launch<TP_GATED, false, 128, 2, ACT>(g, f.st, f.what) : tp_launch<TP_GATED, false, 128, 1, ACT>(g, f.st, f.what);
 }
 template <int ACT>
 static int launch_back(const FeedForward &f, TpArgs &g) {
-  const TpCost cost = cost_of(g, f.f32);   // half of its blocks have two projections' columns, half one's
-  if (f.f32)
+  const TpCost cost = cost_of(g, f.pair);   // half of its blocks have two projections' columns, half one's
+  if (f.pair)
     return cost(2, 64, 96) < cost(1, 64, 96) ? tp_launch<TP_BACK, true, 64, 2, ACT>(g, f.st, f.what) : tp_launch<TP_BACK, true, 64, 1, ACT>(g, f.st, f.what);
   return cost(2, 128, 192) < cost(1, 64, 96) ? tp_launch<TP_BACK, false, 128, 2, ACT>(g, f.st, f.what)
                                              : tp_launch<TP_BACK, false, 64, 1, ACT>(g, f.st, f.what);
@@ -763,13 +776,13 @@ static int row_splits(bool pair, int64_t M, int C, int kblocks, int64_t second) 
 static int launch_rows(const FeedForward &f, TpArgs &g, void *out, int splits, float *partial) {
   if (splits == 1) {
     if (const int rc = set_user_out(g, out, f.f32, f.M, f.C, f.what)) return rc;
-    return launch_plain(f.f32, g, f.st, f.what);
+    return launch_plain(f.pair, g, f.st, f.what);
   }
   const int ld = (int)up(f.C, 4);
   g.splits = splits;
   g.out[1].use_map = 1;
   if (const int rc = encode_tile_map(&g.out[1].map, partial, 4, false, f.C, f.M, splits, ld, f.M * ld, 16, 32, f.what)) return rc;
-  if (const int rc = launch_plain(f.f32, g, f.st, f.what)) return rc;
+  if (const int rc = launch_plain(f.pair, g, f.st, f.what)) return rc;
   const RowsSum r{partial, out, f.M, ld, f.C, splits, f.C % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (f.f32 ? 15 : 7)) == 0};
   const dim3 grid((unsigned)((f.M * ld / 4 + 255) / 256));
   if (f.f32) launch_chained(rows_sum_kernel<float>, grid, dim3(256), (size_t)0, f.st, r);
@@ -885,15 +898,15 @@ static int forward(const FeedForward &f, void *y, Carve &w) {
   PrepArgs prep;
   memset(&prep, 0, sizeof(prep));
   int64_t blocks = 0;
-  Matrix x = take_matrix(w, prep, blocks, f.f32, f.x, f.M, f.C);
-  Matrix wg = take_matrix(w, prep, blocks, f.f32, f.wg, f.C, f.H);
-  Matrix wu = take_matrix(w, prep, blocks, f.f32, f.wu, f.C, f.H);
-  Matrix wd = take_matrix(w, prep, blocks, f.f32, f.wd, f.H, f.C);
-  Matrix h = new_matrix(w, f.f32, f.M, f.H, 1);
-  const int splits = row_splits(f.f32, f.M, f.C, blocks64(f.H), f.f32 ? 10000 : 15000);
+  Matrix x = take_matrix(w, prep, blocks, f, f.x, f.M, f.C);
+  Matrix wg = take_matrix(w, prep, blocks, f, f.wg, f.C, f.H);
+  Matrix wu = take_matrix(w, prep, blocks, f, f.wu, f.C, f.H);
+  Matrix wd = take_matrix(w, prep, blocks, f, f.wd, f.H, f.C);
+  Matrix h = new_matrix(w, f.pair, f.M, f.H, 1);
+  const int splits = row_splits(f.pair, f.M, f.C, blocks64(f.H), f.pair ? 10000 : 15000);
   float *partial = splits > 1 ? w.take<float>(splits * f.M * up(f.C, 4)) : nullptr;
   if (!w.base) return CMACE_OK;
-  const bool bf16 = !f.f32;
+  const bool bf16 = !f.pair;
   int rc = run_prep(prep, blocks, f.st, f.what);
   if (!rc) rc = encode_all({&x, &wg, &wu, &wd, &h}, bf16, f.what);
   TpArgs g = new_args(f.M, f.H, f.status);
@@ -915,19 +928,19 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   PrepArgs prep;
   memset(&prep, 0, sizeof(prep));
   int64_t blocks = 0;
-  Matrix x = take_matrix(w, prep, blocks, f.f32, f.x, f.M, f.C);
-  Matrix wg = take_matrix(w, prep, blocks, f.f32, f.wg, f.C, f.H);
-  Matrix wu = take_matrix(w, prep, blocks, f.f32, f.wu, f.C, f.H);
-  Matrix wd = take_matrix(w, prep, blocks, f.f32, f.wd, f.H, f.C);
-  Matrix gy = take_matrix(w, prep, blocks, f.f32, f.gy, f.M, f.C);
-  Matrix hidden = new_matrix(w, f.f32, f.M, f.H, 3);   // dg, du, h
+  Matrix x = take_matrix(w, prep, blocks, f, f.x, f.M, f.C);
+  Matrix wg = take_matrix(w, prep, blocks, f, f.wg, f.C, f.H);
+  Matrix wu = take_matrix(w, prep, blocks, f, f.wu, f.C, f.H);
+  Matrix wd = take_matrix(w, prep, blocks, f, f.wd, f.H, f.C);
+  Matrix gy = take_matrix(w, prep, blocks, f, f.gy, f.M, f.C);
+  Matrix hidden = new_matrix(w, f.pair, f.M, f.H, 3);   // dg, du, h
   const int64_t ld = up(f.H, 4);
   const int splits = weight_splits(f.M, f.C, f.H);
   float *partial = want_w && splits > 1 ? w.take<float>((int64_t)splits * 3 * f.C * ld) : nullptr;
-  const int x_splits = row_splits(f.f32, f.M, f.C, 2 * blocks64(f.H), 30000);
+  const int x_splits = row_splits(f.pair, f.M, f.C, 2 * blocks64(f.H), 30000);
   float *x_partial = want_x && x_splits > 1 ? w.take<float>(x_splits * f.M * up(f.C, 4)) : nullptr;
   if (!w.base) return CMACE_OK;
-  const bool bf16 = !f.f32;
+  const bool bf16 = !f.pair;
   int rc = run_prep(prep, blocks, f.st, f.what);
   if (!rc) rc = encode_all({&x, &wg, &wu, &wd, &gy, &hidden}, bf16, f.what);
   TpArgs g = new_args(f.M, f.H, f.status);
@@ -962,7 +975,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
       set_k(g, 0, f.M);
       if (!rc) rc = set_user_out(g, gw[0] ? gw[0] : gw[1], f.f32, f.C, f.H, f.what, 0);
       if (!rc && g.batches == 2) rc = set_user_out(g, gw[1], f.f32, f.C, f.H, f.what, 1);
-      if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
+      if (!rc) rc = launch_plain(f.pair, g, f.st, f.what);
     }
     if (gw[2]) {
       g = new_args(f.H, f.C, f.status);
@@ -970,7 +983,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
       set_operand(g.b[0], gy, false);
       set_k(g, 0, f.M);
       if (!rc) rc = set_user_out(g, gw[2], f.f32, f.H, f.C, f.what);
-      if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
+      if (!rc) rc = launch_plain(f.pair, g, f.st, f.what);
     }
   } else if (want_w) {
     // batches dg, du and h: x^T dg, x^T du and, as its transpose, dy^T h
@@ -984,7 +997,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
     set_k(g, 0, f.M);
     g.out[1].use_map = 1;
     if (!rc) rc = encode_tile_map(&g.out[1].map, partial, 4, false, f.H, f.C, (int64_t)splits * 3, ld, (int64_t)f.C * ld, 16, 32, f.what);
-    if (!rc) rc = launch_plain(f.f32, g, f.st, f.what);
+    if (!rc) rc = launch_plain(f.pair, g, f.st, f.what);
     WeightReduce r{partial, {gw[0], gw[1], gw[2]}, ld, splits, f.C, f.H};
     const dim3 grid((unsigned)((f.H + 31) / 32), (unsigned)((f.C + 31) / 32), 3);
     if (!rc) {
@@ -994,6 +1007,12 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
     }
   }
   return rc;
+}
+
+// bf16 rounds h, dg and du once more, which makes 1.4 times the error of a result that is rounded alone: on the mean.  Where an array has few values,
+// chance would make it more (128 hidden values, 300 of a gradient: 1.3 to 1.55), and all goes as pairs, like float32; that costs a kernel, 5 us.
+static bool as_pairs(bool f32, int64_t M, int C, int H, bool backward) {
+  return f32 || M * H <= 512 || M * C <= 1024 || (backward && (int64_t)C * H <= 1024);
 }
 
 static int check_sizes(const char *what, int64_t M, int C, int H, int act) {
@@ -1009,7 +1028,7 @@ static int run_forward(bool f32, const void *x, const void *wg, const void *wu, 
   if (M == 0) return CMACE_OK;
   if (!x || !wg || !wu || !wd || !y || !workspace) return fail(CMACE_ERR_ARG, "%s: null pointer", what);
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(CMACE_ERR_ARG, "%s: the workspace has to be aligned to 256 bytes", what);
-  FeedForward f{f32, x, wg, wu, wd, nullptr, M, C, H, act, status, (cudaStream_t)stream, what};
+  FeedForward f{f32, as_pairs(f32, M, C, H, false), x, wg, wu, wd, nullptr, M, C, H, act, status, (cudaStream_t)stream, what};
   Carve count{nullptr};
   forward(f, y, count);
   count.used = std::max<int64_t>(count.used, 256);   // what is asked for at least
@@ -1035,7 +1054,7 @@ static int run_backward(bool f32, const void *x, const void *wg, const void *wu,
   if (!gx && !want_w) return CMACE_OK;
   if (!x || !wg || !wu || !wd || !gy || !workspace) return fail(CMACE_ERR_ARG, "%s: null pointer", what);
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(CMACE_ERR_ARG, "%s: the workspace has to be aligned to 256 bytes", what);
-  FeedForward f{f32, x, wg, wu, wd, gy, M, C, H, act, status, st, what};
+  FeedForward f{f32, as_pairs(f32, M, C, H, true), x, wg, wu, wd, gy, M, C, H, act, status, st, what};
   Carve count{nullptr};
   backward(f, gx, gw, gx != nullptr, want_w, count);
   if (bytes < count.used) return fail(CMACE_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes, (long long)count.used);
@@ -1055,7 +1074,7 @@ int64_t cmace_gated_ff_workspace_bytes(int is_f32, int64_t rows, int width, int 
   if (check_sizes("cmace_gated_ff_workspace_bytes", rows, width, hidden, TP_SILU)) return -1;
   if (rows == 0) return 256;
   // addresses are not known here: room for copies of all arrays of a width that is not a multiple of eight, and of those that are
-  FeedForward f{is_f32 != 0, (const void *)1, (const void *)1, (const void *)1, (const void *)1, (const void *)1, rows, width, hidden, TP_SILU, nullptr, nullptr, ""};
+  FeedForward f{is_f32 != 0, as_pairs(is_f32 != 0, rows, width, hidden, backward_pass != 0), (const void *)1, (const void *)1, (const void *)1, (const void *)1, (const void *)1, rows, width, hidden, TP_SILU, nullptr, nullptr, ""};
   Carve count{nullptr};
   void *const none[3] = {nullptr, nullptr, nullptr};
   if (backward_pass) backward(f, nullptr, none, true, true, count);

@@ -504,3 +504,27 @@ def test_sums_over_many_hidden_columns(M, C, H, dtype, dev):
     for name, a, b in zip(("y", "x", "w_gate", "w_up", "w_down"), got, again):
         inside(a, want[name])
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("M,C,H", [(1, 64, 128), (1, 300, 17), (9, 130, 56), (3, 352, 170), (16, 200, 32), (8, 33, 63), (2, 1024, 256), (9, 36, 2931), (1, 1000, 1500)])
+def test_few_hidden_values_bfloat16(M, C, H, activation, dev):
+    """Few hidden values are not rounded to bfloat16 between the products: every result is off by its own rounding and float32's part."""
+    t = case(M + C + H + 3, M, C, H, BF16, dev)
+    got = run_all(*t, activation)
+    want = reference(*(v.double() for v in t), activation, F32)
+    for name, a in zip(("y", "x", "w_gate", "w_up", "w_down"), got):
+        v, bound = want[name]
+        inside(a, (v, bound + 2.0 ** -8 * (v.abs() + bound)))
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("M,C,H", [(5000, 16, 24), (700, 32, 32)])
+def test_gradients_of_few_weights_bfloat16(M, C, H, activation, dev):
+    """Neither are they where the weights are few, for the gradients (the forward pass may)."""
+    t = case(M + C + H + 4, M, C, H, BF16, dev)
+    got = run_all(*t, activation)
+    want = reference(*(v.double() for v in t), activation, F32)
+    for name, a in zip(("x", "w_gate", "w_up", "w_down"), got[1:]):
+        v, bound = want[name]
+        inside(a, (v, bound + 2.0 ** -8 * (v.abs() + bound)))

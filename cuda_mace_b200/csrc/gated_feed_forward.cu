@@ -8,9 +8,9 @@
 //             dWg = x^T dg, dWu = x^T du, dWd = h^T dy    one launch of three products over M, split where M is long
 // What bounds them (B200, us alone, cold): widths 1 024 and 4 096, 8 192 rows of bf16: the gated kernel 88 (1 560 TFLOP/s), h Wd 52, the
 // backward's hidden values 178 (1 160: 56 bytes of operands for 48 of products a cycle, and 200 MB put down), dx 96, dW 97 + 51; float32 as
-// pairs: 300, 152, 550, 300, 305 + 148 (1 350 to 1 450 TFLOP/s of fp16 products).  Widths 128 and 512, 64 000 rows: K is two blocks
-// long, so the elementwise epilogue bounds the first and third: 30, 17, 68, 27, 37 in bf16, 61, 31, 150, 52, 74 in float32, where h goes out
-// at 2.1 and h, dg, du at 2.6 TB/s.
+// pairs: 283, 152, 540, 298, 306 + 149 (1 350 to 1 450 TFLOP/s of fp16 products), operands 37 before the first and 71 before the third.  Widths
+// 128 and 512, 64 000 rows: K is two blocks long, so the elementwise epilogue bounds the first and third: 30, 17, 68, 27, 37 in bf16, 63, 32, 149, 54,
+// 74 in float32, where h goes out at 2.1 and h, dg, du at 2.6 TB/s; operands take 14 before the first and 54 before the third.
 // Only x and the weights are kept for the backward: forming g and u again costs 4 M C H operations, keeping them in float32 16 bytes
 // a hidden value written and read (what would be as exact as the products are), which pays from C of about 1 000 only.
 //
@@ -35,89 +35,215 @@ struct PrepJob {
   int64_t rows, first; // first block of this job
   int cols, ld, blocks_n, bf16;   // bf16: of the source of a pair
 };
+// Rows of x, and going back of dL/dy, as pairs.  A block of 64 x 64 values has one scale, under which a row 2^-40 of the largest is zeros, and
+// h goes with the square of a small row.  So the rows of 64 are brought to the size of their largest before they are split, each by a
+// power of two: x~ = x / s, dy~ = dy / t with s, t <= 1 of the row.  A product's rows follow, and what is linear in them: h~ = h / s^2 = g~ sigmoid(g~ s) u~ (SiLU),
+// dg~ = dg / (s t), du~ = du / (s t); y = (h~ Wd) s^2 and dx = (..) s t at the end.  A sum over rows has each at the size of its
+// contribution: dWg = (x s t)^T dg~, dWu = (x s t)^T du~, dWd = h~^T (dy s^2), for which x and dy are laid out a second time.
+struct RowsJob {
+  const void *src[2];   // x, dy or null
+  __half *hi[4];        // x~, dy~, x s t, dy s^2 (null: not wanted), the lo parts a plane behind
+  float *scale[4], *size[2];   // inverse scales of the blocks; s and t, ones behind the last row up to a multiple of 256
+  float *most[2];       // largest finite magnitudes of the rows' slabs, [slabs][rows]; null: x alone, of up to two blocks of columns, which a CTA has whole
+  int64_t rows, plane, blocks;   // blocks: CTAs
+  int cols, ld, blocks_n, bf16, wide, sources, slabs, slab;   // slab: columns
+};
 struct PrepArgs {
   PrepJob job[5];
+  RowsJob rows;
   int jobs;
 };
 constexpr int PREP_THREADS = 256;
 
-// One block of 64 x 64 values a CTA: a thread takes four columns of every 16th row, or one column of every 4th.
-__global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const __grid_constant__ PrepArgs p) {
-  __shared__ float most_of[PREP_THREADS / 32];
+// Four values of a row, zeros for those that are not among the n that it still has.  wide: rows start on 16 bytes.
+__device__ __forceinline__ float4 prep_load(const void *src, int64_t at, int n, bool bf16, bool wide) {
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (wide) {
+    if (n > 0) x = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(src) + at));
+  } else if (bf16) {
+    const __nv_bfloat16 *s = static_cast<const __nv_bfloat16 *>(src) + at;
+    if (n > 0) x.x = __bfloat162float(s[0]);
+    if (n > 1) x.y = __bfloat162float(s[1]);
+    if (n > 2) x.z = __bfloat162float(s[2]);
+    if (n > 3) x.w = __bfloat162float(s[3]);
+  } else {
+    const float *s = static_cast<const float *>(src) + at;
+    if (n > 0) x.x = __ldg(s);
+    if (n > 1) x.y = __ldg(s + 1);
+    if (n > 2) x.z = __ldg(s + 2);
+    if (n > 3) x.w = __ldg(s + 3);
+  }
+  return x;
+}
+__device__ __forceinline__ float prep_most(float4 x) {
+  return fmaxf(fmaxf(tp_finite_abs(x.x), tp_finite_abs(x.y)), fmaxf(tp_finite_abs(x.z), tp_finite_abs(x.w)));
+}
+__device__ __forceinline__ float4 times(float4 x, float f) { return make_float4(x.x * f, x.y * f, x.z * f, x.w * f); }
+
+constexpr int PREP_SLABS = 16;
+// A thread has four columns of every 16th row of a block of 64 x 64.
+struct PrepThread {
+  int64_t row0;
+  int first, in, n;   // its first row and column, rows of the block
+  __device__ __forceinline__ PrepThread(int64_t row0, int64_t rows)
+      : row0(row0), first(threadIdx.x >> 4), in(4 * (threadIdx.x & 15)), n((int)(rows - row0 < 64 ? rows - row0 : 64)) {}
+  __device__ __forceinline__ void fetch(float4 (&x)[4], const void *src, int col, int cols, bool bf16, bool wide) const {
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = prep_load(src, (row0 + first + 16 * i) * cols + col, first + 16 * i < n ? cols - col : 0, bf16, wide);
+  }
+};
+__device__ __forceinline__ void prep_row_most(float (&most)[4]) {   // of the 16 lanes that have a row
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], d));
+}
+
+// Largest finite magnitudes of 64 rows' slabs of columns
+__global__ void __launch_bounds__(PREP_THREADS) row_most_kernel(const RowsJob R) {
   grid_begin();
+  const PrepThread T((int64_t)blockIdx.x * 64, R.rows);
+  const int k = blockIdx.z, end = min(R.cols, (int)(blockIdx.y + 1) * R.slab);
+  float most[4] = {};
+#pragma unroll 4
+  for (int col = (int)blockIdx.y * R.slab + T.in; col < end; col += 64) {
+    float4 x[4];
+    T.fetch(x, R.src[k], col, R.cols, R.bf16, R.wide);
+#pragma unroll
+    for (int i = 0; i < 4; i++) most[i] = fmaxf(most[i], prep_most(x[i]));
+  }
+  prep_row_most(most);
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (T.in == 0 && T.first + 16 * i < T.n) R.most[k][blockIdx.y * R.rows + T.row0 + T.first + 16 * i] = most[i];
+}
+
+// COPY: 64 x 64 bf16 values.  Otherwise pairs: a block of a weight, or of 64 rows of x the whole (WHOLE), or one block of x or dy.
+enum PrepKind { PREP_COPY, PREP_WHOLE, PREP_BLOCKS };
+template <int KIND>
+__global__ void __launch_bounds__(PREP_THREADS, KIND == PREP_COPY ? 8 : KIND == PREP_WHOLE ? 4 : 5) prep_kernel(const __grid_constant__ PrepArgs p) {
+  constexpr int NB = KIND == PREP_WHOLE ? 2 : 1;       // blocks of a CTA
+  __shared__ float most_of[NB][2][PREP_THREADS / 32];   // of both layouts
+  __shared__ int top_of[2][PREP_THREADS / 32];
+  grid_begin();
+  const RowsJob &R = p.rows;
+  const bool rows = KIND != PREP_COPY && (int64_t)blockIdx.x < R.blocks;
   int j = 0;
   while (j + 1 < p.jobs && (int64_t)blockIdx.x >= p.job[j + 1].first) j++;
   const PrepJob &J = p.job[j];
-  const int64_t b = blockIdx.x - J.first;
-  const int64_t rb = b / J.blocks_n;
-  const int cb = (int)(b - rb * J.blocks_n);
-  const int64_t row0 = rb * 64;
-  const int col0 = cb * 64, t = threadIdx.x;
-  if (J.lo == nullptr) {
+  const int across = rows ? (KIND == PREP_WHOLE ? 1 : R.blocks_n * R.sources) : J.blocks_n, t = threadIdx.x;
+  const int64_t b = rows ? blockIdx.x : blockIdx.x - J.first, rb = b / across;
+  int cb = (int)(b - rb * across);
+  if constexpr (KIND == PREP_COPY) {
     const uint16_t *s = static_cast<const uint16_t *>(J.src);
     uint16_t *d = static_cast<uint16_t *>(J.hi);
-    const int col = col0 + (t & 63);
+    const int64_t row0 = rb * 64;
+    const int col = 64 * cb + (t & 63);
     if (col < J.cols)
       for (int r = t >> 6; r < 64 && row0 + r < J.rows; r += 4) d[(row0 + r) * J.ld + col] = s[(row0 + r) * J.cols + col];
     return;
   }
-  const float *s = static_cast<const float *>(J.src);
-  const bool wide = (J.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(J.src) & 15) == 0 && !J.bf16;
-  float v[16];
-  float most = 0.f;
-  if (wide) {
-    const int col = col0 + 4 * (t & 15);
+  const int k = KIND == PREP_BLOCKS && rows && R.sources == 2 ? cb & 1 : 0;   // x or dy
+  if (KIND == PREP_BLOCKS && rows && R.sources == 2) cb >>= 1;
+  const PrepThread T(rb * 64, rows ? R.rows : J.rows);
+  const int warp = t >> 5, cols = rows ? R.cols : J.cols, ld = rows ? R.ld : J.ld, blocks = KIND == PREP_WHOLE && rows ? R.blocks_n : 1;
+  const bool bf16 = rows ? R.bf16 : J.bf16, wide = rows ? R.wide : (cols & 3) == 0 && (reinterpret_cast<uintptr_t>(J.src) & 15) == 0 && !bf16;
+  float4 x[NB][4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int64_t r = row0 + (t >> 4) + 16 * i;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < J.rows && col < J.cols) x = __ldg(reinterpret_cast<const float4 *>(s + r * J.cols + col));
-      v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
-    }
-  } else {
-    const int col = col0 + (t & 63);
+  for (int e = 0; e < NB; e++)
+    if (e < blocks) T.fetch(x[e], rows ? R.src[k] : J.src, 64 * (cb + e) + T.in, cols, bf16, wide);
+  // The sizes of this thread's rows, its own ([0]) and the other source's, by the exponents of the rows' largest finite values (a
+  // subnormal's counts as -127)
+  constexpr int NONE = -0x7FFFFFFF;
+  int below[2][4] = {};   // exponents, then how far below the group's largest (126 at most); NONE: a row of zeros
+  const auto exp2i = [](int e) { return __uint_as_float((uint32_t)(e + 127) << 23); };   // -126 <= e <= 127
+  if (rows) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const int64_t r = row0 + (t >> 6) + 4 * i;
-      if (J.bf16) v[i] = r < J.rows && col < J.cols ? __bfloat162float(static_cast<const __nv_bfloat16 *>(J.src)[r * J.cols + col]) : 0.f;
-      else v[i] = r < J.rows && col < J.cols ? __ldg(s + r * J.cols + col) : 0.f;
+    for (int o = 0; o < (KIND == PREP_WHOLE ? 1 : 2); o++) {
+      if (o >= R.sources) break;
+      float most[4] = {};
+      if constexpr (KIND == PREP_WHOLE) {
+#pragma unroll
+        for (int e = 0; e < NB; e++) {
+          if (e >= blocks) break;
+#pragma unroll
+          for (int i = 0; i < 4; i++) most[i] = fmaxf(most[i], prep_most(x[e][i]));
+        }
+      } else if ((t & 15) < R.slabs) {
+        const float *from = R.most[o ? 1 - k : k] + (t & 15) * R.rows + T.row0 + T.first;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (T.first + 16 * i < T.n) most[i] = __ldcg(from + 16 * i);
+      }
+      prep_row_most(most);
+      int top = NONE;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        below[o][i] = most[i] == 0.f ? NONE : (int)(__float_as_uint(most[i]) >> 23) - 127;
+        top = max(top, below[o][i]);
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if ((t & 31) == 0) top_of[o][warp] = top;
     }
+    __syncthreads();
+#pragma unroll
+    for (int o = 0; o < (KIND == PREP_WHOLE ? 1 : 2); o++) {
+      if (o >= R.sources) break;
+      int top = NONE;
+#pragma unroll
+      for (int w = 0; w < PREP_THREADS / 32; w++) top = max(top, top_of[o][w]);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (below[o][i] != NONE) below[o][i] = min(top - below[o][i], 126);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (cb == 0 && T.in == 0 && T.first + 16 * i < T.n) R.size[k][T.row0 + T.first + 16 * i] = below[0][i] == NONE ? 1.f : exp2i(-below[0][i]);
+    if (cb == 0 && T.row0 + 64 >= R.rows && R.rows + t < (R.rows + 255) / 256 * 256) R.size[k][R.rows + t] = 1.f;
   }
-  most = tp_most(v);
-  most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-  if ((t & 31) == 0) most_of[t >> 5] = most;
+  // At the group's size, and as a contribution: x s t or dy s^2.  A row of zeros contributes nothing, whatever the other has.
+  const auto value = [&](const float4 &v, int how, int i) {
+    const int own = below[0][i], other = below[1][i];
+    if (how == 0) return times(v, own == NONE ? 1.f : exp2i(own));
+    const float of_own = own == NONE ? 0.f : exp2i(-own), of_other = other == NONE ? 0.f : exp2i(-other);
+    return times(times(v, k ? of_other : of_own), of_other);
+  };
+  __half *const hi[2] = {rows ? R.hi[k] : static_cast<__half *>(J.hi), KIND == PREP_BLOCKS && rows ? R.hi[2 + k] : nullptr};
+#pragma unroll
+  for (int e = 0; e < NB; e++)
+#pragma unroll
+    for (int how = 0; how < 2; how++) {
+      if (e >= blocks || !hi[how]) continue;
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) most = fmaxf(most, prep_most(value(x[e][i], how, i)));
+      most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+      if ((t & 31) == 0) most_of[e][how][warp] = most;
+    }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < PREP_THREADS / 32; w++) most = fmaxf(most, most_of[w]);
-  const float scale = tp_scale(most);
-  if (t == 0) J.scale[b] = 1.0f / scale;
-  __half *hi = static_cast<__half *>(J.hi), *lo = static_cast<__half *>(J.lo);
-  if (wide) {
-    const int col = col0 + 4 * (t & 15);
-    if (col >= J.cols) return;
+  for (int e = 0; e < NB; e++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int64_t r = row0 + (t >> 4) + 16 * i;
-      if (r >= J.rows) break;
-      uint2 h, l;
-      tp_split2(v[4 * i], v[4 * i + 1], scale, h.x, l.x);
-      tp_split2(v[4 * i + 2], v[4 * i + 3], scale, h.y, l.y);
-      *reinterpret_cast<uint2 *>(hi + r * J.ld + col) = h;
-      *reinterpret_cast<uint2 *>(lo + r * J.ld + col) = l;
-    }
-  } else {
-    const int col = col0 + (t & 63);
-    if (col >= J.cols) return;
+    for (int how = 0; how < 2; how++) {
+      if (e >= blocks || !hi[how]) continue;
+      float most = most_of[e][how][0];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const int64_t r = row0 + (t >> 6) + 4 * i;
-      if (r >= J.rows) break;
-      uint32_t h, l;
-      tp_split2(v[i], 0.f, scale, h, l);
-      hi[r * J.ld + col] = __ushort_as_half((unsigned short)h);
-      lo[r * J.ld + col] = __ushort_as_half((unsigned short)l);
+      for (int w = 1; w < PREP_THREADS / 32; w++) most = fmaxf(most, most_of[e][how][w]);
+      const float scale = tp_scale(most);
+      if (t == 0) (rows ? R.scale[2 * how + k] + rb * R.blocks_n + cb + e : J.scale + b)[0] = 1.0f / scale;
+      const int col = 64 * (cb + e) + T.in;
+      __half *const to = hi[how] + (T.row0 + T.first) * ld + col, *const to_lo = to + (rows ? R.plane : static_cast<__half *>(J.lo) - hi[how]);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if (T.first + 16 * i >= T.n || col >= cols) break;   // columns up to the rows' distance, a multiple of eight, take zeros
+        const float4 v = value(x[e][i], how, i);
+        uint2 h, l;
+        tp_split2(v.x, v.y, scale, h.x, l.x);
+        tp_split2(v.z, v.w, scale, h.y, l.y);
+        *reinterpret_cast<uint2 *>(to + (int64_t)(16 * i) * ld) = h;
+        *reinterpret_cast<uint2 *>(to_lo + (int64_t)(16 * i) * ld) = l;
+      }
     }
-  }
 }
 
 // ---- few rows: a pass over the weights -------------------------------------------------------------------------------------------
@@ -706,6 +832,36 @@ static Matrix take_matrix(Carve &w, PrepArgs &prep, int64_t &blocks, const FeedF
   blocks += m.blocks_m() * m.blocks_n();
   return m;
 }
+// Rows as pairs, brought to one size, the first of the launch's jobs; and as contributions to sums over rows.
+struct TakenRows {
+  Matrix x, gy, x_sum, gy_sum;
+  float *s = nullptr, *t = nullptr;
+};
+static TakenRows take_rows(Carve &w, PrepArgs &prep, int64_t &blocks, const FeedForward &f, bool x_sum, bool gy_sum) {
+  TakenRows r;
+  RowsJob &j = prep.rows;
+  const bool back = f.gy != nullptr;
+  Matrix *const all[4] = {&r.x, &r.gy, &r.x_sum, &r.gy_sum};
+  const bool wanted[4] = {true, back, x_sum, gy_sum};
+  r.s = w.take<float>(up(f.M, 256));
+  if (back) r.t = w.take<float>(up(f.M, 256));
+  for (int o = 0; o < 4; o++)
+    if (wanted[o]) {
+      *all[o] = new_matrix(w, true, f.M, f.C, 1);
+      j.hi[o] = reinterpret_cast<__half *>(all[o]->at), j.scale[o] = all[o]->scale;
+    }
+  j.src[0] = f.x, j.src[1] = f.gy, j.size[0] = r.s, j.size[1] = r.t, j.sources = back ? 2 : 1;
+  j.rows = f.M, j.cols = f.C, j.plane = r.x.plane(), j.ld = (int)r.x.ld, j.blocks_n = (int)r.x.blocks_n(), j.bf16 = !f.f32;
+  j.wide = f.f32 && f.C % 4 == 0 && aligned16(f.x) && (!back || aligned16(f.gy));
+  j.blocks = r.x.blocks_m();
+  if (back || j.blocks_n > 2) {   // sizes by a kernel of their own
+    j.slab = (int)up(std::max(256, (f.C + PREP_SLABS - 1) / PREP_SLABS), 64), j.slabs = (f.C + j.slab - 1) / j.slab;
+    for (int k = 0; k < j.sources; k++) j.most[k] = w.take<float>(j.slabs * f.M);
+    j.blocks *= j.blocks_n * j.sources;
+  }
+  blocks += j.blocks;
+  return r;
+}
 static int encode_all(std::initializer_list<Matrix *> all, bool bf16, const char *what) {
   for (Matrix *m : all)
     if (const int rc = encode_matrix(&m->map, *m, 64, 64, bf16, what)) return rc;
@@ -793,7 +949,11 @@ static int launch_rows(const FeedForward &f, TpArgs &g, void *out, int splits, f
 static int run_prep(const PrepArgs &p, int64_t blocks, cudaStream_t st, const char *what) {
   if (blocks == 0) return CMACE_OK;
   if (blocks >= (int64_t)1 << 31) return fail(CMACE_ERR_UNSUPPORTED, "%s: too many rows", what);
-  launch_chained(prep_kernel, dim3((unsigned)blocks), dim3(PREP_THREADS), (size_t)0, st, p);
+  if (p.rows.slabs)
+    launch_chained(row_most_kernel, dim3((unsigned)((p.rows.rows + 63) / 64), (unsigned)p.rows.slabs, (unsigned)p.rows.sources), dim3(PREP_THREADS), (size_t)0,
+                   st, p.rows);
+  const auto kernel = !p.rows.blocks ? prep_kernel<PREP_COPY> : p.rows.slabs ? prep_kernel<PREP_BLOCKS> : prep_kernel<PREP_WHOLE>;
+  launch_chained(kernel, dim3((unsigned)blocks), dim3(PREP_THREADS), (size_t)0, st, p);
   return check_launch(what);
 }
 
@@ -898,7 +1058,10 @@ static int forward(const FeedForward &f, void *y, Carve &w) {
   PrepArgs prep;
   memset(&prep, 0, sizeof(prep));
   int64_t blocks = 0;
-  Matrix x = take_matrix(w, prep, blocks, f, f.x, f.M, f.C);
+  TakenRows rows;
+  if (f.pair) rows = take_rows(w, prep, blocks, f, false, false);
+  else rows.x = take_matrix(w, prep, blocks, f, f.x, f.M, f.C);
+  Matrix &x = rows.x;
   Matrix wg = take_matrix(w, prep, blocks, f, f.wg, f.C, f.H);
   Matrix wu = take_matrix(w, prep, blocks, f, f.wu, f.C, f.H);
   Matrix wd = take_matrix(w, prep, blocks, f, f.wd, f.H, f.C);
@@ -914,12 +1077,14 @@ static int forward(const FeedForward &f, void *y, Carve &w) {
   set_operand(g.b[0], wg, false);
   set_operand(g.b[1], wu, false);
   set_k(g, 0, f.C);
+  g.row_size[0] = rows.s;
   if (!rc) rc = set_hidden_out(g, h, 32, bf16, f.what);
   if (!rc) rc = f.act == TP_SILU ? launch_gated<TP_SILU>(f, g) : launch_gated<TP_GELU>(f, g);
   g = new_args(f.M, f.C, f.status);
   set_operand(g.a[0], h, true);
   set_operand(g.b[0], wd, false);
   set_k(g, 0, f.H);
+  g.row_size[0] = g.row_size[1] = rows.s;
   if (!rc) rc = launch_rows(f, g, y, splits, partial);
   return rc;
 }
@@ -928,11 +1093,18 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   PrepArgs prep;
   memset(&prep, 0, sizeof(prep));
   int64_t blocks = 0;
-  Matrix x = take_matrix(w, prep, blocks, f, f.x, f.M, f.C);
+  TakenRows rows;
+  const bool sum_x = want_w && (!w.base || gw[0] || gw[1]), sum_gy = want_w && (!w.base || gw[2]);   // when counting: room for both
+  if (f.pair) {
+    rows = take_rows(w, prep, blocks, f, sum_x, sum_gy);
+  } else {
+    rows.x_sum = rows.x = take_matrix(w, prep, blocks, f, f.x, f.M, f.C);
+    rows.gy_sum = rows.gy = take_matrix(w, prep, blocks, f, f.gy, f.M, f.C);
+  }
+  Matrix &x = rows.x, &gy = rows.gy, &x_sum = rows.x_sum, &gy_sum = rows.gy_sum;
   Matrix wg = take_matrix(w, prep, blocks, f, f.wg, f.C, f.H);
   Matrix wu = take_matrix(w, prep, blocks, f, f.wu, f.C, f.H);
   Matrix wd = take_matrix(w, prep, blocks, f, f.wd, f.H, f.C);
-  Matrix gy = take_matrix(w, prep, blocks, f, f.gy, f.M, f.C);
   Matrix hidden = new_matrix(w, f.pair, f.M, f.H, 3);   // dg, du, h
   const int64_t ld = up(f.H, 4);
   const int splits = weight_splits(f.M, f.C, f.H);
@@ -943,6 +1115,12 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   const bool bf16 = !f.pair;
   int rc = run_prep(prep, blocks, f.st, f.what);
   if (!rc) rc = encode_all({&x, &wg, &wu, &wd, &gy, &hidden}, bf16, f.what);
+  if (f.pair) {
+    if (!rc && sum_x) rc = encode_all({&x_sum}, bf16, f.what);
+    if (!rc && sum_gy) rc = encode_all({&gy_sum}, bf16, f.what);
+  } else {
+    x_sum.map = x.map, gy_sum.map = gy.map;
+  }
   TpArgs g = new_args(f.M, f.H, f.status);
   set_operand(g.a[0], x, true);
   set_operand(g.a[1], gy, true);
@@ -952,6 +1130,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   g.segments = 2;
   set_k(g, 0, f.C);
   set_k(g, 1, f.C);
+  g.row_size[0] = rows.s;
   if (!rc) rc = set_hidden_out(g, hidden, 16, bf16, f.what);
   if (!rc) rc = f.act == TP_SILU ? launch_back<TP_SILU>(f, g) : launch_back<TP_GELU>(f, g);
   if (want_x) {
@@ -963,12 +1142,13 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
     g.segments = 2;
     set_k(g, 0, f.H);
     set_k(g, 1, f.H);
+    g.row_size[0] = rows.s, g.row_size[1] = rows.t;
     if (!rc) rc = launch_rows(f, g, gx, x_splits, x_partial);
   }
   if (want_w && splits == 1) {
     if (gw[0] || gw[1]) {
       g = new_args(f.C, f.H, f.status);
-      set_operand(g.a[0], x, false);
+      set_operand(g.a[0], x_sum, false);
       set_operand(g.b[0], gw[0] && gw[1] ? hidden : hidden.part(gw[0] ? 0 : 1), false);
       g.batches = gw[0] && gw[1] ? 2 : 1;
       g.out_of_batch = 1;
@@ -980,7 +1160,7 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
     if (gw[2]) {
       g = new_args(f.H, f.C, f.status);
       set_operand(g.a[0], hidden.part(2), false);
-      set_operand(g.b[0], gy, false);
+      set_operand(g.b[0], gy_sum, false);
       set_k(g, 0, f.M);
       if (!rc) rc = set_user_out(g, gw[2], f.f32, f.H, f.C, f.what);
       if (!rc) rc = launch_plain(f.pair, g, f.st, f.what);
@@ -988,8 +1168,8 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
   } else if (want_w) {
     // batches dg, du and h: x^T dg, x^T du and, as its transpose, dy^T h
     g = new_args(f.C, f.H, f.status);
-    set_operand(g.a[0], x, false);
-    set_operand(g.a[1], gy, false);
+    set_operand(g.a[0], sum_x ? x_sum : gy_sum, false);   // one that is not wanted: any, its sums go nowhere
+    set_operand(g.a[1], sum_gy ? gy_sum : x_sum, false);
     set_operand(g.b[0], hidden, false);
     g.batches = 3;
     g.splits = splits;
@@ -1074,7 +1254,7 @@ int64_t cmace_gated_ff_workspace_bytes(int is_f32, int64_t rows, int width, int 
   if (check_sizes("cmace_gated_ff_workspace_bytes", rows, width, hidden, TP_SILU)) return -1;
   if (rows == 0) return 256;
   // addresses are not known here: room for copies of all arrays of a width that is not a multiple of eight, and of those that are
-  FeedForward f{is_f32 != 0, as_pairs(is_f32 != 0, rows, width, hidden, backward_pass != 0), (const void *)1, (const void *)1, (const void *)1, (const void *)1, (const void *)1, rows, width, hidden, TP_SILU, nullptr, nullptr, ""};
+  FeedForward f{is_f32 != 0, as_pairs(is_f32 != 0, rows, width, hidden, backward_pass != 0), (const void *)1, (const void *)1, (const void *)1, (const void *)1, backward_pass ? (const void *)1 : nullptr, rows, width, hidden, TP_SILU, nullptr, nullptr, ""};
   Carve count{nullptr};
   void *const none[3] = {nullptr, nullptr, nullptr};
   if (backward_pass) backward(f, nullptr, none, true, true, count);

@@ -13,7 +13,8 @@
 //  * PAIR: float32 values as two fp16 values, x = (hi + lo) / scale, hi and lo rounded to nearest: at most 2^-22 |x| off, about 2^-24
 //    on the average.  Three MMAs a k step (lo hi, hi lo, hi hi; lo lo is below 2^-22 of hi hi).  fp16 lacks float32's range, so
 //    every block of 64 x 64 values has a power of two of its own, from the block's largest value: within a block the precision
-//    holds over 2^18 below that value and degrades to an absolute 2^-39 of it beyond.  A block of 64 k is one chunk: its sum goes
+//    holds over 2^18 below that value and degrades to an absolute 2^-39 of it beyond (rows of a caller's array are brought to one size
+//    first, row_size).  A block of 64 k is one chunk: its sum goes
 //    to its own accumulator columns and the epilogue warps add it, times the two blocks' scales, to float32 registers, rounding to
 //    nearest.  That also keeps the tensor core's own accumulation, which truncates, to 12 instructions: summed in tensor
 //    memory over K = 512, three terms of it are off by 4e-6 of the largest value; in chunks all sums come out smaller by 2.0e-7 (terms of
@@ -82,6 +83,7 @@ struct TpArgs {
   int64_t out_scale_ld, out_scale_batch;
   CUtensorMap cin;               // POLY: S, APPLY: X, in boxes of 32 rows of a warp's columns; batch b is hi 2 b and lo 2 b + 1
   float alpha, beta, pair_scale;   // D = alpha * product + beta * cin, times pair_scale where D is a pair
+  const float *row_size[2];        // PAIR: powers of two that A's rows were brought to one size by, [rows up to a multiple of 256]; PLAIN: null: none
   int32_t *status;
   int64_t rows, cols;            // of the output
   int kblocks[2], segments;      // blocks of 64 k a segment
@@ -297,16 +299,17 @@ __device__ __forceinline__ float tp_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float tp_sigmoid(float x) {
+// of x times a power of two, which goes into the constant
+__device__ __forceinline__ float tp_sigmoid(float x, float size) {
   float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + tp_ex2(-1.4426950408889634f * x)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + tp_ex2(-1.4426950408889634f * size * x)));
   return y;
 }
 // Cumulative normal distribution by formula 7.1.26 of Abramowitz and Stegun's Handbook (after Hastings): erfc(z) = e^(-z^2) times a polynomial
 // of 1 / (1 + p z), to 1.5e-7, without a branch and without the cancellation of 1 + erf far below zero.  e: e^(-g^2 / 2), which the derivative
 // takes as well.  (erff: two ways for small and large arguments, which the lanes of a warp both go.)
-__device__ __forceinline__ float tp_normal_cdf(float g, float &e) {
-  const float z = fabsf(g) * 0.70710678118654752f;
+__device__ __forceinline__ float tp_normal_cdf(float g, float size, float &e) {
+  const float z = fabsf(g) * (0.70710678118654752f * size);
   float t;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f, z, 1.0f)));
   e = tp_ex2(-1.4426950408889634f * z * z);
@@ -314,26 +317,27 @@ __device__ __forceinline__ float tp_normal_cdf(float g, float &e) {
   const float tail = 0.5f * poly * e;
   return g < 0.f ? tail : 1.0f - tail;   // NaN stays NaN
 }
-// act(g); with the derivative
+// act(x) / x of x = g size, size a power of two; with act'(x)
 template <int ACT>
-__device__ __forceinline__ float tp_act(float g) {
-  if (ACT == TP_SILU) return g * tp_sigmoid(g);
+__device__ __forceinline__ float tp_gate(float g, float size) {
+  if (ACT == TP_SILU) return tp_sigmoid(g, size);
   float e;
-  return g * tp_normal_cdf(g, e);
+  return tp_normal_cdf(g, size, e);
 }
 template <int ACT>
-__device__ __forceinline__ float tp_act(float g, float &d) {
+__device__ __forceinline__ float tp_gate(float g, float size, float &d) {
   if (ACT == TP_SILU) {
-    const float s = tp_sigmoid(g);
-    const float a = g * s;
-    d = s * (1.0f + (g - a));
-    return a;
+    const float s = tp_sigmoid(g, size);
+    d = s * fmaf(size, g - g * s, 1.0f);
+    return s;
   }
   float e;
-  const float cdf = tp_normal_cdf(g, e);
-  d = cdf + 0.39894228040143268f * g * e;
-  return g * cdf;
+  const float cdf = tp_normal_cdf(g, size, e);
+  d = cdf + 0.39894228040143268f * size * g * e;
+  return cdf;
 }
+template <int ACT>
+__device__ __forceinline__ float tp_act(float g) { return g * tp_gate<ACT>(g, 1.f); }
 
 // ---- an epilogue warp's stores ------------------------------------------------------------------------------------------
 struct TpStager {
@@ -711,6 +715,13 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       constexpr bool CIN = KIND == TP_POLY || KIND == TP_APPLY;
       constexpr uint32_t LOW = 32 * S::PART * 2;   // bytes from a warp's hi to its lo
       const bool here = row < g.rows && col0 < g.cols;
+      // of this lane's row: known long before the sums are
+      float size[2] = {1.f, 1.f};   // PAIR alone has others
+      if constexpr (PAIR && (KIND == TP_GATED || KIND == TP_BACK)) {
+        size[0] = __ldcg(g.row_size[0] + (uint32_t)row + lane);
+      } else if constexpr (PAIR && KIND == TP_PLAIN) {
+        if (g.row_size[0]) size[0] = __ldcg(g.row_size[0] + (uint32_t)row + lane), size[1] = __ldcg(g.row_size[1] + (uint32_t)row + lane);
+      }
       if (CIN && here && t != first_tile) {   // the first tile's: by the thread that issues the copies
         if (elect_one()) {
           tma_store_wait_read();
@@ -768,7 +779,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
       const auto take = [&](int i, float (&v)[16]) {
         if (PAIR) {
 #pragma unroll
-          for (int j = 0; j < 16; j++) v[j] = acc[PAIR ? i : 0][j];
+          for (int j = 0; j < 16; j++) v[j] = KIND == TP_PLAIN ? acc[PAIR ? i : 0][j] * size[0] * size[1] : acc[PAIR ? i : 0][j];
         } else {
           uint32_t u[16];
           tmem_ld16_nowait(at + column(i) + (S::LATE && i >= SEG0_GROUPS ? 128u * (uint32_t)buf : 0u), u);
@@ -784,7 +795,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < EACH; i++) {
 #pragma unroll
-            for (int j = 0; j < 16; j++) acc[i][j] = tp_act<ACT>(acc[i][j]) * acc[PAIR ? EACH + i : 0][j];
+            for (int j = 0; j < 16; j++) acc[i][j] = acc[i][j] * tp_gate<ACT>(acc[i][j], size[0]) * acc[PAIR ? EACH + i : 0][j];
             most = tp_most(acc[i], most);
           }
           // a block of 64 x 64 values is two quarters' and two parts' warps'
@@ -818,7 +829,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           st.send(&g.out[0].map, 0, col0, row, 0);
         }
       } else if constexpr (KIND == TP_BACK) {
-        // h = act(g) u, dL/dg = dL/dh u act'(g), dL/du = dL/dh act(g)
+        // h = act(g) u, dL/dg = dL/dh u act'(g), dL/du = dL/dh act(g); PAIR: all of the rows' common size, but for the g of the gate
         static_assert(!PAIR || TN == 64, "a block of 64 columns a tile");
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
@@ -829,7 +840,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
 #pragma unroll
           for (int j = 0; j < 16; j++) {
             float d;
-            const float act = tp_act<ACT>(a[j], d);
+            const float act = a[j] * tp_gate<ACT>(a[j], size[0], d);
             const float h = act * u[j], dg = dh[j] * (u[j] * d), du = dh[j] * act;
             a[j] = h;
             u[j] = dg;

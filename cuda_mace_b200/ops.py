@@ -297,7 +297,8 @@ def _workspace(device, nbytes):
 def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
     """(act(x @ w_gate) * (x @ w_up)) @ w_down for rows of node features x [..., C], w_gate and w_up [C, H], w_down [H, C], all
     float32 or all bfloat16; `activation` is "silu" or "gelu" (with erf).  Differentiable (once) in x and the three weights.
-    Sums are float32 in both types; float32 runs on the tensor cores in three terms (cmace_gated_ff_fwd_f32), bfloat16 rounds the hidden
+    Sums are float32 in both types; float32 runs on the tensor cores in three terms, each row precise against its own size
+    (cmace_gated_ff_fwd_f32), bfloat16 rounds the hidden
     values to bfloat16 between the products (few of them are kept to 16 bits or more).  The backward keeps x and the weights only and forms the hidden values again."""
     code = _ACTIVATIONS.get(activation)
     if code is None:

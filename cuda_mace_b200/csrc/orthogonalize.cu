@@ -8,7 +8,7 @@
 // vectors by the rounding and is not multiplied.  float32 takes pairs there too.  bf16 takes the high values alone (2^-12 instead of the
 // result's 2^-9) but for S S, the smallest of the products, whose rounding weighs most: with pairs there the error of a result is 1.2 to
 // 1.4 times that of its own rounding, without 1.6 to 1.8.  fp16's range suffices without looking at the values: |X|_2 <= 1 bounds every entry of X, S and b S + c S S in
-// every step, and the host makes powers of two of the bounds.
+// every step, and the host makes powers of two of the bounds (ns_step).
 //
 // Measured (B200, us a call of five steps, launches and all): one kernel: 4 of 64 x 64 20, 40 of 128 x 128 37, 3 of 128 x 512 in four CTAs each 59;
 // a kernel a product: 1 of 1 001 x 250 149 (17 launches of 6 to 9: chains of first copies, four to 16 blocks of 64 k, an epilogue),
@@ -147,16 +147,21 @@ constexpr int NSF_IMAGE = 128 * 128;      // 128 rows of 64 fp16
 constexpr int NSF_S_BYTES = 4 * NSF_IMAGE;   // two chunks, hi and lo
 constexpr int NSF_MAX_STEPS = 100;
 
+// One step on X 2^-k, with k from the bound of the singular values (ns_step): what it multiplies with, and powers of two of the pairs of S and P
+struct NsStep {
+  float a, b, c, ss, sp, out;   // out: of what the step leaves
+};
+constexpr float NS_SX = 0x1p15f;   // of the pairs of X 2^-k
+
 struct NsFused {
   const void *src;
   void *out;
   int64_t count;
   int side, length, tall, bf16, steps, columns, chunks;   // columns of a CTA, its chunks of 64
   int cluster;
-  float a, b, c;
   double eps;
   int32_t *status;
-  float sx[NSF_MAX_STEPS + 1], ss[NSF_MAX_STEPS], sp[NSF_MAX_STEPS];   // powers of two of X, S and P of every step
+  NsStep step[NSF_MAX_STEPS];
 };
 
 __device__ __forceinline__ void peer_store2(uint32_t addr, uint32_t x, uint32_t y) {
@@ -320,11 +325,11 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
     tmem_ld16_nowait(at, w);
     tmem_ld_wait();
 #pragma unroll
-    for (int k = 0; k < 16; k++) x[k] = inv * __uint_as_float(w[k]);
+    for (int k = 0; k < 16; k++) x[k] = 0.5f * (inv * __uint_as_float(w[k]));   // |X| <= 1: the first k is 1
 #pragma unroll
     for (int k = 0; k < 16; k++) w[k] = __float_as_uint(x[k]);
     tmem_st16(at, w);
-    put_x(ch, x, g.sx[0]);
+    put_x(ch, x, NS_SX);
   }
   tmem_st_wait();
 
@@ -386,13 +391,14 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
     }
   };
   for (int step = 0; step < g.steps; step++) {
-    const float sx = g.sx[step], ss = g.ss[step], sp = g.sp[step];
+    const NsStep &now = g.step[step];
+    const float ss = now.ss, sp = now.sp;
     uint32_t u[32] = {}, hi[16] = {}, lo[16] = {};
     float s[32];
     // S = X X^T
     products(x_first, x_desc, lo_of_x, x_desc, lo_of_x, x_steps, std::false_type{}, idesc_s);
     if (mine) tmem_ld32(acc + (uint32_t)(32 * group), u);
-    const float to_s = 1.0f / (sx * sx);
+    const float to_s = 1.0f / (NS_SX * NS_SX);
 #pragma unroll
     for (int j = 0; j < 32; j++) s[j] = __uint_as_float(u[j]) * to_s;
     if (CLUSTER == 1) {
@@ -456,9 +462,9 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
     products(s_first, s_desc, lo_of_s, s_desc, lo_of_s, side16 / 16, std::false_type{}, idesc_s);
     if (mine) {
       tmem_ld32(acc + (uint32_t)(32 * group), u);
-      const float from_ss = g.c / (ss * ss);
+      const float from_ss = now.c / (ss * ss);
 #pragma unroll
-      for (int j = 0; j < 32; j++) s[j] = g.b * s[j] + from_ss * __uint_as_float(u[j]);
+      for (int j = 0; j < 32; j++) s[j] = now.b * s[j] + from_ss * __uint_as_float(u[j]);
       split_row(s, sp, hi, lo);
       if (!A_TMEM) {
         put_row(s_hi + s_at, row, s_piece, hi);
@@ -472,7 +478,7 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
     }
     // X = a X + P X
     products(s_first, s_desc, lo_of_s, x_rows, lo_of_x, side16 / 16, std::true_type{}, idesc_x);
-    const float from_p = 1.0f / (sp * sx);
+    const float from_p = now.out / (sp * NS_SX), from_x = now.a * now.out;
     const bool last = step + 1 == g.steps;
 #pragma unroll(A_TMEM ? 2 : 1)
     for (int ch = 0; ch < g.chunks; ch++) {
@@ -483,12 +489,12 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
       tmem_ld16_nowait(master + col, m);
       tmem_ld_wait();
 #pragma unroll
-      for (int k = 0; k < 16; k++) x[k] = g.a * __uint_as_float(m[k]) + from_p * __uint_as_float(w[k]);
+      for (int k = 0; k < 16; k++) x[k] = from_x * __uint_as_float(m[k]) + from_p * __uint_as_float(w[k]);
       if (!last) {
 #pragma unroll
         for (int k = 0; k < 16; k++) m[k] = __float_as_uint(x[k]);
         tmem_st16(master + col, m);
-        put_x(ch, x, g.sx[step + 1]);
+        put_x(ch, x, NS_SX);
       } else {
         __syncthreads();   // every warp has its sums: the image of S is free; and the stores of the chunk before are done
 #pragma unroll
@@ -544,12 +550,25 @@ static double most_square(double b, double c, double most) {
   if (c != 0 && -b / (2 * c) > 0 && -b / (2 * c) < most) best = std::max(best, at(-b / (2 * c)));
   return best;
 }
-// power of two that keeps values up to `most`, and 5 % more for what rounding adds, below 2^15
-static float fp16_scale(double most) {
-  if (most == 0) return 1.f;
-  int e;
-  std::frexp(most * 1.05, &e);   // most * 1.05 < 2^e
-  return (float)std::ldexp(1.0, 15 - e);
+// The power of two above `most` and 5 % more, for what rounding adds
+static int exponent_of(double most) {
+  int e = 0;
+  if (most != 0) std::frexp(most * 1.05, &e);   // most * 1.05 < 2^e
+  return e;
+}
+// keeps values up to `most` below 2^15.  What is below 2^-45 of the other values may be lost: products of scales stay float32 values.
+static float fp16_scale(double most) { return (float)std::ldexp(1.0, 15 - std::max(exponent_of(most), -45)); }
+// A step on X^ = X 2^-k, whose singular values (those of X up to `most`) are below 1, to X'^ = X' 2^-k':
+// X'^ = a 2^(k-k') X^ + P^ X^ with P^ = b 2^(3k-k') S^ + c 2^(5k-k') S^ S^.  So the values of every step are of one size however far the polynomial
+// shrinks X or lets it grow, and the last step brings 2^k' back.  most, k: of the step, then of the next one
+static NsStep ns_step(double a, double b, double c, bool last, double &most, int &k) {
+  const double next = most_odd(a, b, c, most), size = std::ldexp(most, -k), size_s = size * size;
+  const int to = exponent_of(next);
+  const double b_k = std::ldexp(b, 3 * k - to), c_k = std::ldexp(c, 5 * k - to);
+  const NsStep s = {(float)std::ldexp(a, k - to), (float)b_k, (float)c_k, fp16_scale(size_s), fp16_scale(most_square(b_k, c_k, size_s)),
+                    last ? (float)std::ldexp(1.0, to) : 1.f};
+  most = next, k = to;
+  return s;
 }
 
 struct NsCall {
@@ -609,14 +628,10 @@ static int run_fused(const NsCall &f, int cluster) {
   g.bf16 = !f.f32, g.steps = f.steps, g.cluster = cluster;
   g.columns = (int)up((g.length + cluster - 1) / cluster, 16);
   g.chunks = (g.columns + 63) / 64;
-  g.a = (float)f.a, g.b = (float)f.b, g.c = (float)f.c, g.eps = f.eps, g.status = f.status;
+  g.eps = f.eps, g.status = f.status;
   double most = 1.0;
-  for (int k = 0; k < f.steps; k++) {
-    g.sx[k] = fp16_scale(most);
-    g.ss[k] = fp16_scale(most * most);
-    g.sp[k] = fp16_scale(most_square(f.b, f.c, most * most));
-    most = most_odd(f.a, f.b, f.c, most);
-  }
+  int k = exponent_of(most);
+  for (int i = 0; i < f.steps; i++) g.step[i] = ns_step(f.a, f.b, f.c, i + 1 == f.steps, most, k);
   const int smem = 2 * g.chunks * NSF_IMAGE + NSF_S_BYTES + (cluster > 1 ? 128 * 512 : 0) + 1024;
   switch (cluster) {
     case 2: return launch_fused<2, true>(f, g, smem);
@@ -650,9 +665,9 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   if (!w.base) return CMACE_OK;
 
   double most = 1.0;   // bound of the singular values
-  float sx = fp16_scale(most);
+  int k = exponent_of(most);
   const int blocks = (int)((f.rows * ((f.cols + 7) / 8) + 4 * NS_THREADS - 1) / (4 * NS_THREADS));
-  NsPrep p{f.src, partial, reinterpret_cast<__half *>(x[0].at), f.count, f.rows, f.cols, (int)x[0].ld, chunks, f.f32 ? 0 : 1, blocks, f.eps, sx};
+  NsPrep p{f.src, partial, reinterpret_cast<__half *>(x[0].at), f.count, f.rows, f.cols, (int)x[0].ld, chunks, f.f32 ? 0 : 1, blocks, f.eps, std::ldexp(NS_SX, -k)};
   launch_chained(ns_norm_kernel, dim3((unsigned)(f.count * chunks)), dim3(NS_THREADS), (size_t)0, f.st, p);
   launch_chained(ns_prep_kernel, dim3((unsigned)(f.count * blocks)), dim3(NS_THREADS), (size_t)0, f.st, p);
   int rc = check_launch(f.what);
@@ -676,9 +691,8 @@ static int orthogonalize(const NsCall &f, Carve &w) {
 
   for (int step = 0; step < f.steps && !rc; step++) {
     const Matrix &now = x[step & 1];
-    const double most_s = most * most, most_next = most_odd(f.a, f.b, f.c, most);
-    const float ss = fp16_scale(most_s), sp = fp16_scale(most_square(f.b, f.c, most_s)), sn = fp16_scale(most_next);
     const bool last = step + 1 == f.steps;
+    const NsStep by = ns_step(f.a, f.b, f.c, last, most, k);
     TpArgs g = new_args(side, side, f.status);
     g.batches = (int)f.count;
     g.in_f16 = 1;
@@ -686,8 +700,8 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     set_operand(g.a[0], now, wide);
     set_operand(g.b[0], now, wide);
     g.out[0].map = to_s;
-    g.alpha = 1.0f / (sx * sx);
-    g.pair_scale = ss;
+    g.alpha = 1.0f / (NS_SX * NS_SX);
+    g.pair_scale = by.ss;
     rc = f.f32 ? launch_ns<TP_GRAM>(v_gram, g, f.st, f.what) : launch_ns_single<TP_GRAM>(v_gram, g, f.st, f.what);
 
     set_k(g, 0, side);
@@ -695,7 +709,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     set_operand(g.b[0], s, true);
     g.out[0].map = to_poly;
     g.cin = from_s;
-    g.alpha = (float)f.c / (ss * ss), g.beta = (float)f.b / ss, g.pair_scale = sp;
+    g.alpha = by.c / (by.ss * by.ss), g.beta = by.b / by.ss, g.pair_scale = by.sp;
     if (!rc) rc = launch_ns<TP_POLY>(v_poly, g, f.st, f.what);
 
     g.rows = f.rows, g.cols = f.cols;
@@ -705,10 +719,8 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     g.out[1] = to_out;
     g.out_bf16 = !f.f32;
     g.cin = part_x[step & 1];
-    g.alpha = 1.0f / (sp * sx), g.beta = (float)f.a / sx, g.pair_scale = last ? 0.f : sn;
+    g.alpha = by.out / (by.sp * NS_SX), g.beta = by.a * by.out / NS_SX, g.pair_scale = last ? 0.f : NS_SX;
     if (!rc) rc = f.f32 ? launch_ns<TP_APPLY>(v_apply, g, f.st, f.what) : launch_ns_single<TP_APPLY>(v_apply, g, f.st, f.what);
-    most = most_next;
-    sx = sn;
   }
   return rc;
 }

@@ -25,6 +25,60 @@ namespace cmace {
 constexpr int NS_THREADS = 256;
 constexpr int NS_CHUNKS = 512;   // partial sums of a matrix at most
 
+// ---- the powers of two of a step ----------------------------------------------------------------------------------------------
+// Largest |t (a + b t^2 + c t^4)| over [0, most], from its ends and the zeros of its derivative
+__host__ __device__ inline double most_odd(double a, double b, double c, double most) {
+  const auto at = [=](double t) { return fabs(t * (a + t * t * (b + t * t * c))); };
+  double best = at(most);
+  // a + 3 b q + 5 c q^2 = 0, q = t^2
+  if (c != 0) {
+    const double d = 9 * b * b - 20 * a * c;
+    if (d >= 0)
+      for (int k = -1; k <= 1; k += 2) {
+        const double q = (-3 * b + k * sqrt(d)) / (10 * c);
+        if (q > 0 && q < most * most) best = fmax(best, at(sqrt(q)));
+      }
+  } else if (b != 0 && -a / (3 * b) > 0 && -a / (3 * b) < most * most) {
+    best = fmax(best, at(sqrt(-a / (3 * b))));
+  }
+  return best;
+}
+// largest |t (b + c t)|
+__host__ __device__ inline double most_square(double b, double c, double most) {
+  const auto at = [=](double t) { return fabs(t * (b + t * c)); };
+  const double best = at(most);
+  return c != 0 && -b / (2 * c) > 0 && -b / (2 * c) < most ? fmax(best, at(-b / (2 * c))) : best;
+}
+// The power of two above `most` and 5 % more, for what rounding adds
+__host__ __device__ inline int exponent_of(double most) {
+  int e = 0;
+  if (most != 0) frexp(most * 1.05, &e);   // most * 1.05 < 2^e
+  return e;
+}
+// keeps values up to `most` below 2^15.  What is below 2^-45 of the other values may be lost: products of scales stay float32 values.
+__host__ __device__ inline float fp16_scale(double most) {
+  const int e = exponent_of(most);
+  return (float)ldexp(1.0, 15 - (e > -45 ? e : -45));
+}
+// One step on X^ = X 2^-k, whose singular values (those of X up to `most`) are below 1, to X'^ = X' 2^-k':
+// X'^ = a 2^(k-k') X^ + P^ X^ with P^ = b 2^(3k-k') S^ + c 2^(5k-k') S^ S^.  So the values of every step are of one size however far the polynomial
+// shrinks X or lets it grow, and the last step brings 2^k' back.
+struct alignas(32) NsStep {
+  float a, b, c, ss, sp, out, unused[2];   // ss, sp: powers of two of the pairs of S^ and P^; out: of what the step leaves
+};
+constexpr float NS_SX = 0x1p15f;   // of the pairs of X^
+constexpr int NS_MAX_STEPS = 100;
+// most, k: of the step, then of the next one
+__host__ __device__ inline NsStep ns_step(double a, double b, double c, bool last, double &most, int &k) {
+  const double next = most_odd(a, b, c, most), size = ldexp(most, -k), size_s = size * size;
+  const int to = exponent_of(next);
+  const double b_k = ldexp(b, 3 * k - to), c_k = ldexp(c, 5 * k - to);
+  const NsStep s = {(float)ldexp(a, k - to), (float)b_k, (float)c_k, fp16_scale(size_s), fp16_scale(most_square(b_k, c_k, size_s)),
+                    last ? (float)ldexp(1.0, to) : 1.f, {0.f, 0.f}};
+  most = next, k = to;
+  return s;
+}
+
 struct NsPrep {
   const void *src;
   double *partial;   // [count][chunks]
@@ -32,7 +86,9 @@ struct NsPrep {
   int64_t count, rows;
   int cols, ld, chunks, bf16, blocks;   // blocks of ns_prep_kernel a matrix
   double eps;
-  float scale;
+  double a, b, c;
+  int steps;
+  NsStep *own;       // [count][NS_MAX_STEPS]: of a matrix far smaller than eps, whose X begins far below the bound of 1; ss = 0: the call's
 };
 
 __device__ __forceinline__ float ns_load(const void *p, int64_t i, int bf16) {
@@ -55,11 +111,11 @@ __device__ __forceinline__ void ns_load8(float (&v)[8], const void *p, int64_t i
   }
 }
 
-// 1 / (|U| + eps) as two factors, the first a power of two: |U| of a matrix of float32's largest or smallest values leaves float32's range.
+// size / (|U| + eps) as two factors, the first a power of two: |U| of a matrix of float32's largest or smallest values leaves float32's range.
 struct NsInverse {
   float first, second;
-  __device__ __forceinline__ NsInverse(double square, double eps) {
-    const double inv = 1.0 / (sqrt(square) + eps);
+  __device__ __forceinline__ NsInverse(double square, double eps, double size = 1.0) {
+    const double inv = size / (sqrt(square) + eps);
     first = inv > 0x1p100 ? 0x1p100f : inv < 0x1p-100 ? 0x1p-100f : 1.0f;
     second = (float)(inv / first);
   }
@@ -98,7 +154,8 @@ __global__ void __launch_bounds__(NS_THREADS) ns_norm_kernel(const NsPrep p) {
   }
 }
 
-// X of the first step as pairs; a thread takes eight columns of a row, four times.
+// X of the first step as pairs; a thread takes eight columns of a row, four times.  Where |U| is far below eps, X begins far below 1, and the
+// bounds with it: the matrix has steps of its own.
 __global__ void __launch_bounds__(NS_THREADS) ns_prep_kernel(const NsPrep p) {
   grid_begin();
   const int64_t m = blockIdx.x / (unsigned)p.blocks, b = blockIdx.x - m * p.blocks;
@@ -106,7 +163,16 @@ __global__ void __launch_bounds__(NS_THREADS) ns_prep_kernel(const NsPrep p) {
   for (int c = threadIdx.x & 31; c < p.chunks; c += 32) s += __ldcg(p.partial + m * p.chunks + c);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-  const NsInverse inv(s, p.eps);
+  double most = sqrt(s) / (sqrt(s) + p.eps);
+  const bool small = most < 0.25 && most > 0;
+  int k = exponent_of(small ? most : 1.0);
+  const NsInverse inv(s, p.eps, ldexp((double)NS_SX, -k));
+  if (b == 0 && threadIdx.x == 0)
+    for (int i = 0; i < p.steps; i++) {
+      NsStep own = {};
+      if (small) own = ns_step(p.a, p.b, p.c, i + 1 == p.steps, most, k);
+      p.own[m * NS_MAX_STEPS + i] = own;
+    }
   const int per_row = (p.cols + 7) / 8;
   const int64_t items = p.rows * per_row, plane = p.rows * p.ld;
   const bool wide = p.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(p.src) & 15) == 0;
@@ -121,7 +187,7 @@ __global__ void __launch_bounds__(NS_THREADS) ns_prep_kernel(const NsPrep p) {
     ns_load8(v, p.src, (m * p.rows + row) * p.cols + col, p.cols - col < 8 ? p.cols - col : 8, p.bf16, wide);
     uint32_t h[4], l[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) tp_split2(inv * v[2 * k], inv * v[2 * k + 1], p.scale, h[k], l[k]);
+    for (int k = 0; k < 4; k++) tp_split2(inv * v[2 * k], inv * v[2 * k + 1], 1.f, h[k], l[k]);
     __half *to = hi + row * p.ld + col;   // rows have a multiple of 64 elements
     *reinterpret_cast<uint4 *>(to) = make_uint4(h[0], h[1], h[2], h[3]);
     *reinterpret_cast<uint4 *>(to + plane) = make_uint4(l[0], l[1], l[2], l[3]);
@@ -145,13 +211,6 @@ constexpr int NSF_THREADS = 512;
 constexpr int NSF_STAGE_LD = 65;          // floats a row of the transposing buffer
 constexpr int NSF_IMAGE = 128 * 128;      // 128 rows of 64 fp16
 constexpr int NSF_S_BYTES = 4 * NSF_IMAGE;   // two chunks, hi and lo
-constexpr int NSF_MAX_STEPS = 100;
-
-// One step on X 2^-k, with k from the bound of the singular values (ns_step): what it multiplies with, and powers of two of the pairs of S and P
-struct NsStep {
-  float a, b, c, ss, sp, out;   // out: of what the step leaves
-};
-constexpr float NS_SX = 0x1p15f;   // of the pairs of X 2^-k
 
 struct NsFused {
   const void *src;
@@ -161,7 +220,7 @@ struct NsFused {
   int cluster;
   double eps;
   int32_t *status;
-  NsStep step[NSF_MAX_STEPS];
+  NsStep step[NS_MAX_STEPS];
 };
 
 __device__ __forceinline__ void peer_store2(uint32_t addr, uint32_t x, uint32_t y) {
@@ -527,50 +586,6 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
-// largest |p| over [0, most] of a polynomial c1 t + c3 t^3 + c5 t^5 (odd) or c1 t + c2 t^2, from its ends and the zeros of its derivative
-static double most_odd(double a, double b, double c, double most) {
-  const auto at = [&](double t) { return std::fabs(t * (a + t * t * (b + t * t * c))); };
-  double best = at(most);
-  // a + 3 b q + 5 c q^2 = 0, q = t^2
-  if (c != 0) {
-    const double d = 9 * b * b - 20 * a * c;
-    if (d >= 0)
-      for (double sign : {-1.0, 1.0}) {
-        const double q = (-3 * b + sign * std::sqrt(d)) / (10 * c);
-        if (q > 0 && q < most * most) best = std::max(best, at(std::sqrt(q)));
-      }
-  } else if (b != 0 && -a / (3 * b) > 0 && -a / (3 * b) < most * most) {
-    best = std::max(best, at(std::sqrt(-a / (3 * b))));
-  }
-  return best;
-}
-static double most_square(double b, double c, double most) {
-  const auto at = [&](double t) { return std::fabs(t * (b + t * c)); };
-  double best = at(most);
-  if (c != 0 && -b / (2 * c) > 0 && -b / (2 * c) < most) best = std::max(best, at(-b / (2 * c)));
-  return best;
-}
-// The power of two above `most` and 5 % more, for what rounding adds
-static int exponent_of(double most) {
-  int e = 0;
-  if (most != 0) std::frexp(most * 1.05, &e);   // most * 1.05 < 2^e
-  return e;
-}
-// keeps values up to `most` below 2^15.  What is below 2^-45 of the other values may be lost: products of scales stay float32 values.
-static float fp16_scale(double most) { return (float)std::ldexp(1.0, 15 - std::max(exponent_of(most), -45)); }
-// A step on X^ = X 2^-k, whose singular values (those of X up to `most`) are below 1, to X'^ = X' 2^-k':
-// X'^ = a 2^(k-k') X^ + P^ X^ with P^ = b 2^(3k-k') S^ + c 2^(5k-k') S^ S^.  So the values of every step are of one size however far the polynomial
-// shrinks X or lets it grow, and the last step brings 2^k' back.  most, k: of the step, then of the next one
-static NsStep ns_step(double a, double b, double c, bool last, double &most, int &k) {
-  const double next = most_odd(a, b, c, most), size = std::ldexp(most, -k), size_s = size * size;
-  const int to = exponent_of(next);
-  const double b_k = std::ldexp(b, 3 * k - to), c_k = std::ldexp(c, 5 * k - to);
-  const NsStep s = {(float)std::ldexp(a, k - to), (float)b_k, (float)c_k, fp16_scale(size_s), fp16_scale(most_square(b_k, c_k, size_s)),
-                    last ? (float)std::ldexp(1.0, to) : 1.f};
-  most = next, k = to;
-  return s;
-}
-
 struct NsCall {
   bool f32;
   const void *src;
@@ -659,6 +674,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   const int64_t n = f.rows * f.cols;
   const int chunks = (int)std::min<int64_t>(NS_CHUNKS, (n + 8191) / 8192);
   double *partial = w.take<double>(f.count * chunks);
+  NsStep *own = w.take<NsStep>(f.count * NS_MAX_STEPS);
   Matrix x[2];
   for (Matrix &m : x) m = new_matrix(w, true, f.rows, f.cols, f.count, 64, false);
   Matrix s = new_matrix(w, true, side, side, f.count, 64, false), poly = new_matrix(w, true, side, side, f.count, 64, false);
@@ -667,7 +683,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   double most = 1.0;   // bound of the singular values
   int k = exponent_of(most);
   const int blocks = (int)((f.rows * ((f.cols + 7) / 8) + 4 * NS_THREADS - 1) / (4 * NS_THREADS));
-  NsPrep p{f.src, partial, reinterpret_cast<__half *>(x[0].at), f.count, f.rows, f.cols, (int)x[0].ld, chunks, f.f32 ? 0 : 1, blocks, f.eps, std::ldexp(NS_SX, -k)};
+  NsPrep p{f.src, partial, reinterpret_cast<__half *>(x[0].at), f.count, f.rows, f.cols, (int)x[0].ld, chunks, f.f32 ? 0 : 1, blocks, f.eps, f.a, f.b, f.c, f.steps, own};
   launch_chained(ns_norm_kernel, dim3((unsigned)(f.count * chunks)), dim3(NS_THREADS), (size_t)0, f.st, p);
   launch_chained(ns_prep_kernel, dim3((unsigned)(f.count * blocks)), dim3(NS_THREADS), (size_t)0, f.st, p);
   int rc = check_launch(f.what);
@@ -696,6 +712,7 @@ static int orthogonalize(const NsCall &f, Carve &w) {
     TpArgs g = new_args(side, side, f.status);
     g.batches = (int)f.count;
     g.in_f16 = 1;
+    g.own = reinterpret_cast<const float4 *>(own + step), g.own_stride = NS_MAX_STEPS * (int)(sizeof(NsStep) / sizeof(float4));
     set_k(g, 0, wide ? f.cols : f.rows);
     set_operand(g.a[0], now, wide);
     set_operand(g.b[0], now, wide);

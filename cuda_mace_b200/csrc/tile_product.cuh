@@ -83,6 +83,8 @@ struct TpArgs {
   int64_t out_scale_ld, out_scale_batch;
   CUtensorMap cin;               // POLY: S, APPLY: X, in boxes of 32 rows of a warp's columns; batch b is hi 2 b and lo 2 b + 1
   float alpha, beta, pair_scale;   // D = alpha * product + beta * cin, times pair_scale where D is a pair
+  const float4 *own;               // Newton-Schulz: a batch's own (a, b, c, ss), (sp, out, ..) of the step, own_stride apart; ss = 0: the three above
+  int own_stride;
   const float *row_size[2];        // PAIR: powers of two that A's rows were brought to one size by, [rows up to a multiple of 256]; PLAIN: null: none
   int32_t *status;
   int64_t rows, cols;            // of the output
@@ -731,6 +733,15 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         }
         __syncwarp();
       }
+      float alpha = g.alpha, beta = g.beta, pair_scale = g.pair_scale;
+      if constexpr (KIND >= TP_GRAM) {
+        const float4 own = __ldcg(g.own + (int64_t)T.batch * g.own_stride), more = __ldcg(g.own + (int64_t)T.batch * g.own_stride + 1);
+        if (own.w != 0.f) {
+          if (KIND == TP_GRAM) pair_scale = own.w;
+          else if (KIND == TP_POLY) alpha = own.z / (own.w * own.w), beta = own.y / own.w, pair_scale = more.x;
+          else alpha = more.y / (more.x * 0x1p15f), beta = own.x * more.y * 0x1p-15f;
+        }
+      }
       float acc[PAIR ? GROUPS : 1][16];
       if (PAIR) {
 #pragma unroll
@@ -948,17 +959,17 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
 #pragma unroll
             for (int k = 0; k < 8; k++) {
               const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&hw[k])), e = __half22float2(*reinterpret_cast<const __half2 *>(&lw[k]));
-              v[2 * k] = g.alpha * v[2 * k] + g.beta * (a.x + e.x);
-              v[2 * k + 1] = g.alpha * v[2 * k + 1] + g.beta * (a.y + e.y);
+              v[2 * k] = alpha * v[2 * k] + beta * (a.x + e.x);
+              v[2 * k + 1] = alpha * v[2 * k + 1] + beta * (a.y + e.y);
             }
           } else {
 #pragma unroll
-            for (int j = 0; j < 16; j++) v[j] *= g.alpha;
+            for (int j = 0; j < 16; j++) v[j] *= alpha;
           }
           if (!result) {
             uint32_t w[8], lo[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) tp_split2(v[2 * j], v[2 * j + 1], g.pair_scale, w[j], lo[j]);
+            for (int j = 0; j < 8; j++) tp_split2(v[2 * j], v[2 * j + 1], pair_scale, w[j], lo[j]);
             st.put<ROW>(0, 2 * i, w);
             if (CIN) st.put<ROW>(LOW, 2 * i, lo);
             else

@@ -76,3 +76,33 @@ def test_usual_coefficients_of_many_steps(shape, dtype, dev):
 
     U = update(43, shape, dtype, dev, "even")
     check(ops.orthogonalize(U, steps=12), U, steps=12, coefficients=USUAL)
+
+
+@pytest.mark.parametrize("ratio", [0.3, 1e-1, 1e-3, 1e-6, 1e-9, 1e-15, 1e-25])
+@pytest.mark.parametrize("steps", [1, 5, 9])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shape", [(3, 48, 80), (3, 200, 150), (3, 130, 300)])
+def test_updates_far_below_eps(shape, dtype, steps, ratio, dev):
+    """Norms at `ratio` of eps, so that X begins at `ratio`, beside matrices that are not small.  float32: the bound of the products' rounding,
+    which is relative to X.  bfloat16: its rounding of the result, once, and twice that for the products, whose rounding is 2^-3 of it."""
+    from cuda_mace_b200 import ops
+
+    U = update(51, shape, F32, dev, "even").double()
+    U[1] *= ratio * 1e-7 / U[1].norm()
+    U = U.to(dtype)
+    out = ops.orthogonalize(U, steps=steps)
+    want = products(U, steps, USUAL, 1e-7)
+    if dtype == F32:
+        check(out, U, steps=steps)
+    for got, w in zip(out, want):
+        assert torch.isfinite(got).all() and relative(got, w) <= (2.0 ** -8 * 3 if dtype == BF16 else 2.0 ** -16)
+    assert torch.equal(out[0], ops.orthogonalize(U[:1], steps=steps)[0]) or shape[1] > 128
+
+
+@pytest.mark.parametrize("shape", [(2, 48, 80), (2, 200, 150)])
+def test_large_eps(shape, dev):
+    from cuda_mace_b200 import ops
+
+    U = update(53, shape, F32, dev)
+    for eps in (1e3, 1e12, 1e30):
+        check(ops.orthogonalize(U, eps=eps), U, eps=eps)

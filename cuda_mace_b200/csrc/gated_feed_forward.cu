@@ -980,7 +980,7 @@ static int launch_few(FewArgs g, cudaStream_t st, const char *what) {
   g.wide = g.N % V == 0;
   for (int i = 0; i < (GATED ? 2 : 1); i++) g.wide = g.wide && reinterpret_cast<uintptr_t>(g.w[i]) % (V * sizeof(T)) == 0;
   constexpr int SUMS = FEW_THREADS / 32 * (GATED ? 2 : 1) * FEW_COLS, SMEM = M * (FEW_K > SUMS ? FEW_K : SUMS) * 4;
-  if (const int rc = allow_smem<few_rows_kernel<T, M, GATED, ACT>>(SMEM, what)) return rc;
+  if (const int rc = allow_smem<few_rows_kernel<T, M, GATED, ACT>, SMEM>(what)) return rc;
   return launch_cluster(few_rows_kernel<T, M, GATED, ACT>, g.cluster, blocks * g.cluster, FEW_THREADS, SMEM, st, what, g);
 }
 template <typename T, int M, int ACT>
@@ -1019,7 +1019,7 @@ static int launch_some(const FeedForward &f, void *y) {
            ((reinterpret_cast<uintptr_t>(f.x) | reinterpret_cast<uintptr_t>(f.wd) | reinterpret_cast<uintptr_t>(y)) & (4 * SIZE - 1)) == 0;
   const int smem = (SIZE == 4 ? 2 : 1) * SOME_ROWS * g.ld * SIZE + SOME_WARPS * SOME_ROWS * 32 * CT * 4;
   constexpr int MOST = (SIZE == 4 ? 2 : 1) * SOME_ROWS * (32 * CT * SIZE + 128 + 64) + SOME_WARPS * SOME_ROWS * 32 * CT * 4;
-  if (const int rc = allow_smem<some_rows_kernel<T, CT, ACT>>(MOST, f.what)) return rc;
+  if (const int rc = allow_smem<some_rows_kernel<T, CT, ACT>, MOST>(f.what)) return rc;
   return launch_cluster(some_rows_kernel<T, CT, ACT>, g.cluster, blocks * g.cluster, SOME_THREADS, smem, f.st, f.what, g);
 }
 template <typename T, int ACT>

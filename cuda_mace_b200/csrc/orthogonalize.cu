@@ -628,9 +628,11 @@ static int fused_cluster(int64_t count, int64_t rows, int cols) {
   return p;
 }
 
+constexpr int fused_smem(int cluster, int chunks) { return 2 * chunks * NSF_IMAGE + NSF_S_BYTES + (cluster > 1 ? 128 * 512 : 0) + 1024; }
 template <int CLUSTER, bool A_TMEM>
 static int launch_fused(const NsCall &f, const NsFused &g, int smem) {
-  if (const int rc = allow_smem<ns_fused_kernel<CLUSTER, A_TMEM>>(smem, f.what)) return rc;
+  constexpr int MOST = fused_smem(CLUSTER, A_TMEM ? 2 : 4);
+  if (const int rc = allow_smem<ns_fused_kernel<CLUSTER, A_TMEM>, MOST>(f.what)) return rc;
   return launch_cluster(ns_fused_kernel<CLUSTER, A_TMEM>, CLUSTER, f.count * CLUSTER, NSF_THREADS, smem, f.st, f.what, g);
 }
 
@@ -647,7 +649,7 @@ static int run_fused(const NsCall &f, int cluster) {
   double most = 1.0;
   int k = exponent_of(most);
   for (int i = 0; i < f.steps; i++) g.step[i] = ns_step(f.a, f.b, f.c, i + 1 == f.steps, most, k);
-  const int smem = 2 * g.chunks * NSF_IMAGE + NSF_S_BYTES + (cluster > 1 ? 128 * 512 : 0) + 1024;
+  const int smem = fused_smem(cluster, g.chunks);
   switch (cluster) {
     case 2: return launch_fused<2, true>(f, g, smem);
     case 4: return launch_fused<4, true>(f, g, smem);

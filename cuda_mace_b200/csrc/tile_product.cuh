@@ -1047,15 +1047,16 @@ int encode_tile_map(CUtensorMap *map, const void *base, int bytes, bool bf16, in
                     int64_t batch_stride, int box_cols, int box_rows, const char *what);
 
 // ---- layout of a call's workspace -------------------------------------------------------------------------------------------
-// Dynamic shared memory a kernel may ask for: said once a device, to at least `bytes`
-template <auto KERNEL>
-int allow_smem(int bytes, const char *what) {
-  static std::atomic<int> allowed[64];
+// Dynamic shared memory that calls of a kernel ask for at most, said once a device.  One number a kernel: threads that say it at once say the same, and
+// none takes back what another's launch needs.
+template <auto KERNEL, int BYTES>
+int allow_smem(const char *what) {
+  static std::atomic<bool> allowed[64];
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess && (device < 0 || device >= 64 || allowed[device].load(std::memory_order_relaxed) < bytes)) {
-    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && device >= 0 && device < 64) allowed[device].store(bytes, std::memory_order_relaxed);
+  if (e == cudaSuccess && (device < 0 || device >= 64 || !allowed[device].load(std::memory_order_relaxed))) {
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+    if (e == cudaSuccess && device >= 0 && device < 64) allowed[device].store(true, std::memory_order_relaxed);
   }
   return e == cudaSuccess ? CMACE_OK : fail(CMACE_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
@@ -1171,7 +1172,7 @@ int tp_launch(TpArgs &g, cudaStream_t st, const char *what) {
   if (g.total >= (int64_t)1 << 31) return fail(CMACE_ERR_UNSUPPORTED, "%s: too many tiles", what);
   g.by_nt = tp_div((uint32_t)g.nt), g.by_mt = tp_div((uint32_t)g.mt), g.by_batches = tp_div((uint32_t)g.batches), g.by_splits = tp_div((uint32_t)g.splits);
   const auto kernel = tile_product_kernel<KIND, PAIR, TN, CTAS, ACT>;
-  if (const int rc = allow_smem<tile_product_kernel<KIND, PAIR, TN, CTAS, ACT>>(S::SMEM, what)) return rc;
+  if (const int rc = allow_smem<tile_product_kernel<KIND, PAIR, TN, CTAS, ACT>, S::SMEM>(what)) return rc;
   return launch_cluster(kernel, CTAS, (int)(CTAS * (g.total < 148 / CTAS ? g.total : 148 / CTAS)), TP_THREADS, S::SMEM, st, what, g);
 }
 

@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_rows_kernel(const FewArgs 
     if (threadIdx.x == 0) peer_arrive(smem_u32(&joined), 0);
     return;
   }
-  if (g.cluster > 1 && !peer_wait(smem_u32(&joined), 0) && g.status) atomicCAS(g.status, 0, 51);
+  if (g.cluster > 1 && !peer_wait(smem_u32(&joined), 0) && g.status) atomicCAS(g.status, 0, 112);
   for (int e = threadIdx.x; e < M * FEW_COLS; e += FEW_THREADS) {
     const int m = e / FEW_COLS, c = (int)(blockIdx.x / g.cluster) * FEW_COLS + e % FEW_COLS;
     float v[W];

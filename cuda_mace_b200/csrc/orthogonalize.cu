@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
       umma_commit(bar);
     }
     if (ok && !warp_wait(bar, phase, lane)) {   // a block that gave up goes on: the others of its cluster meet it at the barriers
-      if (lane == 0 && g.status) atomicCAS(g.status, 0, 47);
+      if (lane == 0 && g.status) atomicCAS(g.status, 0, 107);
       ok = false;
     }
     phase ^= 1;
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
     __syncthreads();
     if (tid < CLUSTER) peer_arrive(peer_bar, (uint32_t)tid);
     if (ok && !peer_wait(peer_bar, peer_phase)) {
-      if (lane == 0 && g.status) atomicCAS(g.status, 0, 50);
+      if (lane == 0 && g.status) atomicCAS(g.status, 0, 110);
       ok = false;
     }
   };

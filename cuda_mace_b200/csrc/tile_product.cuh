@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           const int row0 = (int)T.row0 + 128 * rank;
           for (int kb = k0; kb < k1; kb++) {
             if (!mbar_wait(empty + 8 * stage, phase ^ 1)) {
-              tp_report(g, 40);
+              tp_report(g, 100);
               ok = false;
               break;
             }
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         const TpTile T = tp_tile(g, t, TN, ROWS);
         if (!PAIR) {
           if (!mbar_wait(acc_empty + 8 * buf, (uses >> buf & 1) ^ 1)) {
-            tp_report(g, 41);
+            tp_report(g, 101);
             break;
           }
           tc_fence_after();
@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;   // 16 k, in units of 16 bytes
           if (KIND == TP_BACK) begun = 0;
           if (S::LATE && seg == 0 && !mbar_wait(acc_empty + 8 * (buf ^ 1), (uses >> (buf ^ 1) & 1) ^ 1)) {
-            tp_report(g, 48);
+            tp_report(g, 108);
             ok = false;
             break;
           }
@@ -579,14 +579,14 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           for (int kb = k0; kb < k1; kb++) {
             if (PAIR) {
               if (!mbar_wait(acc_empty + 8 * buf, (uses >> buf & 1) ^ 1)) {
-                tp_report(g, 42);
+                tp_report(g, 102);
                 ok = false;
                 break;
               }
               begun = 0;
             }
             if (!mbar_wait(full + 8 * stage, phase)) {
-              tp_report(g, 43);
+              tp_report(g, 103);
               ok = false;
               break;
             }
@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         }
       }
       commit(drain);   // nothing of this block's products is in flight when the columns are given back
-      if (!mbar_wait(drain, 0)) tp_report(g, 44);
+      if (!mbar_wait(drain, 0)) tp_report(g, 104);
     }
   } else if (warp == TP_EPILOGUE_WARPS + 2) {
     // ================================ scales ================================
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             for (int i = 0; ok && i < n; i++, chunk++) {
               const uint32_t set = chunk % S::BUFFERS;
               if (!warp_wait(scale_empty + 8 * set, (chunk / S::BUFFERS & 1) ^ 1, lane)) {
-                if (lane == 0) tp_report(g, 51);
+                if (lane == 0) tp_report(g, 111);
                 ok = false;
                 break;
               }
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
           constexpr bool TWO = KIND == TP_GATED || KIND == TP_BACK;
           for (int kb = k0; kb < k1; kb++) {
             if (ok && !warp_wait_all(acc_full + 8 * buf, uses >> buf & 1, lane)) {
-              if (lane == 0) tp_report(g, 45);
+              if (lane == 0) tp_report(g, 105);
               ok = false;
             }
             const float *scale = scales[buf] + 4 * (q >> 1) + 2 * (part >> 1);   // TN = 64: both blocks of columns are the one
@@ -780,7 +780,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         }
       } else {
         if (ok && !warp_wait_all(acc_full + 8 * buf, uses >> buf & 1, lane)) {
-          if (lane == 0) tp_report(g, 46);
+          if (lane == 0) tp_report(g, 106);
           ok = false;
         }
         tc_fence_after();
@@ -941,7 +941,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
         constexpr int ROW = 2 * S::PART;   // bytes of a row of a piece
         if (CIN && here) {
           if (!warp_wait(cin_bar, cin_phase, lane)) {   // after another wait gave up too: no copy outlives the block
-            if (lane == 0) tp_report(g, 49);
+            if (lane == 0) tp_report(g, 109);
             ok = false;
           }
           cin_phase ^= 1;

@@ -83,6 +83,7 @@ SIGNATURES = {
     "cmace_bounded_wait_probe": [_P, _I, _D, _P],
     "cmace_gemm3x_gradr_f32": [_P, _P, _P, _P, _P, _P, _L, _I, _I, _P, _P, _P],
     "cmace_gated_ff_workspace_bytes": [_I, _L, _I, _I, _I],
+    "cmace_dense_launches": [],
     "cmace_gated_ff_fwd_f32": [_P, _P, _P, _P, _L, _I, _I, _I, _P, _P, _L, _P, _P],
     "cmace_gated_ff_fwd_bf16": [_P, _P, _P, _P, _L, _I, _I, _I, _P, _P, _L, _P, _P],
     "cmace_gated_ff_bwd_f32": [_P, _P, _P, _P, _P, _L, _I, _I, _I, _P, _P, _P, _P, _P, _L, _P, _P],
@@ -127,6 +128,7 @@ _RESTYPES = {
     "cmace_imp_bwd_scratch_elems": _L,
     "cmace_gemm_packed_floats": _L,
     "cmace_gated_ff_workspace_bytes": _L,
+    "cmace_dense_launches": _L,
     "cmace_orthogonalize_workspace_bytes": _L,
     "cmace_radial_hidden_saved_floats": _L,
     "cmace_nl_num_cells": _L,
@@ -138,7 +140,8 @@ _RESTYPES = {
     "cmace_symcon_plan_destroy": None,
 }
 # functions whose integer result is a value, not a status
-_VALUE_FUNCS = {"cmace_abi_version", "cmace_gated_ff_workspace_bytes", "cmace_orthogonalize_workspace_bytes", "cmace_sender_order_workspace_bytes", "cmace_imp_bwd_scratch_elems",
+_VALUE_FUNCS = {"cmace_abi_version", "cmace_gated_ff_workspace_bytes", "cmace_orthogonalize_workspace_bytes", "cmace_dense_launches",
+                "cmace_sender_order_workspace_bytes", "cmace_imp_bwd_scratch_elems",
                 "cmace_gemm_packed_floats", "cmace_imp_bwd_edge_f64_noalloc_max_elems",
                 "cmace_radial_hidden_saved_floats", "cmace_nl_num_cells", "cmace_nl_workspace_bytes", "cmace_scan_workspace_bytes",
                 "cmace_imp_staged_stalled", "cmace_step_workspace_bytes", "cmace_step_count", "cmace_step_struct_bytes", "cmace_step_name",
@@ -148,7 +151,7 @@ _VALUE_FUNCS = {"cmace_abi_version", "cmace_gated_ff_workspace_bytes", "cmace_or
 _lib = None
 
 # entry points that launch kernels, with the number of kernels of ours each call launches
-# (cub's radix sort inside the two grouping calls is counted as one)
+# (cub's radix sort inside the two grouping calls is counted as one; the dense operators count theirs themselves, some in autograd's thread)
 KERNEL_LAUNCHES = {
     "cmace_receiver_csr": 1, "cmace_sender_order": 3, "cmace_group_by_element": 3,
     "cmace_sph_fwd": 1, "cmace_sph_bwd": 1, "cmace_edge_basis_fwd": 1, "cmace_edge_basis_bwd": 1,
@@ -156,12 +159,18 @@ KERNEL_LAUNCHES = {
     "cmace_spline_fwd": 1, "cmace_spline_bwd": 1, "cmace_imp_fwd": 1, "cmace_imp_bwd_edge": 1, "cmace_imp_bwd_edge_f64_noalloc": 2,
     "cmace_imp_bwd_node": 1, "cmace_imp_bwd_node_edges": 1, "cmace_linear": 1, "cmace_symcon_fwd": 1, "cmace_symcon_bwd": 1,
     "cmace_gemm_pack_weights": 1, "cmace_gemm3x": 1, "cmace_gemm": 1, "cmace_gemm3x_gradr": 1, "cmace_bounded_wait_probe": 1, "cmace_linear_tc": 1,
-    "cmace_gated_ff_fwd": 3, "cmace_gated_ff_fwd_bf16": 2, "cmace_gated_ff_bwd": 5, "cmace_gated_ff_bwd_bf16": 4,
     "cmace_radial_hidden_fwd": 1, "cmace_radial_hidden_bwd": 1, "cmace_imp_radial_fused_fwd": 1,
     "cmace_symcon_effective_weights": 1, "cmace_symcon_apply": 1, "cmace_nl_build": 4, "cmace_nl_emit": 1, "cmace_nl_cell_ids": 1, "cmace_nl_count": 1, "cmace_exclusive_scan_i32": 1, "cmace_nl_fill": 1,
 }
-launch_count = 0       # kernels launched through this binding since import
+_launched = 0          # kernels launched through call() and run_steps() since import
 _timing = None         # list of (name, start_event, end_event) while timing is on
+
+
+def __getattr__(name):
+    """launch_count: kernels launched through this binding since import."""
+    if name == "launch_count":
+        return _launched + (0 if _lib is None else _lib.cmace_dense_launches())
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def load():
@@ -191,7 +200,7 @@ def load():
 def call(name, *args, tag=None):
     """Calls a status-returning entry point; raises RuntimeError with the library's message.
     `tag` only labels the call in the optional kernel timing (e.g. the GEMM shape)."""
-    global launch_count
+    global _launched
     lib = load()
     if name in _VALUE_FUNCS:
         return getattr(lib, name)(*args)
@@ -207,7 +216,7 @@ def call(name, *args, tag=None):
         _timing.append((name if tag is None else f"{name}[{tag}]", ev0, ev1))
     else:
         rc = getattr(lib, name)(*args)
-    launch_count += n_launch
+    _launched += n_launch
     if rc != 0:
         raise RuntimeError(f"{name} failed ({rc}): {lib.cmace_last_error().decode()}")
     return 0
@@ -215,7 +224,7 @@ def call(name, *args, tag=None):
 
 def run_steps(model, io, first, last, stream):
     """cmace_step_run on a StepModel and a StepIO; while timing is on, every step is bracketed by events of its own."""
-    global launch_count
+    global _launched
     lib = _lib if _lib is not None else load()
     before = io.launches
     if _timing is None:
@@ -230,7 +239,7 @@ def run_steps(model, io, first, last, stream):
             rc = rc or lib.cmace_step_run(ctypes.byref(model), ctypes.byref(io), s, s + 1, stream)
             ev1.record()
             _timing.append((f"step[{lib.cmace_step_name(s).decode()}]", ev0, ev1))
-    launch_count += io.launches - before
+    _launched += io.launches - before
     if rc != 0:
         raise RuntimeError(f"cmace_step_run failed ({rc}): {lib.cmace_last_error().decode()}")
 

@@ -941,8 +941,8 @@ static int launch_rows(const FeedForward &f, TpArgs &g, void *out, int splits, f
   if (const int rc = launch_plain(f.pair, g, f.st, f.what)) return rc;
   const RowsSum r{partial, out, f.M, ld, f.C, splits, f.C % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (f.f32 ? 15 : 7)) == 0};
   const dim3 grid((unsigned)((f.M * ld / 4 + 255) / 256));
-  if (f.f32) launch_chained(rows_sum_kernel<float>, grid, dim3(256), (size_t)0, f.st, r);
-  else launch_chained(rows_sum_kernel<__nv_bfloat16>, grid, dim3(256), (size_t)0, f.st, r);
+  if (f.f32) launch_dense(rows_sum_kernel<float>, grid, 256, f.st, r);
+  else launch_dense(rows_sum_kernel<__nv_bfloat16>, grid, 256, f.st, r);
   return check_launch(f.what);
 }
 
@@ -950,10 +950,10 @@ static int run_prep(const PrepArgs &p, int64_t blocks, cudaStream_t st, const ch
   if (blocks == 0) return CMACE_OK;
   if (blocks >= (int64_t)1 << 31) return fail(CMACE_ERR_UNSUPPORTED, "%s: too many rows", what);
   if (p.rows.slabs)
-    launch_chained(row_most_kernel, dim3((unsigned)((p.rows.rows + 63) / 64), (unsigned)p.rows.slabs, (unsigned)p.rows.sources), dim3(PREP_THREADS), (size_t)0,
+    launch_dense(row_most_kernel, dim3((unsigned)((p.rows.rows + 63) / 64), (unsigned)p.rows.slabs, (unsigned)p.rows.sources), PREP_THREADS,
                    st, p.rows);
   const auto kernel = !p.rows.blocks ? prep_kernel<PREP_COPY> : p.rows.slabs ? prep_kernel<PREP_BLOCKS> : prep_kernel<PREP_WHOLE>;
-  launch_chained(kernel, dim3((unsigned)blocks), dim3(PREP_THREADS), (size_t)0, st, p);
+  launch_dense(kernel, dim3((unsigned)blocks), PREP_THREADS, st, p);
   return check_launch(what);
 }
 
@@ -1181,8 +1181,8 @@ static int backward(const FeedForward &f, void *gx, void *const gw[3], bool want
     WeightReduce r{partial, {gw[0], gw[1], gw[2]}, ld, splits, f.C, f.H};
     const dim3 grid((unsigned)((f.H + 31) / 32), (unsigned)((f.C + 31) / 32), 3);
     if (!rc) {
-      if (f.f32) launch_chained(weight_reduce_kernel<float>, grid, dim3(256), (size_t)0, f.st, r);
-      else launch_chained(weight_reduce_kernel<__nv_bfloat16>, grid, dim3(256), (size_t)0, f.st, r);
+      if (f.f32) launch_dense(weight_reduce_kernel<float>, grid, 256, f.st, r);
+      else launch_dense(weight_reduce_kernel<__nv_bfloat16>, grid, 256, f.st, r);
       rc = check_launch(f.what);
     }
   }
@@ -1249,6 +1249,8 @@ static int run_backward(bool f32, const void *x, const void *wg, const void *wu,
 using namespace cmace;
 
 extern "C" {
+
+int64_t cmace_dense_launches(void) { return dense_launches().load(std::memory_order_relaxed); }
 
 int64_t cmace_gated_ff_workspace_bytes(int is_f32, int64_t rows, int width, int hidden, int backward_pass) {
   if (check_sizes("cmace_gated_ff_workspace_bytes", rows, width, hidden, TP_SILU)) return -1;

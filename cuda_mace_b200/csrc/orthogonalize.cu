@@ -686,8 +686,8 @@ static int orthogonalize(const NsCall &f, Carve &w) {
   int k = exponent_of(most);
   const int blocks = (int)((f.rows * ((f.cols + 7) / 8) + 4 * NS_THREADS - 1) / (4 * NS_THREADS));
   NsPrep p{f.src, partial, reinterpret_cast<__half *>(x[0].at), f.count, f.rows, f.cols, (int)x[0].ld, chunks, f.f32 ? 0 : 1, blocks, f.eps, f.a, f.b, f.c, f.steps, own};
-  launch_chained(ns_norm_kernel, dim3((unsigned)(f.count * chunks)), dim3(NS_THREADS), (size_t)0, f.st, p);
-  launch_chained(ns_prep_kernel, dim3((unsigned)(f.count * blocks)), dim3(NS_THREADS), (size_t)0, f.st, p);
+  launch_dense(ns_norm_kernel, dim3((unsigned)(f.count * chunks)), NS_THREADS, f.st, p);
+  launch_dense(ns_prep_kernel, dim3((unsigned)(f.count * blocks)), NS_THREADS, f.st, p);
   int rc = check_launch(f.what);
   // maps: operands; what is added and written, in boxes of the variants' columns a warp
   const int kb_s = blocks64(wide ? f.cols : f.rows), kb = blocks64(side);

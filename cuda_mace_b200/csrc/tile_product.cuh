@@ -1141,6 +1141,16 @@ struct TpCost {
   }
 };
 
+// kernels that the dense operators have launched, from any thread
+inline std::atomic<int64_t> &dense_launches() {
+  static std::atomic<int64_t> count{0};
+  return count;
+}
+template <typename... Params, typename... Args>
+void launch_dense(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t st, Args &&...args) {
+  launch_chained(kernel, grid, dim3((unsigned)threads), (size_t)0, st, std::forward<Args>(args)...);
+  dense_launches().fetch_add(1, std::memory_order_relaxed);
+}
 // launch_chained() with clusters of `ctas`
 template <typename Args>
 int launch_cluster(void (*kernel)(Args), int ctas, int64_t blocks, int threads, int smem, cudaStream_t st, const char *what, const Args &args) {
@@ -1159,6 +1169,7 @@ int launch_cluster(void (*kernel)(Args), int ctas, int64_t blocks, int threads, 
   cfg.attrs = ctas > 1 ? attr : attr + 1;
   cfg.numAttrs = (ctas > 1 ? 1 : 0) + (chained ? 1 : 0);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
+  dense_launches().fetch_add(1, std::memory_order_relaxed);
   return e == cudaSuccess ? check_launch(what) : fail(CMACE_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 

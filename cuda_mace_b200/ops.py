@@ -307,7 +307,6 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
         raise RuntimeError("cuda_mace_b200 operators need CUDA tensors (there is no CPU path)")
     if _gated_feed_forward is None:
         _load_dense()
-    _abi.launch_count += 3 if x.dtype is torch.float32 else 2
     return _gated_feed_forward(x, w_gate, w_up, w_down, code, _status_tensor(x.device))
 
 
@@ -362,7 +361,6 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
     ws = _workspace(u.device, nbytes)
     _abi.call("cmace_orthogonalize_f32" if f32 else "cmace_orthogonalize_bf16", _ptr(u), count, m, n, int(steps), a, b, c, float(eps), _ptr(out), _ptr(ws), nbytes,
               _ptr(_status_tensor(u.device)), _stream())
-    _abi.launch_count += 1 if nbytes == 256 else 2 + 3 * int(steps)   # one kernel needs no workspace
     return out
 
 

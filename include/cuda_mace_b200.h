@@ -299,6 +299,9 @@ int cmace_gated_ff_bwd_bf16(const void *x, const void *w_gate, const void *w_up,
                             void *grad_up, void *grad_down, void *workspace, int64_t workspace_bytes, int32_t *status,
                             cmace_stream_t stream);
 
+/* kernels that the feed-forward block's and the orthogonalised updates' entry points have launched so far, from any thread */
+int64_t cmace_dense_launches(void);
+
 /* ---- orthogonalised updates (no counterpart in the reference) -----------------------------------------
  * out = Newton-Schulz products of update [count, rows, cols], contiguous: X = U / (|U| + eps) with the Frobenius norm of each matrix,
  * then steps (1 to 100) times X <- a X + (b S + c S S) X, S = X X^T (rows > cols: X <- a X + X (b S + c S S), S = X^T X, the same values).

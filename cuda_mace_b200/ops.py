@@ -18,6 +18,7 @@ fallback: a CPU tensor raises.
 """
 import functools
 import math
+import operator
 import os
 from collections import OrderedDict
 
@@ -338,6 +339,7 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
     with the Frobenius norm of each matrix, then `steps` times X <- a X + (b S + c S S) X with S = X X^T and
     (a, b, c) = `coefficients`.  float32 or bfloat16; a new tensor of the same shape and type.  For the updates of weight
     matrices, stacks like Linear's [4, K, N] and ElementalLinear's [Z, 4, K, N] included; has no gradient."""
+    steps = operator.index(steps)
     _check_cuda(update)
     if update.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"orthogonalize needs float32 or bfloat16, got {update.dtype}")
@@ -359,7 +361,7 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
     f32 = u.dtype == torch.float32
     nbytes = _orthogonalize_bytes(f32, count, m, n)
     ws = _workspace(u.device, nbytes)
-    _abi.call("cmace_orthogonalize_f32" if f32 else "cmace_orthogonalize_bf16", _ptr(u), count, m, n, int(steps), a, b, c, float(eps), _ptr(out), _ptr(ws), nbytes,
+    _abi.call("cmace_orthogonalize_f32" if f32 else "cmace_orthogonalize_bf16", _ptr(u), count, m, n, steps, a, b, c, float(eps), _ptr(out), _ptr(ws), nbytes,
               _ptr(_status_tensor(u.device)), _stream())
     return out
 

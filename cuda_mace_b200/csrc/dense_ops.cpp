@@ -106,6 +106,8 @@ Tensor gated_feed_forward(const Tensor &x_, const Tensor &wg_, const Tensor &wu_
   TORCH_CHECK(width >= 1 && hidden >= 1 && x_.size(-1) == width && wu_.size(0) == width && wu_.size(1) == hidden && wd_.size(0) == hidden && wd_.size(1) == width,
               "shape mismatch: x ", x_.sizes(), ", w_gate ", wg_.sizes(), ", w_up ", wu_.sizes(), ", w_down ", wd_.sizes());
   TORCH_CHECK(width <= 1 << 20 && hidden <= 1 << 20, "gated_feed_forward: widths up to 2^20");
+  TORCH_CHECK(status.is_cuda() && status.get_device() == device && status.scalar_type() == torch::kInt32 && status.numel() >= 1,
+              "gated_feed_forward: status has to be an int32 of the current device");
   const Tensor x = x_.contiguous(), wg = wg_.contiguous(), wu = wu_.contiguous(), wd = wd_.contiguous();
   if (at::GradMode::is_enabled() && (x.requires_grad() || wg.requires_grad() || wu.requires_grad() || wd.requires_grad()))
     return GatedFeedForward::apply(x, wg, wu, wd, activation, status);

@@ -345,6 +345,8 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
         raise TypeError(f"orthogonalize needs float32 or bfloat16, got {update.dtype}")
     if update.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("orthogonalize has no gradient: detach the update or call it under torch.no_grad()")
+    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError("orthogonalize cannot be recorded by a tracer")
     if forward_ad._current_level >= 0 and forward_ad.unpack_dual(update).tangent is not None:
         raise NotImplementedError("orthogonalize has no forward-mode derivative")
     if update.dim() < 2 or update.shape[-1] < 1 or update.shape[-2] < 1:

@@ -60,6 +60,8 @@ def test_batched_by_transforms():
 
 
 def test_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
     from cuda_mace_b200 import ops
 
     x, wg, wu, wd, _ = operands()
@@ -67,6 +69,8 @@ def test_refused():
         torch.func.grad(lambda a: ops.gated_feed_forward(a, wg, wu, wd).sum())(x)
     with pytest.raises(NotImplementedError):
         torch.func.jvp(lambda a: ops.gated_feed_forward(a, wg, wu, wd), (x,), (x,))
+    with pytest.raises(RuntimeError, match="tracer"):
+        make_fx(lambda u: ops.orthogonalize(u))(x)
     with pytest.raises(RuntimeError):
         torch.func.vmap(ops.orthogonalize)(x[None])
     with pytest.raises(RuntimeError):

@@ -116,7 +116,10 @@ _STATUS_INPUTS = {90: "an edge's shift index is beyond the shift table",
 def _status_tensor(device):
     idx = device.index if device.index is not None else torch.cuda.current_device()
     if idx not in _status:
-        _status[idx] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        status = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        if type(status) is not torch.Tensor:   # a tracer's, without memory: not for the calls that follow
+            return status
+        _status[idx] = status
     return _status[idx]
 
 

@@ -1,4 +1,8 @@
 """The dense operators under tracers and function transforms: the values of a plain call, or a refusal, never a recording that computes nothing."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -6,11 +10,33 @@ from tests.test_feed_forward_gpu import case
 
 pytestmark = pytest.mark.gpu
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 F32, BF16 = torch.float32, torch.bfloat16
 
 
 def operands(M=20, dtype=F32):
     return case(7, M, 16, 24, dtype, "cuda")
+
+
+FIRST = """
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from cuda_mace_b200 import ops
+
+with FakeTensorMode():
+    x, w, d = (torch.randn(*s, device="cuda") for s in ((20, 16), (16, 24), (24, 16)))
+    y = ops.gated_feed_forward(x, w, w, d)
+    assert tuple(y.shape) == (20, 16) and type(y) is not torch.Tensor
+x, w, d = (torch.randn(*s, device="cuda") for s in ((20, 16), (16, 24), (24, 16)))
+assert torch.isfinite(ops.gated_feed_forward(x, w, w, d)).all()
+ops.check_status()
+"""
+
+
+def test_traced_before_the_first_call():
+    """What a tracer makes for itself is not kept for the calls that follow."""
+    r = subprocess.run([sys.executable, "-c", FIRST], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])

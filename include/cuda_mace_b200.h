@@ -279,7 +279,7 @@ int cmace_gemm3x_gradr_f32(const float *X, const float *G, const float *Y, const
  * workspace: cmace_gated_ff_workspace_bytes(...) bytes, aligned to 256, not shared by calls that may overlap; what it holds afterwards is not
  * for the caller.  A row of x with an infinity or a NaN makes that row of y and grad_x, and the weights' gradients, not finite, no other row.
  * float operands of more than a few rows go as pairs of fp16 values with one scale a block of 64 x 64 values: a value that is smaller than its
- * block's largest keeps 22 bits over 2^18 below it and is gone from 2^40 below it on.  That is so for the weights.  Rows of x and grad_y are
+ * block's largest keeps 22 bits over 2^28 below it and is gone from 2^51 below it on.  That is so for the weights.  Rows of x and grad_y are
  * brought to one size first, by powers of two: a row of y and grad_x has its precision against its own size, whatever the other rows' is,
  * and the weights' gradients theirs against their largest terms.
  * status: as for cmace_gemm3x_f32. */

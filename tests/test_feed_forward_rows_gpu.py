@@ -43,11 +43,11 @@ def product(A, B, dA, dB, size_A, size_B):
     return A @ B, off
 
 
-def reference(x, wg, wu, wd, gy, activation):
-    """Values and bounds of a float32 call, row by row."""
+def reference(x, wg, wu, wd, gy, activation, low=1.0):
+    """Values and bounds of a float32 call, row by row.  low: of the 2^-38 that is lost of a block's largest value."""
     s, t = power(x), power(gy)
-    of = lambda v, p: (v / p).abs().max() * p  # noqa: E731: the block's largest value at a row's own size
-    flat = lambda w: w.abs().max()  # noqa: E731
+    of = lambda v, p: low * (v / p).abs().max() * p  # noqa: E731: the block's largest value at a row's own size
+    flat = lambda w: low * w.abs().max()  # noqa: E731
     g, eg = product(x, wg, 0.0, 0.0, of(x, s), flat(wg))
     u, eu = product(x, wu, 0.0, 0.0, of(x, s), flat(wu))
     a, da = act_of(g, activation)
@@ -66,7 +66,7 @@ def reference(x, wg, wu, wd, gy, activation):
     out = {"y": (y, ey), "x": (x1 + x2, e1 + e2 + 2.0 ** -23 * (x1.abs() + x2.abs()))}
     # sums over rows, of rows at the size of their contributions: x s t by dg / (s t), dy s^2 by h / s^2
     for name, A, p, B, eB in (("w_gate", x, s * t, dg, edg), ("w_up", x, s * t, du, edu), ("w_down", gy, s * s, h, eh)):
-        v, e = product((A * p).t(), B / p, 0.0, eB / p, (A * p).abs().max(), (B / p).abs().max())
+        v, e = product((A * p).t(), B / p, 0.0, eB / p, low * (A * p).abs().max(), low * (B / p).abs().max())
         out[name] = (v.t(), e.t()) if name == "w_down" else (v, e)
     return {k: (v, e + 2.0 ** -24 * v.abs()) for k, (v, e) in out.items()}
 

@@ -238,8 +238,8 @@ __global__ void __launch_bounds__(PREP_THREADS, KIND == PREP_COPY ? 8 : KIND == 
         if (T.first + 16 * i >= T.n || col >= cols) break;   // columns up to the rows' distance, a multiple of eight, take zeros
         const float4 v = value(x[e][i], how, i);
         uint2 h, l;
-        tp_split2<true>(v.x, v.y, scale, h.x, l.x);
-        tp_split2<true>(v.z, v.w, scale, h.y, l.y);
+        tp_split2(v.x, v.y, scale, h.x, l.x);
+        tp_split2(v.z, v.w, scale, h.y, l.y);
         *reinterpret_cast<uint2 *>(to + (int64_t)(16 * i) * ld) = h;
         *reinterpret_cast<uint2 *>(to_lo + (int64_t)(16 * i) * ld) = l;
       }

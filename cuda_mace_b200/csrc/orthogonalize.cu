@@ -3,7 +3,8 @@
 // value s goes to a s + b s^3 + c s^5, so all of them meet near 1.
 //
 // What the precision asks for: a small singular value is multiplied by a up to `steps` times (485 with the usual coefficients), and so is
-// what rounding adds along its direction.  X itself is therefore kept to 22 bits or more, as a pair of fp16 values (tile_product.cuh), and
+// what rounding adds along its direction.  X itself is therefore kept to 22 bits or more, as a pair of fp16 values (tile_product.cuh; 2^-50 of its bound
+// where values are far below that), and
 // a X formed from both; the operands of the products may be rounded further, since what that adds lies in the rows or in the columns of the large values, turns their
 // vectors by the rounding and is not multiplied.  float32 takes pairs there too.  bf16 takes the high values alone (2^-12 instead of the
 // result's 2^-9) but for S S, the smallest of the products, whose rounding weighs most: with pairs there the error of a result is 1.2 to
@@ -11,8 +12,8 @@
 // every step, and the host makes powers of two of the bounds (ns_step).
 //
 // Measured (B200, us a call of five steps, launches and all): one kernel: 4 of 64 x 64 20, 40 of 128 x 128 37, 3 of 128 x 512 in four CTAs each 59;
-// a kernel a product: 1 of 1 001 x 250 149 (17 launches of 6 to 9: chains of first copies, four to 16 blocks of 64 k, an epilogue),
-// 2 of 1 024 x 4 096 in bf16 290 to 325 (X X^T 20, S S 12, P X 28 a step; at 50 to 64 bytes a cycle and SM the copies of 128 x 256 operands
+// a kernel a product: 1 of 1 001 x 250 154 (17 launches of 6 to 9: chains of first copies, four to 16 blocks of 64 k, an epilogue),
+// 2 of 1 024 x 4 096 in bf16 320 (X X^T 20, S S 12, P X 28 a step; at 50 to 64 bytes a cycle and SM the copies of 128 x 256 operands
 // take as long as their products).
 #include <algorithm>
 #include <cmath>
@@ -239,10 +240,19 @@ __device__ __forceinline__ uint4 smem_load4(uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
+// D = A B + D 2^-11, A in tensor memory
+__device__ __forceinline__ void umma_f16_ts_low(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, 11;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc)
+      : "memory");
+}
 // two packed fp16 of each part as the floats that they stand for, times their power of two
 __device__ __forceinline__ float2 pair_value(uint32_t hi, uint32_t lo) {
   const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&hi)), y = __half22float2(*reinterpret_cast<const __half2 *>(&lo));
-  return make_float2(x.x + y.x, x.y + y.y);
+  return make_float2(fmaf(y.x, 0x1p-11f, x.x), fmaf(y.y, 0x1p-11f, x.y));
 }
 // WORDS packed values of one row (16-byte pieces `piece`, ... of its 128 bytes) into an image
 template <int WORDS>
@@ -413,14 +423,17 @@ __global__ void __launch_bounds__(NSF_THREADS, 1) ns_fused_kernel(const __grid_c
         if (A_TMEM) umma_f16_ts(tmem, a_tmem + (uint32_t)(8 * k) + (al ? 64u : 0u), b, idesc, accumulate);
         else umma_16(tmem, A + al + (uint64_t)((k >> 2) * (NSF_IMAGE >> 4) + (k & 3) * 2), b, idesc, accumulate);
       };
+      // the terms with a low part, which is kept times 2^11, then the first of the others on 2^-11 of their sum
 #pragma unroll
       for (int k = 0; k < MOST; k++) {
         if (k >= steps16) break;
         product(k, a_lo, 0, k > 0);
         product(k, 0, b_lo, 1);
       }
+      if (A_TMEM) umma_f16_ts_low(tmem, a_tmem, B, idesc);
+      else umma_16_low(tmem, A, B, idesc);
 #pragma unroll
-      for (int k = 0; k < MOST; k++) {
+      for (int k = 1; k < MOST; k++) {
         if (k >= steps16) break;
         product(k, 0, 0, 1);
       }

@@ -14,8 +14,7 @@
 //    on the average.  Three MMAs a k step (lo hi, hi lo, hi hi; lo lo is below 2^-22 of hi hi).  fp16 lacks float32's range, so
 //    every block of 64 x 64 values has a power of two of its own, from the block's largest value, and lo is kept times 2^11: the terms that it
 //    is in are summed first and the first hi hi adds 2^-11 of them.  Within a block the precision holds over 2^28 below that value
-//    and degrades to an absolute 2^-50 of it beyond (rows of a caller's array are brought to one size first, row_size).  Newton-Schulz pairs, whose
-//    powers of two are the call's, keep lo as it is: 2^18 and 2^-39.  A block of 64 k is one chunk: its sum goes
+//    and degrades to an absolute 2^-50 of it beyond (rows of a caller's array are brought to one size first, row_size).  A block of 64 k is one chunk: its sum goes
 //    to its own accumulator columns and the epilogue warps add it, times the two blocks' scales, to float32 registers, rounding to
 //    nearest.  That also keeps the tensor core's own accumulation, which truncates, to the four instructions of hi hi: summed in tensor
 //    memory over K = 512, three terms of it are off by 4e-6 of the largest value; in chunks all sums come out smaller by 0.9e-7 (terms of
@@ -285,18 +284,14 @@ __device__ __forceinline__ float tp_most(const float (&v)[N], float most = 0.f) 
   }
   return most;
 }
-// Two values times a power of two as (hi, lo) pairs of fp16, LOW: lo times 2^11.  What is not finite has NaN for lo, and products with it come out
-// NaN.
-template <bool LOW = false>
+// Two values times a power of two as (hi, lo) pairs of fp16, lo times 2^11.  What is not finite has NaN for lo, and products with it come out NaN.
 __device__ __forceinline__ void tp_split2(float x, float y, float scale, uint32_t &hi, uint32_t &lo) {
   const unsigned long long v = mul2(pack2(x, y), pack2(scale, scale));
   float a, b;
   unpack2(v, a, b);
   const __half2 h = __floats2half2_rn(a, b);
   const float2 f = __half22float2(h);
-  unsigned long long rest = sub2(v, pack2(f.x, f.y));
-  if (LOW) rest = mul2(rest, pack2(0x1p11f, 0x1p11f));
-  unpack2(rest, a, b);
+  unpack2(mul2(sub2(v, pack2(f.x, f.y)), pack2(0x1p11f, 0x1p11f)), a, b);
   const __half2 l = __floats2half2_rn(a, b);
   hi = *reinterpret_cast<const uint32_t *>(&h);
   lo = *reinterpret_cast<const uint32_t *>(&l);
@@ -609,7 +604,6 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
                 ok = false;
                 break;
               }
-              begun = 0;
             }
             if (!mbar_wait(full + 8 * stage, phase)) {
               tp_report(g, 103);
@@ -621,7 +615,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             if (KIND == TP_BACK && !PAIR) d = S::LATE ? tmem + (seg == 0 ? 0u : 256u + 128u * (uint32_t)buf) : d + (seg == 0 ? 0u : 2u * TN);
             const uint32_t sA = smem + (uint32_t)(stage * S::STAGE), sB = sA + TERMS * S::A_BYTES;
             const uint64_t a_hi = tp_desc(sA, a_mn), b_hi = tp_desc(sB, b_mn);
-            if (PAIR && KIND <= TP_BACK) {   // low parts first: what they sum to is 2^11 times itself
+            if (PAIR) {   // low parts first: what they sum to is 2^11 times itself
               const uint64_t a_lo = tp_desc(sA + S::A_BYTES, a_mn), b_lo = tp_desc(sB + S::B_BYTES, b_mn);
 #pragma unroll
               for (int ks = 0; ks < 4; ks++) {
@@ -634,15 +628,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
               for (int ks = 1; ks < 4; ks++) product(d, a_hi + ks * a_step, b_hi + ks * b_step, idesc, 1);
             }
 #pragma unroll
-            for (int ks = 0; ks < (PAIR && KIND <= TP_BACK ? 0 : 4); ks++) {
-              if (PAIR) {
-                const uint64_t a_lo = tp_desc(sA + S::A_BYTES, a_mn), b_lo = tp_desc(sB + S::B_BYTES, b_mn);
-                product(d, a_lo + ks * a_step, b_hi + ks * b_step, idesc, begun);
-                product(d, a_hi + ks * a_step, b_lo + ks * b_step, idesc, 1);
-                product(d, a_hi + ks * a_step, b_hi + ks * b_step, idesc, 1);
-              } else {
-                product(d, a_hi + ks * a_step, b_hi + ks * b_step, idesc, begun);
-              }
+            for (int ks = 0; ks < (PAIR ? 0 : 4); ks++) {
+              product(d, a_hi + ks * a_step, b_hi + ks * b_step, idesc, begun);
               begun = 1;
             }
             commit(empty + 8 * stage);
@@ -688,7 +675,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             const int mine = kb + (lane >> 3), n = k1 - kb < 4 ? k1 - kb : 4;
             // what truncation takes, by the additions that have something to add
             const int steps = mine + 1 == g.kblocks[seg] ? g.last16[seg] : 4;
-            float a = KIND <= TP_BACK ? (steps > 2 ? 1.f + 0x1p-23f : 1.f) : steps == 4 ? 1.f + 0x1p-22f : (steps > 1 ? 1.f + 0x1p-23f : 1.f), b = 1.f;
+            float a = steps > 2 ? 1.f + 0x1p-23f : 1.f, b = 1.f;
             if (mine < k1) {
               if (pa) a *= __ldcg(pa + mine * A.sc_k);
               if (pb) b = __ldcg(pb + mine * B.sc_k);
@@ -856,7 +843,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             g.out_scale[0][(row >> 6) * g.out_scale_ld + (col0 >> 6)] = 1.0f / scale;
           uint32_t w[16], lo[16];
 #pragma unroll
-          for (int j = 0; j < 16; j++) tp_split2<true>(acc[j >> 3][2 * (j & 7)], acc[j >> 3][2 * (j & 7) + 1], scale, w[j], lo[j]);
+          for (int j = 0; j < 16; j++) tp_split2(acc[j >> 3][2 * (j & 7)], acc[j >> 3][2 * (j & 7) + 1], scale, w[j], lo[j]);
           st.begin();
           st.put<64>(0, 0, w);
           st.send(&g.out[0].map, 0, col0, row, 0);
@@ -921,7 +908,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
             for (int j = 0; j < 8; j++) {
               const float x = p == 0 ? u[2 * j] : (p == 1 ? dh[2 * j] : a[2 * j]);
               const float y = p == 0 ? u[2 * j + 1] : (p == 1 ? dh[2 * j + 1] : a[2 * j + 1]);
-              if (PAIR) tp_split2<true>(x, y, scale[p], w[j], lo[j]);
+              if (PAIR) tp_split2(x, y, scale[p], w[j], lo[j]);
               else w[j] = tp_bf16x2(x, y);
             }
             if (PAIR) {
@@ -997,8 +984,8 @@ __global__ void __launch_bounds__(TP_THREADS, 1) tile_product_kernel(const __gri
 #pragma unroll
             for (int k = 0; k < 8; k++) {
               const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&hw[k])), e = __half22float2(*reinterpret_cast<const __half2 *>(&lw[k]));
-              v[2 * k] = alpha * v[2 * k] + beta * (a.x + e.x);
-              v[2 * k + 1] = alpha * v[2 * k + 1] + beta * (a.y + e.y);
+              v[2 * k] = alpha * v[2 * k] + beta * fmaf(e.x, 0x1p-11f, a.x);
+              v[2 * k + 1] = alpha * v[2 * k + 1] + beta * fmaf(e.y, 0x1p-11f, a.y);
             }
           } else {
 #pragma unroll

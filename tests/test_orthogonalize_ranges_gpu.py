@@ -106,3 +106,23 @@ def test_large_eps(shape, dev):
     U = update(53, shape, F32, dev)
     for eps in (1e3, 1e12, 1e30):
         check(ops.orthogonalize(U, eps=eps), U, eps=eps)
+
+
+@pytest.mark.parametrize("which", ["rows", "columns"])
+@pytest.mark.parametrize("least", [1e-3, 1e-6])
+@pytest.mark.parametrize("shape", [(2, 48, 80), (2, 30, 700), (1, 200, 300), (1, 300, 130), (1, 140, 1030)])
+def test_rows_and_columns_that_are_small(shape, least, which, dev):
+    """float32 updates some of whose rows (columns) are `least` of others, against their own size.  Everything that a step adds to such a row goes with the
+    row itself, as does what it is off by: operands 2^-22 and sums 2^-21 of |P| |X| <= 9 a row, five steps of each, on what grows by 3.4 a
+    step: below 5 * 9 / 3.4 * 2^-20 = 2^-16 of the row."""
+    from cuda_mace_b200 import ops
+
+    U = update(61, shape, F32, dev).double()
+    m, n = shape[1:]
+    k = m if which == "rows" else n
+    f = least ** ((torch.arange(k, device=dev, dtype=torch.float64) * 7 % 10) / 9)
+    U = (U * (f[:, None] if which == "rows" else f)).float()
+    out, want = ops.orthogonalize(U).double(), products(U, 5, USUAL, 1e-7)
+    dim = -1 if which == "rows" else -2
+    error = (out - want).norm(dim=dim) / want.norm(dim=dim)
+    assert (error <= 2.0 ** -16).all(), error.max().item()

@@ -13,7 +13,8 @@ Each class keeps the reference's ``forward`` signature and autograd contract:
 * ``CubicSpline.forward(r, r_knots, coeffs, r_width, r_max)`` (src/cubic_spline.cpp:54-68) -> [E,F].
 
 All tensors must live on a CUDA device; float32 and float64 are supported everywhere (the
-reference's Linear is float32 only).  Kernels run on torch's current stream.  There is no
+reference's Linear is float32 only), but by the dense block and its updates (gated_feed_forward, orthogonalize), which take
+float32 and bfloat16.  Kernels run on torch's current stream.  There is no
 fallback: a CPU tensor raises.
 """
 import functools

@@ -305,7 +305,8 @@ int64_t cmace_dense_launches(void);
 /* ---- orthogonalised updates (no counterpart in the reference) -----------------------------------------
  * out = Newton-Schulz products of update [count, rows, cols], contiguous: X = U / (|U| + eps) with the Frobenius norm of each matrix,
  * then steps (1 to 100) times X <- a X + (b S + c S S) X, S = X X^T (rows > cols: X <- a X + X (b S + c S S), S = X^T X, the same values).
- * float or bfloat16 in and out; X is held in float32.  Coefficients under which a singular value in [0, 1] could pass 1e12 are refused.
+ * float or bfloat16 in and out.  Between the steps X is held in float32 where one kernel has them all (shorter side up to 128, longer up to
+ * 1024), as two fp16 values otherwise: 22 bits, and 2^-50 of the bound of its singular values.  Coefficients under which a singular value in [0, 1] could pass 1e12 are refused.
  * out may be update itself.  workspace: cmace_orthogonalize_workspace_bytes(...) bytes, aligned to 256, not shared by calls that may
  * overlap.  A matrix with an infinity or a NaN comes out not finite, no other one.  status: as for cmace_gemm3x_f32. */
 int64_t cmace_orthogonalize_workspace_bytes(int is_f32, int64_t count, int64_t rows, int cols);

@@ -10,7 +10,7 @@
 // backward's hidden values 178 (1 160: 56 bytes of operands for 48 of products a cycle, and 200 MB put down), dx 96, dW 97 + 51; float32 as
 // pairs: 283, 152, 540, 298, 306 + 149 (1 350 to 1 450 TFLOP/s of fp16 products), operands 37 before the first and 71 before the third.  Widths
 // 128 and 512, 64 000 rows: K is two blocks long, so the elementwise epilogue bounds the first and third: 30, 17, 68, 27, 37 in bf16, 63, 32, 149, 54,
-// 74 in float32, where h goes out at 2.1 and h, dg, du at 2.6 TB/s; operands take 14 before the first and 54 before the third.
+// 74 in float32, where h goes out at 2.1 and h, dg, du at 2.6 TB/s; operands take 14 before the first and 43 before the third.
 // Only x and the weights are kept for the backward: forming g and u again costs 4 M C H operations, keeping them in float32 16 bytes
 // a hidden value written and read (what would be as exact as the products are), which pays from C of about 1 000 only.
 //
@@ -44,7 +44,7 @@ struct RowsJob {
   const void *src[2];   // x, dy or null
   __half *hi[4];        // x~, dy~, x s t, dy s^2 (null: not wanted), the lo parts a plane behind
   float *scale[4], *size[2];   // inverse scales of the blocks; s and t, ones behind the last row up to a multiple of 256
-  float *most[2];       // largest finite magnitudes of the rows' slabs, [slabs][rows]; null: x alone, of up to two blocks of columns, which a CTA has whole
+  float *most[2];       // largest finite magnitudes of the rows' slabs, [slabs][rows]; null: rows of up to two blocks of columns, which a CTA has whole
   int64_t rows, plane, blocks;   // blocks: CTAs
   int cols, ld, blocks_n, bf16, wide, sources, slabs, slab;   // slab: columns
 };
@@ -85,8 +85,8 @@ constexpr int PREP_SLABS = 16;
 struct PrepThread {
   int64_t row0;
   int first, in, n;   // its first row and column, rows of the block
-  __device__ __forceinline__ PrepThread(int64_t row0, int64_t rows)
-      : row0(row0), first(threadIdx.x >> 4), in(4 * (threadIdx.x & 15)), n((int)(rows - row0 < 64 ? rows - row0 : 64)) {}
+  __device__ __forceinline__ PrepThread(int t, int64_t row0, int64_t rows)
+      : row0(row0), first(t >> 4), in(4 * (t & 15)), n((int)(rows - row0 < 64 ? rows - row0 : 64)) {}
   __device__ __forceinline__ void fetch(float4 (&x)[4], const void *src, int col, int cols, bool bf16, bool wide) const {
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = prep_load(src, (row0 + first + 16 * i) * cols + col, first + 16 * i < n ? cols - col : 0, bf16, wide);
@@ -102,7 +102,7 @@ __device__ __forceinline__ void prep_row_most(float (&most)[4]) {   // of the 16
 // Largest finite magnitudes of 64 rows' slabs of columns
 __global__ void __launch_bounds__(PREP_THREADS) row_most_kernel(const RowsJob R) {
   grid_begin();
-  const PrepThread T((int64_t)blockIdx.x * 64, R.rows);
+  const PrepThread T(threadIdx.x, (int64_t)blockIdx.x * 64, R.rows);
   const int k = blockIdx.z, end = min(R.cols, (int)(blockIdx.y + 1) * R.slab);
   float most[4] = {};
 #pragma unroll 4
@@ -118,20 +118,25 @@ __global__ void __launch_bounds__(PREP_THREADS) row_most_kernel(const RowsJob R)
     if (T.in == 0 && T.first + 16 * i < T.n) R.most[k][blockIdx.y * R.rows + T.row0 + T.first + 16 * i] = most[i];
 }
 
-// COPY: 64 x 64 bf16 values.  Otherwise pairs: a block of a weight, or of 64 rows of x the whole (WHOLE), or one block of x or dy.
-enum PrepKind { PREP_COPY, PREP_WHOLE, PREP_BLOCKS };
+// COPY: 64 x 64 bf16 values.  Otherwise pairs: a block of a weight, or one block of x or dy (BLOCKS), or 64 rows of x (WHOLE) or of x and dy (BOTH, a
+// half of the threads each) of up to 128 columns, whose sizes the CTA finds itself: 64 000 rows of 128, x and dy: 43 us, by blocks
+// and a kernel for the sizes 54.
+enum PrepKind { PREP_COPY, PREP_WHOLE, PREP_BOTH, PREP_BLOCKS };
+constexpr int prep_threads(int kind) { return (kind == PREP_BOTH ? 2 : 1) * PREP_THREADS; }
 template <int KIND>
-__global__ void __launch_bounds__(PREP_THREADS, KIND == PREP_COPY ? 8 : KIND == PREP_WHOLE ? 4 : 5) prep_kernel(const __grid_constant__ PrepArgs p) {
-  constexpr int NB = KIND == PREP_WHOLE ? 2 : 1;       // blocks of a CTA
-  __shared__ float most_of[NB][2][PREP_THREADS / 32];   // of both layouts
-  __shared__ int top_of[2][PREP_THREADS / 32];
+__global__ void __launch_bounds__(prep_threads(KIND), KIND == PREP_COPY ? 8 : KIND == PREP_WHOLE ? 4 : KIND == PREP_BOTH ? 2 : 5)
+    prep_kernel(const __grid_constant__ PrepArgs p) {
+  constexpr bool ROWS = KIND == PREP_WHOLE || KIND == PREP_BOTH;
+  constexpr int NB = ROWS ? 2 : 1;                         // blocks of a CTA
+  __shared__ float most_of[2][NB][2][PREP_THREADS / 32];   // of both sources and layouts
+  __shared__ int top_of[2][PREP_THREADS / 32], exponent_of[2][64];
   grid_begin();
   const RowsJob &R = p.rows;
   const bool rows = KIND != PREP_COPY && (int64_t)blockIdx.x < R.blocks;
   int j = 0;
   while (j + 1 < p.jobs && (int64_t)blockIdx.x >= p.job[j + 1].first) j++;
   const PrepJob &J = p.job[j];
-  const int across = rows ? (KIND == PREP_WHOLE ? 1 : R.blocks_n * R.sources) : J.blocks_n, t = threadIdx.x;
+  const int across = rows ? (ROWS ? 1 : R.blocks_n * R.sources) : J.blocks_n, t = threadIdx.x % PREP_THREADS, half = threadIdx.x / PREP_THREADS;
   const int64_t b = rows ? blockIdx.x : blockIdx.x - J.first, rb = b / across;
   int cb = (int)(b - rb * across);
   if constexpr (KIND == PREP_COPY) {
@@ -143,10 +148,11 @@ __global__ void __launch_bounds__(PREP_THREADS, KIND == PREP_COPY ? 8 : KIND == 
       for (int r = t >> 6; r < 64 && row0 + r < J.rows; r += 4) d[(row0 + r) * J.ld + col] = s[(row0 + r) * J.cols + col];
     return;
   }
-  const int k = KIND == PREP_BLOCKS && rows && R.sources == 2 ? cb & 1 : 0;   // x or dy
+  if (!rows && half) return;
+  const int k = KIND == PREP_BOTH ? half : KIND == PREP_BLOCKS && rows && R.sources == 2 ? cb & 1 : 0;   // x or dy
   if (KIND == PREP_BLOCKS && rows && R.sources == 2) cb >>= 1;
-  const PrepThread T(rb * 64, rows ? R.rows : J.rows);
-  const int warp = t >> 5, cols = rows ? R.cols : J.cols, ld = rows ? R.ld : J.ld, blocks = KIND == PREP_WHOLE && rows ? R.blocks_n : 1;
+  const PrepThread T(t, rb * 64, rows ? R.rows : J.rows);
+  const int warp = t >> 5, cols = rows ? R.cols : J.cols, ld = rows ? R.ld : J.ld, blocks = ROWS && rows ? R.blocks_n : 1;
   const bool bf16 = rows ? R.bf16 : J.bf16, wide = rows ? R.wide : (cols & 3) == 0 && (reinterpret_cast<uintptr_t>(J.src) & 15) == 0 && !bf16;
   float4 x[NB][4];
 #pragma unroll
@@ -159,10 +165,10 @@ __global__ void __launch_bounds__(PREP_THREADS, KIND == PREP_COPY ? 8 : KIND == 
   const auto exp2i = [](int e) { return __uint_as_float((uint32_t)(e + 127) << 23); };   // -126 <= e <= 127
   if (rows) {
 #pragma unroll
-    for (int o = 0; o < (KIND == PREP_WHOLE ? 1 : 2); o++) {
+    for (int o = 0; o < (ROWS ? 1 : 2); o++) {
       if (o >= R.sources) break;
       float most[4] = {};
-      if constexpr (KIND == PREP_WHOLE) {
+      if constexpr (ROWS) {
 #pragma unroll
         for (int e = 0; e < NB; e++) {
           if (e >= blocks) break;
@@ -181,9 +187,10 @@ __global__ void __launch_bounds__(PREP_THREADS, KIND == PREP_COPY ? 8 : KIND == 
       for (int i = 0; i < 4; i++) {
         below[o][i] = most[i] == 0.f ? NONE : (int)(__float_as_uint(most[i]) >> 23) - 127;
         top = max(top, below[o][i]);
+        if (KIND == PREP_BOTH && T.in == 0) exponent_of[k][T.first + 16 * i] = below[o][i];
       }
       top = __reduce_max_sync(0xffffffffu, top);
-      if ((t & 31) == 0) top_of[o][warp] = top;
+      if ((t & 31) == 0) top_of[o ? 1 - k : k][warp] = top;
     }
     __syncthreads();
 #pragma unroll
@@ -191,10 +198,12 @@ __global__ void __launch_bounds__(PREP_THREADS, KIND == PREP_COPY ? 8 : KIND == 
       if (o >= R.sources) break;
       int top = NONE;
 #pragma unroll
-      for (int w = 0; w < PREP_THREADS / 32; w++) top = max(top, top_of[o][w]);
+      for (int w = 0; w < PREP_THREADS / 32; w++) top = max(top, top_of[o ? 1 - k : k][w]);
 #pragma unroll
-      for (int i = 0; i < 4; i++)
+      for (int i = 0; i < 4; i++) {
+        if (KIND == PREP_BOTH && o) below[o][i] = exponent_of[1 - k][T.first + 16 * i];
         if (below[o][i] != NONE) below[o][i] = min(top - below[o][i], 126);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -208,7 +217,7 @@ __global__ void __launch_bounds__(PREP_THREADS, KIND == PREP_COPY ? 8 : KIND == 
     const float of_own = own == NONE ? 0.f : exp2i(-own), of_other = other == NONE ? 0.f : exp2i(-other);
     return times(times(v, k ? of_other : of_own), of_other);
   };
-  __half *const hi[2] = {rows ? R.hi[k] : static_cast<__half *>(J.hi), KIND == PREP_BLOCKS && rows ? R.hi[2 + k] : nullptr};
+  __half *const hi[2] = {rows ? R.hi[k] : static_cast<__half *>(J.hi), KIND != PREP_WHOLE && rows ? R.hi[2 + k] : nullptr};
 #pragma unroll
   for (int e = 0; e < NB; e++)
 #pragma unroll
@@ -218,7 +227,7 @@ __global__ void __launch_bounds__(PREP_THREADS, KIND == PREP_COPY ? 8 : KIND == 
 #pragma unroll
       for (int i = 0; i < 4; i++) most = fmaxf(most, prep_most(value(x[e][i], how, i)));
       most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-      if ((t & 31) == 0) most_of[e][how][warp] = most;
+      if ((t & 31) == 0) most_of[half][e][how][warp] = most;
     }
   __syncthreads();
 #pragma unroll
@@ -226,9 +235,9 @@ __global__ void __launch_bounds__(PREP_THREADS, KIND == PREP_COPY ? 8 : KIND == 
 #pragma unroll
     for (int how = 0; how < 2; how++) {
       if (e >= blocks || !hi[how]) continue;
-      float most = most_of[e][how][0];
+      float most = most_of[half][e][how][0];
 #pragma unroll
-      for (int w = 1; w < PREP_THREADS / 32; w++) most = fmaxf(most, most_of[e][how][w]);
+      for (int w = 1; w < PREP_THREADS / 32; w++) most = fmaxf(most, most_of[half][e][how][w]);
       const float scale = tp_scale(most);
       if (t == 0) (rows ? R.scale[2 * how + k] + rb * R.blocks_n + cb + e : J.scale + b)[0] = 1.0f / scale;
       const int col = 64 * (cb + e) + T.in;
@@ -854,7 +863,7 @@ static TakenRows take_rows(Carve &w, PrepArgs &prep, int64_t &blocks, const Feed
   j.rows = f.M, j.cols = f.C, j.plane = r.x.plane(), j.ld = (int)r.x.ld, j.blocks_n = (int)r.x.blocks_n(), j.bf16 = !f.f32;
   j.wide = f.f32 && f.C % 4 == 0 && aligned16(f.x) && (!back || aligned16(f.gy));
   j.blocks = r.x.blocks_m();
-  if (back || j.blocks_n > 2) {   // sizes by a kernel of their own
+  if (j.blocks_n > 2) {   // sizes by a kernel of their own
     j.slab = (int)up(std::max(256, (f.C + PREP_SLABS - 1) / PREP_SLABS), 64), j.slabs = (f.C + j.slab - 1) / j.slab;
     for (int k = 0; k < j.sources; k++) j.most[k] = w.take<float>(j.slabs * f.M);
     j.blocks *= j.blocks_n * j.sources;
@@ -952,8 +961,11 @@ static int run_prep(const PrepArgs &p, int64_t blocks, cudaStream_t st, const ch
   if (p.rows.slabs)
     launch_dense(row_most_kernel, dim3((unsigned)((p.rows.rows + 63) / 64), (unsigned)p.rows.slabs, (unsigned)p.rows.sources), PREP_THREADS,
                    st, p.rows);
-  const auto kernel = !p.rows.blocks ? prep_kernel<PREP_COPY> : p.rows.slabs ? prep_kernel<PREP_BLOCKS> : prep_kernel<PREP_WHOLE>;
-  launch_dense(kernel, dim3((unsigned)blocks), PREP_THREADS, st, p);
+  const dim3 grid((unsigned)blocks);
+  if (!p.rows.blocks) launch_dense(prep_kernel<PREP_COPY>, grid, prep_threads(PREP_COPY), st, p);
+  else if (p.rows.slabs) launch_dense(prep_kernel<PREP_BLOCKS>, grid, prep_threads(PREP_BLOCKS), st, p);
+  else if (p.rows.sources == 2) launch_dense(prep_kernel<PREP_BOTH>, grid, prep_threads(PREP_BOTH), st, p);
+  else launch_dense(prep_kernel<PREP_WHOLE>, grid, prep_threads(PREP_WHOLE), st, p);
   return check_launch(what);
 }
 

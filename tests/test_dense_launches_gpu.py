@@ -18,8 +18,8 @@ def launches(f):
 
 
 # forward: a pass over the weights 2, the whole block 1, rows and weights laid out 1 (2 with sizes of wide rows) and two products, bf16 where it lies 2;
-# backward: layout 2 (bf16: 0), hidden values, gradient of x, two products or one and a sum for the weights
-@pytest.mark.parametrize("M,C,H,dtype,forward,backward", [(4, 512, 1024, F32, 2, None), (100, 64, 128, F32, 1, None), (9000, 64, 128, F32, 3, 6),
+# backward: layout as for the forward pass (bf16: 0), hidden values, gradient of x, two products or one and a sum for the weights
+@pytest.mark.parametrize("M,C,H,dtype,forward,backward", [(4, 512, 1024, F32, 2, None), (100, 64, 128, F32, 1, None), (9000, 64, 128, F32, 3, 5),
                                                           (9000, 192, 256, F32, 4, 6), (9000, 64, 128, BF16, 2, 4), (9000, 65, 128, BF16, 3, 5)])
 def test_feed_forward(M, C, H, dtype, forward, backward):
     from cuda_mace_b200 import ops

@@ -342,7 +342,7 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
     """Matrices of `update` [..., m, n] brought near their orthogonal factors by Newton-Schulz products: X = U / (|U| + eps)
     with the Frobenius norm of each matrix, then `steps` times X <- a X + (b S + c S S) X with S = X X^T and
     (a, b, c) = `coefficients`.  float32 or bfloat16; a new tensor of the same shape and type.  For the updates of weight
-    matrices, stacks like Linear's [4, K, N] and ElementalLinear's [Z, 4, K, N] included; has no gradient."""
+    matrices, stacks of them included; has no gradient, and tracers cannot record it."""
     steps = operator.index(steps)
     _check_cuda(update)
     if update.dtype not in (torch.float32, torch.bfloat16):

@@ -35,11 +35,12 @@ struct PrepJob {
   int64_t rows, first; // first block of this job
   int cols, ld, blocks_n, bf16;   // bf16: of the source of a pair
 };
-// Rows of x, and going back of dL/dy, as pairs.  A block of 64 x 64 values has one scale, under which a row 2^-40 of the largest is zeros, and
-// h goes with the square of a small row.  So the rows of 64 are brought to the size of their largest before they are split, each by a
-// power of two: x~ = x / s, dy~ = dy / t with s, t <= 1 of the row.  A product's rows follow, and what is linear in them: h~ = h / s^2 = g~ sigmoid(g~ s) u~ (SiLU),
-// dg~ = dg / (s t), du~ = du / (s t); y = (h~ Wd) s^2 and dx = (..) s t at the end.  A sum over rows has each at the size of its
-// contribution: dWg = (x s t)^T dg~, dWu = (x s t)^T du~, dWd = h~^T (dy s^2), for which x and dy are laid out a second time.
+// Rows of x, and going back of dL/dy, as pairs.  A block of 64 x 64 values has one scale, under which a row far below the largest is zeros, and
+// h goes with the square of a small row.  So the rows of 64 are brought to one size before they are split, each by a power of two: x~ = x / s, dy~ = dy / t.
+// A product's rows follow, and what is linear in them: h~ = h / s^2 = g~ sigmoid(g~ s) u~ (SiLU), dg~ = dg / (s t), du~ = du / (s t); y = (h~ Wd) s^2 and
+// dx = (..) s t at the end.  A sum over rows has each at the size of its contribution: dWg = (x s t)^T dg~, dWu = (x s t)^T du~,
+// dWd = h~^T (dy s^2), for which x and dy are laid out a second time.
+// The one size is the mean of the rows' exponents: a row of 1e30, whose own h is no float32 value, then leaves the other rows' h~ where it was.
 struct RowsJob {
   const void *src[2];   // x, dy or null
   __half *hi[4];        // x~, dy~, x s t, dy s^2 (null: not wanted), the lo parts a plane behind
@@ -129,7 +130,7 @@ __global__ void __launch_bounds__(prep_threads(KIND), KIND == PREP_COPY ? 8 : KI
   constexpr bool ROWS = KIND == PREP_WHOLE || KIND == PREP_BOTH;
   constexpr int NB = ROWS ? 2 : 1;                         // blocks of a CTA
   __shared__ float most_of[2][NB][2][PREP_THREADS / 32];   // of both sources and layouts
-  __shared__ int top_of[2][PREP_THREADS / 32], exponent_of[2][64];
+  __shared__ int sum_of[2][PREP_THREADS / 32], top_of[2][PREP_THREADS / 32], exponent_of[2][64];
   grid_begin();
   const RowsJob &R = p.rows;
   const bool rows = KIND != PREP_COPY && (int64_t)blockIdx.x < R.blocks;
@@ -158,10 +159,9 @@ __global__ void __launch_bounds__(prep_threads(KIND), KIND == PREP_COPY ? 8 : KI
 #pragma unroll
   for (int e = 0; e < NB; e++)
     if (e < blocks) T.fetch(x[e], rows ? R.src[k] : J.src, 64 * (cb + e) + T.in, cols, bf16, wide);
-  // The sizes of this thread's rows, its own ([0]) and the other source's, by the exponents of the rows' largest finite values (a
-  // subnormal's counts as -127)
-  constexpr int NONE = -0x7FFFFFFF;
-  int below[2][4] = {};   // exponents, then how far below the group's largest (126 at most); NONE: a row of zeros
+  // The sizes of this thread's rows, its own ([0]) and the other source's, by the exponents of the rows' largest finite values
+  constexpr int NONE = 1 << 20;
+  int below[2][4] = {};   // exponents with float32's bias, then how far below the group's mean (126 at most); NONE: a row of zeros
   const auto exp2i = [](int e) { return __uint_as_float((uint32_t)(e + 127) << 23); };   // -126 <= e <= 127
   if (rows) {
 #pragma unroll
@@ -182,27 +182,28 @@ __global__ void __launch_bounds__(prep_threads(KIND), KIND == PREP_COPY ? 8 : KI
           if (T.first + 16 * i < T.n) most[i] = __ldcg(from + 16 * i);
       }
       prep_row_most(most);
-      int top = NONE;
+      int sum = 0;   // and the number of them, above
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        below[o][i] = most[i] == 0.f ? NONE : (int)(__float_as_uint(most[i]) >> 23) - 127;
-        top = max(top, below[o][i]);
+        below[o][i] = most[i] == 0.f ? NONE : (int)(__float_as_uint(most[i]) >> 23);
+        if (T.in == 0 && below[o][i] != NONE) sum += below[o][i] + (1 << 16);
         if (KIND == PREP_BOTH && T.in == 0) exponent_of[k][T.first + 16 * i] = below[o][i];
       }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if ((t & 31) == 0) top_of[o ? 1 - k : k][warp] = top;
+      sum = __reduce_add_sync(0xffffffffu, sum);
+      if ((t & 31) == 0) sum_of[o ? 1 - k : k][warp] = sum;
     }
     __syncthreads();
 #pragma unroll
     for (int o = 0; o < (KIND == PREP_WHOLE ? 1 : 2); o++) {
       if (o >= R.sources) break;
-      int top = NONE;
+      int sum = 0;
 #pragma unroll
-      for (int w = 0; w < PREP_THREADS / 32; w++) top = max(top, top_of[o ? 1 - k : k][w]);
+      for (int w = 0; w < PREP_THREADS / 32; w++) sum += sum_of[o ? 1 - k : k][w];
+      const int count = max(sum >> 16, 1), mean = ((sum & 0xFFFF) + count / 2) / count;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         if (KIND == PREP_BOTH && o) below[o][i] = exponent_of[1 - k][T.first + 16 * i];
-        if (below[o][i] != NONE) below[o][i] = min(top - below[o][i], 126);
+        if (below[o][i] != NONE) below[o][i] = min(max(mean - below[o][i], -126), 126);
       }
     }
 #pragma unroll
@@ -210,12 +211,29 @@ __global__ void __launch_bounds__(prep_threads(KIND), KIND == PREP_COPY ? 8 : KI
       if (cb == 0 && T.in == 0 && T.first + 16 * i < T.n) R.size[k][T.row0 + T.first + 16 * i] = below[0][i] == NONE ? 1.f : exp2i(-below[0][i]);
     if (cb == 0 && T.row0 + 64 >= R.rows && R.rows + t < (R.rows + 255) / 256 * 256) R.size[k][R.rows + t] = 1.f;
   }
-  // At the group's size, and as a contribution: x s t or dy s^2.  A row of zeros contributes nothing, whatever the other has.
+  // As a contribution, x s t or dy s^2, below the group's largest s t or s^2.  A row of zeros contributes nothing, whatever the other has.
+  int less[4] = {}, top = -NONE;
+  if (KIND != PREP_WHOLE && rows && R.sources == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int own = below[0][i], other = below[1][i];
+      less[i] = own == NONE || other == NONE ? -NONE : k ? -2 * other : -own - other;
+      top = max(top, less[i]);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((t & 31) == 0) top_of[half][warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < PREP_THREADS / 32; w++) top = max(top, top_of[half][w]);
+    if (top == -NONE) top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) less[i] -= top;
+  }
+  const auto twice = [&](int e) { return make_float2(exp2i(e / 2), exp2i(e - e / 2)); };   // 2^e as two factors, |e| <= 252
   const auto value = [&](const float4 &v, int how, int i) {
-    const int own = below[0][i], other = below[1][i];
-    if (how == 0) return times(v, own == NONE ? 1.f : exp2i(own));
-    const float of_own = own == NONE ? 0.f : exp2i(-own), of_other = other == NONE ? 0.f : exp2i(-other);
-    return times(times(v, k ? of_other : of_own), of_other);
+    if (how == 0) return times(v, below[0][i] == NONE ? 1.f : exp2i(below[0][i]));
+    const float2 f = less[i] < -252 ? make_float2(0.f, 0.f) : twice(less[i]);
+    return times(times(v, f.x), f.y);
   };
   __half *const hi[2] = {rows ? R.hi[k] : static_cast<__half *>(J.hi), KIND != PREP_WHOLE && rows ? R.hi[2 + k] : nullptr};
 #pragma unroll
@@ -239,7 +257,10 @@ __global__ void __launch_bounds__(prep_threads(KIND), KIND == PREP_COPY ? 8 : KI
 #pragma unroll
       for (int w = 1; w < PREP_THREADS / 32; w++) most = fmaxf(most, most_of[half][e][how][w]);
       const float scale = tp_scale(most);
-      if (t == 0) (rows ? R.scale[2 * how + k] + rb * R.blocks_n + cb + e : J.scale + b)[0] = 1.0f / scale;
+      if (t == 0) {
+        const float2 f = how ? twice(top) : make_float2(1.f, 1.f);
+        (rows ? R.scale[2 * how + k] + rb * R.blocks_n + cb + e : J.scale + b)[0] = 1.0f / scale * f.x * f.y;
+      }
       const int col = 64 * (cb + e) + T.in;
       __half *const to = hi[how] + (T.row0 + T.first) * ld + col, *const to_lo = to + (rows ? R.plane : static_cast<__half *>(J.lo) - hi[how]);
 #pragma unroll

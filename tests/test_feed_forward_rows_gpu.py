@@ -2,7 +2,7 @@
 block of 64 with it, and the weights' gradients against the sums of their terms.
 
 Bounds, all in float64.  float32 goes as pairs of fp16 values: an operand is off by at most 2^-22 of itself and by 2^-39 of the largest value
-of its block of 64 x 64, where the rows of a block have been brought to the size of their largest first.  With s a row's power of two (of x; t: of
+of its block of 64 x 64, where the rows of a block have been brought to one size first.  With s a row's power of two (of x; t: of
 dL/dy), a block's largest value is therefore at most 2 max|x / s| of the whole matrix, and that loses 2^-38 max|x / s| s of a value of the row.
 The like holds for h / s^2, dg / (s t), du / (s t), and for the contributions x s t and dy s^2 of the sums over rows.  The product of two low
 parts (2^-22) is left out, 64 k are summed in 12 truncating additions (2^-22 of the magnitudes) and added with rounding (2^-24)."""
@@ -224,3 +224,53 @@ def test_layouts_of_spread_rows(M, C, H, apart, dev):
         (g,) = torch.autograd.grad(ops.gated_feed_forward(*leaves), leaves[k], args[4])
         assert torch.equal(g, got[name]), name
         inside({name: g}, want, (name,))
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("M,C,H", [(130, 128, 200), (150, 200, 136)])
+@pytest.mark.parametrize("size", [1e15, 1e20, 1e30, 3e37])
+def test_rows_whose_hidden_values_overflow(M, C, H, size, activation, dev):
+    """Rows so large that their own h, or y, is no float32 value, beside rows that are not: those keep theirs."""
+    args = case(M + 83, M, C, H, F32, dev)
+    large = torch.zeros(M, dtype=torch.bool, device=dev)
+    large[[2, 40, 70, M - 1]] = True
+    few = [t.clone() for t in args]
+    few[0][large], few[4][large] = 0, 0
+    args[0][large] = (args[0][large].double() * size / 8).clamp(-3e38, 3e38).float()
+    want = reference(*(v.double() for v in few), activation)   # of the other rows
+    got = run(args, activation)
+    for name in ("y", "x"):
+        v, bound = want[name]
+        off = (got[name].double() - v).abs()[~large]
+        assert torch.isfinite(off).all() and (off <= bound[~large] + 1e-37).all(), name
+    # rows that do not count leave the weights' gradients alone, as far as zero times their h is one
+    if size < 1e18:
+        args[4][large] = 0
+        inside(run(args, activation), want, ("w_gate", "w_up", "w_down"))
+
+
+@pytest.mark.parametrize("M,C,H", [(130, 128, 200), (150, 200, 136)])
+def test_weights_and_rows_far_apart(M, C, H, dev):
+    """Weights of 1e20: half of the rows are small enough for them, the others overflow."""
+    x, wg, wu, wd, gy = case(M + 89, M, C, H, F32, dev)
+    wg, wu = wg * 1e20, wu * 1e20
+    x[::2] *= 1e-20
+    few = [x.clone(), wg, wu, wd, gy.clone()]
+    few[0][1::2], few[4][1::2] = 0, 0
+    want = reference(*(v.double() for v in few), "silu")
+    got = run([x, wg, wu, wd, gy])
+    for name in ("y", "x"):
+        v, bound = want[name]
+        off = (got[name].double() - v).abs()[::2]
+        assert torch.isfinite(off).all() and (off <= bound[::2] + 1e-37).all(), name
+
+
+def test_contributions_of_large_rows(dev):
+    """Rows of 1e20 with gradients of 1e-25 and weights that keep h a float32 value: the weights' gradients are finite sums of all rows."""
+    M, C, H = 200, 128, 136
+    x, wg, wu, wd, gy = case(97, M, C, H, F32, dev)
+    wg, wu = wg * 1e-12, wu * 1e-12
+    x[::3] *= 1e20
+    gy[::3] *= 1e-25
+    args = [x, wg, wu, wd, gy]
+    inside(run(args), reference(*(v.double() for v in args), "silu"))
